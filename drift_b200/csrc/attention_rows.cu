@@ -1,0 +1,718 @@
+// attention_chunks for few rows: a decoding step, drafted tokens, and every
+// chunk in F32.
+//
+// A unit is a key head of one sequence with up to 8 NT of the (token, query
+// head) rows that read it; a CTA takes one split of the unit's key tiles,
+// each of its 8 warps every eighth tile. The products are turned round --
+// scores^T = K q^T and out^T = V^T p^T by mma.sync m16n8k16, keys and then
+// dimensions as the 16 rows and the query rows as the 8 columns -- because
+// there are few query rows: 8 columns leave nothing idle where 16 rows would
+// be half empty. Keys and values go from the cache straight into the
+// registers that the matrix instruction reads: a lane's 16 bytes of a key row
+// (or of a dimension's consecutive positions) become its A fragments by
+// numbering the product's inner index as the bytes lie, which the query
+// fragments, laid out once in shared memory, follow. Codes become F16 by two
+// byte permutes and a subtraction, exactly; a key's scale multiplies its
+// score, and a value's its weight.
+//
+// F32 rows: q and the weights are two F16 terms each (x = hi + lo to 2^-22),
+// keys and values exact, so the products are F32-grade. BF16 rows: q is one
+// term, exactly (after a power of two per row), and a weight is rounded to
+// F16 (off by 2^-11 at most, the result's own rounding is 2^-8).
+//
+// Softmax in F32, a running maximum and sum per warp; the warps meet
+// in shared memory, the splits in a second launch (attention_join_kernel).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "chunks.cuh"
+#include "common.cuh"
+#include "registry.cuh"
+
+namespace drift {
+
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int THREADS = 32 * WARPS;
+constexpr float LOG2E = 1.4426950408889634f;
+// A weight is e^WEIGHT_LOG = 2^14 at the row's largest score, and a row of q
+// 2^Q_BITS and more at its largest value: F16's second terms stop at 2^-24, which is
+// then 2^-38 of the largest weight (it is 2^-19 of a weight of 2^-6 without:
+// the typical one of 4096 random scores).
+constexpr float WEIGHT_LOG = 9.704060527839234f;
+constexpr int Q_BITS = 12;
+
+// e^(score - base), 0 for a score that is not seen.
+__device__ __forceinline__ float weight_of(float score, float base) {
+  return score == -INFINITY ? 0.0f : exp2f((score - base) * LOG2E);
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The 8 x 8 tile of 16-bit values turned round (lane 4 i + j holds row i's
+// values 2 j and 2 j + 1).
+__device__ __forceinline__ uint32_t turn(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 pair_value(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+// Four codes as two pairs of F16: a byte u = code + 128 under the exponent of
+// 1024 is 1024 + u, less 1152.
+__device__ __forceinline__ void code_pairs(uint32_t codes, uint32_t& first, uint32_t& second) {
+  const uint32_t u = codes ^ 0x80808080u;
+  const __half2 less = __half2half2(__ushort_as_half(0x6480));  // 1152
+  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), less);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), less);
+  first = *reinterpret_cast<const uint32_t*>(&x);
+  second = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// How a lane's loads cover rows of D values, 16 of them to a k-step: chunks of
+// 16 bytes a lane while whole ones last, then (D = 80) one k-step of 4 values
+// a lane. first_of(k-step) is where lane t's four values of the step start.
+template <int D, bool CODES>
+struct RowMap {
+  static constexpr int PER = CODES ? 16 : 8;            // values of a 16-byte chunk
+  static constexpr int STEPS_PER = PER / 4;             // k-steps of a chunk
+  static constexpr int CHUNKS = D / (4 * PER);          // whole chunks
+  static constexpr int STEPS = D / 16;
+  static constexpr int TAIL = STEPS - CHUNKS * STEPS_PER;  // 0 or 1
+  static constexpr int WORDS = CODES ? STEPS : 2 * STEPS;  // 32-bit words a lane holds of a row
+  static_assert(TAIL <= 1, "one k-step past the chunks at most");
+  __device__ static int first_of(int step, int t) {
+    return step < CHUNKS * STEPS_PER ? (step / STEPS_PER) * 4 * PER + PER * t + 4 * (step % STEPS_PER)
+                                     : CHUNKS * 4 * PER + 4 * t;
+  }
+};
+
+template <int D_, bool CODES_, bool BF16_, int NT_, int TILE_>
+struct RowsTraits {
+  static constexpr int D = D_, NT = NT_, TILE = TILE_;
+  static constexpr bool CODES = CODES_, BF16 = BF16_;
+  static constexpr int TERMS = BF16 ? 1 : 2;
+  using Map = RowMap<D, CODES>;
+  static constexpr int MT = TILE / 16;   // 16-key tiles of a warp's tile
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int DM = D / 16;      // 16-dimension tiles of the output
+  static constexpr int VWORDS = CODES ? TILE / 16 : TILE / 8;  // words a lane holds of a dimension's positions
+  static constexpr int Q_BYTES = Map::STEPS * NT * TERMS * 32 * 8;
+  static constexpr int MERGE_BYTES = WARPS * ROWS * (D + 4) * 4;
+  static constexpr int BYTES = Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;
+};
+
+template <class T>
+struct RowsWarp {
+  static constexpr int D = T::D, TILE = T::TILE, MT = T::MT, DM = T::DM;
+  static constexpr bool CODES = T::CODES;
+  using Map = typename T::Map;
+
+  const AttentionChunksArgs& a;
+  const Chunk& chunk;
+  const SeenTiles& seen;
+  const int head, lane, g, t;
+  uint32_t k[MT][2][Map::WORDS];
+  uint32_t v[DM][2][T::VWORDS];
+  float k_scale[MT][2], v_scale[MT][2];
+
+  __device__ RowsWarp(const AttentionChunksArgs& a, const Chunk& c, const SeenTiles& s, int head, int lane)
+      : a(a), chunk(c), seen(s), head(head), lane(lane), g(lane / 4), t(lane % 4) {}
+
+  // The page that holds the sixteen positions from `position` on, or -1: past
+  // the last key, or a page that the cache does not have.
+  __device__ int page_of(int position) const {
+    if (position >= seen.end) return -1;
+    const int page = chunk.table[position / a.at.page_size];
+    if (page >= 0 && page < a.at.pages) return page;
+    chunk_error(a.error);
+    return -1;
+  }
+  // Row r of the score tile m, r = g or g + 8, is this position of the tile:
+  // the product of weights and values then meets the positions in the order
+  // in which a lane's value words hold them.
+  __device__ int position_of(int m, int half) const {
+    return TILE / 4 * (g / 2) + 4 * m + g % 2 + 2 * half;
+  }
+
+  __device__ void load_keys(int key0) {
+    const int base = key0 + TILE / 4 * (g / 2) / 16 * 16;  // the sixteen this lane's rows are in
+    const int page = page_of(base);
+    const int in_page = base % a.at.page_size;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int place = in_page + (position_of(m, half) + key0 - base);
+        const long long row = (((long long)page * a.at.page_size + place) * a.kv_heads + head) * D;
+#pragma unroll
+        for (int c = 0; c < Map::CHUNKS; ++c) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (page >= 0) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.keys) + (CODES ? row : 2 * row)) + 4 * c + t);
+          k[m][half][4 * c] = x.x, k[m][half][4 * c + 1] = x.y;
+          k[m][half][4 * c + 2] = x.z, k[m][half][4 * c + 3] = x.w;
+        }
+        if constexpr (Map::TAIL) {
+          constexpr int W = 4 * Map::CHUNKS;
+          const uint8_t* from = static_cast<const uint8_t*>(a.keys) + (CODES ? 1 : 2) * (row + Map::CHUNKS * 4 * Map::PER + 4 * t);
+          if constexpr (CODES) {
+            k[m][half][W] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0;
+          } else {
+            const uint2 x = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
+            k[m][half][W] = x.x, k[m][half][W + 1] = x.y;
+          }
+        }
+        if constexpr (CODES) {
+          const long long at = ((long long)page * a.kv_heads + head) * a.at.page_size + place;
+          k_scale[m][half] = page >= 0 ? __ldg(a.key_scales + at) : 0.0f;
+          v_scale[m][half] = page >= 0 ? __ldg(a.value_scales + at) : 0.0f;
+        }
+      }
+  }
+
+  __device__ void load_values(int key0) {
+    const int first = key0 + TILE / 4 * t;  // this lane's TILE / 4 positions
+    const int page = page_of(first / 16 * 16);
+    const int place = first % a.at.page_size;
+    const long long column = ((long long)page * a.kv_heads + head) * D * a.at.page_size + place;
+#pragma unroll
+    for (int m = 0; m < DM; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int d = 16 * m + g + 8 * half;
+        const uint8_t* from = static_cast<const uint8_t*>(a.values) + (CODES ? 1 : 2) * (column + (long long)d * a.at.page_size);
+        uint32_t (&to)[T::VWORDS] = v[m][half];
+        if constexpr (T::VWORDS == 1) {
+          to[0] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0;
+        } else if constexpr (T::VWORDS == 2) {
+          const uint2 x = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
+          to[0] = x.x, to[1] = x.y;
+        } else {
+          const uint4 x = page >= 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+          to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+        }
+      }
+  }
+
+  // Score tile m's A fragment of a k-step (rows g, g + 8; the step's first and
+  // second eight).
+  __device__ void key_fragment(int m, int step, uint32_t (&f)[4]) const {
+    if constexpr (CODES) {
+      code_pairs(k[m][0][step], f[0], f[2]);
+      code_pairs(k[m][1][step], f[1], f[3]);
+    } else {
+      f[0] = k[m][0][2 * step], f[2] = k[m][0][2 * step + 1];
+      f[1] = k[m][1][2 * step], f[3] = k[m][1][2 * step + 1];
+    }
+  }
+  __device__ void value_fragment(int m, int step, uint32_t (&f)[4]) const {
+    if constexpr (CODES) {
+      code_pairs(v[m][0][step], f[0], f[2]);
+      code_pairs(v[m][1][step], f[1], f[3]);
+    } else {
+      f[0] = v[m][0][2 * step], f[2] = v[m][0][2 * step + 1];
+      f[1] = v[m][1][2 * step], f[3] = v[m][1][2 * step + 1];
+    }
+  }
+};
+
+// `word` (positions p and p + 1 of a dimension) with zeros for what no row
+// sees and for what is not finite; `found` tells of the latter.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t word, int p, int end, int lowest, int first, bool& found) {
+  const bool low = p < end && (p >= lowest || p < first);
+  const bool high = p + 1 < end && (p + 1 >= lowest || p + 1 < first);
+  word &= (low ? 0xffffu : 0u) | (high ? 0xffff0000u : 0u);
+  const bool low_bad = (word & 0x7c00u) == 0x7c00u, high_bad = (word & 0x7c000000u) == 0x7c000000u;
+  found = found || low_bad || high_bad;
+  return word & ((low_bad ? 0u : 0xffffu) | (high_bad ? 0u : 0xffff0000u));
+}
+
+template <class T>
+__global__ void __launch_bounds__(THREADS) attention_rows_kernel(const AttentionChunksArgs a) {
+  pdl_trigger();  // the next kernel may launch and wait for this one
+  pdl_wait();     // what the kernels before this one wrote is visible
+  constexpr int D = T::D, NT = T::NT, TILE = T::TILE, MT = T::MT, ROWS = T::ROWS, TERMS = T::TERMS;
+  constexpr bool CODES = T::CODES;
+  using Map = typename T::Map;
+  using X = typename std::conditional<T::BF16, __nv_bfloat16, float>::type;
+  extern __shared__ __align__(16) uint8_t shared[];
+  __shared__ float q_unit[ROWS];  // the power of two each row was divided by
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
+  const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits, head = blockIdx.y, z = blockIdx.z;
+  const Chunk chunk(a.at, z);
+  if (!chunk.ok && blockIdx.x == 0 && head == 0 && tid == 0) chunk_error(a.error);
+  // this unit's rows [row0, row1) of the sequence's tokens x group, row r
+  // being token r / group, query head r % group of the key head
+  const int row0 = unit * ROWS, row1 = min(row0 + ROWS, chunk.tokens * a.group);
+  if (row0 >= row1) return;
+  const int token0 = row0 / a.group, token1 = (row1 - 1) / a.group + 1;
+  const SeenTiles seen(a, chunk, token0, token1, TILE);
+  const int tile0 = split * a.tiles_per_split, tile1 = min(tile0 + a.tiles_per_split, seen.count);
+  if (tile0 >= tile1) return;
+
+  RowsWarp<T> w(a, chunk, seen, head, lane);
+  int tile = tile0 + warp;
+  if (tile < tile1) {
+    w.load_keys(seen.key_of(tile));
+    w.load_values(seen.key_of(tile));
+  }
+
+  // q: each row divided by a power of two near its largest value, in F16
+  // terms, as B fragments [step][column tile][term][lane]
+  for (int r = warp; r < ROWS; r += WARPS) {
+    float largest = 0.0f;
+    if (row0 + r < row1) {
+      const int row = row0 + r;
+      const X* q = static_cast<const X*>(a.q) + ((chunk.row + row / a.group) * a.q_heads + head * a.group + row % a.group) * D;
+      for (int d = lane; d < D; d += 32) largest = fmaxf(largest, fabsf(float(q[d])));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    // 2^(floor(log2 largest) - Q_BITS), from the exponent bits, kept where it
+    // and its inverse are normal
+    const uint32_t exponent = __float_as_uint(largest) & 0x7f800000u;
+    const uint32_t shift = uint32_t(Q_BITS) << 23;
+    if (lane == 0) q_unit[r] = __uint_as_float(max(exponent, shift + 0x00800000u) - shift);
+  }
+  __syncthreads();
+  uint2* fragments = reinterpret_cast<uint2*>(shared);
+  for (int i = tid; i < Map::STEPS * NT * 32; i += THREADS) {
+    const int l = i % 32, n = i / 32 % NT, step = i / 32 / NT;
+    const int r = 8 * n + l / 4, row = row0 + r, d = Map::first_of(step, l % 4);
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row < row1) {
+      const X* q = static_cast<const X*>(a.q) + ((chunk.row + row / a.group) * a.q_heads + head * a.group + row % a.group) * D + d;
+      const float unit_inverse = 1.0f / q_unit[r];  // exact
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = float(q[e]) * unit_inverse;
+    }
+    const uint2 hi = make_uint2(half_pair(x[0], x[1]), half_pair(x[2], x[3]));
+    fragments[((step * NT + n) * TERMS) * 32 + l] = hi;
+    if constexpr (TERMS == 2) {
+      const float2 u = pair_value(hi.x), y = pair_value(hi.y);
+      fragments[((step * NT + n) * TERMS + 1) * 32 + l] =
+          make_uint2(half_pair(x[0] - u.x, x[1] - u.y), half_pair(x[2] - y.x, x[3] - y.y));
+    }
+  }
+  __syncthreads();
+
+  // this lane's columns: rows 8 n + 2 t and + 1
+  float multiplier[NT][2];
+  int position[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * t + e;
+      multiplier[n][e] = a.scale * q_unit[r];
+      position[n][e] = chunk.position + min(row0 + r, row1 - 1) / a.group;
+    }
+  // what every row sees: keys below `all_end` and from `all_low` on (or below
+  // `first`)
+  const int first = a.window > 0 ? a.first : 0;
+  const int all_end = a.causal ? chunk.position + token0 + 1 : seen.end;
+  const int all_low = a.window > 0 ? chunk.position + token1 - a.window : 0;
+  const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;  // what some row sees
+
+  float out[NT][T::DM][4];
+  float largest[NT][2], sum[NT][2], v_unit = 0.0f;
+  bool taken_out = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    largest[n][0] = largest[n][1] = -INFINITY;
+    sum[n][0] = sum[n][1] = 0.0f;
+#pragma unroll
+    for (int m = 0; m < T::DM; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
+  }
+
+  for (; tile < tile1; tile += WARPS) {
+    const int key0 = seen.key_of(tile);
+    const int next = tile + WARPS;
+    float s[NT][MT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s[n][m][0] = s[n][m][1] = s[n][m][2] = s[n][m][3] = 0.0f;
+#pragma unroll
+    for (int step = 0; step < Map::STEPS; ++step) {
+      uint32_t f[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) w.key_fragment(m, step, f[m]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int term = TERMS - 1; term >= 0; --term) {
+          const uint2 b = fragments[((step * NT + n) * TERMS + term) * 32 + lane];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) mma_f16(s[n][m], f[m], b.x, b.y);
+        }
+    }
+    float k_scale[MT][2], v_scale[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        k_scale[m][half] = CODES ? w.k_scale[m][half] : 1.0f;
+        v_scale[m][half] = CODES ? w.v_scale[m][half] : 1.0f;
+      }
+    if (next < tile1) w.load_keys(seen.key_of(next));  // on their way under the rest of this tile
+
+    // scores, and each column's largest
+    const bool whole = key0 + TILE <= all_end && (key0 >= all_low || key0 + TILE <= first);
+    float rescale[NT][2];
+    bool grown = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float x = s[n][m][2 * half + e] * multiplier[n][e];
+            if (CODES) x *= k_scale[m][half];
+            if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
+            if (!whole) {
+              const int key = key0 + w.position_of(m, half);
+              const bool sees = key < seen.end && (!a.causal || key <= position[n][e]) &&
+                                (a.window == 0 || key > position[n][e] - a.window || key < first);
+              x = sees ? x : -INFINITY;
+            }
+            s[n][m][2 * half + e] = x;
+            top = fmaxf(top, x);
+          }
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float before = largest[n][e];
+        const float now = fmaxf(before, top - WEIGHT_LOG);
+        rescale[n][e] = weight_of(before, now);
+        grown = grown || now > before;
+        largest[n][e] = now;
+      }
+    // a weight is p times its value's scale over the warp's running unit, a
+    // power of two at or above every scale so far: at most 1, as F16 wants
+    float shrink = 1.0f;
+    if constexpr (CODES) {
+      float top = 0.0f;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int key = key0 + w.position_of(m, half);
+          if (key >= seen.end || (key < lowest && key >= first)) v_scale[m][half] = 0.0f;
+          top = fmaxf(top, v_scale[m][half]);
+        }
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (top > v_unit) {
+        const uint32_t bits = __float_as_uint(top);
+        const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
+        const float unit = __uint_as_float(max(up, 0x01000000u));  // (its inverse is normal too)
+        shrink = v_unit / unit;
+        v_unit = unit;
+        grown = true;
+      }
+    }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        sum[n][0] *= rescale[n][0], sum[n][1] *= rescale[n][1];
+        const float f0 = rescale[n][0] * shrink, f1 = rescale[n][1] * shrink;
+#pragma unroll
+        for (int m = 0; m < T::DM; ++m) {
+          out[n][m][0] *= f0, out[n][m][1] *= f1;
+          out[n][m][2] *= f0, out[n][m][3] *= f1;
+        }
+      }
+    }
+    const float v_inverse = CODES && v_unit > 0.0f ? 1.0f / v_unit : 0.0f;  // exact
+    uint32_t p[NT][MT][TERMS][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = s[n][m][2 * half + e];
+            const float weight = weight_of(x, largest[n][e]);
+            sum[n][e] += weight;
+            y[e] = CODES ? (x == -INFINITY ? 0.0f : weight * (v_scale[m][half] * v_inverse)) : weight;
+          }
+          const uint32_t hi = half_pair(y[0], y[1]);
+          p[n][m][0][half] = turn(hi);
+          if constexpr (TERMS == 2) {
+            const float2 u = pair_value(hi);
+            p[n][m][1][half] = turn(half_pair(y[0] - u.x, y[1] - u.y));
+          }
+        }
+    // where rows differ in what they see, a value that is not finite must not
+    // meet the zero weights of those that do not see it: it is taken out here
+    // and added to the rows that see it at the end
+    if (!CODES && !whole) {
+#pragma unroll
+      for (int m = 0; m < T::DM; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < T::VWORDS; ++j)
+            w.v[m][half][j] = finite_halves(w.v[m][half][j], key0 + TILE / 4 * t + 2 * j, seen.end, lowest, first, taken_out);
+    }
+#pragma unroll
+    for (int m = 0; m < T::DM; ++m)
+#pragma unroll
+      for (int step = 0; step < MT; ++step) {
+        uint32_t f[4];
+        w.value_fragment(m, step, f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int term = TERMS - 1; term >= 0; --term)
+            mma_f16(out[n][m], f, p[n][step][term][0], p[n][step][term][1]);
+      }
+    if (next < tile1) w.load_values(seen.key_of(next));
+  }
+
+  // the warps' results: [warp][row][D] and [warp][row] (largest, sum)
+  __syncthreads();  // (past the q fragments)
+  float* merged = reinterpret_cast<float*>(shared);
+  float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
+  const float unit_scale = CODES ? v_unit : 1.0f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float total = sum[n][e];
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const int r = 8 * n + 2 * t + e;
+      if (g == 0) stats[warp * ROWS + r] = make_float2(largest[n][e], total);
+#pragma unroll
+      for (int m = 0; m < T::DM; ++m) {
+        merged[(warp * ROWS + r) * D + 16 * m + g] = out[n][m][e] * unit_scale;
+        merged[(warp * ROWS + r) * D + 16 * m + g + 8] = out[n][m][2 + e] * unit_scale;
+      }
+    }
+  taken_out = __syncthreads_or(taken_out);
+  for (int i = tid; i < (row1 - row0) * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row0 + r, q_head = head * a.group + row % a.group;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) top = fmaxf(top, stats[j * ROWS + r].x);
+    float total = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) {
+      const float2 stat = stats[j * ROWS + r];
+      const float f = weight_of(stat.x, top);
+      total += stat.y * f;  // (a NaN stays one)
+      if (f == 0.0f) continue;
+      const float4 y = *reinterpret_cast<const float4*>(merged + (j * ROWS + r) * D + d);
+      x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+    }
+    if (!CODES && taken_out) {
+      const int own = chunk.position + row / a.group;
+      for (int j = tile0; j < tile1; ++j) {
+        const int key0 = seen.key_of(j);
+        if (key0 + TILE <= all_end && (key0 >= all_low || key0 + TILE <= first)) continue;
+        const long long page_stride = (long long)a.kv_heads * D * a.at.page_size;
+        const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + d) * a.at.page_size,
+                                    page_stride, chunk.table, a.at.pages, a.at.page_size, key0,
+                                    min(key0 + TILE, a.causal ? own + 1 : seen.end),
+                                    a.window > 0 ? own - a.window + 1 : 0, first);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      }
+    }
+    const long long at = (chunk.row + row / a.group) * a.q_heads + q_head;
+    if (a.part_o) {
+      *reinterpret_cast<float4*>(a.part_o + (at * a.splits + split) * D + d) = x;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.splits + split) * 2) = make_float2(top, total);
+      continue;
+    }
+    if (a.sinks) {
+      const float sink = a.sinks[q_head], all = fmaxf(top, sink);
+      const float f = weight_of(top, all);
+      x.x *= f, x.y *= f, x.z *= f, x.w *= f;
+      total = total * f + weight_of(sink, all);
+    }
+    X* to = static_cast<X*>(a.out) + at * D + d;
+    const bool any = total != 0.0f;
+    to[0] = X(any ? x.x / total : 0.0f), to[1] = X(any ? x.y / total : 0.0f);
+    to[2] = X(any ? x.z / total : 0.0f), to[3] = X(any ? x.w / total : 0.0f);
+  }
+}
+
+// The splits' join, a warp per (token, query head) row: out = sum_s o_s
+// e^(m_s - M) / (sum_s l_s e^(m_s - M) + e^(sink - M)), M the largest of the
+// m_s and the sink. A row's splits are those that held tiles of its unit, as
+// the kernel that wrote them counted them.
+struct JoinArgs {
+  AttentionChunksArgs a;
+  int rows_per_unit, keys_per_tile;
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(THREADS) attention_chunks_join_kernel(const JoinArgs j) {
+  pdl_trigger();  // the next kernel may launch and wait for this one
+  pdl_wait();     // what the kernels before this one wrote is visible
+  using X = typename std::conditional<BF16, __nv_bfloat16, float>::type;
+  const AttentionChunksArgs& a = j.a;
+  const int lane = threadIdx.x % 32, z = blockIdx.y;
+  const Chunk chunk(a.at, z);
+  const long long i = (long long)blockIdx.x * WARPS + threadIdx.x / 32;  // token x q_heads + head
+  if (i >= (long long)chunk.tokens * a.q_heads) return;
+  const int token = int(i / a.q_heads), head = int(i % a.q_heads);
+  const int row0 = (token * a.group + head % a.group) / j.rows_per_unit * j.rows_per_unit;
+  const int row1 = min(row0 + j.rows_per_unit, chunk.tokens * a.group);
+  const SeenTiles seen(a, chunk, row0 / a.group, (row1 - 1) / a.group + 1, j.keys_per_tile);
+  const int splits = seen.splits(a.tiles_per_split);
+  const long long at = (chunk.row + token) * a.q_heads + head;
+  const float2* stats = reinterpret_cast<const float2*>(a.part_ml) + at * a.splits;
+  const float* parts = a.part_o + at * a.splits * D;
+  float top = a.sinks ? a.sinks[head] : -INFINITY;
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, stats[s].x);
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float total = a.sinks ? weight_of(a.sinks[head], top) : 0.0f;
+  constexpr int PER = (D + 127) / 128;
+  float x[PER][4] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float2 stat = stats[s];
+    const float f = weight_of(stat.x, top);
+    total += stat.y * f;  // (a NaN stays one)
+    if (f == 0.0f) continue;
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      const int d = 4 * (lane + 32 * c);
+      if (d >= D) continue;
+      const float4 y = *reinterpret_cast<const float4*>(parts + (long long)s * D + d);
+      x[c][0] += y.x * f, x[c][1] += y.y * f, x[c][2] += y.z * f, x[c][3] += y.w * f;
+    }
+  }
+  const bool any = total != 0.0f;
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int d = 4 * (lane + 32 * c);
+    if (d >= D) continue;
+    X* to = static_cast<X*>(a.out) + at * D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = X(any ? x[c][e] / total : 0.0f);
+  }
+}
+
+template <class T>
+int launch_rows(const AttentionChunksArgs& a, cudaStream_t stream) {
+  static PerDevice configured;
+  DRIFT_TRY(ensure_shared_memory(configured, attention_rows_kernel<T>, T::BYTES));
+  const int units = (a.at.longest * a.group + T::ROWS - 1) / T::ROWS;
+  DRIFT_CUDA(launch_pdl(attention_rows_kernel<T>, dim3(unsigned(units) * a.splits, a.kv_heads, a.at.batch), THREADS,
+                        T::BYTES, stream, a));
+  DRIFT_LAUNCHED("attention_rows");
+  return 0;
+}
+
+// Keys of a warp's tile: 32 where its keys and values (16 bytes a lane and
+// key-row chunk) leave the output room in registers, else 16.
+constexpr int tile_of(int head_dim, bool codes, int columns) {
+  return codes && head_dim <= 128 && columns <= 2 ? 32 : 16;
+}
+
+template <int D, bool CODES, bool BF16>
+int launch_columns(const AttentionChunksArgs& a, int columns, cudaStream_t stream) {
+  if constexpr (D <= 128) {
+    if (columns == 4) return launch_rows<RowsTraits<D, CODES, BF16, 4, tile_of(D, CODES, 4)>>(a, stream);
+    if (columns == 2) return launch_rows<RowsTraits<D, CODES, BF16, 2, tile_of(D, CODES, 2)>>(a, stream);
+  }
+  return launch_rows<RowsTraits<D, CODES, BF16, 1, tile_of(D, CODES, 1)>>(a, stream);
+}
+
+template <int D>
+int launch_dim(const AttentionChunksArgs& a, bool codes, bool bf16, int columns, cudaStream_t stream) {
+  if (codes) return bf16 ? launch_columns<D, true, true>(a, columns, stream) : launch_columns<D, true, false>(a, columns, stream);
+  return bf16 ? launch_columns<D, false, true>(a, columns, stream) : launch_columns<D, false, false>(a, columns, stream);
+}
+
+#define DRIFT_ROWS_REGISTER_AS(D, codes, bf16, nt, name) \
+  DRIFT_REGISTER(name, (attention_rows_kernel<RowsTraits<D, codes, bf16, nt, tile_of(D, codes, nt)>>))
+#define DRIFT_ROWS_REGISTER(D, nt)                                             \
+  DRIFT_ROWS_REGISTER_AS(D, true, true, nt, attention_rows_i8_bf16_d##D##_n##nt)    \
+  DRIFT_ROWS_REGISTER_AS(D, true, false, nt, attention_rows_i8_f32_d##D##_n##nt)    \
+  DRIFT_ROWS_REGISTER_AS(D, false, true, nt, attention_rows_f16_bf16_d##D##_n##nt)  \
+  DRIFT_ROWS_REGISTER_AS(D, false, false, nt, attention_rows_f16_f32_d##D##_n##nt)
+DRIFT_ROWS_REGISTER(64, 1)
+DRIFT_ROWS_REGISTER(64, 2)
+DRIFT_ROWS_REGISTER(64, 4)
+DRIFT_ROWS_REGISTER(80, 1)
+DRIFT_ROWS_REGISTER(80, 2)
+DRIFT_ROWS_REGISTER(80, 4)
+DRIFT_ROWS_REGISTER(128, 1)
+DRIFT_ROWS_REGISTER(128, 2)
+DRIFT_ROWS_REGISTER(128, 4)
+DRIFT_ROWS_REGISTER(256, 1)
+#define DRIFT_JOIN_REGISTER(D)                                                            \
+  DRIFT_REGISTER(attention_chunks_join_f32_d##D, (attention_chunks_join_kernel<D, false>)) \
+  DRIFT_REGISTER(attention_chunks_join_bf16_d##D, (attention_chunks_join_kernel<D, true>))
+DRIFT_JOIN_REGISTER(64)
+DRIFT_JOIN_REGISTER(80)
+DRIFT_JOIN_REGISTER(128)
+DRIFT_JOIN_REGISTER(256)
+
+}  // namespace
+
+int attention_rows_tile(int head_dim, bool codes, int columns) { return tile_of(head_dim, codes, columns); }
+
+int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int columns,
+                          cudaStream_t stream) {
+  const bool bf16 = x_dtype == DRIFT_BF16, codes = cache_dtype == DRIFT_I8;
+  switch (head_dim) {
+    case 64: return launch_dim<64>(a, codes, bf16, columns, stream);
+    case 80: return launch_dim<80>(a, codes, bf16, columns, stream);
+    case 128: return launch_dim<128>(a, codes, bf16, columns, stream);
+    default: return launch_dim<256>(a, codes, bf16, columns, stream);
+  }
+}
+
+template <int D>
+static int launch_join(const JoinArgs& j, bool bf16, cudaStream_t stream) {
+  const long long rows = (long long)j.a.at.longest * j.a.q_heads;
+  const dim3 grid(unsigned((rows + WARPS - 1) / WARPS), j.a.at.batch);
+  if (bf16) DRIFT_CUDA(launch_pdl(attention_chunks_join_kernel<D, true>, grid, THREADS, 0, stream, j));
+  else DRIFT_CUDA(launch_pdl(attention_chunks_join_kernel<D, false>, grid, THREADS, 0, stream, j));
+  DRIFT_LAUNCHED("attention_chunks_join");
+  return 0;
+}
+
+int launch_attention_join(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
+                          int keys_per_tile, cudaStream_t stream) {
+  const JoinArgs j = {a, rows_per_unit, keys_per_tile};
+  const bool bf16 = x_dtype == DRIFT_BF16;
+  switch (head_dim) {
+    case 64: return launch_join<64>(j, bf16, stream);
+    case 80: return launch_join<80>(j, bf16, stream);
+    case 128: return launch_join<128>(j, bf16, stream);
+    default: return launch_join<256>(j, bf16, stream);
+  }
+}
+
+}  // namespace drift

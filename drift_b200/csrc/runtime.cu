@@ -77,6 +77,7 @@ const char* dtype_name(int dtype) {
     case DRIFT_F32: return "F32";
     case DRIFT_F16: return "F16";
     case DRIFT_BF16: return "BF16";
+    case DRIFT_I8: return "I8";
     case DRIFT_I32: return "I32";
     case DRIFT_Q4_0: return "Q4_0";
     case DRIFT_Q4_1: return "Q4_1";

@@ -23,7 +23,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import BF16, F32, Q4_0, Q4_1, Q8_0, check
+from ._lib import BF16, F16, F32, I8, Q4_0, Q4_1, Q8_0, check
 from .dtypes import DTYPES, byte_size
 
 # Activation codes (runner/src/drift/runner/ops/Activation.scala:5-19).
@@ -94,13 +94,65 @@ class KvCache:
 
 
 @dataclass
+class QuantizedKvCache:
+    """A KvCache in 8 bits: int8 codes in its two layouts and, for each side,
+    one F32 scale per position and head, [pages, kv_heads, page_size]; a value
+    is code x scale. cache_write_chunks makes them."""
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_scales: torch.Tensor
+    value_scales: torch.Tensor
+    page_size: int
+
+    @property
+    def pages(self) -> int:
+        return int(self.keys.shape[0])
+
+    @property
+    def kv_heads(self) -> int:
+        return int(self.keys.shape[2])
+
+    @property
+    def head_dim(self) -> int:
+        return int(self.keys.shape[3])
+
+    @staticmethod
+    def allocate(pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 device=None) -> "QuantizedKvCache":
+        device = device or torch.device("cuda")
+        codes = dict(dtype=torch.int8, device=device)
+        scales = dict(dtype=torch.float32, device=device)
+        return QuantizedKvCache(torch.zeros(pages, page_size, kv_heads, head_dim, **codes),
+                                torch.zeros(pages, kv_heads, head_dim, page_size, **codes),
+                                torch.zeros(pages, kv_heads, page_size, **scales),
+                                torch.zeros(pages, kv_heads, page_size, **scales), page_size)
+
+
+@dataclass
+class Chunks:
+    """A batch of sequences' new tokens: sequence z's are rows starts[z] ..
+    starts[z + 1] - 1, at positions positions[z], positions[z] + 1, ... of the
+    pages in page_tables[z]. All three are I32 on the device (a captured call
+    replays at other lengths); `longest` bounds a sequence's new tokens and
+    `max_key_count` its positions with them."""
+    starts: torch.Tensor
+    positions: torch.Tensor
+    page_tables: torch.Tensor
+    longest: int
+    max_key_count: int
+
+
+@dataclass
 class Attention:
-    """An attention's parameters (ops/Attention.scala:11-17)."""
+    """An attention's parameters (ops/Attention.scala:11-17). `first`: this
+    many of a sequence's first positions stay visible whatever the window
+    (attention_chunks only)."""
     scale: float
     causal: bool = True
     window: Optional[int] = None
     softcap: Optional[float] = None
     sinks: Optional[torch.Tensor] = None
+    first: int = 0
 
 
 @dataclass
@@ -369,6 +421,7 @@ class CudaOps:
                  f"attention: queries {list(q.shape)} against heads of {cache.head_dim}")
         _require(page_table.dtype == torch.int32 and page_table.dim() == 1,
                  f"a page table is I32 [pages], not {page_table.dtype} {list(page_table.shape)}")
+        _require(attention.first == 0, "attention: first keys are attention_chunks'")
         tokens, q_heads, _ = q.shape
         sinks = attention.sinks
         if sinks is not None:
@@ -433,6 +486,7 @@ class CudaOps:
         _require(positions.dtype == torch.int32 and tuple(positions.shape) == (b,),
                  f"attention: positions {list(positions.shape)} for {b} sequences")
         _require(attention.causal, "a decode step's attention is causal")
+        _require(attention.first == 0, "attention: first keys are attention_chunks'")
         args = (_ptr(q), b, q_heads, _ptr(cache.keys), _ptr(cache.values), cache.pages,
                 cache.page_size, cache.kv_heads, dim, _ptr(page_tables), int(page_tables.shape[1]),
                 _ptr(positions), max_key_count, attention.scale, int(attention.window or 0),
@@ -453,6 +507,123 @@ class CudaOps:
             status = self.lib.drift_attention_decode_prepared(*args, _ptr(prepared),
                                                               self._stream())
         check("drift_attention_decode", status)
+
+    # -- a batch of sequences' new tokens ----------------------------------------------------------
+    @staticmethod
+    def _check_cache(name: str, cache) -> tuple:
+        """The cache's arguments: its type, codes or values, and scales."""
+        quantized = isinstance(cache, QuantizedKvCache)
+        held = torch.int8 if quantized else torch.float16
+        pages, page_size, kv_heads, dim = cache.keys.shape
+        _require(cache.page_size == page_size
+                 and tuple(cache.values.shape) == (pages, kv_heads, dim, page_size),
+                 f"{name}: a cache of keys {list(cache.keys.shape)}, values "
+                 f"{list(cache.values.shape)}, pages of {cache.page_size}")
+        sides = [(cache.keys, held), (cache.values, held)]
+        if quantized:
+            for scales in (cache.key_scales, cache.value_scales):
+                _require(tuple(scales.shape) == (pages, kv_heads, page_size),
+                         f"{name}: scales {list(scales.shape)} for keys {list(cache.keys.shape)}")
+                sides.append((scales, torch.float32))
+        for tensor, dtype in sides:
+            _require(tensor.dtype == dtype and tensor.is_cuda and tensor.is_contiguous(),
+                     f"{name}: the cache is contiguous device memory, {dtype} here")
+        return (I8 if quantized else F16, _ptr(cache.keys), _ptr(cache.values),
+                _ptr(cache.key_scales) if quantized else None,
+                _ptr(cache.value_scales) if quantized else None, pages, page_size)
+
+    def _check_chunks(self, name: str, chunks: Chunks) -> tuple:
+        """The chunks' arguments."""
+        starts, positions, tables = chunks.starts, chunks.positions, chunks.page_tables
+        for t in (starts, positions, tables):
+            _require(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous(),
+                     f"{name}: starts, positions and page tables are contiguous I32 device memory")
+        batch = positions.numel()
+        _require(positions.dim() == 1 and tuple(starts.shape) == (batch + 1,) and tables.dim() == 2
+                 and tables.shape[0] == batch,
+                 f"{name}: starts {list(starts.shape)}, page tables {list(tables.shape)} for "
+                 f"{batch} sequences")
+        return _ptr(tables), int(tables.shape[1]), _ptr(starts), _ptr(positions), batch, \
+            int(chunks.longest)
+
+    def _check_rows(self, name: str, cache, *tensors) -> int:
+        """Rows of the cache's heads: their type, shape and device."""
+        first = tensors[0]
+        _same_shape(name, *tensors)
+        for t in tensors:
+            _require(t.dtype == first.dtype, f"{name}: {first.dtype} and {t.dtype}")
+            _require(t.device == cache.keys.device, f"{name}: {t.device}, the cache on {cache.keys.device}")
+            x_dtype = _x_dtype(name, t)
+        _require(first.dim() == 3 and first.shape[2] == cache.head_dim,
+                 f"{name}: {list(first.shape)} for a cache of {cache.kv_heads} heads of "
+                 f"{cache.head_dim}")
+        _require(first.device.index == torch.cuda.current_device(),
+                 f"{name}: tensors on {first.device}, the current device is "
+                 f"{torch.cuda.current_device()}")
+        return x_dtype
+
+    def cache_write_chunks(self, k, v, cache, chunks: Chunks) -> None:
+        """k, v [tokens, kv_heads, D] (F32 or BF16) of every sequence into its
+        pages, in one launch: rounded to F16 (a KvCache, as cache_write), or
+        to 8-bit codes with a scale per position and head (a
+        QuantizedKvCache): scale = max |row| / 127, code = row / scale to the
+        nearest, halves to even, as in exact arithmetic."""
+        x_dtype = self._check_rows("cacheWrite", cache, k, v)
+        _require(k.shape[1] == cache.kv_heads,
+                 f"cacheWrite: {list(k.shape)} into a cache of {cache.kv_heads} heads of "
+                 f"{cache.head_dim}")
+        dtype, keys, values, key_scales, value_scales, pages, page_size = \
+            self._check_cache("cacheWrite", cache)
+        status = self.lib.drift_cache_write_chunks(
+            x_dtype, _ptr(k), _ptr(v), k.shape[0], cache.kv_heads, cache.head_dim, dtype, keys,
+            values, key_scales, value_scales, pages, page_size,
+            *self._check_chunks("cacheWrite", chunks), self._stream())
+        check("drift_cache_write_chunks", status)
+
+    def cache_read_chunks(self, cache, chunks: Chunks, k, v) -> None:
+        """What the cache holds at the chunks' positions, into k and v
+        [tokens, kv_heads, D] (F32 or BF16)."""
+        x_dtype = self._check_rows("cacheRead", cache, k, v)
+        _require(k.shape[1] == cache.kv_heads,
+                 f"cacheRead: {list(k.shape)} from a cache of {cache.kv_heads} heads of "
+                 f"{cache.head_dim}")
+        dtype, keys, values, key_scales, value_scales, pages, page_size = \
+            self._check_cache("cacheRead", cache)
+        status = self.lib.drift_cache_read_chunks(
+            x_dtype, _ptr(k), _ptr(v), k.shape[0], cache.kv_heads, cache.head_dim, dtype, keys,
+            values, key_scales, value_scales, pages, page_size,
+            *self._check_chunks("cacheRead", chunks), self._stream())
+        check("drift_cache_read_chunks", status)
+
+    def attention_chunks(self, q, cache, chunks: Chunks, attention: Attention, out) -> None:
+        """Attention of every sequence's new tokens, q [tokens, q_heads, D]
+        (F32 or BF16), over its positions in a KvCache or a QuantizedKvCache,
+        the new ones included (written before): a decoding step, drafted
+        tokens, prompts or pieces of them, of different lengths in one call.
+        With a window, the first `attention.first` positions stay visible."""
+        x_dtype = self._check_rows("attention", cache, q, out)
+        tokens, q_heads, dim = q.shape
+        dtype, keys, values, key_scales, value_scales, pages, page_size = \
+            self._check_cache("attention", cache)
+        sinks = attention.sinks
+        if sinks is not None:
+            _f32("attention sinks", sinks)
+            _require(tuple(sinks.shape) == (q_heads,),
+                     f"attention: sinks {list(sinks.shape)} for {q_heads} heads")
+        window, first, longest = int(attention.window or 0), int(attention.first), int(chunks.longest)
+        chunk_args = self._check_chunks("attention", chunks)
+        max_keys = int(chunks.max_key_count)
+        size = self.lib.drift_attention_chunks_workspace_bytes(
+            x_dtype, tokens, q_heads, cache.kv_heads, dim, dtype, chunk_args[4], longest, max_keys,
+            window, first)
+        # the call's own: freed to torch's allocator behind it in the stream
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        status = self.lib.drift_attention_chunks(
+            x_dtype, _ptr(q), tokens, q_heads, cache.kv_heads, dim, dtype, keys, values, key_scales,
+            value_scales, pages, page_size, *chunk_args, max_keys, attention.scale,
+            int(attention.causal), window, first, float(attention.softcap or 0.0), _ptr(sinks),
+            _ptr(out), _ptr(workspace), size, self._stream())
+        check("drift_attention_chunks", status)
 
     # -- SequenceOps: Gated DeltaNet (ops/SequenceOps.scala) --------------------------------------
     def causal_conv(self, x, weight, dilation: int, state, history, out) -> None:

@@ -46,6 +46,7 @@ extern "C" {
 #define DRIFT_Q8_0 8
 #define DRIFT_Q4_K 12 /* super-blocks of 256 (tensor/KQuants.scala:99) */
 #define DRIFT_Q6_K 14 /* (KQuants.scala:122) */
+#define DRIFT_I8 24  /* an 8-bit cache's codes (tensor/DType.scala:86-175) */
 #define DRIFT_I32 26
 #define DRIFT_BF16 30
 
@@ -231,6 +232,67 @@ int drift_attention_decode(const float* q, int batch, int q_heads, const void* k
                            int head_dim, const int32_t* page_tables, int table_stride,
                            const int32_t* positions, int max_key_count, float scale, int window,
                            float softcap, const float* sinks, float* out, drift_stream_t stream);
+
+/* ---- a batch of sequences' new tokens over the paged cache (new) -------------
+ * The three calls below serve sequences with any number of new tokens each in
+ * one launch: prompts and pieces of prompts, drafted tokens, a decoding step.
+ * Sequence z's tokens are rows starts[z] .. starts[z + 1] - 1 of q, k, v and
+ * out, at positions positions[z], positions[z] + 1, ... of the pages in row z
+ * of page_tables [batch][table_stride]; starts (I32 [batch + 1], ascending),
+ * positions (I32 [batch]) and page_tables are on the device, so that a
+ * captured launch replays at other lengths. `longest` bounds a sequence's
+ * tokens. A sequence of no tokens is left out, and rows past the last
+ * sequence stay as they are. A sequence whose starts, length or positions are
+ * out of range sets the device error word (code 1) and is left out; a page id
+ * outside the cache sets it too, is not written, and reads as zeros.
+ * Tensors are F32 or BF16 (x_dtype), 16-byte aligned.
+ *
+ * cache_dtype DRIFT_F16 is drift_cache_write's cache. DRIFT_I8 keeps codes in
+ * its place, int8 in the same two layouts, and a scale for each position and
+ * head of either side, F32 [pages][kv_heads][page_size]: a row x of head_dim
+ * values is scale = max |x| / 127 (rounded to F32) and codes x / scale
+ * rounded to the nearest whole number, halves to the even one, as in exact
+ * arithmetic -- (head_dim + 4) bytes for 2 head_dim, each value within half a
+ * scale of x. A row with a NaN or an infinity reads back as NaNs. Scales are
+ * NULL for DRIFT_F16. */
+/* drift_cache_write for all sequences. Two sequences may share pages if they
+ * write none of them. */
+int drift_cache_write_chunks(int x_dtype, const void* k, const void* v, int64_t tokens, int kv_heads,
+                             int head_dim, int cache_dtype, void* keys, void* values,
+                             float* key_scales, float* value_scales, int pages, int page_size,
+                             const int32_t* page_tables, int table_stride, const int32_t* starts,
+                             const int32_t* positions, int batch, int longest,
+                             drift_stream_t stream);
+/* The reverse: the cache's values at the chunks' positions into k and v
+ * [tokens][kv_heads][head_dim] -- code x scale, rounded to F32 and, for BF16,
+ * again. */
+int drift_cache_read_chunks(int x_dtype, void* k, void* v, int64_t tokens, int kv_heads,
+                            int head_dim, int cache_dtype, const void* keys, const void* values,
+                            const float* key_scales, const float* value_scales, int pages,
+                            int page_size, const int32_t* page_tables, int table_stride,
+                            const int32_t* starts, const int32_t* positions, int batch,
+                            int longest, drift_stream_t stream);
+/* drift_attention for all sequences: q and out [tokens][q_heads][head_dim]. A
+ * token at position p sees the keys at positions up to p when causal, else all
+ * of its sequence's up to its last new token; with window > 0 only those from
+ * p - window + 1 on and, whatever the window, the sequence's first `first`
+ * positions. softcap, sinks and the limits on heads are drift_attention's;
+ * max_key_count bounds positions[z] plus z's tokens. F32 rows are computed to
+ * F32's accuracy, BF16 rows with weights rounded to F16. `workspace`
+ * (16-byte aligned, the caller's: calls that may overlap need one each) holds
+ * drift_attention_chunks_workspace_bytes(...) bytes of partial results. */
+int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_heads, int kv_heads,
+                           int head_dim, int cache_dtype, const void* keys, const void* values,
+                           const float* key_scales, const float* value_scales, int pages,
+                           int page_size, const int32_t* page_tables, int table_stride,
+                           const int32_t* starts, const int32_t* positions, int batch, int longest,
+                           int max_key_count, float scale, int causal, int window, int first,
+                           float softcap, const float* sinks, void* out, void* workspace,
+                           size_t workspace_bytes, drift_stream_t stream);
+size_t drift_attention_chunks_workspace_bytes(int x_dtype, int64_t tokens, int q_heads,
+                                              int kv_heads, int head_dim, int cache_dtype,
+                                              int batch, int longest, int max_key_count,
+                                              int window, int first);
 
 /* ---- Gated DeltaNet (the hybrid decoder's linear-attention layers) ---------
  * SequenceOps.causalConv (ops/SequenceOps.scala; CPU ops/CpuSequence.scala:
