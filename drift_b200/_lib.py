@@ -137,7 +137,7 @@ SIGNATURES = {
                                       _i32, _p, _i32, _p, _p, _i32, _i32, _i32, _f32, _i32, _i32,
                                       _i32, _f32, _p, _p, _p, _sz, _p]),
     "drift_attention_chunks_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
-                                                     _i32, _i32, _i32]),
+                                                     _i32, _i32, _i32, _i32, _i32, _i32]),
     "drift_attention_decode": (_i32, [_p, _i32, _i32, _p, _p, _i32, _i32, _i32, _i32, _p, _i32, _p,
                                       _i32, _f32, _i32, _f32, _p, _p, _p]),
 }

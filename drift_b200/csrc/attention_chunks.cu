@@ -13,30 +13,37 @@ namespace drift {
 namespace {
 
 struct Plan {
-  int columns;          // attention_rows' column tiles
+  int columns;          // attention_rows' column tiles, or
+  int row_tiles;        // attention_tiles' row tiles (0: attention_rows)
   int rows_per_unit;    // rows of a key head that a CTA takes
   int keys_per_tile;
   int splits, tiles_per_split;
 };
 
-// The most key tiles of `width` that a unit of a chunk can see
+struct Call {
+  int x_dtype, cache_dtype, batch, longest, group, kv_heads, head_dim, max_key_count, causal, window, first, pages,
+      page_size;
+};
+
+// The most key tiles of `width` that a unit of `rows` rows can see
 // (SeenTiles::count's bound).
-long long tiles_bound(int longest, int max_key_count, int window, int first, int width) {
-  const long long all = ((long long)max_key_count + width - 1) / width;
-  if (window <= 0) return all;
-  const long long seen = ((long long)window + longest) / width + 2 + ((long long)first + width - 1) / width;
+long long tiles_bound(const Call& c, int rows, int width) {
+  const long long all = ((long long)c.max_key_count + width - 1) / width;
+  if (c.window <= 0) return all;
+  const long long tokens = c.causal ? std::min(c.longest, rows / c.group + 2) : c.longest;
+  const long long seen = (c.window + tokens) / width + 2 + ((long long)c.first + width - 1) / width;
   return std::min(all, seen);
 }
 
-Plan plan_rows(int batch, int longest, int group, int kv_heads, int head_dim, bool codes, int max_key_count,
-               int window, int first) {
+Plan plan_rows(const Call& c) {
   Plan p;
-  const long long rows = (long long)longest * group;
-  p.columns = head_dim > 128 || rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  p.row_tiles = 0;
+  const long long rows = (long long)c.longest * c.group;
+  p.columns = c.head_dim > 128 || rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
   p.rows_per_unit = 8 * p.columns;
-  p.keys_per_tile = attention_rows_tile(head_dim, codes, p.columns);
-  const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * batch * kv_heads;
-  const long long tiles = std::max(1LL, tiles_bound(longest, max_key_count, window, first, p.keys_per_tile));
+  p.keys_per_tile = attention_rows_tile(c.head_dim, c.cache_dtype == DRIFT_I8, p.columns);
+  const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
+  const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
   // CTAs for every SM twice over, of a tile a warp at least
   const long long wanted = std::max(1LL, 4LL * sm_count() / std::max(1LL, units));
   const long long splits = std::min(wanted, (tiles + 7) / 8);
@@ -44,6 +51,46 @@ Plan plan_rows(int batch, int longest, int group, int kv_heads, int head_dim, bo
   p.tiles_per_split = int((each + 7) / 8 * 8);
   p.splits = int((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
   return p;
+}
+
+// Rows of a key head from which BF16 chunks go to the tensor-core tiles.
+constexpr long long TILE_ROWS = 32;
+
+// The split count is the one that leaves the busiest SM the least to do: each
+// CTA pays about TILE_OVERHEAD tiles' time to start and end, and splits cost a
+// join.
+Plan plan_tiles(const Call& c) {
+  constexpr int TILE_OVERHEAD = 3;
+  Plan p;
+  p.columns = 0;
+  const long long rows = (long long)c.longest * c.group;
+  p.row_tiles = c.head_dim > 128 || rows <= 128 ? 1 : 2;
+  p.rows_per_unit = 128 * p.row_tiles;
+  p.keys_per_tile = attention_tiles_keys(c.head_dim);
+  const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
+  const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
+  long long best = 0;
+  for (long long splits = 1; splits <= 64 && splits <= tiles; ++splits) {
+    const long long each = (tiles + splits - 1) / splits;
+    const long long cost = (units * splits + sm_count() - 1) / sm_count() * (each + TILE_OVERHEAD) + (splits > 1 ? 2 : 0);
+    if (best && cost >= best) continue;
+    best = cost;
+    p.tiles_per_split = int(each);
+    p.splits = int((tiles + each - 1) / each);
+  }
+  return p;
+}
+
+Plan plan_chunks(const Call& c) {
+  const long long rows = (long long)c.longest * c.group;
+  // (the copies' coordinates are 32-bit, the grid's unit axis 16-bit)
+  const bool reachable = (long long)c.pages * c.page_size < (1ll << 31) &&
+                         (long long)c.pages * c.kv_heads * c.head_dim < (1ll << 31);
+  if (c.x_dtype == DRIFT_BF16 && c.cache_dtype == DRIFT_F16 && reachable && rows >= TILE_ROWS) {
+    const Plan p = plan_tiles(c);
+    if ((rows + p.rows_per_unit - 1) / p.rows_per_unit * p.splits <= 65535) return p;
+  }
+  return plan_rows(c);
 }
 
 int check_shape(int q_heads, int kv_heads, int max_key_count, int table_stride, int page_size, int longest,
@@ -70,13 +117,13 @@ using namespace drift;
 extern "C" {
 
 size_t drift_attention_chunks_workspace_bytes(int x_dtype, int64_t tokens, int q_heads, int kv_heads, int head_dim,
-                                              int cache_dtype, int batch, int longest, int max_key_count, int window,
-                                              int first) {
-  if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || batch <= 0 || longest <= 0 || max_key_count <= 0)
+                                              int cache_dtype, int pages, int page_size, int batch, int longest,
+                                              int max_key_count, int causal, int window, int first) {
+  if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || pages <= 0 ||
+      page_size <= 0 || batch <= 0 || longest <= 0 || max_key_count <= 0)
     return 0;
-  (void)x_dtype;
-  const Plan p = plan_rows(batch, longest, q_heads / kv_heads, kv_heads, head_dim, cache_dtype == DRIFT_I8, max_key_count,
-                           window, first);
+  const Plan p = plan_chunks({x_dtype, cache_dtype, batch, longest, q_heads / kv_heads, kv_heads, head_dim, max_key_count,
+                              causal, window, first, pages, page_size});
   return parts_bytes(p, tokens, q_heads, head_dim);
 }
 
@@ -93,7 +140,8 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   if (tokens == 0 || batch == 0 || longest == 0) return 0;
   DRIFT_TRY(check_rows_aligned("attention", q, out));
   const int group = q_heads / kv_heads;
-  const Plan p = plan_rows(batch, longest, group, kv_heads, head_dim, cache_dtype == DRIFT_I8, max_key_count, window, first);
+  const Plan p = plan_chunks({x_dtype, cache_dtype, batch, longest, group, kv_heads, head_dim, max_key_count, causal,
+                              window, first, pages, page_size});
   const long long units = ((long long)longest * group + p.rows_per_unit - 1) / p.rows_per_unit;
   if (units * p.splits > 0x7fffffffll || (long long)longest * q_heads > 0x7fffffffll)
     return invalid("attention: chunks of %d tokens of %d heads", longest, q_heads);
@@ -124,7 +172,8 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   a.scale = scale;
   a.softcap = softcap;
   const cudaStream_t s = cudaStream_t(stream);
-  DRIFT_TRY(launch_attention_rows(a, x_dtype, cache_dtype, head_dim, p.columns, s));
+  if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, head_dim, p.row_tiles, s));
+  else DRIFT_TRY(launch_attention_rows(a, x_dtype, cache_dtype, head_dim, p.columns, s));
   if (!needed) return 0;
   return launch_attention_join(a, x_dtype, head_dim, p.rows_per_unit, p.keys_per_tile, s);
 }

@@ -1,0 +1,646 @@
+// attention_chunks for BF16 chunks of many rows, on the tensor cores
+// (tcgen05). A unit is a key head of one sequence with 128 MT of the (token,
+// query head) rows that read it; a CTA takes one split of the unit's key
+// tiles. Per tile of KEYS keys and tile i of 128 rows:
+//
+//   S_i = Q_i K^T      (TMEM; Q and K in shared memory)
+//   P_i = 2^(S_i m - M)  over S_i's columns, as F16 (softmax warps: a thread
+//                       has a row, its maximum and its sum, in F32)
+//   O_i += P_i V       (TMEM; V^T in shared memory, as the cache has it)
+//
+// The cache's layouts are the tensor core's own K-major operands -- keys [..][D],
+// values [D][..positions] -- so pages come straight into shared memory by TMA
+// tensor copies, a page's run of 16, 32 or 64 positions at a time (the largest
+// that divides the page): runs of keys are rows of the 128-byte swizzled tile,
+// and a run of values is a tile of its own, in the swizzle as wide as the run.
+//
+// O stays in TMEM and is rescaled only when a row's maximum has grown by 2^6
+// since the last time (weights are at most 2^14 until then, in F16's range);
+// P's rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). q in BF16 is
+// exact in F16 after a power of two per row.
+//
+// With MT = 2 (D <= 128) the two row tiles take turns: while one's softmax
+// runs the tensor core works on the other. With MT = 1 (heads of 256, whose
+// outputs fill TMEM, and units of 128 rows) S has two buffers, and Q K^T of
+// the next tile runs under the softmax.
+//
+// Warps: 0-3 and 4-7 the softmax of row tiles 0 and 1, 8 the copies, 9 the
+// tensor core, 10 and 11 the edges: in a tile that some row sees only in part
+// they take values that are not finite out of V, since such a value times a
+// zero weight would reach rows that do not see it (they are added at the end,
+// to the rows that do). Every wait is bounded; one that gives up sets device
+// error 2, and the CTA drains its copies and products, frees its TMEM and
+// returns.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "chunks.cuh"
+#include "common.cuh"
+#include "registry.cuh"
+#include "tc_common.cuh"
+#include "tma_host.cuh"
+
+namespace drift {
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int ROW_TILE = 128;
+constexpr int THREADS = 384;
+constexpr int COPY_WARP = 8, MMA_WARP = 9, EDGE_WARP = 10;
+constexpr int EDGE_THREADS = 64;
+constexpr uint32_t TMEM_COLUMNS = 512;
+// A weight is 2^WEIGHT_BITS at the row's largest score when its base is set,
+// and the base moves when one would pass 2^(WEIGHT_BITS + GROWTH_BITS).
+constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f;
+
+template <int D_, int KEYS_, int MT_>
+struct TileTraits {
+  static constexpr int D = D_, KEYS = KEYS_, MT = MT_;
+  static constexpr int UNIT = ROW_TILE * MT;
+  static constexpr int PANELS = (D + 63) / 64;             // 64-column panels of a row
+  static constexpr int Q_PANEL = ROW_TILE * 128;           // bytes
+  static constexpr int Q_BYTES = PANELS * Q_PANEL;         // one row tile
+  static constexpr int K_PANEL = KEYS * 128;
+  static constexpr int K_BYTES = PANELS * K_PANEL;
+  static constexpr int V_BYTES = KEYS * D * 2;
+  static constexpr int STAGES = 2;
+  static constexpr int K_AT = MT * Q_BYTES;
+  static constexpr int V_AT = K_AT + STAGES * K_BYTES;
+  static constexpr int BARRIERS_AT = V_AT + STAGES * ((V_BYTES + 1023) / 1024 * 1024);
+  static constexpr int V_STAGE = (V_BYTES + 1023) / 1024 * 1024;
+  static constexpr int BYTES = BARRIERS_AT + 256 + 1024;   // (and the base's alignment)
+  static constexpr int O_COLUMN = 256;                     // S: columns 0 and KEYS; O: 256 and 384
+  static_assert(MT == 1 || (D <= 128 && KEYS <= 128), "two outputs in TMEM");
+  static_assert(2 * KEYS <= O_COLUMN && O_COLUMN + (MT - 1) * 128 + D <= int(TMEM_COLUMNS), "TMEM");
+  static_assert(BYTES <= 232448, "shared memory");
+};
+
+// K-major operand rows of 32, 64 or 128 bytes in the swizzle of that width,
+// 8-row groups apart by eight rows.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t address, uint32_t row_bytes) {
+  uint64_t d = uint64_t((address >> 4) & 0x3fff);
+  d |= uint64_t(1) << 16;
+  d |= uint64_t((8 * row_bytes) >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void mma_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
+// 32 columns of this thread's lane; the values are there after tmem_load_wait.
+__device__ __forceinline__ void tmem_load_32_async(uint32_t address, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(address)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load_16(uint32_t address, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(address)
+      : "memory");
+  tmem_load_wait();
+}
+__device__ __forceinline__ void tmem_store_16(uint32_t address, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(address),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct TileArgs {
+  AttentionChunksArgs a;
+  int run;  // positions a copy takes of a page: 16, 32 or 64
+};
+
+template <class T>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
+                       const TileArgs args) {
+  constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, STAGES = T::STAGES;
+  pdl_trigger();  // the next kernel may launch and wait for this one
+  pdl_wait();     // what the kernels before this one wrote is visible
+  const AttentionChunksArgs& a = args.a;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int head = blockIdx.x, z = blockIdx.y;
+  // the last rows first: under a causal mask they see the most keys
+  const int at = gridDim.z - 1 - blockIdx.z, split = at % a.splits, unit = at / a.splits;
+  const Chunk chunk(a.at, z);
+  if (!chunk.ok && head == 0 && blockIdx.z == 0 && tid == 0) chunk_error(a.error);
+  const int row0 = unit * T::UNIT, row1 = min(row0 + T::UNIT, chunk.tokens * a.group);
+  if (row0 >= row1) return;
+  const int token0 = row0 / a.group, token1 = (row1 - 1) / a.group + 1;
+  const SeenTiles seen(a, chunk, token0, token1, KEYS);
+  const int tile0 = split * a.tiles_per_split, tile1 = min(tile0 + a.tiles_per_split, seen.count);
+  if (tile0 >= tile1) return;
+  const int tiles = tile1 - tile0;
+  // what some row sees: keys below seen.end that are `lowest` or later or
+  // below `first`; what every row sees: below all_end, from all_low on (or
+  // below `first`)
+  const int first = a.window > 0 ? a.first : 0;
+  const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;
+  const int all_end = a.causal ? chunk.position + token0 + 1 : seen.end;
+  const int all_low = a.window > 0 ? chunk.position + token1 - a.window : 0;
+  auto whole = [&](int key0) { return key0 + KEYS <= all_end && (key0 >= all_low || key0 + KEYS <= first); };
+
+  extern __shared__ uint8_t raw[];
+  uint8_t* shared = raw + ((1024 - (tc::smem_u32(raw) & 1023)) & 1023);
+  const uint32_t base = tc::smem_u32(shared);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(shared + T::BARRIERS_AT);
+  uint64_t* q_full = bars;             // [2]
+  uint64_t* k_full = bars + 2;         // [STAGES] each
+  uint64_t* k_empty = k_full + STAGES;
+  uint64_t* v_full = k_empty + STAGES;
+  uint64_t* v_empty = v_full + STAGES;
+  uint64_t* edge_found = v_empty + STAGES;  // an edge tile's values are there; they are clean
+  uint64_t* edge_clean = edge_found + 1;
+  uint64_t* s_full = edge_clean + 1;    // [2]: of row tile i, or of buffer i
+  uint64_t* p_full = s_full + 2;        // [2]
+  uint64_t* o_full = p_full + 2;        // [2]
+  uint64_t* drained = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* taken_out = abort + 1;
+  volatile int* copied = abort + 2;  // [2]: tiles whose keys, values were asked for
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&q_full[i], ROW_TILE);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], ROW_TILE);
+      tc::mbar_init(&o_full[i], 1);
+    }
+    for (int s = 0; s < STAGES; ++s) {
+      tc::mbar_init(&k_full[s], 1);
+      tc::mbar_init(&k_empty[s], 1);
+      tc::mbar_init(&v_full[s], 1);
+      tc::mbar_init(&v_empty[s], 1);
+    }
+    tc::mbar_init(edge_found, 1);
+    tc::mbar_init(edge_clean, EDGE_THREADS);
+    tc::mbar_init(drained, 1);
+    *abort = 0;
+    *taken_out = 0;
+    copied[0] = copied[1] = 0;
+    tc::fence_barrier_init();
+  }
+  __syncwarp();
+  if (warp == 0) tc::tmem_alloc(tmem_slot, TMEM_COLUMNS);
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return tc::mbar_wait_warp(bar, parity, abort, a.error); };
+
+  if (warp < 4 * MT) {
+    // ---- softmax: this thread's row of row tile i --------------------------------------
+    const int i = warp / 4, r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
+    const bool real = row < row1;
+    const int token = (real ? row : row1 - 1) / a.group, q_head = head * a.group + row % a.group;
+    const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
+    const long long row_at = (chunk.row + token) * a.q_heads + q_head;
+    // q, divided by a power of two (and by the scale's sign), into the
+    // swizzled panels
+    float multiplier;
+    {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + row_at * D);
+      uint32_t largest = 0;
+      if (real)
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 x = q[c];
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) largest = max(largest, max(w[e] & 0x7fff0000u, (w[e] << 16) & 0x7fff0000u));
+        }
+      // 2^floor(log2 largest), kept where its inverse is normal (NaNs and
+      // infinities stay what they are)
+      const uint32_t exponent = min(max(largest & 0x7f800000u, 0x01000000u), 0x7e800000u);
+      const float unit_inverse = 1.0f / __uint_as_float(exponent);
+      const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
+      multiplier = fabsf(a.scale) * __uint_as_float(exponent);
+      uint8_t* panel = shared + i * T::Q_BYTES + r * 128;
+      for (int c = 0; c < T::PANELS * 8; ++c) {
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (real && c < D / 8) {
+          const uint4 x = q[c];
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            h[e] = half_pair(__uint_as_float(w[e] << 16) * by, __uint_as_float(w[e] & 0xffff0000u) * by);
+          y = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        *reinterpret_cast<uint4*>(panel + (c / 8) * T::Q_PANEL + 16 * ((c % 8) ^ (r % 8))) = y;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(&q_full[i]);
+    }
+    // (a softcap leaves natural units behind)
+    const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 1.2e-38f);
+    const int position = chunk.position + token;
+    const int hi = a.causal ? position + 1 : seen.end;
+    const int lo = a.window > 0 ? position - a.window + 1 : 0;
+    // what all of this row tile's rows see
+    const int last = min(row0 + ROW_TILE * (i + 1), row1) - 1;
+    const int tile_end = a.causal ? chunk.position + (row0 + ROW_TILE * i) / a.group + 1 : seen.end;
+    const int tile_low = a.window > 0 ? chunk.position + max(last, 0) / a.group - a.window + 1 : 0;
+
+    float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      const int b = MT == 2 ? i : j & 1;
+      const uint32_t phase = MT == 2 ? j & 1 : (j >> 1) & 1;
+      if (!(ok = wait(&s_full[b], phase))) break;
+      tc::fence_after_sync();
+      const uint32_t s_at = tmem + lanes + b * KEYS;
+      float s[KEYS];
+#pragma unroll
+      for (int c = 0; c < KEYS; c += 32) tmem_load_32_async(s_at + c, s + c);
+      tmem_load_wait();
+      const int key0 = seen.key_of(tile0 + j);
+      if (a.softcap > 0.0f) {
+        // softcap tanh(x / softcap) = softcap (1 - 2 / (1 + e^(2 x / softcap)))
+        const float up = 2.0f * LOG2E * multiplier / a.softcap;
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c) s[c] = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + exp2_approx(s[c] * up));
+      }
+      if (!(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first))) {
+        const int end = hi - key0, low = lo - key0, head_end = first - key0;
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c)
+          if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int c = 1; c < KEYS; ++c) top = fmaxf(top, s[c]);
+      top *= m2;
+      const bool grown = top > base2 + (WEIGHT_BITS + GROWTH_BITS);
+      if (__any_sync(0xffffffffu, grown)) {
+        const float now = fmaxf(base2, top - WEIGHT_BITS);
+        const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
+        base2 = now;
+        sum *= f;
+        if (j > 0) {
+          // O holds every tile before this one: with two row tiles P V of the
+          // last came before this S; with one it is waited for
+          if (MT == 1 && !(ok = wait(&o_full[0], (j - 1) & 1))) break;
+          tc::fence_after_sync();
+          const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tmem_load_16(o_at + c, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] *= f;
+            tmem_store_16(o_at + c, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+      }
+      const float less = base2 == -INFINITY ? 0.0f : base2;
+#pragma unroll
+      for (int c = 0; c < KEYS; c += 32) {
+        uint32_t p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = exp2_approx(fmaf(s[c + 2 * e], m2, -less)), y = exp2_approx(fmaf(s[c + 2 * e + 1], m2, -less));
+          sum += x + y;
+          p[e] = half_pair(x, y);
+        }
+        tmem_store_16(s_at + c / 2, p);
+      }
+      tc::tmem_store_wait();
+      tc::fence_before_sync();
+      tc::mbar_arrive(&p_full[b]);
+    }
+    if (ok) ok = wait(&o_full[i], MT == 2 ? 0 : (tiles - 1) & 1);
+    asm volatile("bar.sync 1, %0;" ::"r"(4 * 32 * MT + EDGE_THREADS) : "memory");  // (taken_out is final)
+    if (ok) {
+      tc::fence_after_sync();
+      const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
+      float scale = 1.0f;
+      if (!a.part_o) {
+        float total = sum;
+        if (a.sinks) {
+          // the sink's weight in the row's units, or the row's in the sink's
+          const float sink = a.sinks[q_head] * LOG2E, all = fmaxf(base2, sink);
+          scale = base2 == -INFINITY ? 0.0f : exp2f(base2 - all);
+          total = total * scale + exp2f(sink - all);
+        }
+        scale = total != 0.0f ? scale / total : 0.0f;
+      } else if (real) {
+        *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, sum);
+      }
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        float o[16];
+        __syncwarp();
+        tmem_load_16(o_at + c, o);
+        if (!real) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] *= scale;
+        if (*taken_out) {
+          for (int j = 0; j < tiles; ++j) {
+            const int key0 = seen.key_of(tile0 + j);
+            if (whole(key0)) continue;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + c + e) * a.at.page_size,
+                                          (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
+                                          a.at.page_size, key0, min(key0 + KEYS, hi), lo, first);
+              o[e] += y.x, o[e + 1] += y.y, o[e + 2] += y.z, o[e + 3] += y.w;
+            }
+          }
+        }
+        if (a.part_o) {
+          float4* to = reinterpret_cast<float4*>(a.part_o + (row_at * a.splits + split) * D + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        } else {
+          __align__(16) __nv_bfloat162 y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
+          uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row_at * D + c);
+          to[0] = reinterpret_cast<const uint4*>(y)[0];
+          to[1] = reinterpret_cast<const uint4*>(y)[1];
+        }
+      }
+    }
+  } else if (warp == COPY_WARP) {
+    // ---- copies: a lane per run of a tile's keys, then of its values --------------------
+    const int run = args.run, runs = KEYS / run;
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j % STAGES;
+      const uint32_t used = ((j / STAGES) & 1) ^ 1;  // (free from the start in the first round)
+      const int key = seen.key_of(tile0 + j) + lane * run;
+      // past the last key, or a page that the cache does not have: out of the
+      // maps' range, which reads as zeros
+      int page = a.at.pages;
+      if (lane < runs && key < seen.end) {
+        page = chunk.table[key / a.at.page_size];
+        if (page < 0 || page >= a.at.pages) {
+          chunk_error(a.error);
+          page = a.at.pages;
+        }
+      }
+      const int place = key % a.at.page_size;
+      if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
+      if (lane == 0) {
+        tc::mbar_expect_tx(&k_full[stage], T::K_BYTES);
+        copied[0] = j + 1;
+      }
+      __syncwarp();
+      if (lane < runs)
+#pragma unroll
+        for (int p = 0; p < T::PANELS; ++p)
+          tma_load_3d(base + T::K_AT + stage * T::K_BYTES + p * T::K_PANEL + lane * run * 128, &key_map, &k_full[stage],
+                      64 * p, head, page * a.at.page_size + (page < a.at.pages ? place : 0));
+      if (j >= STAGES && !(ok = wait(&v_empty[stage], used))) break;
+      if (lane == 0) {
+        tc::mbar_expect_tx(&v_full[stage], T::V_BYTES);
+        copied[1] = j + 1;
+      }
+      __syncwarp();
+      if (lane < runs)
+        tma_load_2d(base + T::V_AT + stage * T::V_STAGE + lane * run * D * 2, &value_map, &v_full[stage], place,
+                    (page * a.kv_heads + (page < a.at.pages ? head : 0)) * D);
+      __syncwarp();
+    }
+  } else if (warp == MMA_WARP) {
+    // ---- tensor core --------------------------------------------------------------------
+    constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
+    const int run = args.run;
+    const uint32_t run_steps = run / 16, run_bytes = uint32_t(run) * D * 2;
+    bool ok = true;
+    int edges = 0;
+    auto scores = [&](int j, int i, int b) {
+      const uint64_t q = operand_desc(base + i * T::Q_BYTES, 128);
+      const uint64_t k = operand_desc(base + T::K_AT + (j % STAGES) * T::K_BYTES, 128);
+#pragma unroll
+      for (int step = 0; step < D / 16; ++step)
+        mma_ss_warp(tmem + b * KEYS, q + ((step / 4 * T::Q_PANEL + step % 4 * 32) >> 4),
+                    k + ((step / 4 * T::K_PANEL + step % 4 * 32) >> 4), qk, step > 0);
+      tc::mma_commit_warp(&s_full[b]);
+    };
+    auto outputs = [&](int j, int i, int b) {
+      const uint64_t v = operand_desc(base + T::V_AT + (j % STAGES) * T::V_STAGE, 2 * run);
+#pragma unroll
+      for (int step = 0; step < KEYS / 16; ++step) {
+        const uint32_t at = step / run_steps * run_bytes + step % run_steps * 32;
+        tc::mma_f16_ts_warp(tmem + T::O_COLUMN + 128 * i, tmem + b * KEYS + 8 * step, v + (at >> 4), pv, j > 0 || step > 0);
+      }
+    };
+    auto keys_ready = [&](int j) { return wait(&k_full[j % STAGES], (j / STAGES) & 1); };
+    auto values_ready = [&](int j) {
+      if (!wait(&v_full[j % STAGES], (j / STAGES) & 1)) return false;
+      if (whole(seen.key_of(tile0 + j))) return true;
+      // (edge tile by edge tile, in turn with the edge warps)
+      if (lane == 0) tc::mbar_arrive(edge_found);
+      return wait(edge_clean, edges++ & 1);
+    };
+    for (int i = 0; i < MT && ok; ++i) ok = wait(&q_full[i], 0);
+    if (ok) ok = keys_ready(0);
+    if (ok) {
+      tc::fence_after_sync();
+      for (int i = 0; i < MT; ++i) scores(0, i, i);
+      tc::mma_commit_warp(&k_empty[0]);
+    }
+    for (int j = 0; j < tiles && ok; ++j) {
+      if constexpr (MT == 2) {
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (i == 0 && !(ok = values_ready(j))) break;
+          if (!(ok = wait(&p_full[i], j & 1))) break;
+          tc::fence_after_sync();
+          outputs(j, i, i);
+          if (i == 1) tc::mma_commit_warp(&v_empty[j % STAGES]);
+          if (j + 1 == tiles) {
+            tc::mma_commit_warp(&o_full[i]);
+            continue;
+          }
+          if (i == 0 && !(ok = keys_ready(j + 1))) break;
+          scores(j + 1, i, i);
+          if (i == 1) tc::mma_commit_warp(&k_empty[(j + 1) % STAGES]);
+        }
+      } else {
+        if (j + 1 < tiles) {
+          if (!(ok = keys_ready(j + 1))) break;
+          scores(j + 1, 0, (j + 1) & 1);
+          tc::mma_commit_warp(&k_empty[(j + 1) % STAGES]);
+        }
+        if (!(ok = values_ready(j))) break;
+        if (!(ok = wait(&p_full[j & 1], (j >> 1) & 1))) break;
+        tc::fence_after_sync();
+        outputs(j, 0, j & 1);
+        tc::mma_commit_warp(&v_empty[j % STAGES]);
+        tc::mma_commit_warp(&o_full[0]);
+      }
+    }
+  } else if (warp >= EDGE_WARP) {
+    // ---- edges: values that are not finite, out of the tiles seen in part -----------------
+    bool ok = true;
+    int edges = 0;
+    const int run = args.run, row_bytes = 2 * run, chunks = run / 8;  // 16-byte chunks of a run's row
+    for (int j = 0; j < tiles && ok; ++j) {
+      const int key0 = seen.key_of(tile0 + j);
+      if (whole(key0)) continue;
+      if (!(ok = wait(edge_found, edges++ & 1))) break;
+      if (!(ok = wait(&v_full[j % STAGES], (j / STAGES) & 1))) break;
+      uint8_t* v = shared + T::V_AT + (j % STAGES) * T::V_STAGE;
+      bool found = false;
+      for (int n = tid - 32 * EDGE_WARP; n < T::V_BYTES / 16; n += EDGE_THREADS) {
+        uint4 x = *reinterpret_cast<uint4*>(v + 16 * n);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool low = (w[e] & 0x7c00u) == 0x7c00u, high = (w[e] & 0x7c000000u) == 0x7c000000u;
+          bad = bad || low || high;
+          w[e] &= (low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u);
+        }
+        if (!bad) continue;
+        *reinterpret_cast<uint4*>(v + 16 * n) = x;
+        // which keys: the run, and the chunk in its row before the swizzle
+        // (which exchanges 16-byte chunks by the address bits 7 and up)
+        const int in_run = 16 * n % (run * D * 2), d = in_run / row_bytes;
+        const int swizzle = row_bytes == 128 ? d % 8 : row_bytes == 64 ? d / 2 % 4 : d / 4 % 2;
+        const int key = key0 + 16 * n / (run * D * 2) * run + 8 * ((n % chunks) ^ swizzle);
+        for (int e = 0; e < 8; ++e)
+          found = found || (key + e < seen.end && (key + e >= lowest || key + e < first));
+      }
+      if (found) *taken_out = 1;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(edge_clean);
+    }
+    asm volatile("bar.arrive 1, %0;" ::"r"(4 * 32 * MT + EDGE_THREADS) : "memory");
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (*abort) {
+    // a wait gave up: what is on its way lands before shared memory and TMEM go
+    int none = 0;
+    if (tid == 32 * COPY_WARP)
+      for (int side = 0; side < 2; ++side) {
+        const int n = copied[side];
+        uint64_t* full = side == 0 ? k_full : v_full;
+        for (int j = max(0, n - STAGES); j < n; ++j) tc::mbar_wait(&full[j % STAGES], (j / STAGES) & 1, &none, nullptr);
+      }
+    if (warp == MMA_WARP) {
+      tc::mma_commit_warp(drained);
+      tc::mbar_wait_warp(drained, 0, &none, nullptr);
+    }
+    __syncthreads();
+  }
+  if (warp == 0) tc::tmem_dealloc(tmem, TMEM_COLUMNS);
+}
+
+// Keys of a tile: 64 where a wider one's scores, or its keys and values beside
+// q, do not fit.
+constexpr int tile_of(int head_dim) { return head_dim > 128 ? 64 : 128; }
+
+template <int D, int MT>
+int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
+  using T = TileTraits<D, tile_of(D), MT>;
+  TileArgs args;
+  args.a = a;
+  const int ps = a.at.page_size;
+  args.run = ps % 64 == 0 ? 64 : ps % 32 == 0 ? 32 : 16;
+  const uint64_t positions = uint64_t(a.at.pages) * ps;
+  CUtensorMap key_map, value_map;
+  {
+    const uint64_t dims[3] = {uint64_t(D), uint64_t(a.kv_heads), positions};
+    const uint64_t strides[2] = {uint64_t(D) * 2, uint64_t(a.kv_heads) * D * 2};
+    const uint32_t box[3] = {64, 1, uint32_t(args.run)};
+    DRIFT_TRY(encode_f16_tiles(&key_map, a.keys, 3, dims, strides, box, 128));
+  }
+  {
+    const uint64_t dims[2] = {uint64_t(ps), uint64_t(a.at.pages) * a.kv_heads * D};
+    const uint64_t strides[1] = {uint64_t(ps) * 2};
+    const uint32_t box[2] = {uint32_t(args.run), uint32_t(D)};
+    DRIFT_TRY(encode_f16_tiles(&value_map, a.values, 2, dims, strides, box, 2 * args.run));
+  }
+  static PerDevice configured;
+  DRIFT_TRY(ensure_shared_memory(configured, attention_tiles_kernel<T>, T::BYTES));
+  const unsigned units = unsigned((a.at.longest * a.group + T::UNIT - 1) / T::UNIT);
+  DRIFT_CUDA(launch_pdl(attention_tiles_kernel<T>, dim3(a.kv_heads, a.at.batch, units * a.splits), THREADS, T::BYTES,
+                        stream, key_map, value_map, args));
+  DRIFT_LAUNCHED("attention_tiles");
+  return 0;
+}
+
+#define DRIFT_TILES_REGISTER(D, MT) \
+  DRIFT_REGISTER(attention_tiles_f16_d##D##_m##MT, (attention_tiles_kernel<TileTraits<D, tile_of(D), MT>>))
+DRIFT_TILES_REGISTER(64, 1)
+DRIFT_TILES_REGISTER(64, 2)
+DRIFT_TILES_REGISTER(80, 1)
+DRIFT_TILES_REGISTER(80, 2)
+DRIFT_TILES_REGISTER(128, 1)
+DRIFT_TILES_REGISTER(128, 2)
+DRIFT_TILES_REGISTER(256, 1)
+
+}  // namespace
+
+int attention_tiles_keys(int head_dim) { return tile_of(head_dim); }
+
+int launch_attention_tiles(const AttentionChunksArgs& a, int head_dim, int row_tiles, cudaStream_t stream) {
+  switch (head_dim) {
+    case 64: return row_tiles == 2 ? launch_tiles<64, 2>(a, stream) : launch_tiles<64, 1>(a, stream);
+    case 80: return row_tiles == 2 ? launch_tiles<80, 2>(a, stream) : launch_tiles<80, 1>(a, stream);
+    case 128: return row_tiles == 2 ? launch_tiles<128, 2>(a, stream) : launch_tiles<128, 1>(a, stream);
+    default: return launch_tiles<256, 1>(a, stream);
+  }
+}
+
+}  // namespace drift

@@ -614,8 +614,8 @@ class CudaOps:
         chunk_args = self._check_chunks("attention", chunks)
         max_keys = int(chunks.max_key_count)
         size = self.lib.drift_attention_chunks_workspace_bytes(
-            x_dtype, tokens, q_heads, cache.kv_heads, dim, dtype, chunk_args[4], longest, max_keys,
-            window, first)
+            x_dtype, tokens, q_heads, cache.kv_heads, dim, dtype, pages, page_size, chunk_args[4],
+            longest, max_keys, int(attention.causal), window, first)
         # the call's own: freed to torch's allocator behind it in the stream
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         status = self.lib.drift_attention_chunks(

@@ -291,8 +291,9 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
                            size_t workspace_bytes, drift_stream_t stream);
 size_t drift_attention_chunks_workspace_bytes(int x_dtype, int64_t tokens, int q_heads,
                                               int kv_heads, int head_dim, int cache_dtype,
-                                              int batch, int longest, int max_key_count,
-                                              int window, int first);
+                                              int pages, int page_size, int batch, int longest,
+                                              int max_key_count, int causal, int window,
+                                              int first);
 
 /* ---- Gated DeltaNet (the hybrid decoder's linear-attention layers) ---------
  * SequenceOps.causalConv (ops/SequenceOps.scala; CPU ops/CpuSequence.scala:

@@ -104,7 +104,8 @@ def test_no_attention_is_nothing_to_do(lib):
 
 def test_workspace_bytes(lib):
     size = lambda **c: lib.drift_attention_chunks_workspace_bytes(*({**dict(  # noqa: E731
-        x_dtype=F32, tokens=8, q_heads=32, kv_heads=8, head_dim=128, cache_dtype=I8, batch=8, longest=1, max_keys=4096,
+        x_dtype=F32, tokens=8, q_heads=32, kv_heads=8, head_dim=128, cache_dtype=I8, pages=64, page_size=16, batch=8,
+        longest=1, max_keys=4096, causal=1,
         window=0, first=0), **c}.values()))
     assert size() > 0                       # few rows: split over the keys
     assert size(max_keys=16) == 0           # one split
