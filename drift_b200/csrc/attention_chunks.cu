@@ -53,7 +53,7 @@ Plan plan_rows(const Call& c) {
   return p;
 }
 
-// Rows of a key head from which BF16 chunks go to the tensor-core tiles.
+// Rows of a key head from which chunks go to the tensor-core tiles.
 constexpr long long TILE_ROWS = 32;
 
 // The split count is the one that leaves the busiest SM the least to do: each
@@ -66,7 +66,7 @@ Plan plan_tiles(const Call& c) {
   const long long rows = (long long)c.longest * c.group;
   p.row_tiles = c.head_dim > 128 || rows <= 128 ? 1 : 2;
   p.rows_per_unit = 128 * p.row_tiles;
-  p.keys_per_tile = attention_tiles_keys(c.head_dim);
+  p.keys_per_tile = attention_tiles_keys(c.head_dim, c.x_dtype == DRIFT_BF16);
   const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
   const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
   long long best = 0;
@@ -86,7 +86,7 @@ Plan plan_chunks(const Call& c) {
   // (the copies' coordinates are 32-bit, the grid's unit axis 16-bit)
   const bool reachable = (long long)c.pages * c.page_size < (1ll << 31) &&
                          (long long)c.pages * c.kv_heads * c.head_dim < (1ll << 31);
-  if (c.x_dtype == DRIFT_BF16 && c.cache_dtype == DRIFT_F16 && reachable && rows >= TILE_ROWS) {
+  if ((c.x_dtype == DRIFT_BF16 || c.head_dim <= 128) && reachable && rows >= TILE_ROWS) {
     const Plan p = plan_tiles(c);
     if ((rows + p.rows_per_unit - 1) / p.rows_per_unit * p.splits <= 65535) return p;
   }
@@ -172,7 +172,7 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   a.scale = scale;
   a.softcap = softcap;
   const cudaStream_t s = cudaStream_t(stream);
-  if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, head_dim, p.row_tiles, s));
+  if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, x_dtype, cache_dtype, head_dim, p.row_tiles, s));
   else DRIFT_TRY(launch_attention_rows(a, x_dtype, cache_dtype, head_dim, p.columns, s));
   if (!needed) return 0;
   return launch_attention_join(a, x_dtype, head_dim, p.rows_per_unit, p.keys_per_tile, s);

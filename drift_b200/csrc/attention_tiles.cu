@@ -1,23 +1,32 @@
-// attention_chunks for BF16 chunks of many rows, on the tensor cores
-// (tcgen05). A unit is a key head of one sequence with 128 MT of the (token,
-// query head) rows that read it; a CTA takes one split of the unit's key
-// tiles. Per tile of KEYS keys and tile i of 128 rows:
+// attention_chunks for chunks of many rows, on the tensor cores (tcgen05). A
+// unit is a key head of one sequence with 128 MT of the (token, query head)
+// rows that read it; a CTA takes one split of the unit's key tiles. Per tile
+// of KEYS keys and tile i of 128 rows:
 //
 //   S_i = Q_i K^T      (TMEM; Q and K in shared memory)
-//   P_i = 2^(S_i m - M)  over S_i's columns, as F16 (softmax warps: a thread
-//                       has a row, its maximum and its sum, in F32)
-//   O_i += P_i V       (TMEM; V^T in shared memory, as the cache has it)
+//   P_i = e^(scale S_i - base)  over S_i's columns, as F16 (softmax warps: a
+//                       thread has a row, its base and its sum, in F32)
+//   O_i (+)= P_i V     (TMEM; V^T in shared memory, as the cache has it)
 //
-// The cache's layouts are the tensor core's own K-major operands -- keys [..][D],
-// values [D][..positions] -- so pages come straight into shared memory by TMA
-// tensor copies, a page's run of 16, 32 or 64 positions at a time (the largest
-// that divides the page): runs of keys are rows of the 128-byte swizzled tile,
-// and a run of values is a tile of its own, in the swizzle as wide as the run.
+// The F16 cache's layouts are the tensor core's own K-major operands -- keys
+// [..][D], values [D][..positions] -- so pages come straight into shared memory
+// by TMA tensor copies, a page's run of 16, 32 or 64 positions at a time (the
+// largest that divides the page): runs of keys are rows of the 128-byte
+// swizzled tile, and a run of values is a tile of its own, in the swizzle as
+// wide as the run. An 8-bit cache's codes come the same way into a buffer of
+// their own, from which converting warps write them as F16, exactly, into the
+// operands; a key's scale multiplies its scores, and a value's scale its
+// weights (over a power of two at or above every scale so far, so that a
+// weight stays in F16's range).
 //
-// O stays in TMEM and is rescaled only when a row's maximum has grown by 2^6
-// since the last time (weights are at most 2^14 until then, in F16's range);
-// P's rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). q in BF16 is
-// exact in F16 after a power of two per row.
+// BF16 rows (TERMS = 1): q is exact in F16 after a power of two per row; P's
+// rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). O stays in TMEM
+// and is rescaled only when a row's largest score has grown by 2^6 since the
+// last time (weights are at most 2^14 until then).
+// F32 rows (TERMS = 2): q and P are two F16 terms each (hi + lo, to 2^-22), the
+// products of both summed. The tensor core's F32 sums drop low bits as a chain
+// grows, so a tile's P V starts a new O, and the softmax threads add it to
+// their row's running output in registers.
 //
 // With MT = 2 (D <= 128) the two row tiles take turns: while one's softmax
 // runs the tensor core works on the other. With MT = 1 (heads of 256, whose
@@ -25,16 +34,18 @@
 // the next tile runs under the softmax.
 //
 // Warps: 0-3 and 4-7 the softmax of row tiles 0 and 1, 8 the copies, 9 the
-// tensor core, 10 and 11 the edges: in a tile that some row sees only in part
-// they take values that are not finite out of V, since such a value times a
-// zero weight would reach rows that do not see it (they are added at the end,
-// to the rows that do). Every wait is bounded; one that gives up sets device
-// error 2, and the CTA drains its copies and products, frees its TMEM and
-// returns.
+// tensor core; then, for an F16 cache, 10 and 11 the edges: in a tile that
+// some row sees only in part they take values that are not finite out of V,
+// since such a value times a zero weight would reach rows that do not see it
+// (they are added at the end, to the rows that do); for an 8-bit cache the
+// converting warps. Every wait is bounded; one that gives up sets device error
+// 2, and the CTA drains its copies and products, frees its TMEM and returns.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "chunks.cuh"
 #include "common.cuh"
@@ -49,35 +60,64 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROW_TILE = 128;
-constexpr int THREADS = 384;
 constexpr int COPY_WARP = 8, MMA_WARP = 9, EDGE_WARP = 10;
 constexpr int EDGE_THREADS = 64;
 constexpr uint32_t TMEM_COLUMNS = 512;
 // A weight is 2^WEIGHT_BITS at the row's largest score when its base is set,
 // and the base moves when one would pass 2^(WEIGHT_BITS + GROWTH_BITS).
 constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f;
+// A row of q is 2^Q_BITS and more at its largest value, so that its second
+// terms end far below F16's last bit, 2^-24.
+constexpr int Q_BITS = 8;
 
-template <int D_, int KEYS_, int MT_>
+template <int D_, int KEYS_, int MT_, bool CODES_, int TERMS_>
 struct TileTraits {
-  static constexpr int D = D_, KEYS = KEYS_, MT = MT_;
+  static constexpr int D = D_, KEYS = KEYS_, MT = MT_, TERMS = TERMS_;
+  static constexpr bool CODES = CODES_;
   static constexpr int UNIT = ROW_TILE * MT;
+  // Converting 128 keys' codes for BF16 rows takes four warps, one to a
+  // scheduler; for F32 rows, at half the keys in the same time, two. The
+  // softmax warps take the registers that the others leave.
+  static constexpr bool WIDE = CODES && TERMS == 1;
+  static constexpr int THREADS = WIDE ? 512 : 384;
+  static constexpr int CONVERT_WARP = WIDE ? 12 : 10;
+  static constexpr int CONVERT_THREADS = THREADS - 32 * CONVERT_WARP;
+  static constexpr int SOFTMAX_REGISTERS = TERMS == 2 ? 224 : WIDE ? 192 : 208;
+  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : WIDE ? 64 : 88;
+  static_assert(256 * SOFTMAX_REGISTERS + (THREADS - 256) * OTHER_REGISTERS <= THREADS * (65536 / THREADS / 8 * 8),
+                "what the block is launched with");
   static constexpr int PANELS = (D + 63) / 64;             // 64-column panels of a row
   static constexpr int Q_PANEL = ROW_TILE * 128;           // bytes
-  static constexpr int Q_BYTES = PANELS * Q_PANEL;         // one row tile
+  static constexpr int Q_BYTES = PANELS * Q_PANEL;         // one term of one row tile
   static constexpr int K_PANEL = KEYS * 128;
   static constexpr int K_BYTES = PANELS * K_PANEL;
   static constexpr int V_BYTES = KEYS * D * 2;
-  static constexpr int STAGES = 2;
-  static constexpr int K_AT = MT * Q_BYTES;
-  static constexpr int V_AT = K_AT + STAGES * K_BYTES;
-  static constexpr int BARRIERS_AT = V_AT + STAGES * ((V_BYTES + 1023) / 1024 * 1024);
   static constexpr int V_STAGE = (V_BYTES + 1023) / 1024 * 1024;
-  static constexpr int BYTES = BARRIERS_AT + 256 + 1024;   // (and the base's alignment)
+  static constexpr int CODE_BYTES = KEYS * D;              // of one side of a tile
+  static constexpr int STAGES = 2;
+  static constexpr int COPY_STAGES = CODES ? 1 : STAGES;   // of what the copies fill
+  static constexpr int K_AT = MT * TERMS * Q_BYTES;
+  static constexpr int V_AT = K_AT + STAGES * K_BYTES;
+  static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;
+  static constexpr int SCALES_AT = CODES_AT + (CODES ? 2 * CODE_BYTES : 0);  // [STAGES][2][KEYS]
+  static constexpr int BARRIERS_AT = SCALES_AT + (CODES ? STAGES * 2 * KEYS * 4 : 0);
+  static constexpr int BYTES = BARRIERS_AT + 320;
   static constexpr int O_COLUMN = 256;                     // S: columns 0 and KEYS; O: 256 and 384
   static_assert(MT == 1 || (D <= 128 && KEYS <= 128), "two outputs in TMEM");
   static_assert(2 * KEYS <= O_COLUMN && O_COLUMN + (MT - 1) * 128 + D <= int(TMEM_COLUMNS), "TMEM");
+  static_assert(KEYS % 64 == 0 && TERMS * KEYS / 2 <= KEYS, "P fits over S");
+  static_assert(TERMS == 1 || D <= 128, "the running output of a row in registers");
   static_assert(BYTES <= 232448, "shared memory");
 };
+
+template <int REGISTERS>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+}
+template <int REGISTERS>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+}
 
 // K-major operand rows of 32, 64 or 128 bytes in the swizzle of that width,
 // 8-row groups apart by eight rows.
@@ -161,6 +201,37 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// What F16 leaves of a pair.
+__device__ __forceinline__ uint32_t left_pair(float a, float b, uint32_t pair) {
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+  return half_pair(a - h.x, b - h.y);
+}
+
+// Four codes as two pairs of F16: a byte u = code + 128 under the exponent of
+// 1024 is 1024 + u, less 1152.
+__device__ __forceinline__ uint2 code_pairs(uint32_t codes) {
+  const uint32_t u = codes ^ 0x80808080u;
+  const __half2 less = __half2half2(__ushort_as_half(0x6480));  // 1152
+  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), less);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), less);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// softcap tanh(x / softcap): near zero x / softcap times a polynomial in its
+// square (least squares on Chebyshev points of |y| <= 0.55, reweighted towards
+// the least largest relative error, 1e-9), farther off 1 - 2 / (1 + e^(2 y)),
+// which loses bits only near zero.
+__device__ __forceinline__ float capped(float x, float inverse, float softcap) {
+  const float y = x * inverse, u = y * y;
+  float p = fmaf(u, -0.006235556676983833f, 0.021039674058556557f);
+  p = fmaf(u, p, -0.053842708468437195f);
+  p = fmaf(u, p, 0.13332460820674896f);
+  p = fmaf(u, p, -0.3333331048488617f);
+  const float near = fmaf(y * u, p, y);
+  const float far = 1.0f - __fdividef(2.0f, 1.0f + exp2_approx(2.0f * LOG2E * y));
+  return softcap * (fabsf(y) <= 0.55f ? near : far);
+}
 
 struct TileArgs {
   AttentionChunksArgs a;
@@ -168,10 +239,12 @@ struct TileArgs {
 };
 
 template <class T>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(T::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                        const TileArgs args) {
-  constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, STAGES = T::STAGES;
+  constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
+  constexpr bool CODES = T::CODES;
+  using X = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
   const AttentionChunksArgs& a = args.a;
@@ -197,25 +270,33 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   const int all_low = a.window > 0 ? chunk.position + token1 - a.window : 0;
   auto whole = [&](int key0) { return key0 + KEYS <= all_end && (key0 >= all_low || key0 + KEYS <= first); };
 
-  extern __shared__ uint8_t raw[];
-  uint8_t* shared = raw + ((1024 - (tc::smem_u32(raw) & 1023)) & 1023);
+  extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = tc::smem_u32(shared);
+  if (base & 1023) {  // (the operands' swizzles want it; a kernel without static shared memory has it)
+    if (tid == 0 && a.error) atomicCAS(a.error, 0, 2);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(shared + T::BARRIERS_AT);
   uint64_t* q_full = bars;             // [2]
   uint64_t* k_full = bars + 2;         // [STAGES] each
   uint64_t* k_empty = k_full + STAGES;
   uint64_t* v_full = k_empty + STAGES;
   uint64_t* v_empty = v_full + STAGES;
-  uint64_t* edge_found = v_empty + STAGES;  // an edge tile's values are there; they are clean
+  uint64_t* scales_full = v_empty + STAGES;
+  uint64_t* s_full = scales_full + STAGES;  // [2]: of row tile i, or of buffer i
+  uint64_t* p_full = s_full + 2;            // [2]
+  uint64_t* o_full = p_full + 2;            // [2]
+  uint64_t* edge_found = o_full + 2;        // an edge tile's values are there; they are clean
   uint64_t* edge_clean = edge_found + 1;
-  uint64_t* s_full = edge_clean + 1;    // [2]: of row tile i, or of buffer i
-  uint64_t* p_full = s_full + 2;        // [2]
-  uint64_t* o_full = p_full + 2;        // [2]
-  uint64_t* drained = o_full + 2;
+  uint64_t* codes_full = edge_clean + 1;    // [2]: of the keys, of the values
+  uint64_t* codes_empty = codes_full + 2;   // [2]
+  uint64_t* drained = codes_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* taken_out = abort + 1;
-  volatile int* copied = abort + 2;  // [2]: tiles whose keys, values were asked for
+  volatile int* copied = abort + 2;         // [2]: tiles whose keys, values were asked for
+  volatile float* v_unit = reinterpret_cast<volatile float*>(abort + 4);  // [STAGES]: the scales' power of two
+  float* scales = reinterpret_cast<float*>(shared + T::SCALES_AT);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -225,10 +306,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_init(&o_full[i], 1);
     }
     for (int s = 0; s < STAGES; ++s) {
-      tc::mbar_init(&k_full[s], 1);
+      tc::mbar_init(&k_full[s], CODES ? T::CONVERT_THREADS : 1);
       tc::mbar_init(&k_empty[s], 1);
-      tc::mbar_init(&v_full[s], 1);
+      tc::mbar_init(&v_full[s], CODES ? T::CONVERT_THREADS : 1);
       tc::mbar_init(&v_empty[s], 1);
+      tc::mbar_init(&scales_full[s], T::CONVERT_THREADS);
+      tc::mbar_init(&codes_full[s], 1);
+      tc::mbar_init(&codes_empty[s], T::CONVERT_THREADS);
     }
     tc::mbar_init(edge_found, 1);
     tc::mbar_init(edge_clean, EDGE_THREADS);
@@ -245,6 +329,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return tc::mbar_wait_warp(bar, parity, abort, a.error); };
 
+  // (warpgroups 0 and 1: warps 0-7)
+  if (warp < 4 * MT) more_registers<T::SOFTMAX_REGISTERS>();
+  else fewer_registers<T::OTHER_REGISTERS>();
+
   if (warp < 4 * MT) {
     // ---- softmax: this thread's row of row tile i --------------------------------------
     const int i = warp / 4, r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
@@ -253,37 +341,51 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
     const long long row_at = (chunk.row + token) * a.q_heads + q_head;
     // q, divided by a power of two (and by the scale's sign), into the
-    // swizzled panels
+    // swizzled panels of its terms
     float multiplier;
     {
-      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + row_at * D);
-      uint32_t largest = 0;
+      const X* q = static_cast<const X*>(a.q) + row_at * D;
+      float x[8];
+      auto load = [&](int c) {  // values 8 c .. 8 c + 7
+        if constexpr (TERMS == 1) {
+          const uint4 v = reinterpret_cast<const uint4*>(q)[c];
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        } else {
+          const float4 u = reinterpret_cast<const float4*>(q)[2 * c], v = reinterpret_cast<const float4*>(q)[2 * c + 1];
+          x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+        }
+      };
+      float largest = 0.0f;
       if (real)
         for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = q[c];
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          load(c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) largest = max(largest, max(w[e] & 0x7fff0000u, (w[e] << 16) & 0x7fff0000u));
+          for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[e]));
         }
-      // 2^floor(log2 largest), kept where its inverse is normal (NaNs and
-      // infinities stay what they are)
-      const uint32_t exponent = min(max(largest & 0x7f800000u, 0x01000000u), 0x7e800000u);
+      // 2^(floor(log2 largest) - Q_BITS), kept where it and its inverse are
+      // normal (NaNs and infinities stay what they are)
+      constexpr uint32_t SHIFT = uint32_t(Q_BITS) << 23;
+      const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, SHIFT + 0x01000000u) - SHIFT;
       const float unit_inverse = 1.0f / __uint_as_float(exponent);
       const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
       multiplier = fabsf(a.scale) * __uint_as_float(exponent);
-      uint8_t* panel = shared + i * T::Q_BYTES + r * 128;
+      uint8_t* panel = shared + i * TERMS * T::Q_BYTES + r * 128;
       for (int c = 0; c < T::PANELS * 8; ++c) {
-        uint4 y = make_uint4(0, 0, 0, 0);
+        uint4 hi = make_uint4(0, 0, 0, 0), low = hi;
         if (real && c < D / 8) {
-          const uint4 x = q[c];
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          uint32_t h[4];
+          load(c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            h[e] = half_pair(__uint_as_float(w[e] << 16) * by, __uint_as_float(w[e] & 0xffff0000u) * by);
-          y = make_uint4(h[0], h[1], h[2], h[3]);
+          for (int e = 0; e < 8; ++e) x[e] *= by;
+          hi = make_uint4(half_pair(x[0], x[1]), half_pair(x[2], x[3]), half_pair(x[4], x[5]), half_pair(x[6], x[7]));
+          if constexpr (TERMS == 2)
+            low = make_uint4(left_pair(x[0], x[1], hi.x), left_pair(x[2], x[3], hi.y), left_pair(x[4], x[5], hi.z),
+                             left_pair(x[6], x[7], hi.w));
         }
-        *reinterpret_cast<uint4*>(panel + (c / 8) * T::Q_PANEL + 16 * ((c % 8) ^ (r % 8))) = y;
+        uint8_t* to = panel + (c / 8) * T::Q_PANEL + 16 * ((c % 8) ^ (r % 8));
+        *reinterpret_cast<uint4*>(to) = hi;
+        if constexpr (TERMS == 2) *reinterpret_cast<uint4*>(to + T::Q_BYTES) = low;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&q_full[i]);
@@ -297,13 +399,36 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int last = min(row0 + ROW_TILE * (i + 1), row1) - 1;
     const int tile_end = a.causal ? chunk.position + (row0 + ROW_TILE * i) / a.group + 1 : seen.end;
     const int tile_low = a.window > 0 ? chunk.position + max(last, 0) / a.group - a.window + 1 : 0;
+    const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
 
     float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
+    float unit = 0.0f;                    // and, for codes, values are over this
+    float total[TERMS == 2 ? D : 1] = {};  // the running output (F32 rows)
+    // the last tile's output, which the tensor core has left in O
+    auto take_output = [&]() {
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          tmem_load_16(o_at + c, o);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) total[c + e] += o[e];
+        }
+      }
+    };
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      const int b = MT == 2 ? i : j & 1;
+      const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
       const uint32_t phase = MT == 2 ? j & 1 : (j >> 1) & 1;
       if (!(ok = wait(&s_full[b], phase))) break;
+      if (CODES && !(ok = wait(&scales_full[stage], (j / STAGES) & 1))) break;
+      // O holds the tile before this one, or every one: with two row tiles
+      // that P V came before this S; with one it is waited for
+      if (TERMS == 2 && j > 0) {
+        if (MT == 1 && !(ok = wait(&o_full[0], (j - 1) & 1))) break;
+        tc::fence_after_sync();
+        take_output();
+      }
       tc::fence_after_sync();
       const uint32_t s_at = tmem + lanes + b * KEYS;
       float s[KEYS];
@@ -311,13 +436,22 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       for (int c = 0; c < KEYS; c += 32) tmem_load_32_async(s_at + c, s + c);
       tmem_load_wait();
       const int key0 = seen.key_of(tile0 + j);
-      if (a.softcap > 0.0f) {
-        // softcap tanh(x / softcap) = softcap (1 - 2 / (1 + e^(2 x / softcap)))
-        const float up = 2.0f * LOG2E * multiplier / a.softcap;
+      const float* k_scales = scales + stage * 2 * KEYS;
+      const float* v_scales = k_scales + KEYS;
+      if constexpr (CODES) {
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c) s[c] = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + exp2_approx(s[c] * up));
+        for (int c = 0; c < KEYS; c += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
+          s[c] *= x.x, s[c + 1] *= x.y, s[c + 2] *= x.z, s[c + 3] *= x.w;
+        }
       }
-      if (!(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first))) {
+      if (a.softcap > 0.0f) {
+        const float inverse = multiplier / a.softcap;
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c) s[c] = capped(s[c], inverse, a.softcap);
+      }
+      const bool edge = !(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first));
+      if (edge) {
         const int end = hi - key0, low = lo - key0, head_end = first - key0;
 #pragma unroll
         for (int c = 0; c < KEYS; ++c)
@@ -327,71 +461,91 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll
       for (int c = 1; c < KEYS; ++c) top = fmaxf(top, s[c]);
       top *= m2;
-      const bool grown = top > base2 + (WEIGHT_BITS + GROWTH_BITS);
+      float shrink = 1.0f;
+      if constexpr (CODES) {
+        const float now = v_unit[stage];
+        if (now > unit) {
+          shrink = unit / now;
+          unit = now;
+        }
+      }
+      const bool grown = top > base2 + (WEIGHT_BITS + GROWTH_BITS) || shrink != 1.0f;
       if (__any_sync(0xffffffffu, grown)) {
         const float now = fmaxf(base2, top - WEIGHT_BITS);
         const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
         base2 = now;
         sum *= f;
-        if (j > 0) {
-          // O holds every tile before this one: with two row tiles P V of the
-          // last came before this S; with one it is waited for
+        const float g = f * shrink;
+        if constexpr (TERMS == 2) {
+#pragma unroll
+          for (int c = 0; c < D; ++c) total[c] *= g;
+        } else if (j > 0) {
           if (MT == 1 && !(ok = wait(&o_full[0], (j - 1) & 1))) break;
           tc::fence_after_sync();
-          const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
             float o[16];
             tmem_load_16(o_at + c, o);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] *= f;
+            for (int e = 0; e < 16; ++e) o[e] *= g;
             tmem_store_16(o_at + c, reinterpret_cast<const uint32_t*>(o));
           }
         }
       }
       const float less = base2 == -INFINITY ? 0.0f : base2;
+      float part = 0.0f;  // (a tile's own sum: short chains)
 #pragma unroll
       for (int c = 0; c < KEYS; c += 32) {
-        uint32_t p[16];
+        uint32_t p[16], p_low[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = exp2_approx(fmaf(s[c + 2 * e], m2, -less)), y = exp2_approx(fmaf(s[c + 2 * e + 1], m2, -less));
-          sum += x + y;
-          p[e] = half_pair(x, y);
+        for (int e = 0; e < 16; e += 2) {
+          float w[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) w[n] = exp2_approx(fmaf(s[c + 2 * e + n], m2, -less));
+          part += (w[0] + w[1]) + (w[2] + w[3]);
+          if constexpr (CODES) {
+            const float4 x = *reinterpret_cast<const float4*>(v_scales + c + 2 * e);
+            w[0] *= x.x, w[1] *= x.y, w[2] *= x.z, w[3] *= x.w;
+            if (edge) {  // (a hidden value's scale may be a NaN)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) w[n] = s[c + 2 * e + n] == -INFINITY ? 0.0f : w[n];
+            }
+          }
+          p[e] = half_pair(w[0], w[1]);
+          p[e + 1] = half_pair(w[2], w[3]);
+          if constexpr (TERMS == 2) p_low[e] = left_pair(w[0], w[1], p[e]), p_low[e + 1] = left_pair(w[2], w[3], p[e + 1]);
         }
         tmem_store_16(s_at + c / 2, p);
+        if constexpr (TERMS == 2) tmem_store_16(s_at + KEYS / 2 + c / 2, p_low);
       }
+      sum += part;
       tc::tmem_store_wait();
       tc::fence_before_sync();
       tc::mbar_arrive(&p_full[b]);
     }
     if (ok) ok = wait(&o_full[i], MT == 2 ? 0 : (tiles - 1) & 1);
-    asm volatile("bar.sync 1, %0;" ::"r"(4 * 32 * MT + EDGE_THREADS) : "memory");  // (taken_out is final)
+    if constexpr (!CODES) asm volatile("bar.sync 1, %0;" ::"n"(4 * 32 * MT + EDGE_THREADS) : "memory");  // (taken_out is final)
     if (ok) {
       tc::fence_after_sync();
-      const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
-      float scale = 1.0f;
+      take_output();
+      float scale = CODES ? unit : 1.0f;
       if (!a.part_o) {
-        float total = sum;
+        float all_sum = sum;
         if (a.sinks) {
           // the sink's weight in the row's units, or the row's in the sink's
           const float sink = a.sinks[q_head] * LOG2E, all = fmaxf(base2, sink);
-          scale = base2 == -INFINITY ? 0.0f : exp2f(base2 - all);
-          total = total * scale + exp2f(sink - all);
+          const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - all);
+          all_sum = all_sum * f + exp2f(sink - all);
+          scale *= f;
         }
-        scale = total != 0.0f ? scale / total : 0.0f;
+        scale = all_sum != 0.0f ? scale / all_sum : 0.0f;
       } else if (real) {
         *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, sum);
       }
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        float o[16];
-        __syncwarp();
-        tmem_load_16(o_at + c, o);
-        if (!real) continue;
+      auto put = [&](int c, float (&o)[16]) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[e] *= scale;
-        if (*taken_out) {
+        if (!CODES && *taken_out) {
           for (int j = 0; j < tiles; ++j) {
             const int key0 = seen.key_of(tile0 + j);
             if (whole(key0)) continue;
@@ -404,8 +558,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             }
           }
         }
-        if (a.part_o) {
-          float4* to = reinterpret_cast<float4*>(a.part_o + (row_at * a.splits + split) * D + c);
+        if (a.part_o || TERMS == 2) {
+          float4* to = reinterpret_cast<float4*>(a.part_o ? a.part_o + (row_at * a.splits + split) * D + c
+                                                          : static_cast<float*>(a.out) + row_at * D + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         } else {
@@ -416,6 +571,23 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           to[0] = reinterpret_cast<const uint4*>(y)[0];
           to[1] = reinterpret_cast<const uint4*>(y)[1];
         }
+      };
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = total[c + e];
+          if (real) put(c, o);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          __syncwarp();
+          tmem_load_16(o_at + c, o);
+          if (real) put(c, o);
+        }
       }
     }
   } else if (warp == COPY_WARP) {
@@ -423,8 +595,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int run = args.run, runs = KEYS / run;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      const int stage = j % STAGES;
-      const uint32_t used = ((j / STAGES) & 1) ^ 1;  // (free from the start in the first round)
+      const int stage = j % T::COPY_STAGES;
+      const uint32_t used = ((j / T::COPY_STAGES) & 1) ^ 1;
       const int key = seen.key_of(tile0 + j) + lane * run;
       // past the last key, or a page that the cache does not have: out of the
       // maps' range, which reads as zeros
@@ -437,56 +609,73 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         }
       }
       const int place = key % a.at.page_size;
-      if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
+      const int k_row = page * a.at.page_size + (page < a.at.pages ? place : 0);
+      const int v_row = (page * a.kv_heads + (page < a.at.pages ? head : 0)) * D;
+      if (j >= T::COPY_STAGES && !(ok = wait(CODES ? &codes_empty[0] : &k_empty[stage], used))) break;
+      uint64_t* full = CODES ? &codes_full[0] : &k_full[stage];
       if (lane == 0) {
-        tc::mbar_expect_tx(&k_full[stage], T::K_BYTES);
+        tc::mbar_expect_tx(full, CODES ? T::CODE_BYTES : T::K_BYTES);
         copied[0] = j + 1;
       }
       __syncwarp();
-      if (lane < runs)
+      if (lane < runs) {
+        if constexpr (CODES) {
+          tma_load_3d(base + T::CODES_AT + lane * run * D, &key_map, full, 0, head, k_row);
+        } else {
 #pragma unroll
-        for (int p = 0; p < T::PANELS; ++p)
-          tma_load_3d(base + T::K_AT + stage * T::K_BYTES + p * T::K_PANEL + lane * run * 128, &key_map, &k_full[stage],
-                      64 * p, head, page * a.at.page_size + (page < a.at.pages ? place : 0));
-      if (j >= STAGES && !(ok = wait(&v_empty[stage], used))) break;
+          for (int p = 0; p < T::PANELS; ++p)
+            tma_load_3d(base + T::K_AT + stage * T::K_BYTES + p * T::K_PANEL + lane * run * 128, &key_map, full, 64 * p,
+                        head, k_row);
+        }
+      }
+      if (j >= T::COPY_STAGES && !(ok = wait(CODES ? &codes_empty[1] : &v_empty[stage], used))) break;
+      full = CODES ? &codes_full[1] : &v_full[stage];
       if (lane == 0) {
-        tc::mbar_expect_tx(&v_full[stage], T::V_BYTES);
+        tc::mbar_expect_tx(full, CODES ? T::CODE_BYTES : T::V_BYTES);
         copied[1] = j + 1;
       }
       __syncwarp();
       if (lane < runs)
-        tma_load_2d(base + T::V_AT + stage * T::V_STAGE + lane * run * D * 2, &value_map, &v_full[stage], place,
-                    (page * a.kv_heads + (page < a.at.pages ? head : 0)) * D);
+        tma_load_2d(CODES ? base + T::CODES_AT + T::CODE_BYTES + lane * run * D
+                          : base + T::V_AT + stage * T::V_STAGE + lane * run * D * 2,
+                    &value_map, full, place, v_row);
       __syncwarp();
     }
   } else if (warp == MMA_WARP) {
     // ---- tensor core --------------------------------------------------------------------
     constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
-    const int run = args.run;
+    const int run = CODES ? 64 : args.run;  // keys of a tile of V
     const uint32_t run_steps = run / 16, run_bytes = uint32_t(run) * D * 2;
     bool ok = true;
     int edges = 0;
+    // (second terms first, while the sums are small)
     auto scores = [&](int j, int i, int b) {
-      const uint64_t q = operand_desc(base + i * T::Q_BYTES, 128);
       const uint64_t k = operand_desc(base + T::K_AT + (j % STAGES) * T::K_BYTES, 128);
 #pragma unroll
-      for (int step = 0; step < D / 16; ++step)
-        mma_ss_warp(tmem + b * KEYS, q + ((step / 4 * T::Q_PANEL + step % 4 * 32) >> 4),
-                    k + ((step / 4 * T::K_PANEL + step % 4 * 32) >> 4), qk, step > 0);
+      for (int term = TERMS - 1; term >= 0; --term) {
+        const uint64_t q = operand_desc(base + (i * TERMS + term) * T::Q_BYTES, 128);
+#pragma unroll
+        for (int step = 0; step < D / 16; ++step)
+          mma_ss_warp(tmem + b * KEYS, q + ((step / 4 * T::Q_PANEL + step % 4 * 32) >> 4),
+                      k + ((step / 4 * T::K_PANEL + step % 4 * 32) >> 4), qk, term < TERMS - 1 || step > 0);
+      }
       tc::mma_commit_warp(&s_full[b]);
     };
     auto outputs = [&](int j, int i, int b) {
       const uint64_t v = operand_desc(base + T::V_AT + (j % STAGES) * T::V_STAGE, 2 * run);
 #pragma unroll
-      for (int step = 0; step < KEYS / 16; ++step) {
-        const uint32_t at = step / run_steps * run_bytes + step % run_steps * 32;
-        tc::mma_f16_ts_warp(tmem + T::O_COLUMN + 128 * i, tmem + b * KEYS + 8 * step, v + (at >> 4), pv, j > 0 || step > 0);
-      }
+      for (int term = TERMS - 1; term >= 0; --term)
+#pragma unroll
+        for (int step = 0; step < KEYS / 16; ++step) {
+          const uint32_t at = step / run_steps * run_bytes + step % run_steps * 32;
+          tc::mma_f16_ts_warp(tmem + T::O_COLUMN + 128 * i, tmem + b * KEYS + term * KEYS / 2 + 8 * step, v + (at >> 4), pv,
+                              (TERMS == 1 && j > 0) || term < TERMS - 1 || step > 0);
+        }
     };
     auto keys_ready = [&](int j) { return wait(&k_full[j % STAGES], (j / STAGES) & 1); };
     auto values_ready = [&](int j) {
       if (!wait(&v_full[j % STAGES], (j / STAGES) & 1)) return false;
-      if (whole(seen.key_of(tile0 + j))) return true;
+      if (CODES || whole(seen.key_of(tile0 + j))) return true;
       // (edge tile by edge tile, in turn with the edge warps)
       if (lane == 0) tc::mbar_arrive(edge_found);
       return wait(edge_clean, edges++ & 1);
@@ -528,7 +717,95 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         tc::mma_commit_warp(&o_full[0]);
       }
     }
-  } else if (warp >= EDGE_WARP) {
+  } else if (CODES && warp >= T::CONVERT_WARP) {
+    // ---- conversion: codes to F16 operands, and the tile's scales ------------------------
+    const int t = tid - 32 * T::CONVERT_WARP;
+    const int run = args.run;
+    const uint8_t* k_codes = shared + T::CODES_AT;
+    const uint8_t* v_codes = k_codes + T::CODE_BYTES;
+    // the scales of tile j, zeros where no row sees the key: key t's of the
+    // keys, and of the values those of every 32nd from this lane's (each warp
+    // finds the largest for itself)
+    constexpr int PER = KEYS / 32;
+    auto load_scales = [&](int j, float& k, float (&v)[PER]) {
+      k = 0.0f;
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        v[n] = 0.0f;
+        const int key = seen.key_of(tile0 + j) + lane + 32 * n;
+        if (key >= seen.end || (key < lowest && key >= first)) continue;
+        const int page = chunk.table[key / a.at.page_size];
+        if (page < 0 || page >= a.at.pages) continue;
+        const long long at = ((long long)page * a.kv_heads + head) * a.at.page_size + key % a.at.page_size;
+        v[n] = a.value_scales[at];
+        if (n == t / 32) k = a.key_scales[at];
+      }
+    };
+    float k_scale, v_scale[PER], power = 0.0f;
+    load_scales(0, k_scale, v_scale);
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j % STAGES;
+      const uint32_t used = ((j / STAGES) & 1) ^ 1;
+      // keys
+      if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
+      if (!(ok = wait(&codes_full[0], j & 1))) break;
+      uint8_t* k = shared + T::K_AT + stage * T::K_BYTES;
+#pragma unroll 4
+      for (int n = t; n < KEYS * D / 16; n += T::CONVERT_THREADS) {
+        const int row = n / (D / 16), c = n % (D / 16);
+        const uint4 x = *reinterpret_cast<const uint4*>(k_codes + 16 * n);
+        const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
+        uint8_t* to = k + c / 4 * T::K_PANEL + row * 128;
+        *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4)) ^ (row % 8))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4) + 1) ^ (row % 8))) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(&k_full[stage]);
+      tc::mbar_arrive(&codes_empty[0]);
+      // scales: the stage's were last read by the softmax before the P V that
+      // freed its values
+      if (j >= STAGES && !(ok = wait(&v_empty[stage], used))) break;
+      float most = 0.0f;  // (fmaxf passes NaNs over)
+#pragma unroll
+      for (int n = 0; n < PER; ++n) most = fmaxf(most, v_scale[n]);
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (most > power) {
+        // a power of two at or above it whose inverse is normal
+        const uint32_t bits = __float_as_uint(most);
+        const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
+        power = __uint_as_float(max(up, 0x01000000u));
+      }
+      if (t < KEYS) {
+        float own = v_scale[0];
+#pragma unroll
+        for (int n = 1; n < PER; ++n) own = n == t / 32 ? v_scale[n] : own;
+        scales[stage * 2 * KEYS + t] = k_scale;
+        scales[stage * 2 * KEYS + KEYS + t] = power > 0.0f ? own * (1.0f / power) : own;
+      }
+      if (t == 0) v_unit[stage] = power;
+      tc::mbar_arrive(&scales_full[stage]);
+      if (j + 1 < tiles) load_scales(j + 1, k_scale, v_scale);
+      // values: sixteen positions of a dimension
+      if (!(ok = wait(&codes_full[1], j & 1))) break;
+      uint8_t* v = shared + T::V_AT + stage * T::V_STAGE;
+#pragma unroll 4
+      for (int n = t; n < KEYS * D / 16; n += T::CONVERT_THREADS) {
+        const int in_run = 16 * n % (run * D), d = in_run / run;
+        const int place = 16 * n / (run * D) * run + in_run % run;
+        const uint4 x = *reinterpret_cast<const uint4*>(v_codes + 16 * n);
+        const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
+        uint8_t* to = v + place / 64 * (D * 128) + d * 128;
+        const int c = place % 64 / 8;
+        *reinterpret_cast<uint4*>(to + 16 * (c ^ (d % 8))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        *reinterpret_cast<uint4*>(to + 16 * ((c + 1) ^ (d % 8))) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(&v_full[stage]);
+      tc::mbar_arrive(&codes_empty[1]);
+    }
+  } else if (!CODES && warp >= EDGE_WARP) {
     // ---- edges: values that are not finite, out of the tiles seen in part -----------------
     bool ok = true;
     int edges = 0;
@@ -564,7 +841,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(edge_clean);
     }
-    asm volatile("bar.arrive 1, %0;" ::"r"(4 * 32 * MT + EDGE_THREADS) : "memory");
+    asm volatile("bar.arrive 1, %0;" ::"n"(4 * 32 * MT + EDGE_THREADS) : "memory");
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -574,8 +851,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     if (tid == 32 * COPY_WARP)
       for (int side = 0; side < 2; ++side) {
         const int n = copied[side];
-        uint64_t* full = side == 0 ? k_full : v_full;
-        for (int j = max(0, n - STAGES); j < n; ++j) tc::mbar_wait(&full[j % STAGES], (j / STAGES) & 1, &none, nullptr);
+        uint64_t* full = CODES ? &codes_full[side] : side == 0 ? k_full : v_full;
+        for (int j = max(0, n - T::COPY_STAGES); j < n; ++j)
+          tc::mbar_wait(&full[j % T::COPY_STAGES], (j / T::COPY_STAGES) & 1, &none, nullptr);
       }
     if (warp == MMA_WARP) {
       tc::mma_commit_warp(drained);
@@ -586,60 +864,77 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   if (warp == 0) tc::tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
-// Keys of a tile: 64 where a wider one's scores, or its keys and values beside
-// q, do not fit.
-constexpr int tile_of(int head_dim) { return head_dim > 128 ? 64 : 128; }
+// Keys of a tile: 64 where a wider one's scores (two terms of weights and the
+// running output), or its keys and values beside q, do not fit.
+constexpr int tile_of(int head_dim, int terms) { return head_dim > 128 || terms == 2 ? 64 : 128; }
 
-template <int D, int MT>
+template <int D, int MT, bool CODES, int TERMS>
 int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
-  using T = TileTraits<D, tile_of(D), MT>;
+  using T = TileTraits<D, tile_of(D, TERMS), MT, CODES, TERMS>;
   TileArgs args;
   args.a = a;
   const int ps = a.at.page_size;
   args.run = ps % 64 == 0 ? 64 : ps % 32 == 0 ? 32 : 16;
   const uint64_t positions = uint64_t(a.at.pages) * ps;
+  constexpr uint64_t SIZE = CODES ? 1 : 2;
   CUtensorMap key_map, value_map;
   {
     const uint64_t dims[3] = {uint64_t(D), uint64_t(a.kv_heads), positions};
-    const uint64_t strides[2] = {uint64_t(D) * 2, uint64_t(a.kv_heads) * D * 2};
-    const uint32_t box[3] = {64, 1, uint32_t(args.run)};
-    DRIFT_TRY(encode_f16_tiles(&key_map, a.keys, 3, dims, strides, box, 128));
+    const uint64_t strides[2] = {uint64_t(D) * SIZE, uint64_t(a.kv_heads) * D * SIZE};
+    const uint32_t box[3] = {CODES ? uint32_t(D) : 64u, 1, uint32_t(args.run)};
+    DRIFT_TRY(encode_cache_tiles(&key_map, a.keys, CODES, 3, dims, strides, box, CODES ? 0 : 128));
   }
   {
     const uint64_t dims[2] = {uint64_t(ps), uint64_t(a.at.pages) * a.kv_heads * D};
-    const uint64_t strides[1] = {uint64_t(ps) * 2};
+    const uint64_t strides[1] = {uint64_t(ps) * SIZE};
     const uint32_t box[2] = {uint32_t(args.run), uint32_t(D)};
-    DRIFT_TRY(encode_f16_tiles(&value_map, a.values, 2, dims, strides, box, 2 * args.run));
+    DRIFT_TRY(encode_cache_tiles(&value_map, a.values, CODES, 2, dims, strides, box, CODES ? 0 : 2 * args.run));
   }
   static PerDevice configured;
   DRIFT_TRY(ensure_shared_memory(configured, attention_tiles_kernel<T>, T::BYTES));
   const unsigned units = unsigned((a.at.longest * a.group + T::UNIT - 1) / T::UNIT);
-  DRIFT_CUDA(launch_pdl(attention_tiles_kernel<T>, dim3(a.kv_heads, a.at.batch, units * a.splits), THREADS, T::BYTES,
+  DRIFT_CUDA(launch_pdl(attention_tiles_kernel<T>, dim3(a.kv_heads, a.at.batch, units * a.splits), T::THREADS, T::BYTES,
                         stream, key_map, value_map, args));
   DRIFT_LAUNCHED("attention_tiles");
   return 0;
 }
 
-#define DRIFT_TILES_REGISTER(D, MT) \
-  DRIFT_REGISTER(attention_tiles_f16_d##D##_m##MT, (attention_tiles_kernel<TileTraits<D, tile_of(D), MT>>))
+template <int D, int MT>
+int launch_types(const AttentionChunksArgs& a, bool codes, bool bf16, cudaStream_t stream) {
+  if (bf16) return codes ? launch_tiles<D, MT, true, 1>(a, stream) : launch_tiles<D, MT, false, 1>(a, stream);
+  if constexpr (D <= 128) return codes ? launch_tiles<D, MT, true, 2>(a, stream) : launch_tiles<D, MT, false, 2>(a, stream);
+  else return invalid("attention: no F32 tiles for heads of %d", D);
+}
+
+#define DRIFT_TILES_REGISTER_AS(D, MT, codes, terms, name) \
+  DRIFT_REGISTER(name, (attention_tiles_kernel<TileTraits<D, tile_of(D, terms), MT, codes, terms>>))
+#define DRIFT_TILES_REGISTER_BF16(D, MT)                                            \
+  DRIFT_TILES_REGISTER_AS(D, MT, false, 1, attention_tiles_f16_bf16_d##D##_m##MT)    \
+  DRIFT_TILES_REGISTER_AS(D, MT, true, 1, attention_tiles_i8_bf16_d##D##_m##MT)
+#define DRIFT_TILES_REGISTER(D, MT)                                                 \
+  DRIFT_TILES_REGISTER_BF16(D, MT)                                                  \
+  DRIFT_TILES_REGISTER_AS(D, MT, false, 2, attention_tiles_f16_f32_d##D##_m##MT)     \
+  DRIFT_TILES_REGISTER_AS(D, MT, true, 2, attention_tiles_i8_f32_d##D##_m##MT)
 DRIFT_TILES_REGISTER(64, 1)
 DRIFT_TILES_REGISTER(64, 2)
 DRIFT_TILES_REGISTER(80, 1)
 DRIFT_TILES_REGISTER(80, 2)
 DRIFT_TILES_REGISTER(128, 1)
 DRIFT_TILES_REGISTER(128, 2)
-DRIFT_TILES_REGISTER(256, 1)
+DRIFT_TILES_REGISTER_BF16(256, 1)
 
 }  // namespace
 
-int attention_tiles_keys(int head_dim) { return tile_of(head_dim); }
+int attention_tiles_keys(int head_dim, bool bf16) { return tile_of(head_dim, bf16 ? 1 : 2); }
 
-int launch_attention_tiles(const AttentionChunksArgs& a, int head_dim, int row_tiles, cudaStream_t stream) {
+int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int row_tiles,
+                           cudaStream_t stream) {
+  const bool bf16 = x_dtype == DRIFT_BF16, codes = cache_dtype == DRIFT_I8;
   switch (head_dim) {
-    case 64: return row_tiles == 2 ? launch_tiles<64, 2>(a, stream) : launch_tiles<64, 1>(a, stream);
-    case 80: return row_tiles == 2 ? launch_tiles<80, 2>(a, stream) : launch_tiles<80, 1>(a, stream);
-    case 128: return row_tiles == 2 ? launch_tiles<128, 2>(a, stream) : launch_tiles<128, 1>(a, stream);
-    default: return launch_tiles<256, 1>(a, stream);
+    case 64: return row_tiles == 2 ? launch_types<64, 2>(a, codes, bf16, stream) : launch_types<64, 1>(a, codes, bf16, stream);
+    case 80: return row_tiles == 2 ? launch_types<80, 2>(a, codes, bf16, stream) : launch_types<80, 1>(a, codes, bf16, stream);
+    case 128: return row_tiles == 2 ? launch_types<128, 2>(a, codes, bf16, stream) : launch_types<128, 1>(a, codes, bf16, stream);
+    default: return launch_types<256, 1>(a, codes, bf16, stream);
   }
 }
 

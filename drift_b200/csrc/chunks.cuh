@@ -121,10 +121,11 @@ int check_rows_aligned(const char* call, const void* a, const void* b);
 int attention_rows_tile(int head_dim, bool codes, int columns);
 int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int columns,
                           cudaStream_t stream);
-// attention_tiles.cu, for BF16 rows over F16 caches: `row_tiles` tiles of 128
-// rows a unit (1 or 2; 1 for heads of 256), and the keys of one of its tiles.
-int attention_tiles_keys(int head_dim);
-int launch_attention_tiles(const AttentionChunksArgs& a, int head_dim, int row_tiles, cudaStream_t stream);
+// attention_tiles.cu (F32 rows: heads up to 128): `row_tiles` tiles of 128 rows
+// a unit (1 or 2; 1 for heads of 256), and the keys of one of its tiles.
+int attention_tiles_keys(int head_dim, bool bf16);
+int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int row_tiles,
+                           cudaStream_t stream);
 // Joins the splits (attention_rows.cu).
 int launch_attention_join(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                           int keys_per_tile, cudaStream_t stream);

@@ -66,7 +66,7 @@ int encode_f16_sw128(CUtensorMap* map, const void* base, int64_t cols, int64_t r
   return 0;
 }
 
-int encode_f16_tiles(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+int encode_cache_tiles(CUtensorMap* map, const void* base, bool bytes, int rank, const uint64_t* dims,
                      const uint64_t* strides, const uint32_t* box, int swizzle_bytes) {
   EncodeTiled encode = encode_tiled();
   if (!encode) return invalid("cuTensorMapEncodeTiled is not available from the driver");
@@ -77,8 +77,9 @@ int encode_f16_tiles(CUtensorMap* map, const void* base, int rank, const uint64_
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
   const CUtensorMapSwizzle swizzle = swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                      : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                           : CU_TENSOR_MAP_SWIZZLE_32B;
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, cuuint32_t(rank),
+                                     : swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                                           : CU_TENSOR_MAP_SWIZZLE_NONE;
+  const CUresult r = encode(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, cuuint32_t(rank),
                             const_cast<void*>(base), d, s, b, element, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

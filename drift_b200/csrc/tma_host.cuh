@@ -19,10 +19,11 @@ int encode_word_rows(CUtensorMap* map, const void* base, int64_t row_words, int6
 // 128-byte swizzle that UMMA's K-major canonical layout reads.
 int encode_f16_sw128(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int box_rows);
 
-// F16 tiles of up to 5 dimensions, the innermost first: `strides` are bytes
-// from the second dimension on, the box's innermost extent is as wide as the
-// swizzle (128, 64 or 32 bytes), zero fill past the ends.
-int encode_f16_tiles(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+// Tiles of F16 values (or bytes) of up to 5 dimensions, the innermost first:
+// `strides` are bytes from the second dimension on, the box's innermost extent
+// is as wide as the swizzle (128, 64 or 32 bytes; 0 for none), zero fill past
+// the ends.
+int encode_cache_tiles(CUtensorMap* map, const void* base, bool bytes, int rank, const uint64_t* dims,
                      const uint64_t* strides, const uint32_t* box, int swizzle_bytes);
 
 }  // namespace drift

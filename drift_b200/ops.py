@@ -93,7 +93,7 @@ class KvCache:
                                    device=device), page_size)
 
 
-@dataclass
+@dataclass(frozen=True)
 class QuantizedKvCache:
     """A KvCache in 8 bits: int8 codes in its two layouts and, for each side,
     one F32 scale per position and head, [pages, kv_heads, page_size]; a value
@@ -103,6 +103,17 @@ class QuantizedKvCache:
     key_scales: torch.Tensor
     value_scales: torch.Tensor
     page_size: int
+
+    def __post_init__(self):
+        # once, so that a call need not
+        shape = (self.pages, self.kv_heads, self.page_size)
+        _check_cache("cache", self.keys, self.values, self.page_size, torch.int8)
+        for scales in (self.key_scales, self.value_scales):
+            _require(tuple(scales.shape) == shape,
+                     f"cache: scales {list(scales.shape)} for keys {list(self.keys.shape)}")
+            _require(scales.dtype == torch.float32 and scales.is_contiguous()
+                     and scales.device == self.keys.device,
+                     "cache: scales are contiguous F32 beside the codes")
 
     @property
     def pages(self) -> int:
@@ -128,7 +139,7 @@ class QuantizedKvCache:
                                 torch.zeros(pages, kv_heads, page_size, **scales), page_size)
 
 
-@dataclass
+@dataclass(frozen=True)
 class Chunks:
     """A batch of sequences' new tokens: sequence z's are rows starts[z] ..
     starts[z + 1] - 1, at positions positions[z], positions[z] + 1, ... of the
@@ -140,6 +151,19 @@ class Chunks:
     page_tables: torch.Tensor
     longest: int
     max_key_count: int
+
+    def __post_init__(self):
+        # once, so that a call need not
+        tensors = (self.starts, self.positions, self.page_tables)
+        for t in tensors:
+            _require(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous()
+                     and t.device == self.starts.device,
+                     "chunks: starts, positions and page tables are contiguous I32 device memory")
+        batch = self.positions.numel()
+        _require(self.positions.dim() == 1 and tuple(self.starts.shape) == (batch + 1,)
+                 and self.page_tables.dim() == 2 and self.page_tables.shape[0] == batch,
+                 f"chunks: starts {list(self.starts.shape)}, page tables "
+                 f"{list(self.page_tables.shape)} for {batch} sequences")
 
 
 @dataclass
@@ -187,6 +211,18 @@ def _ptr(t: Optional[torch.Tensor]):
 def _require(condition: bool, message: str) -> None:
     if not condition:
         raise ValueError(message)
+
+
+def _check_cache(name: str, keys, values, page_size: int, dtype) -> None:
+    """A paged cache's two sides."""
+    shape = keys.shape
+    if len(shape) != 4 or shape[1] != page_size or \
+            values.shape != (shape[0], shape[2], shape[3], page_size):
+        raise ValueError(f"{name}: a cache of keys {list(shape)}, values {list(values.shape)}, "
+                         f"pages of {page_size}")
+    for t in (keys, values):
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.device != keys.device:
+            raise ValueError(f"{name}: the cache is contiguous device memory, {dtype} here")
 
 
 def _f32(name: str, *tensors: torch.Tensor) -> None:
@@ -510,57 +546,42 @@ class CudaOps:
 
     # -- a batch of sequences' new tokens ----------------------------------------------------------
     @staticmethod
-    def _check_cache(name: str, cache) -> tuple:
-        """The cache's arguments: its type, codes or values, and scales."""
-        quantized = isinstance(cache, QuantizedKvCache)
-        held = torch.int8 if quantized else torch.float16
-        pages, page_size, kv_heads, dim = cache.keys.shape
-        _require(cache.page_size == page_size
-                 and tuple(cache.values.shape) == (pages, kv_heads, dim, page_size),
-                 f"{name}: a cache of keys {list(cache.keys.shape)}, values "
-                 f"{list(cache.values.shape)}, pages of {cache.page_size}")
-        sides = [(cache.keys, held), (cache.values, held)]
-        if quantized:
-            for scales in (cache.key_scales, cache.value_scales):
-                _require(tuple(scales.shape) == (pages, kv_heads, page_size),
-                         f"{name}: scales {list(scales.shape)} for keys {list(cache.keys.shape)}")
-                sides.append((scales, torch.float32))
-        for tensor, dtype in sides:
-            _require(tensor.dtype == dtype and tensor.is_cuda and tensor.is_contiguous(),
-                     f"{name}: the cache is contiguous device memory, {dtype} here")
-        return (I8 if quantized else F16, _ptr(cache.keys), _ptr(cache.values),
-                _ptr(cache.key_scales) if quantized else None,
-                _ptr(cache.value_scales) if quantized else None, pages, page_size)
+    def _chunk_rows(name: str, a, b, cache, chunks: Chunks) -> int:
+        """Two arrays of rows of the cache's heads; their type. (The checks of
+        a decoding step's calls, so the messages are made only when needed.)"""
+        dtype, shape, device = a.dtype, a.shape, a.device
+        if b.dtype != dtype or b.shape != shape:
+            raise ValueError(f"{name}: {dtype} and {b.dtype}, {list(shape)} and {list(b.shape)}")
+        if dtype != torch.float32 and dtype != torch.bfloat16:
+            raise ValueError(f"{name} takes F32 (or BF16), not {dtype}")
+        if len(shape) != 3 or shape[2] != cache.keys.shape[3]:
+            raise ValueError(f"{name}: {list(shape)} for a cache of {cache.kv_heads} heads of "
+                             f"{cache.head_dim}")
+        if not (a.is_contiguous() and b.is_contiguous()):
+            raise ValueError(f"{name}: tensors are contiguous device memory")
+        if device.index != torch.cuda.current_device() or not (
+                device == b.device == cache.keys.device == chunks.starts.device):
+            raise ValueError(f"{name}: tensors on {device}, {b.device}, {cache.keys.device} and "
+                             f"{chunks.starts.device}, the current device is "
+                             f"{torch.cuda.current_device()}")
+        return F32 if dtype == torch.float32 else BF16
 
-    def _check_chunks(self, name: str, chunks: Chunks) -> tuple:
-        """The chunks' arguments."""
-        starts, positions, tables = chunks.starts, chunks.positions, chunks.page_tables
-        for t in (starts, positions, tables):
-            _require(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous(),
-                     f"{name}: starts, positions and page tables are contiguous I32 device memory")
-        batch = positions.numel()
-        _require(positions.dim() == 1 and tuple(starts.shape) == (batch + 1,) and tables.dim() == 2
-                 and tables.shape[0] == batch,
-                 f"{name}: starts {list(starts.shape)}, page tables {list(tables.shape)} for "
-                 f"{batch} sequences")
-        return _ptr(tables), int(tables.shape[1]), _ptr(starts), _ptr(positions), batch, \
-            int(chunks.longest)
+    @staticmethod
+    def _cache_args(name: str, cache) -> tuple:
+        """kv_heads, head_dim, the type, the two sides, their scales, pages and page_size."""
+        keys, values = cache.keys, cache.values
+        pages, page_size, kv_heads, dim = keys.shape
+        if isinstance(cache, QuantizedKvCache):
+            return (kv_heads, dim, I8, keys.data_ptr(), values.data_ptr(), cache.key_scales.data_ptr(),
+                    cache.value_scales.data_ptr(), pages, page_size)
+        _check_cache(name, keys, values, cache.page_size, torch.float16)
+        return kv_heads, dim, F16, keys.data_ptr(), values.data_ptr(), None, None, pages, page_size
 
-    def _check_rows(self, name: str, cache, *tensors) -> int:
-        """Rows of the cache's heads: their type, shape and device."""
-        first = tensors[0]
-        _same_shape(name, *tensors)
-        for t in tensors:
-            _require(t.dtype == first.dtype, f"{name}: {first.dtype} and {t.dtype}")
-            _require(t.device == cache.keys.device, f"{name}: {t.device}, the cache on {cache.keys.device}")
-            x_dtype = _x_dtype(name, t)
-        _require(first.dim() == 3 and first.shape[2] == cache.head_dim,
-                 f"{name}: {list(first.shape)} for a cache of {cache.kv_heads} heads of "
-                 f"{cache.head_dim}")
-        _require(first.device.index == torch.cuda.current_device(),
-                 f"{name}: tensors on {first.device}, the current device is "
-                 f"{torch.cuda.current_device()}")
-        return x_dtype
+    @staticmethod
+    def _chunk_args(chunks: Chunks) -> tuple:
+        tables = chunks.page_tables
+        return (tables.data_ptr(), tables.shape[1], chunks.starts.data_ptr(),
+                chunks.positions.data_ptr(), tables.shape[0], chunks.longest)
 
     def cache_write_chunks(self, k, v, cache, chunks: Chunks) -> None:
         """k, v [tokens, kv_heads, D] (F32 or BF16) of every sequence into its
@@ -568,31 +589,27 @@ class CudaOps:
         to 8-bit codes with a scale per position and head (a
         QuantizedKvCache): scale = max |row| / 127, code = row / scale to the
         nearest, halves to even, as in exact arithmetic."""
-        x_dtype = self._check_rows("cacheWrite", cache, k, v)
-        _require(k.shape[1] == cache.kv_heads,
-                 f"cacheWrite: {list(k.shape)} into a cache of {cache.kv_heads} heads of "
-                 f"{cache.head_dim}")
-        dtype, keys, values, key_scales, value_scales, pages, page_size = \
-            self._check_cache("cacheWrite", cache)
+        x_dtype = self._chunk_rows("cacheWrite", k, v, cache, chunks)
+        args = self._cache_args("cacheWrite", cache)
+        if k.shape[1] != args[0]:
+            raise ValueError(f"cacheWrite: {list(k.shape)} into a cache of {args[0]} heads of "
+                             f"{args[1]}")
         status = self.lib.drift_cache_write_chunks(
-            x_dtype, _ptr(k), _ptr(v), k.shape[0], cache.kv_heads, cache.head_dim, dtype, keys,
-            values, key_scales, value_scales, pages, page_size,
-            *self._check_chunks("cacheWrite", chunks), self._stream())
+            x_dtype, k.data_ptr(), v.data_ptr(), k.shape[0], *args, *self._chunk_args(chunks),
+            self._stream())
         check("drift_cache_write_chunks", status)
 
     def cache_read_chunks(self, cache, chunks: Chunks, k, v) -> None:
         """What the cache holds at the chunks' positions, into k and v
         [tokens, kv_heads, D] (F32 or BF16)."""
-        x_dtype = self._check_rows("cacheRead", cache, k, v)
-        _require(k.shape[1] == cache.kv_heads,
-                 f"cacheRead: {list(k.shape)} from a cache of {cache.kv_heads} heads of "
-                 f"{cache.head_dim}")
-        dtype, keys, values, key_scales, value_scales, pages, page_size = \
-            self._check_cache("cacheRead", cache)
+        x_dtype = self._chunk_rows("cacheRead", k, v, cache, chunks)
+        args = self._cache_args("cacheRead", cache)
+        if k.shape[1] != args[0]:
+            raise ValueError(f"cacheRead: {list(k.shape)} from a cache of {args[0]} heads of "
+                             f"{args[1]}")
         status = self.lib.drift_cache_read_chunks(
-            x_dtype, _ptr(k), _ptr(v), k.shape[0], cache.kv_heads, cache.head_dim, dtype, keys,
-            values, key_scales, value_scales, pages, page_size,
-            *self._check_chunks("cacheRead", chunks), self._stream())
+            x_dtype, k.data_ptr(), v.data_ptr(), k.shape[0], *args, *self._chunk_args(chunks),
+            self._stream())
         check("drift_cache_read_chunks", status)
 
     def attention_chunks(self, q, cache, chunks: Chunks, attention: Attention, out) -> None:
@@ -601,28 +618,26 @@ class CudaOps:
         the new ones included (written before): a decoding step, drafted
         tokens, prompts or pieces of them, of different lengths in one call.
         With a window, the first `attention.first` positions stay visible."""
-        x_dtype = self._check_rows("attention", cache, q, out)
-        tokens, q_heads, dim = q.shape
-        dtype, keys, values, key_scales, value_scales, pages, page_size = \
-            self._check_cache("attention", cache)
+        x_dtype = self._chunk_rows("attention", q, out, cache, chunks)
+        tokens, q_heads, _ = q.shape
+        args = self._cache_args("attention", cache)
+        kv_heads, dim, dtype, pages, page_size = args[0], args[1], args[2], args[7], args[8]
         sinks = attention.sinks
         if sinks is not None:
             _f32("attention sinks", sinks)
-            _require(tuple(sinks.shape) == (q_heads,),
+            _require(tuple(sinks.shape) == (q_heads,) and sinks.device == q.device,
                      f"attention: sinks {list(sinks.shape)} for {q_heads} heads")
-        window, first, longest = int(attention.window or 0), int(attention.first), int(chunks.longest)
-        chunk_args = self._check_chunks("attention", chunks)
-        max_keys = int(chunks.max_key_count)
+        window, causal = attention.window or 0, int(attention.causal)
+        chunk_args = self._chunk_args(chunks)
         size = self.lib.drift_attention_chunks_workspace_bytes(
-            x_dtype, tokens, q_heads, cache.kv_heads, dim, dtype, pages, page_size, chunk_args[4],
-            longest, max_keys, int(attention.causal), window, first)
+            x_dtype, tokens, q_heads, kv_heads, dim, dtype, pages, page_size, chunk_args[4],
+            chunk_args[5], chunks.max_key_count, causal, window, attention.first)
         # the call's own: freed to torch's allocator behind it in the stream
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         status = self.lib.drift_attention_chunks(
-            x_dtype, _ptr(q), tokens, q_heads, cache.kv_heads, dim, dtype, keys, values, key_scales,
-            value_scales, pages, page_size, *chunk_args, max_keys, attention.scale,
-            int(attention.causal), window, first, float(attention.softcap or 0.0), _ptr(sinks),
-            _ptr(out), _ptr(workspace), size, self._stream())
+            x_dtype, q.data_ptr(), tokens, q_heads, *args, *chunk_args, chunks.max_key_count,
+            attention.scale, causal, window, attention.first, attention.softcap or 0.0, _ptr(sinks),
+            out.data_ptr(), workspace.data_ptr() if size else None, size, self._stream())
         check("drift_attention_chunks", status)
 
     # -- SequenceOps: Gated DeltaNet (ops/SequenceOps.scala) --------------------------------------
