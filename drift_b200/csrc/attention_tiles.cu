@@ -66,6 +66,8 @@ constexpr uint32_t TMEM_COLUMNS = 512;
 // A weight is 2^WEIGHT_BITS at the row's largest score when its base is set,
 // and the base moves when one would pass 2^(WEIGHT_BITS + GROWTH_BITS).
 constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f;
+// Of eight pairs of BF16 rows' weights, those made by exp2_cubic.
+constexpr int CUBIC_PAIRS = 3;
 // A row of q is 2^Q_BITS and more at its largest value, so that its second
 // terms end far below F16's last bit, 2^-24.
 constexpr int Q_BITS = 8;
@@ -197,6 +199,61 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// The largest of three, a NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Pairs: one instruction for two F32 operations.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 2^x for x <= 15 on the multiply-add units, to 8e-5 (a sixth of F16's
+// rounding): x = n + f with |f| <= 1/2, by the F32 sum that has no room for a
+// fraction; a cubic in f (least squares on Chebyshev points, reweighted
+// towards the least largest relative error) and n added to its exponent. The
+// special function unit makes 16 values a clock and SM, the tensor core needs
+// a tile's 16384 in as many clocks as it takes to make them: a share of them
+// made here leaves the tensor core the one that is waited for.
+__device__ __forceinline__ float2 exp2_cubic(float2 x) {
+  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  const float2 whole = make_float2(12582912.0f, 12582912.0f);  // 1.5 x 2^23
+  const float2 t = add2(x, whole);
+  const float2 f = add2(x, mul2(add2(t, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f)));
+  float2 p = fma2(f, make_float2(0.05517164245247841f, 0.05517164245247841f), make_float2(0.2426111251115799f, 0.2426111251115799f));
+  p = fma2(f, p, make_float2(0.6932609677314758f, 0.6932609677314758f));
+  p = fma2(f, p, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(p.x)),
+                     __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
+}
+
 __device__ __forceinline__ uint32_t half_pair(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -285,7 +342,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   uint64_t* scales_full = v_empty + STAGES;
   uint64_t* s_full = scales_full + STAGES;  // [2]: of row tile i, or of buffer i
   uint64_t* p_full = s_full + 2;            // [2]
-  uint64_t* o_full = p_full + 2;            // [2]
+  uint64_t* p_half = p_full + 2;            // [2] (BF16 rows)
+  uint64_t* o_full = p_half + 2;            // [2]
   uint64_t* edge_found = o_full + 2;        // an edge tile's values are there; they are clean
   uint64_t* edge_clean = edge_found + 1;
   uint64_t* codes_full = edge_clean + 1;    // [2]: of the keys, of the values
@@ -303,6 +361,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_init(&q_full[i], ROW_TILE);
       tc::mbar_init(&s_full[i], 1);
       tc::mbar_init(&p_full[i], ROW_TILE);
+      tc::mbar_init(&p_half[i], ROW_TILE);
       tc::mbar_init(&o_full[i], 1);
     }
     for (int s = 0; s < STAGES; ++s) {
@@ -442,7 +501,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll
         for (int c = 0; c < KEYS; c += 4) {
           const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
-          s[c] *= x.x, s[c + 1] *= x.y, s[c + 2] *= x.z, s[c + 3] *= x.w;
+          const float2 u = mul2(make_float2(s[c], s[c + 1]), make_float2(x.x, x.y));
+          const float2 v = mul2(make_float2(s[c + 2], s[c + 3]), make_float2(x.z, x.w));
+          s[c] = u.x, s[c + 1] = u.y, s[c + 2] = v.x, s[c + 3] = v.y;
         }
       }
       if (a.softcap > 0.0f) {
@@ -457,10 +518,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         for (int c = 0; c < KEYS; ++c)
           if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
       }
-      float top = s[0];
+      float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 1; c < KEYS; ++c) top = fmaxf(top, s[c]);
-      top *= m2;
+      for (int c = 4; c < KEYS - 4; c += 8)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[KEYS - 4 + n]);
+      const float top = max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * m2;
       float shrink = 1.0f;
       if constexpr (CODES) {
         const float now = v_unit[stage];
@@ -492,33 +557,37 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           }
         }
       }
-      const float less = base2 == -INFINITY ? 0.0f : base2;
-      float part = 0.0f;  // (a tile's own sum: short chains)
+      // (a NaN makes the whole row NaNs)
+      const float less = top != top ? top : base2 == -INFINITY ? 0.0f : -base2;
+      float2 part = make_float2(0.0f, 0.0f);  // (a tile's own sum: short chains)
 #pragma unroll
       for (int c = 0; c < KEYS; c += 32) {
         uint32_t p[16], p_low[16];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          float w[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) w[n] = exp2_approx(fmaf(s[c + 2 * e + n], m2, -less));
-          part += (w[0] + w[1]) + (w[2] + w[3]);
+        for (int e = 0; e < 16; ++e) {
+          float2 w = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), make_float2(m2, m2), make_float2(less, less));
+          if (TERMS == 1 && e % 8 < CUBIC_PAIRS) w = exp2_cubic(w);
+          else w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
+          part = add2(part, w);
           if constexpr (CODES) {
-            const float4 x = *reinterpret_cast<const float4*>(v_scales + c + 2 * e);
-            w[0] *= x.x, w[1] *= x.y, w[2] *= x.z, w[3] *= x.w;
+            w = mul2(w, *reinterpret_cast<const float2*>(v_scales + c + 2 * e));
             if (edge) {  // (a hidden value's scale may be a NaN)
-#pragma unroll
-              for (int n = 0; n < 4; ++n) w[n] = s[c + 2 * e + n] == -INFINITY ? 0.0f : w[n];
+              w.x = s[c + 2 * e] == -INFINITY ? 0.0f : w.x;
+              w.y = s[c + 2 * e + 1] == -INFINITY ? 0.0f : w.y;
             }
           }
-          p[e] = half_pair(w[0], w[1]);
-          p[e + 1] = half_pair(w[2], w[3]);
-          if constexpr (TERMS == 2) p_low[e] = left_pair(w[0], w[1], p[e]), p_low[e + 1] = left_pair(w[2], w[3], p[e + 1]);
+          p[e] = half_pair(w.x, w.y);
+          if constexpr (TERMS == 2) p_low[e] = left_pair(w.x, w.y, p[e]);
         }
         tmem_store_16(s_at + c / 2, p);
         if constexpr (TERMS == 2) tmem_store_16(s_at + KEYS / 2 + c / 2, p_low);
+        if (TERMS == 1 && c + 32 == KEYS / 2) {  // the first half's products start
+          tc::tmem_store_wait();
+          tc::fence_before_sync();
+          tc::mbar_arrive(&p_half[b]);
+        }
       }
-      sum += part;
+      sum += part.x + part.y;
       tc::tmem_store_wait();
       tc::fence_before_sync();
       tc::mbar_arrive(&p_full[b]);
@@ -645,7 +714,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     // ---- tensor core --------------------------------------------------------------------
     constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
     const int run = CODES ? 64 : args.run;  // keys of a tile of V
-    const uint32_t run_steps = run / 16, run_bytes = uint32_t(run) * D * 2;
+    const uint32_t run_shift = run == 64 ? 2 : run == 32 ? 1 : 0, run_bytes = uint32_t(run) * D * 2;  // 2^shift steps
     bool ok = true;
     int edges = 0;
     // (second terms first, while the sums are small)
@@ -661,16 +730,28 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
       tc::mma_commit_warp(&s_full[b]);
     };
-    auto outputs = [&](int j, int i, int b) {
+    // (false if the weights did not come)
+    auto outputs = [&](int j, int i, int b, uint32_t phase) {
       const uint64_t v = operand_desc(base + T::V_AT + (j % STAGES) * T::V_STAGE, 2 * run);
+      if (TERMS == 1) {
+        if (!wait(&p_half[b], phase)) return false;
+      } else if (!wait(&p_full[b], phase)) {
+        return false;
+      }
+      tc::fence_after_sync();
 #pragma unroll
       for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
         for (int step = 0; step < KEYS / 16; ++step) {
-          const uint32_t at = step / run_steps * run_bytes + step % run_steps * 32;
+          if (TERMS == 1 && step == KEYS / 32) {
+            if (!wait(&p_full[b], phase)) return false;
+            tc::fence_after_sync();
+          }
+          const uint32_t at = (step >> run_shift) * run_bytes + (step & ((1u << run_shift) - 1)) * 32;
           tc::mma_f16_ts_warp(tmem + T::O_COLUMN + 128 * i, tmem + b * KEYS + term * KEYS / 2 + 8 * step, v + (at >> 4), pv,
                               (TERMS == 1 && j > 0) || term < TERMS - 1 || step > 0);
         }
+      return true;
     };
     auto keys_ready = [&](int j) { return wait(&k_full[j % STAGES], (j / STAGES) & 1); };
     auto values_ready = [&](int j) {
@@ -691,9 +772,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if constexpr (MT == 2) {
         for (int i = 0; i < 2 && ok; ++i) {
           if (i == 0 && !(ok = values_ready(j))) break;
-          if (!(ok = wait(&p_full[i], j & 1))) break;
-          tc::fence_after_sync();
-          outputs(j, i, i);
+          if (!(ok = outputs(j, i, i, j & 1))) break;
           if (i == 1) tc::mma_commit_warp(&v_empty[j % STAGES]);
           if (j + 1 == tiles) {
             tc::mma_commit_warp(&o_full[i]);
@@ -710,9 +789,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           tc::mma_commit_warp(&k_empty[(j + 1) % STAGES]);
         }
         if (!(ok = values_ready(j))) break;
-        if (!(ok = wait(&p_full[j & 1], (j >> 1) & 1))) break;
-        tc::fence_after_sync();
-        outputs(j, 0, j & 1);
+        if (!(ok = outputs(j, 0, j & 1, (j >> 1) & 1))) break;
         tc::mma_commit_warp(&v_empty[j % STAGES]);
         tc::mma_commit_warp(&o_full[0]);
       }
