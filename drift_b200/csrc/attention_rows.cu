@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
         for (int half = 0; half < 2; ++half) {
           const int key = key0 + w.position_of(m, half);
           if (key >= seen.end || (key < lowest && key >= first)) v_scale[m][half] = 0.0f;
-          top = fmaxf(top, v_scale[m][half]);
+          if (v_scale[m][half] <= 3.402823466e38f) top = fmaxf(top, v_scale[m][half]);  // (the finite ones)
         }
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

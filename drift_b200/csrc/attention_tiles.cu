@@ -5,7 +5,8 @@
 //
 //   S_i = Q_i K^T      (TMEM; Q and K in shared memory)
 //   P_i = e^(scale S_i - base)  over S_i's columns, as F16 (softmax warps: a
-//                       thread has a row, its base and its sum, in F32)
+//                       thread has a row, or half of one's columns, its base
+//                       and its sum, in F32)
 //   O_i (+)= P_i V     (TMEM; V^T in shared memory, as the cache has it)
 //
 // The F16 cache's layouts are the tensor core's own K-major operands -- keys
@@ -14,15 +15,22 @@
 // largest that divides the page): runs of keys are rows of the 128-byte
 // swizzled tile, and a run of values is a tile of its own, in the swizzle as
 // wide as the run. An 8-bit cache's codes come the same way into a buffer of
-// their own, from which converting warps write them as F16, exactly, into the
-// operands; a key's scale multiplies its scores, and a value's scale its
-// weights (over a power of two at or above every scale so far, so that a
-// weight stays in F16's range).
+// their own, from which converting warps write them as F16 into the operands:
+// for BF16 rows times their scales over a power of two (of the tile's keys; of
+// the values so far), each rounded to F16 like the weights; for F32 rows
+// exactly, and there a key's scale multiplies its scores, and a value's its
+// weights.
+//
+// A weight is at most 2^15 or the row's base moves: the sum of a tile's
+// weights tells, so that a tile's largest score is looked for only then (and
+// in the first tile, to set the base) -- the tile is read again, and what was
+// summed so far rescaled. Looking for it in every tile took 27 % of a tile's
+// softmax.
 //
 // BF16 rows (TERMS = 1): q is exact in F16 after a power of two per row; P's
-// rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). O stays in TMEM
-// and is rescaled only when a row's largest score has grown by 2^6 since the
-// last time (weights are at most 2^14 until then).
+// rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). O stays in TMEM.
+// Two threads share a row, half of a tile's columns each, since what a row
+// tile's softmax takes adds to what its products take before the next scores.
 // F32 rows (TERMS = 2): q and P are two F16 terms each (hi + lo, to 2^-22), the
 // products of both summed. The tensor core's F32 sums drop low bits as a chain
 // grows, so a tile's P V starts a new O, and the softmax threads add it to
@@ -33,11 +41,11 @@
 // outputs fill TMEM, and units of 128 rows) S has two buffers, and Q K^T of
 // the next tile runs under the softmax.
 //
-// Warps: 0-3 and 4-7 the softmax of row tiles 0 and 1, 8 the copies, 9 the
-// tensor core; then, for an F16 cache, 10 and 11 the edges: in a tile that
+// Warps: first the softmax, four for 128 rows (eight for BF16 rows); then one
+// for the copies, one for the tensor core, and two for the edges: in a tile that
 // some row sees only in part they take values that are not finite out of V,
 // since such a value times a zero weight would reach rows that do not see it
-// (they are added at the end, to the rows that do); for an 8-bit cache the
+// (they are added at the end, to the rows that do). An 8-bit cache has
 // converting warps. Every wait is bounded; one that gives up sets device error
 // 2, and the CTA drains its copies and products, frees its TMEM and returns.
 #include <cuda.h>
@@ -60,12 +68,11 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROW_TILE = 128;
-constexpr int COPY_WARP = 8, MMA_WARP = 9, EDGE_WARP = 10;
 constexpr int EDGE_THREADS = 64;
 constexpr uint32_t TMEM_COLUMNS = 512;
 // A weight is 2^WEIGHT_BITS at the row's largest score when its base is set,
-// and the base moves when one would pass 2^(WEIGHT_BITS + GROWTH_BITS).
-constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f;
+// and the base moves when a tile's weights sum to more than MOST_WEIGHT.
+constexpr float WEIGHT_BITS = 8.0f, MOST_WEIGHT = 32768.0f;
 // Of eight pairs of BF16 rows' weights, those made by exp2_cubic.
 constexpr int CUBIC_PAIRS = 3;
 // A row of q is 2^Q_BITS and more at its largest value, so that its second
@@ -77,17 +84,24 @@ struct TileTraits {
   static constexpr int D = D_, KEYS = KEYS_, MT = MT_, TERMS = TERMS_;
   static constexpr bool CODES = CODES_;
   static constexpr int UNIT = ROW_TILE * MT;
+  static constexpr int HALVES = TERMS == 1 ? 2 : 1;        // threads that share a row
+  static constexpr int COLUMNS = KEYS / HALVES;            // a thread's, of a tile's scores
+  static constexpr int SOFTMAX_WARPS = 4 * MT * HALVES;
+  static constexpr int COPY_WARP = SOFTMAX_WARPS, MMA_WARP = COPY_WARP + 1, EDGE_WARP = COPY_WARP + 2;
   // Converting 128 keys' codes for BF16 rows takes four warps, one to a
   // scheduler; for F32 rows, at half the keys in the same time, two. The
   // softmax warps take the registers that the others leave.
   static constexpr bool WIDE = CODES && TERMS == 1;
-  static constexpr int THREADS = WIDE ? 512 : 384;
-  static constexpr int CONVERT_WARP = WIDE ? 12 : 10;
-  static constexpr int CONVERT_THREADS = THREADS - 32 * CONVERT_WARP;
-  static constexpr int SOFTMAX_REGISTERS = TERMS == 2 ? 224 : WIDE ? 192 : 208;
-  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : WIDE ? 64 : 88;
-  static_assert(256 * SOFTMAX_REGISTERS + (THREADS - 256) * OTHER_REGISTERS <= THREADS * (65536 / THREADS / 8 * 8),
-                "what the block is launched with");
+  static constexpr int CONVERT_WARP = WIDE ? EDGE_WARP + 2 : EDGE_WARP;
+  static constexpr int CONVERT_THREADS = WIDE ? 128 : 64;
+  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4 + (WIDE ? 4 : 0));
+  static constexpr int LAUNCH_REGISTERS = 65536 / THREADS / 8 * 8 > 248 ? 248 : 65536 / THREADS / 8 * 8;
+  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : WIDE ? 64 : MT == 2 ? 64 : 88;
+  static constexpr int SHARE =
+      (THREADS * LAUNCH_REGISTERS - (THREADS - 32 * SOFTMAX_WARPS) * OTHER_REGISTERS) / (32 * SOFTMAX_WARPS) / 8 * 8;
+  static constexpr int SOFTMAX_REGISTERS = SHARE > 232 ? 232 : SHARE;
+  static constexpr bool MOVES_REGISTERS = THREADS > 256;  // (255 a thread are there otherwise)
+  static constexpr int ROUND_THREADS = 32 * SOFTMAX_WARPS + (CODES ? CONVERT_THREADS : EDGE_THREADS);
   static constexpr int PANELS = (D + 63) / 64;             // 64-column panels of a row
   static constexpr int Q_PANEL = ROW_TILE * 128;           // bytes
   static constexpr int Q_BYTES = PANELS * Q_PANEL;         // one term of one row tile
@@ -102,7 +116,8 @@ struct TileTraits {
   static constexpr int V_AT = K_AT + STAGES * K_BYTES;
   static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;
   static constexpr int SCALES_AT = CODES_AT + (CODES ? 2 * CODE_BYTES : 0);  // [STAGES][2][KEYS]
-  static constexpr int BARRIERS_AT = SCALES_AT + (CODES ? STAGES * 2 * KEYS * 4 : 0);
+  static constexpr int SHARED_AT = SCALES_AT + (CODES && TERMS == 2 ? STAGES * 2 * KEYS * 4 : 0);  // between halves
+  static constexpr int BARRIERS_AT = SHARED_AT + (HALVES == 2 ? MT * 2 * ROW_TILE * 4 : 0);
   static constexpr int BYTES = BARRIERS_AT + 320;
   static constexpr int O_COLUMN = 256;                     // S: columns 0 and KEYS; O: 256 and 384
   static_assert(MT == 1 || (D <= 128 && KEYS <= 128), "two outputs in TMEM");
@@ -173,6 +188,19 @@ __device__ __forceinline__ void tmem_load_32_async(uint32_t address, float* v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load_8(uint32_t address, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(address)
+               : "memory");
+  tmem_load_wait();
+}
+__device__ __forceinline__ void tmem_store_8(uint32_t address, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(address),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_load_16(uint32_t address, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
@@ -206,6 +234,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// Whether some thread of the 256 of a row tile has `any` (one answer for all;
+// and they meet).
+__device__ __forceinline__ bool any_of_tile(int tile, bool any) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+               "barrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(uint32_t(any)), "r"(3 + tile)
+               : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void meet_tile(int tile) { asm volatile("bar.sync %0, 256;" ::"r"(5 + tile) : "memory"); }
+
 // Pairs: one instruction for two F32 operations.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -235,7 +276,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-// 2^x for x <= 15 on the multiply-add units, to 8e-5 (a sixth of F16's
+// 2^x for |x| <= 126 (beyond: 2^-126, 2^126) on the multiply-add units, to 8e-5 (a sixth of F16's
 // rounding): x = n + f with |f| <= 1/2, by the F32 sum that has no room for a
 // fraction; a cubic in f (least squares on Chebyshev points, reweighted
 // towards the least largest relative error) and n added to its exponent. The
@@ -243,7 +284,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // a tile's 16384 in as many clocks as it takes to make them: a share of them
 // made here leaves the tensor core the one that is waited for.
 __device__ __forceinline__ float2 exp2_cubic(float2 x) {
-  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  x.x = fminf(fmaxf(x.x, -126.0f), 126.0f), x.y = fminf(fmaxf(x.y, -126.0f), 126.0f);
   const float2 whole = make_float2(12582912.0f, 12582912.0f);  // 1.5 x 2^23
   const float2 t = add2(x, whole);
   const float2 f = add2(x, mul2(add2(t, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f)));
@@ -301,6 +342,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                        const TileArgs args) {
   constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
   constexpr bool CODES = T::CODES;
+  constexpr int HALVES = T::HALVES, COLUMNS = T::COLUMNS;
   using X = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
@@ -342,8 +384,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   uint64_t* scales_full = v_empty + STAGES;
   uint64_t* s_full = scales_full + STAGES;  // [2]: of row tile i, or of buffer i
   uint64_t* p_full = s_full + 2;            // [2]
-  uint64_t* p_half = p_full + 2;            // [2] (BF16 rows)
-  uint64_t* o_full = p_half + 2;            // [2]
+  uint64_t* o_full = p_full + 2;            // [2]
   uint64_t* edge_found = o_full + 2;        // an edge tile's values are there; they are clean
   uint64_t* edge_clean = edge_found + 1;
   uint64_t* codes_full = edge_clean + 1;    // [2]: of the keys, of the values
@@ -353,15 +394,17 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* taken_out = abort + 1;
   volatile int* copied = abort + 2;         // [2]: tiles whose keys, values were asked for
-  volatile float* v_unit = reinterpret_cast<volatile float*>(abort + 4);  // [STAGES]: the scales' power of two
+  volatile int* failed = abort + 4;         // [2][2]: a wait of row tile i gave up, in an even or odd tile
+  volatile float* k_unit = reinterpret_cast<volatile float*>(abort + 8);  // [STAGES]: the scales' powers of two
+  volatile float* v_unit = k_unit + STAGES;
+  volatile float* between = reinterpret_cast<volatile float*>(shared + T::SHARED_AT);  // [MT][2][ROW_TILE]
   float* scales = reinterpret_cast<float*>(shared + T::SCALES_AT);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&q_full[i], ROW_TILE);
+      tc::mbar_init(&q_full[i], ROW_TILE * HALVES);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&p_full[i], ROW_TILE);
-      tc::mbar_init(&p_half[i], ROW_TILE);
+      tc::mbar_init(&p_full[i], ROW_TILE * HALVES);
       tc::mbar_init(&o_full[i], 1);
     }
     for (int s = 0; s < STAGES; ++s) {
@@ -379,6 +422,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     *abort = 0;
     *taken_out = 0;
     copied[0] = copied[1] = 0;
+    failed[0] = failed[1] = failed[2] = failed[3] = 0;
     tc::fence_barrier_init();
   }
   __syncwarp();
@@ -388,13 +432,15 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return tc::mbar_wait_warp(bar, parity, abort, a.error); };
 
-  // (warpgroups 0 and 1: warps 0-7)
-  if (warp < 4 * MT) more_registers<T::SOFTMAX_REGISTERS>();
-  else fewer_registers<T::OTHER_REGISTERS>();
+  if constexpr (T::MOVES_REGISTERS) {
+    if (warp < T::SOFTMAX_WARPS) more_registers<T::SOFTMAX_REGISTERS>();
+    else fewer_registers<T::OTHER_REGISTERS>();
+  }
 
-  if (warp < 4 * MT) {
-    // ---- softmax: this thread's row of row tile i --------------------------------------
-    const int i = warp / 4, r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
+  if (warp < T::SOFTMAX_WARPS) {
+    // ---- softmax: this thread's row of row tile i, columns [COLUMNS half, + COLUMNS) of a tile ----
+    const int i = warp / (4 * HALVES), half = HALVES == 2 ? warp / 4 % 2 : 0;
+    const int r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
     const bool real = row < row1;
     const int token = (real ? row : row1 - 1) / a.group, q_head = head * a.group + row % a.group;
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
@@ -431,7 +477,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
       multiplier = fabsf(a.scale) * __uint_as_float(exponent);
       uint8_t* panel = shared + i * TERMS * T::Q_BYTES + r * 128;
-      for (int c = 0; c < T::PANELS * 8; ++c) {
+      for (int c = half * (T::PANELS * 8 / HALVES); c < (half + 1) * (T::PANELS * 8 / HALVES); ++c) {
         uint4 hi = make_uint4(0, 0, 0, 0), low = hi;
         if (real && c < D / 8) {
           load(c);
@@ -450,7 +496,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_arrive(&q_full[i]);
     }
     // (a softcap leaves natural units behind)
-    const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 1.2e-38f);
+    // (and a factor of 2^-60 is as good as none; times a tile's power it is normal)
+    const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 8.7e-19f);
     const int position = chunk.position + token;
     const int hi = a.causal ? position + 1 : seen.end;
     const int lo = a.window > 0 ? position - a.window + 1 : 0;
@@ -459,6 +506,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int tile_end = a.causal ? chunk.position + (row0 + ROW_TILE * i) / a.group + 1 : seen.end;
     const int tile_low = a.window > 0 ? chunk.position + max(last, 0) / a.group - a.window + 1 : 0;
     const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
+
+    constexpr int OWN = D / HALVES;  // this thread's dimensions of the output
+    const int d0 = half * OWN;
 
     float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
     float unit = 0.0f;                    // and, for codes, values are over this
@@ -471,7 +521,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           float o[16];
           tmem_load_16(o_at + c, o);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) total[c + e] += o[e];
+          for (int e = 0; e < 16; e += 2) {
+            const float2 x = add2(make_float2(total[c + e], total[c + e + 1]), make_float2(o[e], o[e + 1]));
+            total[c + e] = x.x, total[c + e + 1] = x.y;
+          }
         }
       }
     };
@@ -479,127 +532,156 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     for (int j = 0; j < tiles; ++j) {
       const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
       const uint32_t phase = MT == 2 ? j & 1 : (j >> 1) & 1;
-      if (!(ok = wait(&s_full[b], phase))) break;
-      if (CODES && !(ok = wait(&scales_full[stage], (j / STAGES) & 1))) break;
+      // (the threads of a row tile leave the loop together: they meet in it)
+      ok = ok && wait(&s_full[b], phase);
+      if (CODES) ok = ok && wait(&scales_full[stage], (j / STAGES) & 1);
       // O holds the tile before this one, or every one: with two row tiles
       // that P V came before this S; with one it is waited for
-      if (TERMS == 2 && j > 0) {
-        if (MT == 1 && !(ok = wait(&o_full[0], (j - 1) & 1))) break;
+      if (TERMS == 2 && j > 0 && ok) {
+        if (MT == 1) ok = wait(&o_full[0], (j - 1) & 1);
         tc::fence_after_sync();
-        take_output();
+        if (ok) take_output();
       }
+      if (HALVES == 1 && !ok) break;
       tc::fence_after_sync();
       const uint32_t s_at = tmem + lanes + b * KEYS;
-      float s[KEYS];
-#pragma unroll
-      for (int c = 0; c < KEYS; c += 32) tmem_load_32_async(s_at + c, s + c);
-      tmem_load_wait();
-      const int key0 = seen.key_of(tile0 + j);
+      const int key0 = seen.key_of(tile0 + j), own_key0 = key0 + half * COLUMNS;
       const float* k_scales = scales + stage * 2 * KEYS;
       const float* v_scales = k_scales + KEYS;
-      if constexpr (CODES) {
-#pragma unroll
-        for (int c = 0; c < KEYS; c += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
-          const float2 u = mul2(make_float2(s[c], s[c + 1]), make_float2(x.x, x.y));
-          const float2 v = mul2(make_float2(s[c + 2], s[c + 3]), make_float2(x.z, x.w));
-          s[c] = u.x, s[c + 1] = u.y, s[c + 2] = v.x, s[c + 3] = v.y;
-        }
-      }
-      if (a.softcap > 0.0f) {
-        const float inverse = multiplier / a.softcap;
-#pragma unroll
-        for (int c = 0; c < KEYS; ++c) s[c] = capped(s[c], inverse, a.softcap);
-      }
       const bool edge = !(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first));
-      if (edge) {
-        const int end = hi - key0, low = lo - key0, head_end = first - key0;
+      const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : 1.0f;
+      const float tile_m2 = a.softcap > 0.0f ? m2 : m2 * by_unit;
+      const float now_unit = CODES ? float(v_unit[stage]) : 0.0f;
+      bool slow = j == 0;  // (the same for a row tile's threads)
+      uint32_t p[COLUMNS / 2], p_low[TERMS == 2 ? COLUMNS / 2 : 1];
+      float part;
+#pragma unroll 1
+      for (;;) {
+        float s[COLUMNS];
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c)
-          if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
-      }
-      float tops[4] = {s[0], s[1], s[2], s[3]};
+        for (int c = 0; c < COLUMNS; c += 32) tmem_load_32_async(s_at + half * COLUMNS + c, s + c);
+        tmem_load_wait();
+        if constexpr (CODES && TERMS == 2) {
 #pragma unroll
-      for (int c = 4; c < KEYS - 4; c += 8)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
-#pragma unroll
-      for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[KEYS - 4 + n]);
-      const float top = max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * m2;
-      float shrink = 1.0f;
-      if constexpr (CODES) {
-        const float now = v_unit[stage];
-        if (now > unit) {
-          shrink = unit / now;
-          unit = now;
-        }
-      }
-      const bool grown = top > base2 + (WEIGHT_BITS + GROWTH_BITS) || shrink != 1.0f;
-      if (__any_sync(0xffffffffu, grown)) {
-        const float now = fmaxf(base2, top - WEIGHT_BITS);
-        const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
-        base2 = now;
-        sum *= f;
-        const float g = f * shrink;
-        if constexpr (TERMS == 2) {
-#pragma unroll
-          for (int c = 0; c < D; ++c) total[c] *= g;
-        } else if (j > 0) {
-          if (MT == 1 && !(ok = wait(&o_full[0], (j - 1) & 1))) break;
-          tc::fence_after_sync();
-#pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            float o[16];
-            tmem_load_16(o_at + c, o);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] *= g;
-            tmem_store_16(o_at + c, reinterpret_cast<const uint32_t*>(o));
+          for (int c = 0; c < COLUMNS; c += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
+            const float2 u = mul2(make_float2(s[c], s[c + 1]), make_float2(x.x, x.y));
+            const float2 v = mul2(make_float2(s[c + 2], s[c + 3]), make_float2(x.z, x.w));
+            s[c] = u.x, s[c + 1] = u.y, s[c + 2] = v.x, s[c + 3] = v.y;
           }
         }
-      }
-      // (a NaN makes the whole row NaNs)
-      const float less = top != top ? top : base2 == -INFINITY ? 0.0f : -base2;
-      float2 part = make_float2(0.0f, 0.0f);  // (a tile's own sum: short chains)
+        if (a.softcap > 0.0f) {
+          const float inverse = multiplier * by_unit / a.softcap;
 #pragma unroll
-      for (int c = 0; c < KEYS; c += 32) {
-        uint32_t p[16], p_low[16];
+          for (int c = 0; c < COLUMNS; ++c) s[c] = capped(s[c], inverse, a.softcap);
+        }
+        if (edge) {
+          const int end = hi - own_key0, low = lo - own_key0, head_end = first - own_key0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 w = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), make_float2(m2, m2), make_float2(less, less));
+          for (int c = 0; c < COLUMNS; ++c)
+            if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
+        }
+        bool not_a_number = false;
+        if (slow) {
+          float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int c = 4; c < COLUMNS - 4; c += 8)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[COLUMNS - 4 + n]);
+          float top = max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * tile_m2;
+          if constexpr (HALVES == 2) {
+            volatile float* shared_top = between + 2 * ROW_TILE * i + r;
+            shared_top[ROW_TILE * half] = top;
+            meet_tile(i);
+            top = max3(top, top, shared_top[ROW_TILE * (1 - half)]);
+          }
+          not_a_number = top != top;
+          // (a row without a base takes one; a base that is too high stays)
+          const float now = fmaxf(base2, top - WEIGHT_BITS);
+          const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
+          const float g = CODES && now_unit > unit ? f * (unit / now_unit) : f;
+          if (CODES) unit = fmaxf(unit, now_unit);
+          base2 = now;
+          sum *= f;
+          if constexpr (TERMS == 2) {
+#pragma unroll
+            for (int c = 0; c < D; ++c) total[c] *= g;
+          } else if (j > 0 && ok) {
+            if (MT == 1) ok = wait(&o_full[0], (j - 1) & 1);
+            if (ok) {
+              tc::fence_after_sync();
+#pragma unroll 1
+              for (int c = 0; c < OWN; c += 8) {
+                float o[8];
+                tmem_load_8(o_at + d0 + c, o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] *= g;
+                tmem_store_8(o_at + d0 + c, reinterpret_cast<const uint32_t*>(o));
+              }
+            }
+          }
+        }
+        // (a NaN makes the whole row NaNs)
+        const float less = not_a_number ? __int_as_float(0x7fc00000) : slow && base2 == -INFINITY ? 0.0f : -base2;
+        float2 parts = make_float2(0.0f, 0.0f);  // (a tile's own sum: short chains)
+#pragma unroll
+        for (int e = 0; e < COLUMNS / 2; ++e) {
+          float2 w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
           if (TERMS == 1 && e % 8 < CUBIC_PAIRS) w = exp2_cubic(w);
           else w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
-          part = add2(part, w);
-          if constexpr (CODES) {
-            w = mul2(w, *reinterpret_cast<const float2*>(v_scales + c + 2 * e));
+          parts = add2(parts, w);
+          if constexpr (CODES && TERMS == 2) {
+            w = mul2(w, *reinterpret_cast<const float2*>(v_scales + 2 * e));
             if (edge) {  // (a hidden value's scale may be a NaN)
-              w.x = s[c + 2 * e] == -INFINITY ? 0.0f : w.x;
-              w.y = s[c + 2 * e + 1] == -INFINITY ? 0.0f : w.y;
+              w.x = s[2 * e] == -INFINITY ? 0.0f : w.x;
+              w.y = s[2 * e + 1] == -INFINITY ? 0.0f : w.y;
             }
           }
           p[e] = half_pair(w.x, w.y);
           if constexpr (TERMS == 2) p_low[e] = left_pair(w.x, w.y, p[e]);
         }
-        tmem_store_16(s_at + c / 2, p);
-        if constexpr (TERMS == 2) tmem_store_16(s_at + KEYS / 2 + c / 2, p_low);
-        if (TERMS == 1 && c + 32 == KEYS / 2) {  // the first half's products start
-          tc::tmem_store_wait();
-          tc::fence_before_sync();
-          tc::mbar_arrive(&p_half[b]);
+        part = parts.x + parts.y;
+        if (slow) break;
+        const bool over = !(part <= MOST_WEIGHT) || (CODES && now_unit > unit);
+        if constexpr (HALVES == 2) {
+          if (!ok) failed[2 * i + j % 2] = 1;
+          if (!any_of_tile(i, over || !ok)) break;
+          if (failed[2 * i + j % 2]) break;
+        } else if (!__any_sync(0xffffffffu, over)) {
+          break;
         }
+        slow = true;
       }
-      sum += part.x + part.y;
+      // (only a tile that was met in has an answer for all: one that is taken
+      // slowly from the start is told by the next)
+      if (HALVES == 2 && failed[2 * i + j % 2] && !slow) break;
+      sum += part;
+#pragma unroll
+      for (int c = 0; c < COLUMNS / 2; c += 16) {
+        tmem_store_16(s_at + half * (COLUMNS / 2) + c, p + c);
+        if constexpr (TERMS == 2) tmem_store_16(s_at + KEYS / 2 + c, p_low + c);
+      }
       tc::tmem_store_wait();
       tc::fence_before_sync();
       tc::mbar_arrive(&p_full[b]);
     }
-    if (ok) ok = wait(&o_full[i], MT == 2 ? 0 : (tiles - 1) & 1);
-    if constexpr (!CODES) asm volatile("bar.sync 1, %0;" ::"n"(4 * 32 * MT + EDGE_THREADS) : "memory");  // (taken_out is final)
+    ok = ok && wait(&o_full[i], MT == 2 ? 0 : (tiles - 1) & 1);
+    float all_sum = sum;
+    if constexpr (HALVES == 2) {
+      volatile float* shared_sum = between + 2 * ROW_TILE * i + r;
+      meet_tile(i);  // (past the last exchange)
+      shared_sum[ROW_TILE * half] = sum;
+      meet_tile(i);
+      all_sum = sum + shared_sum[ROW_TILE * (1 - half)];
+    }
+    if constexpr (!(CODES && TERMS == 2)) asm volatile("bar.sync 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");  // (taken_out is final)
     if (ok) {
       tc::fence_after_sync();
       take_output();
       float scale = CODES ? unit : 1.0f;
       if (!a.part_o) {
-        float all_sum = sum;
         if (a.sinks) {
           // the sink's weight in the row's units, or the row's in the sink's
           const float sink = a.sinks[q_head] * LOG2E, all = fmaxf(base2, sink);
@@ -608,58 +690,65 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           scale *= f;
         }
         scale = all_sum != 0.0f ? scale / all_sum : 0.0f;
-      } else if (real) {
-        *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, sum);
+      } else if (real && half == 0) {
+        *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, all_sum);
       }
-      auto put = [&](int c, float (&o)[16]) {
+      // dimensions c .. c + 7 of the row
+      auto put = [&](int c, float (&o)[8]) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] *= scale;
-        if (!CODES && *taken_out) {
+        for (int e = 0; e < 8; ++e) o[e] *= scale;
+        if (!(CODES && TERMS == 2) && *taken_out) {
           for (int j = 0; j < tiles; ++j) {
             const int key0 = seen.key_of(tile0 + j);
             if (whole(key0)) continue;
+            const int end = min(key0 + KEYS, hi);
+            if constexpr (CODES) {
+              const float y = not_finite_scale(a.value_scales + (long long)head * a.at.page_size, (long long)a.kv_heads * a.at.page_size,
+                                               chunk.table, a.at.pages, a.at.page_size, key0, end, lo, first);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + c + e) * a.at.page_size,
-                                          (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
-                                          a.at.page_size, key0, min(key0 + KEYS, hi), lo, first);
-              o[e] += y.x, o[e + 1] += y.y, o[e + 2] += y.z, o[e + 3] += y.w;
+              for (int e = 0; e < 8; ++e) o[e] += y;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; e += 4) {
+                const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + c + e) * a.at.page_size,
+                                            (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
+                                            a.at.page_size, key0, end, lo, first);
+                o[e] += y.x, o[e + 1] += y.y, o[e + 2] += y.z, o[e + 3] += y.w;
+              }
             }
           }
         }
         if (a.part_o || TERMS == 2) {
           float4* to = reinterpret_cast<float4*>(a.part_o ? a.part_o + (row_at * a.splits + split) * D + c
                                                           : static_cast<float*>(a.out) + row_at * D + c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          to[0] = make_float4(o[0], o[1], o[2], o[3]);
+          to[1] = make_float4(o[4], o[5], o[6], o[7]);
         } else {
-          __align__(16) __nv_bfloat162 y[8];
+          __align__(16) __nv_bfloat162 y[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
-          uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row_at * D + c);
-          to[0] = reinterpret_cast<const uint4*>(y)[0];
-          to[1] = reinterpret_cast<const uint4*>(y)[1];
+          for (int e = 0; e < 4; ++e) y[e] = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row_at * D + c) = *reinterpret_cast<const uint4*>(y);
         }
       };
       if constexpr (TERMS == 2) {
 #pragma unroll
-        for (int c = 0; c < D; c += 16) {
-          float o[16];
+        for (int c = 0; c < D; c += 8) {
+          float o[8];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = total[c + e];
+          for (int e = 0; e < 8; ++e) o[e] = total[c + e];
           if (real) put(c, o);
         }
       } else {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          float o[16];
+        for (int c = 0; c < OWN; c += 8) {
+          float o[8];
           __syncwarp();
-          tmem_load_16(o_at + c, o);
-          if (real) put(c, o);
+          tmem_load_8(o_at + d0 + c, o);
+          if (real) put(d0 + c, o);
         }
       }
     }
-  } else if (warp == COPY_WARP) {
+  } else if (warp == T::COPY_WARP) {
     // ---- copies: a lane per run of a tile's keys, then of its values --------------------
     const int run = args.run, runs = KEYS / run;
     bool ok = true;
@@ -710,7 +799,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                     &value_map, full, place, v_row);
       __syncwarp();
     }
-  } else if (warp == MMA_WARP) {
+  } else if (warp == T::MMA_WARP) {
     // ---- tensor core --------------------------------------------------------------------
     constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
     const int run = CODES ? 64 : args.run;  // keys of a tile of V
@@ -733,20 +822,12 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     // (false if the weights did not come)
     auto outputs = [&](int j, int i, int b, uint32_t phase) {
       const uint64_t v = operand_desc(base + T::V_AT + (j % STAGES) * T::V_STAGE, 2 * run);
-      if (TERMS == 1) {
-        if (!wait(&p_half[b], phase)) return false;
-      } else if (!wait(&p_full[b], phase)) {
-        return false;
-      }
+      if (!wait(&p_full[b], phase)) return false;
       tc::fence_after_sync();
 #pragma unroll
       for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
         for (int step = 0; step < KEYS / 16; ++step) {
-          if (TERMS == 1 && step == KEYS / 32) {
-            if (!wait(&p_full[b], phase)) return false;
-            tc::fence_after_sync();
-          }
           const uint32_t at = (step >> run_shift) * run_bytes + (step & ((1u << run_shift) - 1)) * 32;
           tc::mma_f16_ts_warp(tmem + T::O_COLUMN + 128 * i, tmem + b * KEYS + term * KEYS / 2 + 8 * step, v + (at >> 4), pv,
                               (TERMS == 1 && j > 0) || term < TERMS - 1 || step > 0);
@@ -796,46 +877,93 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
   } else if (CODES && warp >= T::CONVERT_WARP) {
     // ---- conversion: codes to F16 operands, and the tile's scales ------------------------
+    constexpr int N = T::CONVERT_THREADS, CHUNKS = D / 16;  // 16-byte chunks of a key's codes
     const int t = tid - 32 * T::CONVERT_WARP;
     const int run = args.run;
     const uint8_t* k_codes = shared + T::CODES_AT;
     const uint8_t* v_codes = k_codes + T::CODE_BYTES;
-    // the scales of tile j, zeros where no row sees the key: key t's of the
-    // keys, and of the values those of every 32nd from this lane's (each warp
-    // finds the largest for itself)
+    auto seen_key = [&](int key) { return key < seen.end && (key >= lowest || key < first); };
+    // where the scales of the sixteen keys around `key` are, or -1
+    auto scales_at = [&](int key) {
+      const int page = key < seen.end ? chunk.table[key / a.at.page_size] : -1;
+      if (page < 0 || page >= a.at.pages) return -1ll;
+      return ((long long)page * a.kv_heads + head) * a.at.page_size + key % a.at.page_size;
+    };
+    // the scales of tile j, of every 32nd key from this lane's, zeros where no
+    // row sees the key (each warp finds the largest for itself)
     constexpr int PER = KEYS / 32;
-    auto load_scales = [&](int j, float& k, float (&v)[PER]) {
-      k = 0.0f;
+    auto load_scales = [&](int j, float (&k)[PER], float (&v)[PER]) {
+      const int key0 = seen.key_of(tile0 + j);
 #pragma unroll
       for (int n = 0; n < PER; ++n) {
-        v[n] = 0.0f;
-        const int key = seen.key_of(tile0 + j) + lane + 32 * n;
-        if (key >= seen.end || (key < lowest && key >= first)) continue;
-        const int page = chunk.table[key / a.at.page_size];
-        if (page < 0 || page >= a.at.pages) continue;
-        const long long at = ((long long)page * a.kv_heads + head) * a.at.page_size + key % a.at.page_size;
+        k[n] = v[n] = 0.0f;
+        const int key = key0 + lane + 32 * n;
+        if (!seen_key(key)) continue;
+        const long long at = scales_at(key);
+        if (at < 0) continue;
+        k[n] = a.key_scales[at];
         v[n] = a.value_scales[at];
-        if (n == t / 32) k = a.key_scales[at];
       }
     };
-    float k_scale, v_scale[PER], power = 0.0f;
+    auto largest_of = [](const float (&x)[PER]) {  // of those that are finite
+      float most = 0.0f;
+#pragma unroll
+      for (int n = 0; n < PER; ++n) most = x[n] <= 3.402823466e38f ? fmaxf(most, x[n]) : most;
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      return most;
+    };
+    // a power of two at or above x, `least` (in exponent bits) at least, whose
+    // inverse is normal
+    auto power_over = [](float x, uint32_t least) {
+      const uint32_t bits = __float_as_uint(x);
+      const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
+      return __uint_as_float(max(up, least));
+    };
+    float k_scale[PER], v_scale[PER], v_power = 0.0f;
     load_scales(0, k_scale, v_scale);
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      const int stage = j % STAGES;
+      const int stage = j % STAGES, key0 = seen.key_of(tile0 + j);
       const uint32_t used = ((j / STAGES) & 1) ^ 1;
-      // keys
+      // keys: a thread takes a row (or, of 64 rows, half of one)
+      const int row = t % KEYS;
+      float own_k = k_scale[0], own_v = v_scale[0];
+#pragma unroll
+      for (int n = 1; n < PER; ++n) {
+        own_k = n == row / 32 ? k_scale[n] : own_k;
+        own_v = n == row / 32 ? v_scale[n] : own_v;
+      }
+      // (2^-64 at least: the scores' factor stays normal with it)
+      const float k_power = power_over(largest_of(k_scale), 0x1f800000u);
       if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
       if (!(ok = wait(&codes_full[0], j & 1))) break;
-      uint8_t* k = shared + T::K_AT + stage * T::K_BYTES;
+      {
+        uint8_t* k = shared + T::K_AT + stage * T::K_BYTES + row * 128;
+        constexpr int TAKES = KEYS * CHUNKS / N;  // chunks a thread takes
+        const int c0 = t / KEYS * TAKES;
+        // the scale over the tile's power of two in two F16 terms
+        const float ratio = own_k * (1.0f / k_power);
+        const __half ratio_hi = __float2half_rn(ratio);
+        const __half2 hi = __half2half2(ratio_hi), low = __half2half2(__float2half_rn(ratio - __half2float(ratio_hi)));
+        auto scaled = [&](uint32_t pair) {
+          if constexpr (TERMS == 2) return pair;
+          const __half2 x = *reinterpret_cast<const __half2*>(&pair);
+          const __half2 y = __hfma2(x, hi, __hmul2(x, low));
+          return *reinterpret_cast<const uint32_t*>(&y);
+        };
 #pragma unroll 4
-      for (int n = t; n < KEYS * D / 16; n += T::CONVERT_THREADS) {
-        const int row = n / (D / 16), c = n % (D / 16);
-        const uint4 x = *reinterpret_cast<const uint4*>(k_codes + 16 * n);
-        const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
-        uint8_t* to = k + c / 4 * T::K_PANEL + row * 128;
-        *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4)) ^ (row % 8))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
-        *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4) + 1) ^ (row % 8))) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+        for (int n = 0; n < TAKES; ++n) {
+          // (each eight lanes' chunks on different banks)
+          const int c = c0 + (TAKES % 8 == 0 ? (n + t) % TAKES : TAKES == 4 ? (n + t / 2) % 4 : n);
+          const uint4 x = *reinterpret_cast<const uint4*>(k_codes + row * D + 16 * c);
+          const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
+          uint8_t* to = k + c / 4 * T::K_PANEL;
+          *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4)) ^ (row % 8))) =
+              make_uint4(scaled(y0.x), scaled(y0.y), scaled(y1.x), scaled(y1.y));
+          *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4) + 1) ^ (row % 8))) =
+              make_uint4(scaled(y2.x), scaled(y2.y), scaled(y3.x), scaled(y3.y));
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&k_full[stage]);
@@ -843,46 +971,70 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       // scales: the stage's were last read by the softmax before the P V that
       // freed its values
       if (j >= STAGES && !(ok = wait(&v_empty[stage], used))) break;
-      float most = 0.0f;  // (fmaxf passes NaNs over)
-#pragma unroll
-      for (int n = 0; n < PER; ++n) most = fmaxf(most, v_scale[n]);
-#pragma unroll
-      for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (most > power) {
-        // a power of two at or above it whose inverse is normal
-        const uint32_t bits = __float_as_uint(most);
-        const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-        power = __uint_as_float(max(up, 0x01000000u));
+      const float most = largest_of(v_scale);
+      if (most > v_power) v_power = power_over(most, 0x01000000u);
+      const float v_inverse = 1.0f / (v_power > 0.0f ? v_power : 1.0f);
+      if (TERMS == 2) {
+        scales[stage * 2 * KEYS + row] = own_k;
+        scales[stage * 2 * KEYS + KEYS + row] = own_v * v_inverse;
       }
-      if (t < KEYS) {
-        float own = v_scale[0];
-#pragma unroll
-        for (int n = 1; n < PER; ++n) own = n == t / 32 ? v_scale[n] : own;
-        scales[stage * 2 * KEYS + t] = k_scale;
-        scales[stage * 2 * KEYS + KEYS + t] = power > 0.0f ? own * (1.0f / power) : own;
-      }
-      if (t == 0) v_unit[stage] = power;
+      if (t == 0) k_unit[stage] = k_power, v_unit[stage] = v_power;
       tc::mbar_arrive(&scales_full[stage]);
       if (j + 1 < tiles) load_scales(j + 1, k_scale, v_scale);
-      // values: sixteen positions of a dimension
+      // values: a thread takes sixteen positions of every (DIMS)th dimension
+      constexpr int DIMS = N / (KEYS / 16);
+      const int per = run / 16;
+      const int group = t % per + per * (t / (DIMS * per)), first_d = t / per % DIMS;
+      __half2 ratios[8];
+      if constexpr (TERMS == 1) {
+        const int key = key0 + 16 * group;
+        const long long at = scales_at(key);
+        const bool check = !whole(key0);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (at >= 0) x = *reinterpret_cast<const float4*>(a.value_scales + at + 4 * n);
+          float y[4] = {x.x, x.y, x.z, x.w};
+          if (check) {
+            // (at an edge, what is not finite is taken out for the rows that
+            // do not see it)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (!seen_key(key + 4 * n + e)) y[e] = 0.0f;
+              else if (!isfinite(y[e])) y[e] = 0.0f, *taken_out = 1;
+            }
+          }
+          ratios[2 * n] = __floats2half2_rn(y[0] * v_inverse, y[1] * v_inverse);
+          ratios[2 * n + 1] = __floats2half2_rn(y[2] * v_inverse, y[3] * v_inverse);
+        }
+      }
       if (!(ok = wait(&codes_full[1], j & 1))) break;
-      uint8_t* v = shared + T::V_AT + stage * T::V_STAGE;
+      {
+        uint8_t* v = shared + T::V_AT + stage * T::V_STAGE + group / 4 * (D * 128);
+        const uint8_t* from = v_codes + group / per * (run * D) + group % per * 16;
+        auto scaled = [&](uint32_t pair, int n) {
+          if constexpr (TERMS == 2) return pair;
+          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), ratios[n]);
+          return *reinterpret_cast<const uint32_t*>(&y);
+        };
 #pragma unroll 4
-      for (int n = t; n < KEYS * D / 16; n += T::CONVERT_THREADS) {
-        const int in_run = 16 * n % (run * D), d = in_run / run;
-        const int place = 16 * n / (run * D) * run + in_run % run;
-        const uint4 x = *reinterpret_cast<const uint4*>(v_codes + 16 * n);
-        const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
-        uint8_t* to = v + place / 64 * (D * 128) + d * 128;
-        const int c = place % 64 / 8;
-        *reinterpret_cast<uint4*>(to + 16 * (c ^ (d % 8))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
-        *reinterpret_cast<uint4*>(to + 16 * ((c + 1) ^ (d % 8))) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+        for (int d = first_d; d < D; d += DIMS) {
+          const uint4 x = *reinterpret_cast<const uint4*>(from + d * run);
+          const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
+          uint8_t* to = v + d * 128;
+          const int c = 2 * (group % 4);
+          *reinterpret_cast<uint4*>(to + 16 * (c ^ (d % 8))) =
+              make_uint4(scaled(y0.x, 0), scaled(y0.y, 1), scaled(y1.x, 2), scaled(y1.y, 3));
+          *reinterpret_cast<uint4*>(to + 16 * ((c + 1) ^ (d % 8))) =
+              make_uint4(scaled(y2.x, 4), scaled(y2.y, 5), scaled(y3.x, 6), scaled(y3.y, 7));
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&v_full[stage]);
       tc::mbar_arrive(&codes_empty[1]);
     }
-  } else if (!CODES && warp >= EDGE_WARP) {
+    if constexpr (TERMS == 1) asm volatile("bar.arrive 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");
+  } else if (!CODES && warp >= T::EDGE_WARP) {
     // ---- edges: values that are not finite, out of the tiles seen in part -----------------
     bool ok = true;
     int edges = 0;
@@ -894,7 +1046,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (!(ok = wait(&v_full[j % STAGES], (j / STAGES) & 1))) break;
       uint8_t* v = shared + T::V_AT + (j % STAGES) * T::V_STAGE;
       bool found = false;
-      for (int n = tid - 32 * EDGE_WARP; n < T::V_BYTES / 16; n += EDGE_THREADS) {
+      for (int n = tid - 32 * T::EDGE_WARP; n < T::V_BYTES / 16; n += EDGE_THREADS) {
         uint4 x = *reinterpret_cast<uint4*>(v + 16 * n);
         uint32_t* w = reinterpret_cast<uint32_t*>(&x);
         bool bad = false;
@@ -918,21 +1070,21 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(edge_clean);
     }
-    asm volatile("bar.arrive 1, %0;" ::"n"(4 * 32 * MT + EDGE_THREADS) : "memory");
+    asm volatile("bar.arrive 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");
   }
   tc::fence_before_sync();
   __syncthreads();
   if (*abort) {
     // a wait gave up: what is on its way lands before shared memory and TMEM go
     int none = 0;
-    if (tid == 32 * COPY_WARP)
+    if (tid == 32 * T::COPY_WARP)
       for (int side = 0; side < 2; ++side) {
         const int n = copied[side];
         uint64_t* full = CODES ? &codes_full[side] : side == 0 ? k_full : v_full;
         for (int j = max(0, n - T::COPY_STAGES); j < n; ++j)
           tc::mbar_wait(&full[j % T::COPY_STAGES], (j / T::COPY_STAGES) & 1, &none, nullptr);
       }
-    if (warp == MMA_WARP) {
+    if (warp == T::MMA_WARP) {
       tc::mma_commit_warp(drained);
       tc::mbar_wait_warp(drained, 0, &none, nullptr);
     }
@@ -968,6 +1120,14 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
     DRIFT_TRY(encode_cache_tiles(&value_map, a.values, CODES, 2, dims, strides, box, CODES ? 0 : 2 * args.run));
   }
   static PerDevice configured;
+  if (T::MOVES_REGISTERS && !configured.done()) {
+    // the warps' shares come out of what a block is launched with; more than
+    // that would be waited for without end
+    cudaFuncAttributes attributes;
+    DRIFT_CUDA(cudaFuncGetAttributes(&attributes, attention_tiles_kernel<T>));
+    if (attributes.numRegs < T::LAUNCH_REGISTERS)
+      return invalid("attention: a kernel of %d registers, built for %d", attributes.numRegs, T::LAUNCH_REGISTERS);
+  }
   DRIFT_TRY(ensure_shared_memory(configured, attention_tiles_kernel<T>, T::BYTES));
   const unsigned units = unsigned((a.at.longest * a.group + T::UNIT - 1) / T::UNIT);
   DRIFT_CUDA(launch_pdl(attention_tiles_kernel<T>, dim3(a.kv_heads, a.at.batch, units * a.splits), T::THREADS, T::BYTES,

@@ -109,6 +109,21 @@ static __device__ __noinline__ float4 not_finite(const __half* values, long long
   return x;
 }
 
+// The same for codes: a scale that is not finite makes NaNs of the key's
+// values in every dimension. `scales`: the key head's in page 0.
+static __device__ __noinline__ float not_finite_scale(const float* scales, long long page_stride, const int* table,
+                                                      int pages, int page_size, int key0, int end, int lowest, int first) {
+  float x = 0.0f;
+  for (int key = key0; key < end; ++key) {
+    if (key < lowest && key >= first) continue;
+    const int page = table[key / page_size];
+    if (page < 0 || page >= pages) continue;
+    const float s = scales[page * page_stride + key % page_size];
+    if (!isfinite(s)) x += s - s;
+  }
+  return x;
+}
+
 // The checks that the calls share (chunks.cu).
 int check_chunks(const char* call, int x_dtype, long long tokens, int kv_heads, int head_dim, int cache_dtype,
                  const void* keys, const void* values, const float* key_scales, const float* value_scales,

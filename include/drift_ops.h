@@ -278,7 +278,8 @@ int drift_cache_read_chunks(int x_dtype, void* k, void* v, int64_t tokens, int k
  * p - window + 1 on and, whatever the window, the sequence's first `first`
  * positions. softcap, sinks and the limits on heads are drift_attention's;
  * max_key_count bounds positions[z] plus z's tokens. F32 rows are computed to
- * F32's accuracy, BF16 rows with weights rounded to F16. `workspace`
+ * F32's accuracy, BF16 rows with weights (and an 8-bit cache's keys and
+ * values) rounded to F16. `workspace`
  * (16-byte aligned, the caller's: calls that may overlap need one each) holds
  * drift_attention_chunks_workspace_bytes(...) bytes of partial results. */
 int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_heads, int kv_heads,

@@ -78,6 +78,7 @@ def attention(q, cache, tables, new, counts, spec):
             at = torch.arange(count, device="cuda")
             page = torch.as_tensor(np.asarray(tables[z]), device="cuda")[at // cache.page_size].long()
             scales = cache.value_scales[page, :, at % cache.page_size].double()
+            key_scales = cache.key_scales[page, :, at % cache.page_size].double()
         key = torch.arange(count, device="cuda")[None]
         position = torch.arange(count - n, count, device="cuda")[:, None]
         seen = key <= position if spec.causal else torch.ones(n, count, dtype=torch.bool, device="cuda")
@@ -93,7 +94,16 @@ def attention(q, cache, tables, new, counts, spec):
             lost = (x.abs().amax(1, keepdim=True) * kh.abs().sum(1)[None]) * abs(spec.scale) * 2.0 ** -21
             if spec.softcap:
                 score = spec.softcap * torch.tanh(score / spec.softcap)
-            delta = lost + magnitude * (2 * dim / 16 * 2.0 ** -22) + score.abs() * 2.0 ** -20
+            rounded = coded = 0.0
+            if scales is not None and q.dtype == torch.bfloat16:
+                # BF16 rows may meet keys and values rounded to F16 over a power
+                # of two under twice the largest scale: 2^-11 of each key, and
+                # 2^-25 of the power at least; a value's scale is rounded
+                # before its product, 2^-11 twice.
+                rounded = magnitude * 2.0 ** -11 + x.abs().sum(1, keepdim=True) * abs(spec.scale) * (
+                    2.0 ** -25 * 2 * key_scales[seen.any(0), h // group].max())
+                coded = 2 * 2.0 ** -11
+            delta = rounded + lost + magnitude * (2 * dim / 16 * 2.0 ** -22) + score.abs() * 2.0 ** -20
             score = score.masked_fill(~seen, -math.inf)
             delta = delta.masked_fill(~seen, 0.0).amax(1, keepdim=True)
             largest = score.amax(1, keepdim=True)
@@ -113,9 +123,14 @@ def attention(q, cache, tables, new, counts, spec):
             # in units of a power of two under twice the largest scale seen:
             # off by 2^-38 of that, times a code of at most 127.
             reach = 254 * scales[seen.any(0), h // group].max() if scales is not None else vh.abs().amax(0, keepdim=True)
-            floor = seen.sum(1, keepdim=True) * 2.0 ** -38 * reach / torch.where(
+            # (and a value so rounded is off by 2^-25 of the power at least; the weights sum to one)
+            if scales is not None and q.dtype == torch.bfloat16:
+                coded_floor = 2.0 ** -25 * 2 * scales[seen.any(0), h // group].max()
+            else:
+                coded_floor = 0.0
+            floor = coded_floor + seen.sum(1, keepdim=True) * 2.0 ** -38 * reach / torch.where(
                 total > 0, torch.minimum(safe, torch.ones_like(safe)), 1.0)
-            tolerance[row:row + n, h] = (mass * (2 * delta + 2.0 ** -21 + rounding + chain) + floor
+            tolerance[row:row + n, h] = (mass * (2 * delta + 2.0 ** -21 + rounding + coded + chain) + floor
                                          + out[row:row + n, h].abs() * UNIT[q.dtype] + 1e-30)
         row += n
     return out, tolerance
