@@ -56,11 +56,12 @@ Plan plan_rows(const Call& c) {
 // Rows of a key head from which chunks go to the tensor-core tiles.
 constexpr long long TILE_ROWS = 32;
 
-// The split count is the one that leaves the busiest SM the least to do: each
-// CTA pays about TILE_OVERHEAD tiles' time to start and end, and splits cost a
-// join.
+// The split count is the one with the least time of the busiest SM, by what
+// was measured on B200 for a tile (per row tile and key: BF16 6 ns, F32 16,
+// heads of 256 14, converted codes half as much again), for a CTA's start and
+// end, and for the join, whose partial rows are written and read once.
 Plan plan_tiles(const Call& c) {
-  constexpr int TILE_OVERHEAD = 3;
+  constexpr double CTA_NS = 5000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 4500;
   Plan p;
   p.columns = 0;
   const long long rows = (long long)c.longest * c.group;
@@ -69,11 +70,16 @@ Plan plan_tiles(const Call& c) {
   p.keys_per_tile = attention_tiles_keys(c.head_dim, c.x_dtype == DRIFT_BF16);
   const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
   const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
-  long long best = 0;
+  const double tile_ns = p.row_tiles * p.keys_per_tile * (c.x_dtype == DRIFT_F32 ? 16 : c.head_dim > 128 ? 14 : 6) *
+                         (c.cache_dtype == DRIFT_I8 ? 1.5 : 1.0);
+  const double parts_bytes = 8.0 * rows * c.batch * c.kv_heads * c.head_dim;  // of a split, there and back
+  double best = 0;
   for (long long splits = 1; splits <= 64 && splits <= tiles; ++splits) {
     const long long each = (tiles + splits - 1) / splits;
-    const long long cost = (units * splits + sm_count() - 1) / sm_count() * (each + TILE_OVERHEAD) + (splits > 1 ? 2 : 0);
-    if (best && cost >= best) continue;
+    const double rounds = double((units * splits + sm_count() - 1) / sm_count());
+    const double cost = rounds * (each * tile_ns + CTA_NS) +
+                        (splits > 1 ? JOIN_NS + splits * parts_bytes / PARTS_BYTES_A_NS : 0);
+    if (splits > 1 && cost >= best) continue;
     best = cost;
     p.tiles_per_split = int(each);
     p.splits = int((tiles + each - 1) / each);

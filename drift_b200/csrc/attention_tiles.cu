@@ -4,9 +4,8 @@
 // of KEYS keys and tile i of 128 rows:
 //
 //   S_i = Q_i K^T      (TMEM; Q and K in shared memory)
-//   P_i = e^(scale S_i - base)  over S_i's columns, as F16 (softmax warps: a
-//                       thread has a row, or half of one's columns, its base
-//                       and its sum, in F32)
+//   P_i = e^(scale S_i - base)  beside S_i, as F16 (softmax warps: a thread
+//                       has a row, its base and its sum, in F32)
 //   O_i (+)= P_i V     (TMEM; V^T in shared memory, as the cache has it)
 //
 // The F16 cache's layouts are the tensor core's own K-major operands -- keys
@@ -21,30 +20,33 @@
 // exactly, and there a key's scale multiplies its scores, and a value's its
 // weights.
 //
-// A weight is at most 2^15 or the row's base moves: the sum of a tile's
-// weights tells, so that a tile's largest score is looked for only then (and
-// in the first tile, to set the base) -- the tile is read again, and what was
-// summed so far rescaled. Looking for it in every tile took 27 % of a tile's
-// softmax.
+// The order: Q K^T of the next tile is issued as soon as the softmax threads
+// have taken S into registers, P V when P is there. So the tensor core works
+// under the softmax and the softmax under the products, and what bounds a tile
+// is the longer of the two: for D = 128 the tensor core's 16 + 10 products of
+// 64 and 52 clocks for 80 keys and 256 rows. (With P over S, and Q K^T behind
+// P V, a tile took both after one another: 3050 clocks for 128 keys.) TMEM's
+// 512 columns set the tile's keys: MT S, MT P, MT outputs.
 //
 // BF16 rows (TERMS = 1): q is exact in F16 after a power of two per row; P's
 // rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). O stays in TMEM.
-// Two threads share a row, half of a tile's columns each, since what a row
-// tile's softmax takes adds to what its products take before the next scores.
+// A weight is at most 2^15 or the row's base moves: the sum of a tile's
+// weights tells, so that a tile's largest score is looked for only then (and
+// in the first tile, to set the base), and the weights made again and O
+// rescaled. Looking for it in every tile took 27 % of a tile's softmax.
 // F32 rows (TERMS = 2): q and P are two F16 terms each (hi + lo, to 2^-22), the
 // products of both summed. The tensor core's F32 sums drop low bits as a chain
 // grows, so a tile's P V starts a new O, and the softmax threads add it to
 // their row's running output in registers.
 //
-// With MT = 2 (D <= 128) the two row tiles take turns: while one's softmax
-// runs the tensor core works on the other. With MT = 1 (heads of 256, whose
-// outputs fill TMEM, and units of 128 rows) S has two buffers, and Q K^T of
-// the next tile runs under the softmax.
+// MT = 2 (D <= 128) shares a tile's keys and values between two row tiles. MT =
+// 1 (heads of 256, whose outputs fill TMEM, and units of 128 rows) has two S.
 //
-// Warps: first the softmax, four for 128 rows (eight for BF16 rows); then one
-// for the copies, one for the tensor core, and two for the edges: in a tile that
-// some row sees only in part they take values that are not finite out of V,
-// since such a value times a zero weight would reach rows that do not see it
+// Warps: first the softmax, four for 128 rows; then one for the copies, two for
+// the tensor core (Q K^T, P V), and for an F16 cache one for the edges: in a
+// tile that some row sees only in part it takes values that are not finite out
+// of V, since such a value times a zero weight would reach rows that do not see
+// it
 // (they are added at the end, to the rows that do). An 8-bit cache has
 // converting warps. Every wait is bounded; one that gives up sets device error
 // 2, and the CTA drains its copies and products, frees its TMEM and returns.
@@ -68,13 +70,16 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROW_TILE = 128;
-constexpr int EDGE_THREADS = 64;
 constexpr uint32_t TMEM_COLUMNS = 512;
 // A weight is 2^WEIGHT_BITS at the row's largest score when its base is set,
-// and the base moves when a tile's weights sum to more than MOST_WEIGHT.
-constexpr float WEIGHT_BITS = 8.0f, MOST_WEIGHT = 32768.0f;
+// and the base moves when a tile's weights sum to more than MOST_WEIGHT (F32
+// rows: when one would pass 2^(WEIGHT_BITS + GROWTH_BITS)).
+constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f, MOST_WEIGHT = 32768.0f;
 // Of eight pairs of BF16 rows' weights, those made by exp2_cubic.
-constexpr int CUBIC_PAIRS = 3;
+#ifndef CUBIC
+#define CUBIC 3
+#endif
+constexpr int CUBIC_PAIRS = CUBIC;
 // A row of q is 2^Q_BITS and more at its largest value, so that its second
 // terms end far below F16's last bit, 2^-24.
 constexpr int Q_BITS = 8;
@@ -84,23 +89,29 @@ struct TileTraits {
   static constexpr int D = D_, KEYS = KEYS_, MT = MT_, TERMS = TERMS_;
   static constexpr bool CODES = CODES_;
   static constexpr int UNIT = ROW_TILE * MT;
-  static constexpr int HALVES = TERMS == 1 ? 2 : 1;        // threads that share a row
-  static constexpr int COLUMNS = KEYS / HALVES;            // a thread's, of a tile's scores
+  // Two threads share a row of BF16, half of a tile's columns each: with one
+  // to a row, two warps to a scheduler, an instruction took 3.7 clocks.
+  static constexpr int HALVES = TERMS == 1 ? 2 : 1, COLUMNS = KEYS / HALVES;
   static constexpr int SOFTMAX_WARPS = 4 * MT * HALVES;
-  static constexpr int COPY_WARP = SOFTMAX_WARPS, MMA_WARP = COPY_WARP + 1, EDGE_WARP = COPY_WARP + 2;
-  // Converting 128 keys' codes for BF16 rows takes four warps, one to a
-  // scheduler; for F32 rows, at half the keys in the same time, two. The
-  // softmax warps take the registers that the others leave.
+  // Q K^T and P V have a warp each: a wait costs one about 100 clocks even when
+  // there is nothing to wait for, and six of them and the products' issue were
+  // longer than the products (for the codes of F32 rows they are not).
+  static constexpr bool TWO_ISSUE = !(CODES && TERMS == 2);
+  static constexpr int COPY_WARP = SOFTMAX_WARPS, QK_WARP = COPY_WARP + 1, PV_WARP = QK_WARP + TWO_ISSUE;
+  static constexpr int EDGE_WARP = PV_WARP + 1, EDGE_THREADS = 32;
+  // Converting codes for BF16 rows takes four warps, one to a scheduler; for
+  // F32 rows, at half the rate, two. The softmax warps take the registers that
+  // the others leave.
   static constexpr bool WIDE = CODES && TERMS == 1;
-  static constexpr int CONVERT_WARP = WIDE ? EDGE_WARP + 2 : EDGE_WARP;
+  static constexpr int CONVERT_WARP = WIDE ? EDGE_WARP + 1 : EDGE_WARP;
   static constexpr int CONVERT_THREADS = WIDE ? 128 : 64;
   static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4 + (WIDE ? 4 : 0));
-  static constexpr int LAUNCH_REGISTERS = 65536 / THREADS / 8 * 8 > 248 ? 248 : 65536 / THREADS / 8 * 8;
-  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : WIDE ? 64 : MT == 2 ? 64 : 88;
-  static constexpr int SHARE =
+  static constexpr bool MOVES_REGISTERS = MT == 2;  // (128 a thread and more are there otherwise)
+  static constexpr int LAUNCH_REGISTERS = 65536 / THREADS / 8 * 8;
+  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : 64;
+  static constexpr int SOFTMAX_REGISTERS =
       (THREADS * LAUNCH_REGISTERS - (THREADS - 32 * SOFTMAX_WARPS) * OTHER_REGISTERS) / (32 * SOFTMAX_WARPS) / 8 * 8;
-  static constexpr int SOFTMAX_REGISTERS = SHARE > 232 ? 232 : SHARE;
-  static constexpr bool MOVES_REGISTERS = THREADS > 256;  // (255 a thread are there otherwise)
+  static_assert(!MOVES_REGISTERS || SOFTMAX_REGISTERS <= 248, "a thread's registers");
   static constexpr int ROUND_THREADS = 32 * SOFTMAX_WARPS + (CODES ? CONVERT_THREADS : EDGE_THREADS);
   static constexpr int PANELS = (D + 63) / 64;             // 64-column panels of a row
   static constexpr int Q_PANEL = ROW_TILE * 128;           // bytes
@@ -110,21 +121,35 @@ struct TileTraits {
   static constexpr int V_BYTES = KEYS * D * 2;
   static constexpr int V_STAGE = (V_BYTES + 1023) / 1024 * 1024;
   static constexpr int CODE_BYTES = KEYS * D;              // of one side of a tile
-  static constexpr int STAGES = 2;
-  static constexpr int COPY_STAGES = CODES ? 1 : STAGES;   // of what the copies fill
+  static constexpr int CODE_STAGE = (CODE_BYTES + 127) / 128 * 128;
   static constexpr int K_AT = MT * TERMS * Q_BYTES;
+  // what the copies fill: the operands, or codes, twice where that fits; and
+  // the operands three times where that does (a copy's 1400 clocks from when
+  // its stage is free are a tile's time)
+  static constexpr int bytes_of(int stages, int code_stages) {
+    return K_AT + stages * (K_BYTES + V_STAGE) + (CODES ? code_stages * 2 * CODE_STAGE : 0) +
+           (CODES && TERMS == 2 ? stages * 2 * KEYS * 4 : 0) + (CODES ? code_stages * 2 * KEYS * 4 : 0) +
+           (HALVES == 2 ? MT * 2 * ROW_TILE * 4 : 0) + 384;
+  }
+  static constexpr int LIMIT = 232448;
+  static constexpr int CODE_STAGES = bytes_of(2, 2) <= LIMIT ? 2 : 1;
+  static constexpr int STAGES = bytes_of(3, CODE_STAGES) <= LIMIT ? 3 : 2;
+  static constexpr int COPY_STAGES = CODES ? CODE_STAGES : STAGES;
   static constexpr int V_AT = K_AT + STAGES * K_BYTES;
-  static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;
-  static constexpr int SCALES_AT = CODES_AT + (CODES ? 2 * CODE_BYTES : 0);  // [STAGES][2][KEYS]
-  static constexpr int SHARED_AT = SCALES_AT + (CODES && TERMS == 2 ? STAGES * 2 * KEYS * 4 : 0);  // between halves
-  static constexpr int BARRIERS_AT = SHARED_AT + (HALVES == 2 ? MT * 2 * ROW_TILE * 4 : 0);
-  static constexpr int BYTES = BARRIERS_AT + 320;
-  static constexpr int O_COLUMN = 256;                     // S: columns 0 and KEYS; O: 256 and 384
-  static_assert(MT == 1 || (D <= 128 && KEYS <= 128), "two outputs in TMEM");
-  static_assert(2 * KEYS <= O_COLUMN && O_COLUMN + (MT - 1) * 128 + D <= int(TMEM_COLUMNS), "TMEM");
-  static_assert(KEYS % 64 == 0 && TERMS * KEYS / 2 <= KEYS, "P fits over S");
-  static_assert(TERMS == 1 || D <= 128, "the running output of a row in registers");
-  static_assert(BYTES <= 232448, "shared memory");
+  static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;  // [COPY_STAGES][2]
+  static constexpr int SCALES_AT = CODES_AT + (CODES ? COPY_STAGES * 2 * CODE_STAGE : 0);  // [STAGES][2][KEYS]
+  static constexpr int COPIED_SCALES_AT = SCALES_AT + (CODES && TERMS == 2 ? STAGES * 2 * KEYS * 4 : 0);  // [COPY_STAGES][2][KEYS]
+  static constexpr int BETWEEN_AT = COPIED_SCALES_AT + (CODES ? COPY_STAGES * 2 * KEYS * 4 : 0);  // [MT][2][ROW_TILE]
+  static constexpr int BARRIERS_AT = BETWEEN_AT + (HALVES == 2 ? MT * 2 * ROW_TILE * 4 : 0);
+  static constexpr int BYTES = BARRIERS_AT + 384;  // 36 barriers and a few words
+  // TMEM: S of row tile i, or (MT = 1) of every other tile; P and O of row tile i
+  static constexpr int S_COLUMNS = (KEYS + 31) / 32 * 32;
+  static constexpr int P_COLUMN = S_COLUMNS + KEYS, P_COLUMNS = TERMS * KEYS / 2;
+  static constexpr int O_COLUMN = int(TMEM_COLUMNS) - MT * ((D + 31) / 32 * 32), O_COLUMNS = (D + 31) / 32 * 32;
+  static_assert(P_COLUMN + MT * P_COLUMNS <= O_COLUMN, "TMEM");
+  static_assert(KEYS % 16 == 0 && KEYS <= 128 && P_COLUMN % 8 == 0, "whole steps");
+  static_assert(TERMS == 1 || (D <= 128 && KEYS == 64), "the running output of a row in registers");
+  static_assert(BYTES <= LIMIT, "shared memory");
 };
 
 template <int REGISTERS>
@@ -187,21 +212,7 @@ __device__ __forceinline__ void tmem_load_32_async(uint32_t address, float* v) {
       : "r"(address)
       : "memory");
 }
-__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_load_8(uint32_t address, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(address)
-               : "memory");
-  tmem_load_wait();
-}
-__device__ __forceinline__ void tmem_store_8(uint32_t address, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(address),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-__device__ __forceinline__ void tmem_load_16(uint32_t address, float* v) {
+__device__ __forceinline__ void tmem_load_16_async(uint32_t address, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
@@ -210,6 +221,41 @@ __device__ __forceinline__ void tmem_load_16(uint32_t address, float* v) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(address)
       : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store_8(uint32_t address, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(address),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load_8_async(uint32_t address, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(address)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store_4(uint32_t address, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// N columns of this thread's lane, in as few instructions as there are.
+template <int N>
+__device__ __forceinline__ void tmem_load_async(uint32_t address, float* v) {
+  if constexpr (N >= 32) {
+    tmem_load_32_async(address, v);
+    if constexpr (N > 32) tmem_load_async<N - 32>(address + 32, v + 32);
+  } else if constexpr (N >= 16) {
+    tmem_load_16_async(address, v);
+    if constexpr (N > 16) tmem_load_async<N - 16>(address + 16, v + 16);
+  } else {
+    static_assert(N == 8, "columns by eights");
+    tmem_load_8_async(address, v);
+  }
+}
+__device__ __forceinline__ void tmem_load_16(uint32_t address, float* v) {
+  tmem_load_16_async(address, v);
   tmem_load_wait();
 }
 __device__ __forceinline__ void tmem_store_16(uint32_t address, const uint32_t* r) {
@@ -221,17 +267,18 @@ __device__ __forceinline__ void tmem_store_16(uint32_t address, const uint32_t* 
       : "memory");
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// The largest of three, a NaN if one is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t address, const uint32_t* r) {
+  if constexpr (N >= 16) {
+    tmem_store_16(address, r);
+    if constexpr (N > 16) tmem_store<N - 16>(address + 16, r + 16);
+  } else if constexpr (N >= 8) {
+    tmem_store_8(address, r);
+    if constexpr (N > 8) tmem_store<N - 8>(address + 8, r + 8);
+  } else {
+    static_assert(N == 4, "columns by fours");
+    tmem_store_4(address, r);
+  }
 }
 
 // Whether some thread of the 256 of a row tile has `any` (one answer for all;
@@ -246,6 +293,19 @@ __device__ __forceinline__ bool any_of_tile(int tile, bool any) {
   return r != 0;
 }
 __device__ __forceinline__ void meet_tile(int tile) { asm volatile("bar.sync %0, 256;" ::"r"(5 + tile) : "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The largest of three, a NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Pairs: one instruction for two F32 operations.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -276,18 +336,25 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-// 2^x for |x| <= 126 (beyond: 2^-126, 2^126) on the multiply-add units, to 8e-5 (a sixth of F16's
-// rounding): x = n + f with |f| <= 1/2, by the F32 sum that has no room for a
-// fraction; a cubic in f (least squares on Chebyshev points, reweighted
-// towards the least largest relative error) and n added to its exponent. The
-// special function unit makes 16 values a clock and SM, the tensor core needs
-// a tile's 16384 in as many clocks as it takes to make them: a share of them
-// made here leaves the tensor core the one that is waited for.
-__device__ __forceinline__ float2 exp2_cubic(float2 x) {
-  x.x = fminf(fmaxf(x.x, -126.0f), 126.0f), x.y = fminf(fmaxf(x.y, -126.0f), 126.0f);
-  const float2 whole = make_float2(12582912.0f, 12582912.0f);  // 1.5 x 2^23
-  const float2 t = add2(x, whole);
-  const float2 f = add2(x, mul2(add2(t, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f)));
+// 2^x of a pair's x = s factor + less on the multiply-add units, to 8e-5 (a
+// sixth of F16's rounding), x held between -126 and 126 (a NaN becomes -126).
+// The caller gives a = factor / 252 and b = less / 252 + 1/2, whose saturating
+// product and sum is x / 252 + 1/2. x = n + f with |f| <= 1/2, by the F32 sum
+// that has no room for a fraction; a cubic in f (least squares on Chebyshev
+// points, reweighted towards the least largest relative error), and n added to
+// its exponent. The special function unit gives a warp's 32 values in 8
+// clocks: 1280 for 80 keys of 256 rows on a scheduler, beside the tensor
+// core's 1440; of eight pairs three made here, in 14 clocks of the multiply-add
+// units each, leave it 800.
+__device__ __forceinline__ float2 exp2_cubic(float s0, float s1, float a, float b) {
+  float2 y;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(y.x) : "f"(s0), "f"(a), "f"(b));
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(y.y) : "f"(s1), "f"(a), "f"(b));
+  constexpr float WHOLE = 12582912.0f;  // 1.5 x 2^23
+  const float2 by = make_float2(252.0f, 252.0f);
+  const float2 t = fma2(y, by, make_float2(WHOLE - 126.0f, WHOLE - 126.0f));                  // n + WHOLE
+  const float2 n = fma2(t, make_float2(-1.0f, -1.0f), make_float2(WHOLE - 126.0f, WHOLE - 126.0f));  // -(n + 126)
+  const float2 f = fma2(y, by, n);
   float2 p = fma2(f, make_float2(0.05517164245247841f, 0.05517164245247841f), make_float2(0.2426111251115799f, 0.2426111251115799f));
   p = fma2(f, p, make_float2(0.6932609677314758f, 0.6932609677314758f));
   p = fma2(f, p, make_float2(0.9999280571937561f, 0.9999280571937561f));
@@ -383,29 +450,32 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   uint64_t* v_empty = v_full + STAGES;
   uint64_t* scales_full = v_empty + STAGES;
   uint64_t* s_full = scales_full + STAGES;  // [2]: of row tile i, or of buffer i
-  uint64_t* p_full = s_full + 2;            // [2]
-  uint64_t* o_full = p_full + 2;            // [2]
-  uint64_t* edge_found = o_full + 2;        // an edge tile's values are there; they are clean
+  uint64_t* s_empty = s_full + 2;           // [2]
+  uint64_t* p_full = s_empty + 2;           // [2]: of row tile i
+  uint64_t* pv_done = p_full + 2;           // [2]: P is read, O written
+  uint64_t* edge_found = pv_done + 2;       // an edge tile's values are there; they are clean
   uint64_t* edge_clean = edge_found + 1;
-  uint64_t* codes_full = edge_clean + 1;    // [2]: of the keys, of the values
-  uint64_t* codes_empty = codes_full + 2;   // [2]
-  uint64_t* drained = codes_empty + 2;
+  uint64_t* codes_full = edge_clean + 1;    // [COPY_STAGES][2]: of the keys, of the values
+  uint64_t* codes_empty = codes_full + 4;   // [COPY_STAGES][2]
+  uint64_t* drained = codes_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* taken_out = abort + 1;
   volatile int* copied = abort + 2;         // [2]: tiles whose keys, values were asked for
-  volatile int* failed = abort + 4;         // [2][2]: a wait of row tile i gave up, in an even or odd tile
-  volatile float* k_unit = reinterpret_cast<volatile float*>(abort + 8);  // [STAGES]: the scales' powers of two
+  volatile float* k_unit = reinterpret_cast<volatile float*>(abort + 4);  // [STAGES]: the scales' powers of two
   volatile float* v_unit = k_unit + STAGES;
-  volatile float* between = reinterpret_cast<volatile float*>(shared + T::SHARED_AT);  // [MT][2][ROW_TILE]
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 5 + 2 * STAGES);  // [2][2]: a wait of row tile i
+                                                                                     // gave up, in an even or odd tile
+  volatile float* between = reinterpret_cast<volatile float*>(shared + T::BETWEEN_AT);  // what a row's halves exchange
   float* scales = reinterpret_cast<float*>(shared + T::SCALES_AT);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&q_full[i], ROW_TILE * HALVES);
       tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&s_empty[i], ROW_TILE * HALVES);
       tc::mbar_init(&p_full[i], ROW_TILE * HALVES);
-      tc::mbar_init(&o_full[i], 1);
+      tc::mbar_init(&pv_done[i], 1);
     }
     for (int s = 0; s < STAGES; ++s) {
       tc::mbar_init(&k_full[s], CODES ? T::CONVERT_THREADS : 1);
@@ -413,12 +483,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_init(&v_full[s], CODES ? T::CONVERT_THREADS : 1);
       tc::mbar_init(&v_empty[s], 1);
       tc::mbar_init(&scales_full[s], T::CONVERT_THREADS);
+    }
+    for (int s = 0; s < 4; ++s) {
       tc::mbar_init(&codes_full[s], 1);
       tc::mbar_init(&codes_empty[s], T::CONVERT_THREADS);
     }
     tc::mbar_init(edge_found, 1);
-    tc::mbar_init(edge_clean, EDGE_THREADS);
-    tc::mbar_init(drained, 1);
+    tc::mbar_init(edge_clean, T::EDGE_THREADS);
+    tc::mbar_init(drained, 1 + T::TWO_ISSUE);
     *abort = 0;
     *taken_out = 0;
     copied[0] = copied[1] = 0;
@@ -438,62 +510,88 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   }
 
   if (warp < T::SOFTMAX_WARPS) {
-    // ---- softmax: this thread's row of row tile i, columns [COLUMNS half, + COLUMNS) of a tile ----
-    const int i = warp / (4 * HALVES), half = HALVES == 2 ? warp / 4 % 2 : 0;
-    const int r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
+    // ---- softmax: this thread's row of row tile i (of a tile's columns, its half) -----------
+    const int i = warp / (4 * HALVES), half = HALVES == 2 ? warp / 4 % 2 : 0, r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
     const bool real = row < row1;
     const int token = (real ? row : row1 - 1) / a.group, q_head = head * a.group + row % a.group;
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
     const long long row_at = (chunk.row + token) * a.q_heads + q_head;
     // q, divided by a power of two (and by the scale's sign), into the
-    // swizzled panels of its terms
+    // swizzled panels of its terms: a warp takes its 32 rows, a few at a time,
+    // a lane eight values of one
     float multiplier;
+    const uint32_t group_magic = a.group > 1 ? 0xffffffffu / uint32_t(a.group) + 1 : 0;  // (2^32 / group, up)
     {
-      const X* q = static_cast<const X*>(a.q) + row_at * D;
-      float x[8];
-      auto load = [&](int c) {  // values 8 c .. 8 c + 7
-        if constexpr (TERMS == 1) {
-          const uint4 v = reinterpret_cast<const uint4*>(q)[c];
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      constexpr int CHUNKS = D / 8, LANES = CHUNKS <= 8 ? 8 : CHUNKS <= 16 ? 16 : 32;  // of a row
+      constexpr int AT_ONCE = 32 / LANES, PASSES = LANES, FLIGHT = 4;
+      const int c = lane % LANES, part = lane / LANES;
+      const int tile_row0 = row0 + ROW_TILE * i + 32 * (warp % 4);
+      const int tile_token0 = tile_row0 / a.group, tile_head0 = tile_row0 % a.group;
+      // (rows past the unit's are zeros, and so are the last panel's columns past D)
+      auto load = [&](int pass, uint4 (&x)[TERMS]) {
+        const int from = tile_row0 + pass * AT_ONCE + part;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        } else {
-          const float4 u = reinterpret_cast<const float4*>(q)[2 * c], v = reinterpret_cast<const float4*>(q)[2 * c + 1];
-          x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-        }
+        for (int n = 0; n < TERMS; ++n) x[n] = make_uint4(0, 0, 0, 0);
+        if (c >= CHUNKS || from >= row1) return;
+        // (row x's token past the first: x below 48 over at most 16, exactly)
+        const int x_row = tile_head0 + pass * AT_ONCE + part, tokens = a.group > 1 ? int(__umulhi(x_row, group_magic)) : x_row;
+        const X* q = static_cast<const X*>(a.q) +
+                     ((chunk.row + tile_token0 + tokens) * a.q_heads + head * a.group + x_row - tokens * a.group) * D + 8 * c;
+#pragma unroll
+        for (int n = 0; n < TERMS; ++n) x[n] = reinterpret_cast<const uint4*>(q)[n];
       };
-      float largest = 0.0f;
-      if (real)
-        for (int c = 0; c < D / 8; ++c) {
-          load(c);
+      multiplier = 0.0f;
+#pragma unroll 1
+      for (int pass0 = half * (PASSES / HALVES); pass0 < (half + 1) * (PASSES / HALVES); pass0 += FLIGHT) {
+        uint4 held[FLIGHT][TERMS];
+#pragma unroll
+        for (int n = 0; n < FLIGHT; ++n) load(pass0 + n, held[n]);
+#pragma unroll
+        for (int n = 0; n < FLIGHT; ++n) {
+          float x[8];
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(held[n]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = __uint_as_float(TERMS == 2 ? w[e % (4 * TERMS)] : e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+          float largest = 0.0f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[e]));
-        }
-      // 2^(floor(log2 largest) - Q_BITS), kept where it and its inverse are
-      // normal (NaNs and infinities stay what they are)
-      constexpr uint32_t SHIFT = uint32_t(Q_BITS) << 23;
-      const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, SHIFT + 0x01000000u) - SHIFT;
-      const float unit_inverse = 1.0f / __uint_as_float(exponent);
-      const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
-      multiplier = fabsf(a.scale) * __uint_as_float(exponent);
-      uint8_t* panel = shared + i * TERMS * T::Q_BYTES + r * 128;
-      for (int c = half * (T::PANELS * 8 / HALVES); c < (half + 1) * (T::PANELS * 8 / HALVES); ++c) {
-        uint4 hi = make_uint4(0, 0, 0, 0), low = hi;
-        if (real && c < D / 8) {
-          load(c);
+#pragma unroll
+          for (int o = 1; o < LANES; o *= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+          // 2^(floor(log2 largest) - Q_BITS), kept where it and its inverse
+          // are normal (NaNs and infinities stay what they are)
+          constexpr uint32_t SHIFT = uint32_t(Q_BITS) << 23;
+          const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, SHIFT + 0x01000000u) - SHIFT;
+          const float unit_inverse = __uint_as_float(0x7f000000u - exponent);
+          const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
+          const int pass = pass0 + n;
+          if constexpr (HALVES == 2) {
+            if (c == 0) between[2 * ROW_TILE * i + 32 * (warp % 4) + pass * AT_ONCE + part] = __uint_as_float(exponent);
+          } else {
+            const uint32_t own = __shfl_sync(0xffffffffu, exponent, lane % AT_ONCE * LANES);
+            if (lane / AT_ONCE == pass) multiplier = fabsf(a.scale) * __uint_as_float(own);
+          }
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= by;
-          hi = make_uint4(half_pair(x[0], x[1]), half_pair(x[2], x[3]), half_pair(x[4], x[5]), half_pair(x[6], x[7]));
-          if constexpr (TERMS == 2)
-            low = make_uint4(left_pair(x[0], x[1], hi.x), left_pair(x[2], x[3], hi.y), left_pair(x[4], x[5], hi.z),
+          const uint4 hi = make_uint4(half_pair(x[0], x[1]), half_pair(x[2], x[3]), half_pair(x[4], x[5]), half_pair(x[6], x[7]));
+          const int to_row = 32 * (warp % 4) + pass * AT_ONCE + part;
+          if (c < T::PANELS * 8) {
+            uint8_t* to = shared + i * TERMS * T::Q_BYTES + to_row * 128 + c / 8 * T::Q_PANEL + 16 * ((c % 8) ^ (to_row % 8));
+            *reinterpret_cast<uint4*>(to) = hi;
+            if constexpr (TERMS == 2)
+              *reinterpret_cast<uint4*>(to + T::Q_BYTES) =
+                  make_uint4(left_pair(x[0], x[1], hi.x), left_pair(x[2], x[3], hi.y), left_pair(x[4], x[5], hi.z),
                              left_pair(x[6], x[7], hi.w));
+          }
         }
-        uint8_t* to = panel + (c / 8) * T::Q_PANEL + 16 * ((c % 8) ^ (r % 8));
-        *reinterpret_cast<uint4*>(to) = hi;
-        if constexpr (TERMS == 2) *reinterpret_cast<uint4*>(to + T::Q_BYTES) = low;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&q_full[i]);
+      if constexpr (HALVES == 2) {
+        meet_tile(i);
+        multiplier = fabsf(a.scale) * between[2 * ROW_TILE * i + r];
+        meet_tile(i);
+      }
     }
     // (a softcap leaves natural units behind)
     // (and a factor of 2^-60 is as good as none; times a tile's power it is normal)
@@ -505,10 +603,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int last = min(row0 + ROW_TILE * (i + 1), row1) - 1;
     const int tile_end = a.causal ? chunk.position + (row0 + ROW_TILE * i) / a.group + 1 : seen.end;
     const int tile_low = a.window > 0 ? chunk.position + max(last, 0) / a.group - a.window + 1 : 0;
-    const uint32_t o_at = tmem + lanes + T::O_COLUMN + 128 * i;
+    const uint32_t o_at = tmem + lanes + T::O_COLUMN + i * T::O_COLUMNS, p_at = tmem + lanes + T::P_COLUMN + i * T::P_COLUMNS;
 
-    constexpr int OWN = D / HALVES;  // this thread's dimensions of the output
-    const int d0 = half * OWN;
 
     float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
     float unit = 0.0f;                    // and, for codes, values are over this
@@ -531,107 +627,107 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
-      const uint32_t phase = MT == 2 ? j & 1 : (j >> 1) & 1;
-      // (the threads of a row tile leave the loop together: they meet in it)
-      ok = ok && wait(&s_full[b], phase);
+      // (a row's halves leave the loop together: they meet in it)
+      ok = ok && wait(&s_full[b], MT == 2 ? j & 1 : (j >> 1) & 1);
       if (CODES) ok = ok && wait(&scales_full[stage], (j / STAGES) & 1);
-      // O holds the tile before this one, or every one: with two row tiles
-      // that P V came before this S; with one it is waited for
-      if (TERMS == 2 && j > 0 && ok) {
-        if (MT == 1) ok = wait(&o_full[0], (j - 1) & 1);
-        tc::fence_after_sync();
-        if (ok) take_output();
-      }
       if (HALVES == 1 && !ok) break;
       tc::fence_after_sync();
-      const uint32_t s_at = tmem + lanes + b * KEYS;
-      const int key0 = seen.key_of(tile0 + j), own_key0 = key0 + half * COLUMNS;
+      float s[COLUMNS];
+      tmem_load_async<COLUMNS>(tmem + lanes + b * T::S_COLUMNS + half * COLUMNS, s);
+      tmem_load_wait();
+      tc::fence_before_sync();
+      tc::mbar_arrive(&s_empty[b]);
+
+      const int key0 = seen.key_of(tile0 + j);
       const float* k_scales = scales + stage * 2 * KEYS;
       const float* v_scales = k_scales + KEYS;
-      const bool edge = !(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first));
       const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : 1.0f;
       const float tile_m2 = a.softcap > 0.0f ? m2 : m2 * by_unit;
       const float now_unit = CODES ? float(v_unit[stage]) : 0.0f;
-      bool slow = j == 0;  // (the same for a row tile's threads)
+      if constexpr (CODES && TERMS == 2) {
+#pragma unroll
+        for (int c = 0; c < COLUMNS; c += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
+          const float2 u = mul2(make_float2(s[c], s[c + 1]), make_float2(x.x, x.y));
+          const float2 v = mul2(make_float2(s[c + 2], s[c + 3]), make_float2(x.z, x.w));
+          s[c] = u.x, s[c + 1] = u.y, s[c + 2] = v.x, s[c + 3] = v.y;
+        }
+      }
+      if (a.softcap > 0.0f) {
+        const float inverse = multiplier * by_unit / a.softcap;
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) s[c] = capped(s[c], inverse, a.softcap);
+      }
+      const bool edge = !(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first));
+      if (edge) {
+        const int own0 = key0 + half * COLUMNS, end = hi - own0, low = lo - own0, head_end = first - own0;
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+          if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
+      }
+      // P and O are free (and O complete) when the last tile's P V is done
+      auto settled = [&]() {
+        if (j == 0) return true;
+        if (!wait(&pv_done[i], (j - 1) & 1)) return false;
+        tc::fence_after_sync();
+        return true;
+      };
+      // the row's base from this tile's largest score, and what is summed in it
+      bool not_a_number = false;
+      auto rebase = [&](float top) {
+        not_a_number = top != top;
+        // (a row without a base takes one; a base that is too high stays)
+        const float now = fmaxf(base2, top - WEIGHT_BITS);
+        const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
+        const float g = CODES && now_unit > unit ? f * (unit / now_unit) : f;
+        if (CODES) unit = fmaxf(unit, now_unit);
+        base2 = now;
+        sum *= f;
+        if constexpr (TERMS == 2) {
+#pragma unroll
+          for (int c = 0; c < D; ++c) total[c] *= g;
+        } else if (j > 0 && ok) {
+#pragma unroll 1
+          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 8) {
+            float o[8];
+            tmem_load_8_async(o_at + c, o);
+            tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] *= g;
+            tmem_store_8(o_at + c, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+      };
+      auto largest = [&]() {
+        float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < COLUMNS - 4; c += 8)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[COLUMNS - 4 + n]);
+        return max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * tile_m2;
+      };
       uint32_t p[COLUMNS / 2], p_low[TERMS == 2 ? COLUMNS / 2 : 1];
-      float part;
-#pragma unroll 1
-      for (;;) {
-        float s[COLUMNS];
-#pragma unroll
-        for (int c = 0; c < COLUMNS; c += 32) tmem_load_32_async(s_at + half * COLUMNS + c, s + c);
-        tmem_load_wait();
-        if constexpr (CODES && TERMS == 2) {
-#pragma unroll
-          for (int c = 0; c < COLUMNS; c += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
-            const float2 u = mul2(make_float2(s[c], s[c + 1]), make_float2(x.x, x.y));
-            const float2 v = mul2(make_float2(s[c + 2], s[c + 3]), make_float2(x.z, x.w));
-            s[c] = u.x, s[c + 1] = u.y, s[c + 2] = v.x, s[c + 3] = v.y;
-          }
-        }
-        if (a.softcap > 0.0f) {
-          const float inverse = multiplier * by_unit / a.softcap;
-#pragma unroll
-          for (int c = 0; c < COLUMNS; ++c) s[c] = capped(s[c], inverse, a.softcap);
-        }
-        if (edge) {
-          const int end = hi - own_key0, low = lo - own_key0, head_end = first - own_key0;
-#pragma unroll
-          for (int c = 0; c < COLUMNS; ++c)
-            if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
-        }
-        bool not_a_number = false;
-        if (slow) {
-          float tops[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int c = 4; c < COLUMNS - 4; c += 8)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[COLUMNS - 4 + n]);
-          float top = max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * tile_m2;
-          if constexpr (HALVES == 2) {
-            volatile float* shared_top = between + 2 * ROW_TILE * i + r;
-            shared_top[ROW_TILE * half] = top;
-            meet_tile(i);
-            top = max3(top, top, shared_top[ROW_TILE * (1 - half)]);
-          }
-          not_a_number = top != top;
-          // (a row without a base takes one; a base that is too high stays)
-          const float now = fmaxf(base2, top - WEIGHT_BITS);
-          const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
-          const float g = CODES && now_unit > unit ? f * (unit / now_unit) : f;
-          if (CODES) unit = fmaxf(unit, now_unit);
-          base2 = now;
-          sum *= f;
-          if constexpr (TERMS == 2) {
-#pragma unroll
-            for (int c = 0; c < D; ++c) total[c] *= g;
-          } else if (j > 0 && ok) {
-            if (MT == 1) ok = wait(&o_full[0], (j - 1) & 1);
-            if (ok) {
-              tc::fence_after_sync();
-#pragma unroll 1
-              for (int c = 0; c < OWN; c += 8) {
-                float o[8];
-                tmem_load_8(o_at + d0 + c, o);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] *= g;
-                tmem_store_8(o_at + d0 + c, reinterpret_cast<const uint32_t*>(o));
-              }
-            }
-          }
-        }
+      // the weights and their sum (a tile's own: short chains); a NaN, or
+      // weights past any use, if exp2_cubic was given what it cannot show
+      auto weigh = [&]() {
         // (a NaN makes the whole row NaNs)
-        const float less = not_a_number ? __int_as_float(0x7fc00000) : slow && base2 == -INFINITY ? 0.0f : -base2;
-        float2 parts = make_float2(0.0f, 0.0f);  // (a tile's own sum: short chains)
+        const float less = not_a_number ? __int_as_float(0x7fc00000) : base2 == -INFINITY ? 0.0f : -base2;
+        float2 part = make_float2(0.0f, 0.0f);
+        const float cubic_a = tile_m2 * (1.0f / 252.0f), cubic_b = fmaf(less, 1.0f / 252.0f, 0.5f);
+        float cubic_top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < COLUMNS / 2; ++e) {
-          float2 w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
-          if (TERMS == 1 && e % 8 < CUBIC_PAIRS) w = exp2_cubic(w);
-          else w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
-          parts = add2(parts, w);
+          float2 w;
+          if (TERMS == 1 && e % 8 < CUBIC_PAIRS) {
+            cubic_top = max3(cubic_top, s[2 * e], s[2 * e + 1]);
+            w = exp2_cubic(s[2 * e], s[2 * e + 1], cubic_a, cubic_b);
+          } else {
+            w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
+            w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
+          }
+          part = add2(part, w);
           if constexpr (CODES && TERMS == 2) {
             w = mul2(w, *reinterpret_cast<const float2*>(v_scales + 2 * e));
             if (edge) {  // (a hidden value's scale may be a NaN)
@@ -642,39 +738,55 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           p[e] = half_pair(w.x, w.y);
           if constexpr (TERMS == 2) p_low[e] = left_pair(w.x, w.y, p[e]);
         }
-        part = parts.x + parts.y;
-        if (slow) break;
-        const bool over = !(part <= MOST_WEIGHT) || (CODES && now_unit > unit);
-        if constexpr (HALVES == 2) {
+        const float shown = fmaf(cubic_top, tile_m2, less);
+        return !(shown <= 120.0f) ? shown : part.x + part.y;
+      };
+      if constexpr (TERMS == 2) {
+        if (!(ok = settled())) break;
+        if (j > 0) take_output();
+        const float top = largest();
+        const bool grown = !(top <= base2 + (WEIGHT_BITS + GROWTH_BITS)) || (CODES && now_unit > unit);
+        if (__any_sync(0xffffffffu, grown)) rebase(top);
+        sum += weigh();
+      } else {
+        // the halves agree on whether the row tile's bases stay; in the first
+        // tile, and where a row without one sees keys, they do not
+        bool slow = j == 0;
+        float part = 0.0f;
+        if (!slow) {
+          part = weigh();
+          const bool sees = key0 < hi && (key0 + KEYS > lo || key0 < first);
+          const bool over = !(part <= MOST_WEIGHT) || (base2 == -INFINITY && sees) || (CODES && now_unit > unit);
           if (!ok) failed[2 * i + j % 2] = 1;
-          if (!any_of_tile(i, over || !ok)) break;
-          if (failed[2 * i + j % 2]) break;
-        } else if (!__any_sync(0xffffffffu, over)) {
-          break;
+          slow = any_of_tile(i, over || !ok);
+          if (slow && failed[2 * i + j % 2]) break;
         }
-        slow = true;
+        ok = ok && settled();
+        if (slow) {
+          volatile float* tops = between + 2 * ROW_TILE * i + r;
+          float top = largest();
+          tops[ROW_TILE * half] = top;
+          meet_tile(i);
+          top = max3(top, top, tops[ROW_TILE * (1 - half)]);
+          rebase(top);
+          part = weigh();
+        }
+        sum += part;
       }
-      // (only a tile that was met in has an answer for all: one that is taken
-      // slowly from the start is told by the next)
-      if (HALVES == 2 && failed[2 * i + j % 2] && !slow) break;
-      sum += part;
-#pragma unroll
-      for (int c = 0; c < COLUMNS / 2; c += 16) {
-        tmem_store_16(s_at + half * (COLUMNS / 2) + c, p + c);
-        if constexpr (TERMS == 2) tmem_store_16(s_at + KEYS / 2 + c, p_low + c);
-      }
+      tmem_store<COLUMNS / 2>(p_at + half * (COLUMNS / 2), p);
+      if constexpr (TERMS == 2) tmem_store<COLUMNS / 2>(p_at + COLUMNS / 2, p_low);
       tc::tmem_store_wait();
       tc::fence_before_sync();
-      tc::mbar_arrive(&p_full[b]);
+      tc::mbar_arrive(&p_full[i]);
     }
-    ok = ok && wait(&o_full[i], MT == 2 ? 0 : (tiles - 1) & 1);
+    if (ok) ok = wait(&pv_done[i], (tiles - 1) & 1);
     float all_sum = sum;
     if constexpr (HALVES == 2) {
-      volatile float* shared_sum = between + 2 * ROW_TILE * i + r;
+      volatile float* sums = between + 2 * ROW_TILE * i + r;
       meet_tile(i);  // (past the last exchange)
-      shared_sum[ROW_TILE * half] = sum;
+      sums[ROW_TILE * half] = sum;
       meet_tile(i);
-      all_sum = sum + shared_sum[ROW_TILE * (1 - half)];
+      all_sum = sum + sums[ROW_TILE * (1 - half)];
     }
     if constexpr (!(CODES && TERMS == 2)) asm volatile("bar.sync 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");  // (taken_out is final)
     if (ok) {
@@ -693,11 +805,35 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       } else if (real && half == 0) {
         *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, all_sum);
       }
-      // dimensions c .. c + 7 of the row
-      auto put = [&](int c, float (&o)[8]) {
+      // PIECE dimensions of every row at a time, through this warp's part of the
+      // row tile's q (which no product reads any more): a row to a thread goes
+      // in, a row to neighbouring threads comes out
+      constexpr int OWN = D / HALVES, ROWS = ROW_TILE * HALVES, Q = TERMS * T::Q_BYTES;
+      constexpr int PIECE = OWN % 32 == 0 && ROWS * 144 <= Q ? 32 : OWN % 16 == 0 && ROWS * 80 <= Q ? 16 : 8;
+      const bool wide = TERMS == 2 || a.part_o;
+      const int size = wide ? 4 : 2, pitch = PIECE * size + 16;
+      const long long row_bytes = (a.part_o ? (long long)a.splits : 1ll) * D * size;
+      uint8_t* out = a.part_o ? reinterpret_cast<uint8_t*>(a.part_o + (long long)split * D) : static_cast<uint8_t*>(a.out);
+      uint8_t* stage = shared + i * Q + 32 * (warp % (4 * HALVES)) * pitch;
+      static_assert(ROWS * (PIECE * 4 + 16) <= Q, "a piece of every row");
+      const int lanes_to_row = PIECE * size / 16, at_once = 32 / lanes_to_row;  // 1 to 8, 32 to 4
+      const int tile_row0 = row0 + ROW_TILE * i + 32 * (warp % 4);
+      const int tile_token0 = tile_row0 / a.group, tile_head0 = tile_row0 % a.group;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] *= scale;
-        if (!(CODES && TERMS == 2) && *taken_out) {
+      for (int c0 = 0; c0 < OWN; c0 += PIECE) {
+        const int c = half * OWN + c0;
+        float o[PIECE];
+        if constexpr (TERMS == 2) {
+#pragma unroll
+          for (int e = 0; e < PIECE; ++e) o[e] = total[c0 + e];
+        } else {
+          tmem_load_async<PIECE>(o_at + c, o);
+          tmem_load_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < PIECE; ++e) o[e] *= scale;
+        if (!(CODES && TERMS == 2) && *taken_out && real) {
+#pragma unroll 1
           for (int j = 0; j < tiles; ++j) {
             const int key0 = seen.key_of(tile0 + j);
             if (whole(key0)) continue;
@@ -706,10 +842,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
               const float y = not_finite_scale(a.value_scales + (long long)head * a.at.page_size, (long long)a.kv_heads * a.at.page_size,
                                                chunk.table, a.at.pages, a.at.page_size, key0, end, lo, first);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] += y;
+              for (int e = 0; e < PIECE; ++e) o[e] += y;
             } else {
 #pragma unroll
-              for (int e = 0; e < 8; e += 4) {
+              for (int e = 0; e < PIECE; e += 4) {
                 const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + c + e) * a.at.page_size,
                                             (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
                                             a.at.page_size, key0, end, lo, first);
@@ -718,34 +854,30 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             }
           }
         }
-        if (a.part_o || TERMS == 2) {
-          float4* to = reinterpret_cast<float4*>(a.part_o ? a.part_o + (row_at * a.splits + split) * D + c
-                                                          : static_cast<float*>(a.out) + row_at * D + c);
-          to[0] = make_float4(o[0], o[1], o[2], o[3]);
-          to[1] = make_float4(o[4], o[5], o[6], o[7]);
+        __syncwarp();  // (the piece before is out of the way)
+        uint8_t* own = stage + lane * pitch;
+        if (wide) {
+#pragma unroll
+          for (int e = 0; e < PIECE; e += 4)
+            *reinterpret_cast<float4*>(own + 4 * e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         } else {
-          __align__(16) __nv_bfloat162 y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row_at * D + c) = *reinterpret_cast<const uint4*>(y);
-        }
-      };
-      if constexpr (TERMS == 2) {
+          for (int e = 0; e < PIECE; e += 8) {
+            __align__(16) __nv_bfloat162 y[4];
 #pragma unroll
-        for (int c = 0; c < D; c += 8) {
-          float o[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = total[c + e];
-          if (real) put(c, o);
+            for (int n = 0; n < 4; ++n) y[n] = __floats2bfloat162_rn(o[e + 2 * n], o[e + 2 * n + 1]);
+            *reinterpret_cast<uint4*>(own + 2 * e) = *reinterpret_cast<const uint4*>(y);
+          }
         }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < OWN; c += 8) {
-          float o[8];
-          __syncwarp();
-          tmem_load_8(o_at + d0 + c, o);
-          if (real) put(d0 + c, o);
+        __syncwarp();
+        for (int x = lane / lanes_to_row; x < 32; x += at_once) {
+          if (tile_row0 + x >= row1) break;
+          const int x_row = tile_head0 + x, tokens = a.group > 1 ? int(__umulhi(x_row, group_magic)) : x_row;
+          const long long to = (chunk.row + tile_token0 + tokens) * a.q_heads + head * a.group + x_row - tokens * a.group;
+          *reinterpret_cast<uint4*>(out + to * row_bytes + c * size + 16 * (lane % lanes_to_row)) =
+              *reinterpret_cast<const uint4*>(stage + x * pitch + 16 * (lane % lanes_to_row));
         }
+        __syncwarp();
       }
     }
   } else if (warp == T::COPY_WARP) {
@@ -769,16 +901,32 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const int place = key % a.at.page_size;
       const int k_row = page * a.at.page_size + (page < a.at.pages ? place : 0);
       const int v_row = (page * a.kv_heads + (page < a.at.pages ? head : 0)) * D;
-      if (j >= T::COPY_STAGES && !(ok = wait(CODES ? &codes_empty[0] : &k_empty[stage], used))) break;
-      uint64_t* full = CODES ? &codes_full[0] : &k_full[stage];
+      const uint32_t codes = base + T::CODES_AT + stage * 2 * T::CODE_STAGE + lane * run * D;
+      // codes come with the scales of their pages' runs (zeros for the others')
+      const long long scales_row = ((long long)page * a.kv_heads + head) * a.at.page_size + place;
+      float* copied_scales = reinterpret_cast<float*>(shared + T::COPIED_SCALES_AT) + stage * 2 * KEYS + lane * run;
+      const bool there = page < a.at.pages;
+      const int bytes = T::CODE_BYTES + 4 * run * __popc(__ballot_sync(0xffffffffu, there));
+      auto copy_scales = [&](const float* from, float* to, uint64_t* bar) {
+        if (there) tc::bulk_load(to, from + scales_row, 4 * run, bar);
+      };
+      auto clear_scales = [&](float* to) {
+        if (CODES && lane < runs && !there)
+          for (int n = 0; n < run; n += 4) *reinterpret_cast<float4*>(to + n) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      };
+      if (j >= T::COPY_STAGES && !(ok = wait(CODES ? &codes_empty[2 * stage] : &k_empty[stage], used))) break;
+      uint64_t* full = CODES ? &codes_full[2 * stage] : &k_full[stage];
+      clear_scales(copied_scales);
+      __syncwarp();
       if (lane == 0) {
-        tc::mbar_expect_tx(full, CODES ? T::CODE_BYTES : T::K_BYTES);
+        tc::mbar_expect_tx(full, CODES ? bytes : T::K_BYTES);
         copied[0] = j + 1;
       }
       __syncwarp();
       if (lane < runs) {
         if constexpr (CODES) {
-          tma_load_3d(base + T::CODES_AT + lane * run * D, &key_map, full, 0, head, k_row);
+          tma_load_3d(codes, &key_map, full, 0, head, k_row);
+          copy_scales(a.key_scales, copied_scales, full);
         } else {
 #pragma unroll
           for (int p = 0; p < T::PANELS; ++p)
@@ -786,25 +934,26 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                         head, k_row);
         }
       }
-      if (j >= T::COPY_STAGES && !(ok = wait(CODES ? &codes_empty[1] : &v_empty[stage], used))) break;
-      full = CODES ? &codes_full[1] : &v_full[stage];
+      if (j >= T::COPY_STAGES && !(ok = wait(CODES ? &codes_empty[2 * stage + 1] : &v_empty[stage], used))) break;
+      full = CODES ? &codes_full[2 * stage + 1] : &v_full[stage];
+      clear_scales(copied_scales + KEYS);
+      __syncwarp();
       if (lane == 0) {
-        tc::mbar_expect_tx(full, CODES ? T::CODE_BYTES : T::V_BYTES);
+        tc::mbar_expect_tx(full, CODES ? bytes : T::V_BYTES);
         copied[1] = j + 1;
       }
       __syncwarp();
       if (lane < runs)
-        tma_load_2d(CODES ? base + T::CODES_AT + T::CODE_BYTES + lane * run * D
-                          : base + T::V_AT + stage * T::V_STAGE + lane * run * D * 2,
-                    &value_map, full, place, v_row);
+        tma_load_2d(CODES ? codes + T::CODE_STAGE : base + T::V_AT + stage * T::V_STAGE + lane * run * D * 2, &value_map,
+                    full, place, v_row);
+      if (CODES && lane < runs) copy_scales(a.value_scales, copied_scales + KEYS, full);
       __syncwarp();
     }
-  } else if (warp == T::MMA_WARP) {
+  } else if (warp == T::QK_WARP || warp == T::PV_WARP) {
     // ---- tensor core --------------------------------------------------------------------
     constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
-    const int run = CODES ? 64 : args.run;  // keys of a tile of V
+    const int run = CODES ? 16 : args.run;  // keys of a piece of V
     const uint32_t run_shift = run == 64 ? 2 : run == 32 ? 1 : 0, run_bytes = uint32_t(run) * D * 2;  // 2^shift steps
-    bool ok = true;
     int edges = 0;
     // (second terms first, while the sums are small)
     auto scores = [&](int j, int i, int b) {
@@ -814,24 +963,27 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const uint64_t q = operand_desc(base + (i * TERMS + term) * T::Q_BYTES, 128);
 #pragma unroll
         for (int step = 0; step < D / 16; ++step)
-          mma_ss_warp(tmem + b * KEYS, q + ((step / 4 * T::Q_PANEL + step % 4 * 32) >> 4),
+          mma_ss_warp(tmem + b * T::S_COLUMNS, q + ((step / 4 * T::Q_PANEL + step % 4 * 32) >> 4),
                       k + ((step / 4 * T::K_PANEL + step % 4 * 32) >> 4), qk, term < TERMS - 1 || step > 0);
       }
       tc::mma_commit_warp(&s_full[b]);
     };
     // (false if the weights did not come)
-    auto outputs = [&](int j, int i, int b, uint32_t phase) {
+    auto outputs = [&](int j, int i) {
       const uint64_t v = operand_desc(base + T::V_AT + (j % STAGES) * T::V_STAGE, 2 * run);
-      if (!wait(&p_full[b], phase)) return false;
+      if (!wait(&p_full[i], j & 1)) return false;
       tc::fence_after_sync();
 #pragma unroll
       for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
         for (int step = 0; step < KEYS / 16; ++step) {
           const uint32_t at = (step >> run_shift) * run_bytes + (step & ((1u << run_shift) - 1)) * 32;
-          tc::mma_f16_ts_warp(tmem + T::O_COLUMN + 128 * i, tmem + b * KEYS + term * KEYS / 2 + 8 * step, v + (at >> 4), pv,
+          tc::mma_f16_ts_warp(tmem + T::O_COLUMN + i * T::O_COLUMNS,
+                              tmem + T::P_COLUMN + i * T::P_COLUMNS + term * KEYS / 2 + 8 * step, v + (at >> 4), pv,
                               (TERMS == 1 && j > 0) || term < TERMS - 1 || step > 0);
         }
+      if (i == MT - 1) tc::mma_commit_warp(&v_empty[j % STAGES]);
+      tc::mma_commit_warp(&pv_done[i]);
       return true;
     };
     auto keys_ready = [&](int j) { return wait(&k_full[j % STAGES], (j / STAGES) & 1); };
@@ -842,67 +994,46 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (lane == 0) tc::mbar_arrive(edge_found);
       return wait(edge_clean, edges++ & 1);
     };
-    for (int i = 0; i < MT && ok; ++i) ok = wait(&q_full[i], 0);
-    if (ok) ok = keys_ready(0);
-    if (ok) {
-      tc::fence_after_sync();
-      for (int i = 0; i < MT; ++i) scores(0, i, i);
-      tc::mma_commit_warp(&k_empty[0]);
+    // scores of tile j (two row tiles: when theirs of the last are read; with
+    // two S, when those of the one before are)
+    auto next_scores = [&](int j) {
+      if (!keys_ready(j)) return false;
+      for (int i = 0; i < MT; ++i) {
+        const int b = MT == 2 ? i : j & 1;
+        if (MT == 2 && j > 0 && !wait(&s_empty[b], (j - 1) & 1)) return false;
+        if (MT == 1 && j > 1 && !wait(&s_empty[b], ((j - 2) >> 1) & 1)) return false;
+        tc::fence_after_sync();
+        scores(j, i, b);
+      }
+      tc::mma_commit_warp(&k_empty[j % STAGES]);
+      return true;
+    };
+    bool ok = true;
+    const bool does_scores = warp == T::QK_WARP, does_outputs = warp == T::PV_WARP;
+    if (does_scores) {
+      for (int i = 0; i < MT && ok; ++i) ok = wait(&q_full[i], 0);
+      if (ok) ok = next_scores(0);
     }
     for (int j = 0; j < tiles && ok; ++j) {
-      if constexpr (MT == 2) {
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (i == 0 && !(ok = values_ready(j))) break;
-          if (!(ok = outputs(j, i, i, j & 1))) break;
-          if (i == 1) tc::mma_commit_warp(&v_empty[j % STAGES]);
-          if (j + 1 == tiles) {
-            tc::mma_commit_warp(&o_full[i]);
-            continue;
-          }
-          if (i == 0 && !(ok = keys_ready(j + 1))) break;
-          scores(j + 1, i, i);
-          if (i == 1) tc::mma_commit_warp(&k_empty[(j + 1) % STAGES]);
-        }
-      } else {
-        if (j + 1 < tiles) {
-          if (!(ok = keys_ready(j + 1))) break;
-          scores(j + 1, 0, (j + 1) & 1);
-          tc::mma_commit_warp(&k_empty[(j + 1) % STAGES]);
-        }
-        if (!(ok = values_ready(j))) break;
-        if (!(ok = outputs(j, 0, j & 1, (j >> 1) & 1))) break;
-        tc::mma_commit_warp(&v_empty[j % STAGES]);
-        tc::mma_commit_warp(&o_full[0]);
-      }
+      if (does_scores && j + 1 < tiles && !(ok = next_scores(j + 1))) break;
+      if (!does_outputs) continue;
+      if (!(ok = values_ready(j))) break;
+      for (int i = 0; i < MT && ok; ++i) ok = outputs(j, i);
     }
   } else if (CODES && warp >= T::CONVERT_WARP) {
     // ---- conversion: codes to F16 operands, and the tile's scales ------------------------
     constexpr int N = T::CONVERT_THREADS, CHUNKS = D / 16;  // 16-byte chunks of a key's codes
     const int t = tid - 32 * T::CONVERT_WARP;
     const int run = args.run;
-    const uint8_t* k_codes = shared + T::CODES_AT;
-    const uint8_t* v_codes = k_codes + T::CODE_BYTES;
     auto seen_key = [&](int key) { return key < seen.end && (key >= lowest || key < first); };
-    // where the scales of the sixteen keys around `key` are, or -1
-    auto scales_at = [&](int key) {
-      const int page = key < seen.end ? chunk.table[key / a.at.page_size] : -1;
-      if (page < 0 || page >= a.at.pages) return -1ll;
-      return ((long long)page * a.kv_heads + head) * a.at.page_size + key % a.at.page_size;
-    };
-    // the scales of tile j, of every 32nd key from this lane's, zeros where no
-    // row sees the key (each warp finds the largest for itself)
-    constexpr int PER = KEYS / 32;
-    auto load_scales = [&](int j, float (&k)[PER], float (&v)[PER]) {
-      const int key0 = seen.key_of(tile0 + j);
+    // a tile's scales, of every 32nd key from this lane's, zeros where no row
+    // sees the key (each warp finds the largest for itself)
+    constexpr int PER = (KEYS + 31) / 32;
+    auto load_scales = [&](int key0, bool check, const float* from, float (&x)[PER]) {
 #pragma unroll
       for (int n = 0; n < PER; ++n) {
-        k[n] = v[n] = 0.0f;
-        const int key = key0 + lane + 32 * n;
-        if (!seen_key(key)) continue;
-        const long long at = scales_at(key);
-        if (at < 0) continue;
-        k[n] = a.key_scales[at];
-        v[n] = a.value_scales[at];
+        const int k = lane + 32 * n;
+        x[n] = k < KEYS && (!check || seen_key(key0 + k)) ? from[k] : 0.0f;
       }
     };
     auto largest_of = [](const float (&x)[PER]) {  // of those that are finite
@@ -920,28 +1051,33 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
       return __uint_as_float(max(up, least));
     };
-    float k_scale[PER], v_scale[PER], v_power = 0.0f;
-    load_scales(0, k_scale, v_scale);
+    float v_power = 0.0f;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       const int stage = j % STAGES, key0 = seen.key_of(tile0 + j);
       const uint32_t used = ((j / STAGES) & 1) ^ 1;
+      const int copy_stage = j % T::COPY_STAGES;
+      const uint32_t copy_phase = (j / T::COPY_STAGES) & 1;
+      const uint8_t* k_codes = shared + T::CODES_AT + copy_stage * 2 * T::CODE_STAGE;
+      const uint8_t* v_codes = k_codes + T::CODE_STAGE;
       // keys: a thread takes a row (or, of 64 rows, half of one)
-      const int row = t % KEYS;
-      float own_k = k_scale[0], own_v = v_scale[0];
-#pragma unroll
-      for (int n = 1; n < PER; ++n) {
-        own_k = n == row / 32 ? k_scale[n] : own_k;
-        own_v = n == row / 32 ? v_scale[n] : own_v;
-      }
+      constexpr int TO_ROW = N >= 2 * KEYS ? 2 : 1;  // threads
+      const int row = TO_ROW == 2 ? t % KEYS : t;
+      const bool has_row = row < KEYS;
+      const float* k_from = reinterpret_cast<const float*>(shared + T::COPIED_SCALES_AT) + copy_stage * 2 * KEYS;
+      const float* v_from = k_from + KEYS;
+      const bool check = !whole(key0);
+      if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
+      if (!(ok = wait(&codes_full[2 * copy_stage], copy_phase))) break;
+      float k_scale[PER];
+      load_scales(key0, check, k_from, k_scale);
+      const float own_k = has_row && (!check || seen_key(key0 + row)) ? k_from[row] : 0.0f;
       // (2^-64 at least: the scores' factor stays normal with it)
       const float k_power = power_over(largest_of(k_scale), 0x1f800000u);
-      if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
-      if (!(ok = wait(&codes_full[0], j & 1))) break;
-      {
+      if (has_row) {
         uint8_t* k = shared + T::K_AT + stage * T::K_BYTES + row * 128;
-        constexpr int TAKES = KEYS * CHUNKS / N;  // chunks a thread takes
-        const int c0 = t / KEYS * TAKES;
+        constexpr int TAKES = CHUNKS / TO_ROW;  // chunks a thread takes
+        const int c0 = TO_ROW == 2 ? t / KEYS * TAKES : 0;
         // the scale over the tile's power of two in two F16 terms
         const float ratio = own_k * (1.0f / k_power);
         const __half ratio_hi = __float2half_rn(ratio);
@@ -967,40 +1103,41 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&k_full[stage]);
-      tc::mbar_arrive(&codes_empty[0]);
+      tc::mbar_arrive(&codes_empty[2 * copy_stage]);
       // scales: the stage's were last read by the softmax before the P V that
       // freed its values
       if (j >= STAGES && !(ok = wait(&v_empty[stage], used))) break;
+      if (!(ok = wait(&codes_full[2 * copy_stage + 1], copy_phase))) break;
+      float v_scale[PER];
+      load_scales(key0, check, v_from, v_scale);
       const float most = largest_of(v_scale);
       if (most > v_power) v_power = power_over(most, 0x01000000u);
       const float v_inverse = 1.0f / (v_power > 0.0f ? v_power : 1.0f);
       if (TERMS == 2) {
         scales[stage * 2 * KEYS + row] = own_k;
-        scales[stage * 2 * KEYS + KEYS + row] = own_v * v_inverse;
+        scales[stage * 2 * KEYS + KEYS + row] = !check || seen_key(key0 + row) ? v_from[row] * v_inverse : 0.0f;
       }
       if (t == 0) k_unit[stage] = k_power, v_unit[stage] = v_power;
       tc::mbar_arrive(&scales_full[stage]);
-      if (j + 1 < tiles) load_scales(j + 1, k_scale, v_scale);
       // values: a thread takes sixteen positions of every (DIMS)th dimension
-      constexpr int DIMS = N / (KEYS / 16);
+      constexpr int GROUPS = KEYS / 16, DIMS = N / GROUPS;
       const int per = run / 16;
       const int group = t % per + per * (t / (DIMS * per)), first_d = t / per % DIMS;
+      const bool has_group = group < GROUPS;
       __half2 ratios[8];
       if constexpr (TERMS == 1) {
         const int key = key0 + 16 * group;
-        const long long at = scales_at(key);
-        const bool check = !whole(key0);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (at >= 0) x = *reinterpret_cast<const float4*>(a.value_scales + at + 4 * n);
+          if (has_group) x = *reinterpret_cast<const float4*>(v_from + 16 * group + 4 * n);
           float y[4] = {x.x, x.y, x.z, x.w};
           if (check) {
             // (at an edge, what is not finite is taken out for the rows that
             // do not see it)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if (!seen_key(key + 4 * n + e)) y[e] = 0.0f;
+              if (!has_group || !seen_key(key + 4 * n + e)) y[e] = 0.0f;
               else if (!isfinite(y[e])) y[e] = 0.0f, *taken_out = 1;
             }
           }
@@ -1008,9 +1145,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           ratios[2 * n + 1] = __floats2half2_rn(y[2] * v_inverse, y[3] * v_inverse);
         }
       }
-      if (!(ok = wait(&codes_full[1], j & 1))) break;
-      {
-        uint8_t* v = shared + T::V_AT + stage * T::V_STAGE + group / 4 * (D * 128);
+      if (has_group) {
+        uint8_t* v = shared + T::V_AT + stage * T::V_STAGE + group * (D * 32);
         const uint8_t* from = v_codes + group / per * (run * D) + group % per * 16;
         auto scaled = [&](uint32_t pair, int n) {
           if constexpr (TERMS == 2) return pair;
@@ -1021,20 +1157,18 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         for (int d = first_d; d < D; d += DIMS) {
           const uint4 x = *reinterpret_cast<const uint4*>(from + d * run);
           const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
-          uint8_t* to = v + d * 128;
-          const int c = 2 * (group % 4);
-          *reinterpret_cast<uint4*>(to + 16 * (c ^ (d % 8))) =
-              make_uint4(scaled(y0.x, 0), scaled(y0.y, 1), scaled(y1.x, 2), scaled(y1.y, 3));
-          *reinterpret_cast<uint4*>(to + 16 * ((c + 1) ^ (d % 8))) =
-              make_uint4(scaled(y2.x, 4), scaled(y2.y, 5), scaled(y3.x, 6), scaled(y3.y, 7));
+          uint8_t* to = v + d * 32;  // (rows of 32 bytes, their halves exchanged in every other four)
+          const int c = d / 4 % 2;
+          *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(scaled(y0.x, 0), scaled(y0.y, 1), scaled(y1.x, 2), scaled(y1.y, 3));
+          *reinterpret_cast<uint4*>(to + 16 * (1 - c)) = make_uint4(scaled(y2.x, 4), scaled(y2.y, 5), scaled(y3.x, 6), scaled(y3.y, 7));
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&v_full[stage]);
-      tc::mbar_arrive(&codes_empty[1]);
+      tc::mbar_arrive(&codes_empty[2 * copy_stage + 1]);
     }
     if constexpr (TERMS == 1) asm volatile("bar.arrive 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");
-  } else if (!CODES && warp >= T::EDGE_WARP) {
+  } else if (!CODES && warp == T::EDGE_WARP) {
     // ---- edges: values that are not finite, out of the tiles seen in part -----------------
     bool ok = true;
     int edges = 0;
@@ -1046,7 +1180,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (!(ok = wait(&v_full[j % STAGES], (j / STAGES) & 1))) break;
       uint8_t* v = shared + T::V_AT + (j % STAGES) * T::V_STAGE;
       bool found = false;
-      for (int n = tid - 32 * T::EDGE_WARP; n < T::V_BYTES / 16; n += EDGE_THREADS) {
+      for (int n = tid - 32 * T::EDGE_WARP; n < T::V_BYTES / 16; n += T::EDGE_THREADS) {
         uint4 x = *reinterpret_cast<uint4*>(v + 16 * n);
         uint32_t* w = reinterpret_cast<uint32_t*>(&x);
         bool bad = false;
@@ -1080,11 +1214,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     if (tid == 32 * T::COPY_WARP)
       for (int side = 0; side < 2; ++side) {
         const int n = copied[side];
-        uint64_t* full = CODES ? &codes_full[side] : side == 0 ? k_full : v_full;
+        uint64_t* full = CODES ? codes_full + side : side == 0 ? k_full : v_full;
         for (int j = max(0, n - T::COPY_STAGES); j < n; ++j)
-          tc::mbar_wait(&full[j % T::COPY_STAGES], (j / T::COPY_STAGES) & 1, &none, nullptr);
+          tc::mbar_wait(&full[j % T::COPY_STAGES * (CODES ? 2 : 1)], (j / T::COPY_STAGES) & 1, &none, nullptr);
       }
-    if (warp == T::MMA_WARP) {
+    if (warp == T::QK_WARP || warp == T::PV_WARP) {
       tc::mma_commit_warp(drained);
       tc::mbar_wait_warp(drained, 0, &none, nullptr);
     }
@@ -1093,9 +1227,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   if (warp == 0) tc::tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
-// Keys of a tile: 64 where a wider one's scores (two terms of weights and the
-// running output), or its keys and values beside q, do not fit.
-constexpr int tile_of(int head_dim, int terms) { return head_dim > 128 || terms == 2 ? 64 : 128; }
+// Keys of a tile: what TMEM holds beside the outputs (P_COLUMN's assertion);
+// F32 rows and heads of 256 have no room in registers or shared memory for more.
+constexpr int tile_of(int head_dim, int terms) {
+  return terms == 2 || head_dim > 128 ? 64 : head_dim > 80 ? 80 : head_dim > 64 ? 96 : 128;
+}
 
 template <int D, int MT, bool CODES, int TERMS>
 int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
@@ -1103,7 +1239,8 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
   TileArgs args;
   args.a = a;
   const int ps = a.at.page_size;
-  args.run = ps % 64 == 0 ? 64 : ps % 32 == 0 ? 32 : 16;
+  // the largest piece that pages and tiles are made of
+  args.run = ps % 64 == 0 && T::KEYS % 64 == 0 ? 64 : ps % 32 == 0 && T::KEYS % 32 == 0 ? 32 : 16;
   const uint64_t positions = uint64_t(a.at.pages) * ps;
   constexpr uint64_t SIZE = CODES ? 1 : 2;
   CUtensorMap key_map, value_map;

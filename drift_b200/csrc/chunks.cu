@@ -335,6 +335,8 @@ int check_chunks(const char* call, int x_dtype, long long tokens, int kv_heads, 
   if (cache_dtype == DRIFT_I8 && (!key_scales || !value_scales)) return invalid("%s: an 8-bit cache without scales", call);
   if ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15)
     return invalid("%s: the cache does not start on a 16-byte boundary", call);
+  if ((reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales)) & 15)
+    return invalid("%s: the cache's scales do not start on a 16-byte boundary", call);
   return 0;
 }
 
