@@ -75,11 +75,6 @@ constexpr uint32_t TMEM_COLUMNS = 512;
 // and the base moves when a tile's weights sum to more than MOST_WEIGHT (F32
 // rows: when one would pass 2^(WEIGHT_BITS + GROWTH_BITS)).
 constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f, MOST_WEIGHT = 32768.0f;
-// Of eight pairs of BF16 rows' weights, those made by exp2_cubic.
-#ifndef CUBIC
-#define CUBIC 3
-#endif
-constexpr int CUBIC_PAIRS = CUBIC;
 // A row of q is 2^Q_BITS and more at its largest value, so that its second
 // terms end far below F16's last bit, 2^-24.
 constexpr int Q_BITS = 8;
@@ -89,10 +84,7 @@ struct TileTraits {
   static constexpr int D = D_, KEYS = KEYS_, MT = MT_, TERMS = TERMS_;
   static constexpr bool CODES = CODES_;
   static constexpr int UNIT = ROW_TILE * MT;
-  // Two threads share a row of BF16, half of a tile's columns each: with one
-  // to a row, two warps to a scheduler, an instruction took 3.7 clocks.
-  static constexpr int HALVES = TERMS == 1 ? 2 : 1, COLUMNS = KEYS / HALVES;
-  static constexpr int SOFTMAX_WARPS = 4 * MT * HALVES;
+  static constexpr int SOFTMAX_WARPS = 4 * MT;
   // Q K^T and P V have a warp each: a wait costs one about 100 clocks even when
   // there is nothing to wait for, and six of them and the products' issue were
   // longer than the products (for the codes of F32 rows they are not).
@@ -108,7 +100,7 @@ struct TileTraits {
   static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4 + (WIDE ? 4 : 0));
   static constexpr bool MOVES_REGISTERS = MT == 2;  // (128 a thread and more are there otherwise)
   static constexpr int LAUNCH_REGISTERS = 65536 / THREADS / 8 * 8;
-  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : 64;
+  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : WIDE ? 64 : 88;
   static constexpr int SOFTMAX_REGISTERS =
       (THREADS * LAUNCH_REGISTERS - (THREADS - 32 * SOFTMAX_WARPS) * OTHER_REGISTERS) / (32 * SOFTMAX_WARPS) / 8 * 8;
   static_assert(!MOVES_REGISTERS || SOFTMAX_REGISTERS <= 248, "a thread's registers");
@@ -128,8 +120,7 @@ struct TileTraits {
   // its stage is free are a tile's time)
   static constexpr int bytes_of(int stages, int code_stages) {
     return K_AT + stages * (K_BYTES + V_STAGE) + (CODES ? code_stages * 2 * CODE_STAGE : 0) +
-           (CODES && TERMS == 2 ? stages * 2 * KEYS * 4 : 0) + (CODES ? code_stages * 2 * KEYS * 4 : 0) +
-           (HALVES == 2 ? MT * 2 * ROW_TILE * 4 : 0) + 384;
+           (CODES && TERMS == 2 ? stages * 2 * KEYS * 4 : 0) + (CODES ? code_stages * 2 * KEYS * 4 : 0) + 384;
   }
   static constexpr int LIMIT = 232448;
   static constexpr int CODE_STAGES = bytes_of(2, 2) <= LIMIT ? 2 : 1;
@@ -139,9 +130,8 @@ struct TileTraits {
   static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;  // [COPY_STAGES][2]
   static constexpr int SCALES_AT = CODES_AT + (CODES ? COPY_STAGES * 2 * CODE_STAGE : 0);  // [STAGES][2][KEYS]
   static constexpr int COPIED_SCALES_AT = SCALES_AT + (CODES && TERMS == 2 ? STAGES * 2 * KEYS * 4 : 0);  // [COPY_STAGES][2][KEYS]
-  static constexpr int BETWEEN_AT = COPIED_SCALES_AT + (CODES ? COPY_STAGES * 2 * KEYS * 4 : 0);  // [MT][2][ROW_TILE]
-  static constexpr int BARRIERS_AT = BETWEEN_AT + (HALVES == 2 ? MT * 2 * ROW_TILE * 4 : 0);
-  static constexpr int BYTES = BARRIERS_AT + 384;  // 36 barriers and a few words
+  static constexpr int BARRIERS_AT = COPIED_SCALES_AT + (CODES ? COPY_STAGES * 2 * KEYS * 4 : 0);
+  static constexpr int BYTES = BARRIERS_AT + 384;  // 38 barriers and a few words
   // TMEM: S of row tile i, or (MT = 1) of every other tile; P and O of row tile i
   static constexpr int S_COLUMNS = (KEYS + 31) / 32 * 32;
   static constexpr int P_COLUMN = S_COLUMNS + KEYS, P_COLUMNS = TERMS * KEYS / 2;
@@ -281,19 +271,6 @@ __device__ __forceinline__ void tmem_store(uint32_t address, const uint32_t* r) 
   }
 }
 
-// Whether some thread of the 256 of a row tile has `any` (one answer for all;
-// and they meet).
-__device__ __forceinline__ bool any_of_tile(int tile, bool any) {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-               "barrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-               : "=r"(r)
-               : "r"(uint32_t(any)), "r"(3 + tile)
-               : "memory");
-  return r != 0;
-}
-__device__ __forceinline__ void meet_tile(int tile) { asm volatile("bar.sync %0, 256;" ::"r"(5 + tile) : "memory"); }
-
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -334,32 +311,6 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
-}
-
-// 2^x of a pair's x = s factor + less on the multiply-add units, to 8e-5 (a
-// sixth of F16's rounding), x held between -126 and 126 (a NaN becomes -126).
-// The caller gives a = factor / 252 and b = less / 252 + 1/2, whose saturating
-// product and sum is x / 252 + 1/2. x = n + f with |f| <= 1/2, by the F32 sum
-// that has no room for a fraction; a cubic in f (least squares on Chebyshev
-// points, reweighted towards the least largest relative error), and n added to
-// its exponent. The special function unit gives a warp's 32 values in 8
-// clocks: 1280 for 80 keys of 256 rows on a scheduler, beside the tensor
-// core's 1440; of eight pairs three made here, in 14 clocks of the multiply-add
-// units each, leave it 800.
-__device__ __forceinline__ float2 exp2_cubic(float s0, float s1, float a, float b) {
-  float2 y;
-  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(y.x) : "f"(s0), "f"(a), "f"(b));
-  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(y.y) : "f"(s1), "f"(a), "f"(b));
-  constexpr float WHOLE = 12582912.0f;  // 1.5 x 2^23
-  const float2 by = make_float2(252.0f, 252.0f);
-  const float2 t = fma2(y, by, make_float2(WHOLE - 126.0f, WHOLE - 126.0f));                  // n + WHOLE
-  const float2 n = fma2(t, make_float2(-1.0f, -1.0f), make_float2(WHOLE - 126.0f, WHOLE - 126.0f));  // -(n + 126)
-  const float2 f = fma2(y, by, n);
-  float2 p = fma2(f, make_float2(0.05517164245247841f, 0.05517164245247841f), make_float2(0.2426111251115799f, 0.2426111251115799f));
-  p = fma2(f, p, make_float2(0.6932609677314758f, 0.6932609677314758f));
-  p = fma2(f, p, make_float2(0.9999280571937561f, 0.9999280571937561f));
-  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(p.x)),
-                     __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
 }
 
 __device__ __forceinline__ uint32_t half_pair(float a, float b) {
@@ -409,7 +360,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                        const TileArgs args) {
   constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
   constexpr bool CODES = T::CODES;
-  constexpr int HALVES = T::HALVES, COLUMNS = T::COLUMNS;
   using X = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
@@ -453,9 +403,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   uint64_t* s_empty = s_full + 2;           // [2]
   uint64_t* p_full = s_empty + 2;           // [2]: of row tile i
   uint64_t* pv_done = p_full + 2;           // [2]: P is read, O written
-  uint64_t* edge_found = pv_done + 2;       // an edge tile's values are there; they are clean
-  uint64_t* edge_clean = edge_found + 1;
-  uint64_t* codes_full = edge_clean + 1;    // [COPY_STAGES][2]: of the keys, of the values
+  uint64_t* edge_found = pv_done + 2;       // [2] each, of every other edge tile (two may be under way):
+  uint64_t* edge_clean = edge_found + 2;    // its values are there; they are clean
+  uint64_t* codes_full = edge_clean + 2;    // [COPY_STAGES][2]: of the keys, of the values
   uint64_t* codes_empty = codes_full + 4;   // [COPY_STAGES][2]
   uint64_t* drained = codes_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
@@ -464,17 +414,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   volatile int* copied = abort + 2;         // [2]: tiles whose keys, values were asked for
   volatile float* k_unit = reinterpret_cast<volatile float*>(abort + 4);  // [STAGES]: the scales' powers of two
   volatile float* v_unit = k_unit + STAGES;
-  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 5 + 2 * STAGES);  // [2][2]: a wait of row tile i
-                                                                                     // gave up, in an even or odd tile
-  volatile float* between = reinterpret_cast<volatile float*>(shared + T::BETWEEN_AT);  // what a row's halves exchange
   float* scales = reinterpret_cast<float*>(shared + T::SCALES_AT);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&q_full[i], ROW_TILE * HALVES);
+      tc::mbar_init(&q_full[i], ROW_TILE);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&s_empty[i], ROW_TILE * HALVES);
-      tc::mbar_init(&p_full[i], ROW_TILE * HALVES);
+      tc::mbar_init(&s_empty[i], ROW_TILE);
+      tc::mbar_init(&p_full[i], ROW_TILE);
       tc::mbar_init(&pv_done[i], 1);
     }
     for (int s = 0; s < STAGES; ++s) {
@@ -488,13 +435,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_init(&codes_full[s], 1);
       tc::mbar_init(&codes_empty[s], T::CONVERT_THREADS);
     }
-    tc::mbar_init(edge_found, 1);
-    tc::mbar_init(edge_clean, T::EDGE_THREADS);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&edge_found[i], 1);
+      tc::mbar_init(&edge_clean[i], T::EDGE_THREADS);
+    }
     tc::mbar_init(drained, 1 + T::TWO_ISSUE);
     *abort = 0;
     *taken_out = 0;
     copied[0] = copied[1] = 0;
-    failed[0] = failed[1] = failed[2] = failed[3] = 0;
     tc::fence_barrier_init();
   }
   __syncwarp();
@@ -510,8 +458,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   }
 
   if (warp < T::SOFTMAX_WARPS) {
-    // ---- softmax: this thread's row of row tile i (of a tile's columns, its half) -----------
-    const int i = warp / (4 * HALVES), half = HALVES == 2 ? warp / 4 % 2 : 0, r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
+    // ---- softmax: this thread's row of row tile i --------------------------------------
+    const int i = warp / 4, r = tid % ROW_TILE, row = row0 + ROW_TILE * i + r;
     const bool real = row < row1;
     const int token = (real ? row : row1 - 1) / a.group, q_head = head * a.group + row % a.group;
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
@@ -542,7 +490,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       };
       multiplier = 0.0f;
 #pragma unroll 1
-      for (int pass0 = half * (PASSES / HALVES); pass0 < (half + 1) * (PASSES / HALVES); pass0 += FLIGHT) {
+      for (int pass0 = 0; pass0 < PASSES; pass0 += FLIGHT) {
         uint4 held[FLIGHT][TERMS];
 #pragma unroll
         for (int n = 0; n < FLIGHT; ++n) load(pass0 + n, held[n]);
@@ -565,12 +513,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const float unit_inverse = __uint_as_float(0x7f000000u - exponent);
           const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
           const int pass = pass0 + n;
-          if constexpr (HALVES == 2) {
-            if (c == 0) between[2 * ROW_TILE * i + 32 * (warp % 4) + pass * AT_ONCE + part] = __uint_as_float(exponent);
-          } else {
-            const uint32_t own = __shfl_sync(0xffffffffu, exponent, lane % AT_ONCE * LANES);
-            if (lane / AT_ONCE == pass) multiplier = fabsf(a.scale) * __uint_as_float(own);
-          }
+          const uint32_t own = __shfl_sync(0xffffffffu, exponent, lane % AT_ONCE * LANES);
+          if (lane / AT_ONCE == pass) multiplier = fabsf(a.scale) * __uint_as_float(own);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= by;
           const uint4 hi = make_uint4(half_pair(x[0], x[1]), half_pair(x[2], x[3]), half_pair(x[4], x[5]), half_pair(x[6], x[7]));
@@ -587,11 +531,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&q_full[i]);
-      if constexpr (HALVES == 2) {
-        meet_tile(i);
-        multiplier = fabsf(a.scale) * between[2 * ROW_TILE * i + r];
-        meet_tile(i);
-      }
     }
     // (a softcap leaves natural units behind)
     // (and a factor of 2^-60 is as good as none; times a tile's power it is normal)
@@ -627,13 +566,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
-      // (a row's halves leave the loop together: they meet in it)
-      ok = ok && wait(&s_full[b], MT == 2 ? j & 1 : (j >> 1) & 1);
-      if (CODES) ok = ok && wait(&scales_full[stage], (j / STAGES) & 1);
-      if (HALVES == 1 && !ok) break;
+      if (!(ok = wait(&s_full[b], MT == 2 ? j & 1 : (j >> 1) & 1))) break;
+      if (CODES && !(ok = wait(&scales_full[stage], (j / STAGES) & 1))) break;
       tc::fence_after_sync();
-      float s[COLUMNS];
-      tmem_load_async<COLUMNS>(tmem + lanes + b * T::S_COLUMNS + half * COLUMNS, s);
+      float s[KEYS];
+      tmem_load_async<KEYS>(tmem + lanes + b * T::S_COLUMNS, s);
       tmem_load_wait();
       tc::fence_before_sync();
       tc::mbar_arrive(&s_empty[b]);
@@ -646,7 +583,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const float now_unit = CODES ? float(v_unit[stage]) : 0.0f;
       if constexpr (CODES && TERMS == 2) {
 #pragma unroll
-        for (int c = 0; c < COLUMNS; c += 4) {
+        for (int c = 0; c < KEYS; c += 4) {
           const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
           const float2 u = mul2(make_float2(s[c], s[c + 1]), make_float2(x.x, x.y));
           const float2 v = mul2(make_float2(s[c + 2], s[c + 3]), make_float2(x.z, x.w));
@@ -656,13 +593,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (a.softcap > 0.0f) {
         const float inverse = multiplier * by_unit / a.softcap;
 #pragma unroll
-        for (int c = 0; c < COLUMNS; ++c) s[c] = capped(s[c], inverse, a.softcap);
+        for (int c = 0; c < KEYS; ++c) s[c] = capped(s[c], inverse, a.softcap);
       }
       const bool edge = !(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first));
       if (edge) {
-        const int own0 = key0 + half * COLUMNS, end = hi - own0, low = lo - own0, head_end = first - own0;
+        const int end = hi - key0, low = lo - key0, head_end = first - key0;
 #pragma unroll
-        for (int c = 0; c < COLUMNS; ++c)
+        for (int c = 0; c < KEYS; ++c)
           if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
       }
       // P and O are free (and O complete) when the last tile's P V is done
@@ -686,47 +623,37 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         if constexpr (TERMS == 2) {
 #pragma unroll
           for (int c = 0; c < D; ++c) total[c] *= g;
-        } else if (j > 0 && ok) {
+        } else if (j > 0) {
 #pragma unroll 1
-          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 8) {
-            float o[8];
-            tmem_load_8_async(o_at + c, o);
-            tmem_load_wait();
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tmem_load_16(o_at + c, o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] *= g;
-            tmem_store_8(o_at + c, reinterpret_cast<const uint32_t*>(o));
+            for (int e = 0; e < 16; ++e) o[e] *= g;
+            tmem_store_16(o_at + c, reinterpret_cast<const uint32_t*>(o));
           }
         }
       };
       auto largest = [&]() {
         float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < COLUMNS - 4; c += 8)
+        for (int c = 4; c < KEYS - 4; c += 8)
 #pragma unroll
           for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[COLUMNS - 4 + n]);
+        for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[KEYS - 4 + n]);
         return max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * tile_m2;
       };
-      uint32_t p[COLUMNS / 2], p_low[TERMS == 2 ? COLUMNS / 2 : 1];
-      // the weights and their sum (a tile's own: short chains); a NaN, or
-      // weights past any use, if exp2_cubic was given what it cannot show
+      uint32_t p[KEYS / 2], p_low[TERMS == 2 ? KEYS / 2 : 1];
+      // the weights and their sum (a tile's own: short chains)
       auto weigh = [&]() {
         // (a NaN makes the whole row NaNs)
         const float less = not_a_number ? __int_as_float(0x7fc00000) : base2 == -INFINITY ? 0.0f : -base2;
         float2 part = make_float2(0.0f, 0.0f);
-        const float cubic_a = tile_m2 * (1.0f / 252.0f), cubic_b = fmaf(less, 1.0f / 252.0f, 0.5f);
-        float cubic_top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < COLUMNS / 2; ++e) {
-          float2 w;
-          if (TERMS == 1 && e % 8 < CUBIC_PAIRS) {
-            cubic_top = max3(cubic_top, s[2 * e], s[2 * e + 1]);
-            w = exp2_cubic(s[2 * e], s[2 * e + 1], cubic_a, cubic_b);
-          } else {
-            w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
-            w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
-          }
+        for (int e = 0; e < KEYS / 2; ++e) {
+          float2 w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
+          w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
           part = add2(part, w);
           if constexpr (CODES && TERMS == 2) {
             w = mul2(w, *reinterpret_cast<const float2*>(v_scales + 2 * e));
@@ -738,8 +665,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           p[e] = half_pair(w.x, w.y);
           if constexpr (TERMS == 2) p_low[e] = left_pair(w.x, w.y, p[e]);
         }
-        const float shown = fmaf(cubic_top, tile_m2, less);
-        return !(shown <= 120.0f) ? shown : part.x + part.y;
+        return part.x + part.y;
       };
       if constexpr (TERMS == 2) {
         if (!(ok = settled())) break;
@@ -749,45 +675,31 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         if (__any_sync(0xffffffffu, grown)) rebase(top);
         sum += weigh();
       } else {
-        // the halves agree on whether the row tile's bases stay; in the first
-        // tile, and where a row without one sees keys, they do not
+        // the bases stay unless a weight might not fit; in the first tile, and
+        // where a row without one sees keys, they are set
         bool slow = j == 0;
         float part = 0.0f;
         if (!slow) {
           part = weigh();
           const bool sees = key0 < hi && (key0 + KEYS > lo || key0 < first);
           const bool over = !(part <= MOST_WEIGHT) || (base2 == -INFINITY && sees) || (CODES && now_unit > unit);
-          if (!ok) failed[2 * i + j % 2] = 1;
-          slow = any_of_tile(i, over || !ok);
-          if (slow && failed[2 * i + j % 2]) break;
+          slow = __any_sync(0xffffffffu, over);
         }
-        ok = ok && settled();
+        if (!(ok = settled())) break;
         if (slow) {
-          volatile float* tops = between + 2 * ROW_TILE * i + r;
-          float top = largest();
-          tops[ROW_TILE * half] = top;
-          meet_tile(i);
-          top = max3(top, top, tops[ROW_TILE * (1 - half)]);
-          rebase(top);
+          rebase(largest());
           part = weigh();
         }
         sum += part;
       }
-      tmem_store<COLUMNS / 2>(p_at + half * (COLUMNS / 2), p);
-      if constexpr (TERMS == 2) tmem_store<COLUMNS / 2>(p_at + COLUMNS / 2, p_low);
+      tmem_store<KEYS / 2>(p_at, p);
+      if constexpr (TERMS == 2) tmem_store<KEYS / 2>(p_at + KEYS / 2, p_low);
       tc::tmem_store_wait();
       tc::fence_before_sync();
       tc::mbar_arrive(&p_full[i]);
     }
     if (ok) ok = wait(&pv_done[i], (tiles - 1) & 1);
     float all_sum = sum;
-    if constexpr (HALVES == 2) {
-      volatile float* sums = between + 2 * ROW_TILE * i + r;
-      meet_tile(i);  // (past the last exchange)
-      sums[ROW_TILE * half] = sum;
-      meet_tile(i);
-      all_sum = sum + sums[ROW_TILE * (1 - half)];
-    }
     if constexpr (!(CODES && TERMS == 2)) asm volatile("bar.sync 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");  // (taken_out is final)
     if (ok) {
       tc::fence_after_sync();
@@ -802,30 +714,28 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           scale *= f;
         }
         scale = all_sum != 0.0f ? scale / all_sum : 0.0f;
-      } else if (real && half == 0) {
+      } else if (real) {
         *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, all_sum);
       }
       // PIECE dimensions of every row at a time, through this warp's part of the
       // row tile's q (which no product reads any more): a row to a thread goes
       // in, a row to neighbouring threads comes out
-      constexpr int OWN = D / HALVES, ROWS = ROW_TILE * HALVES, Q = TERMS * T::Q_BYTES;
-      constexpr int PIECE = OWN % 32 == 0 && ROWS * 144 <= Q ? 32 : OWN % 16 == 0 && ROWS * 80 <= Q ? 16 : 8;
+      constexpr int PIECE = D % 32 == 0 && ROW_TILE * 144 <= TERMS * T::Q_BYTES ? 32 : 16;
       const bool wide = TERMS == 2 || a.part_o;
       const int size = wide ? 4 : 2, pitch = PIECE * size + 16;
       const long long row_bytes = (a.part_o ? (long long)a.splits : 1ll) * D * size;
       uint8_t* out = a.part_o ? reinterpret_cast<uint8_t*>(a.part_o + (long long)split * D) : static_cast<uint8_t*>(a.out);
-      uint8_t* stage = shared + i * Q + 32 * (warp % (4 * HALVES)) * pitch;
-      static_assert(ROWS * (PIECE * 4 + 16) <= Q, "a piece of every row");
-      const int lanes_to_row = PIECE * size / 16, at_once = 32 / lanes_to_row;  // 1 to 8, 32 to 4
+      uint8_t* stage = shared + i * TERMS * T::Q_BYTES + 32 * (warp % 4) * pitch;
+      static_assert(ROW_TILE * (PIECE * 4 + 16) <= TERMS * T::Q_BYTES, "a piece of every row");
+      const int lanes_to_row = PIECE * size / 16, at_once = 32 / lanes_to_row;  // 2 to 8, 16 to 4
       const int tile_row0 = row0 + ROW_TILE * i + 32 * (warp % 4);
       const int tile_token0 = tile_row0 / a.group, tile_head0 = tile_row0 % a.group;
 #pragma unroll
-      for (int c0 = 0; c0 < OWN; c0 += PIECE) {
-        const int c = half * OWN + c0;
+      for (int c = 0; c < D; c += PIECE) {
         float o[PIECE];
         if constexpr (TERMS == 2) {
 #pragma unroll
-          for (int e = 0; e < PIECE; ++e) o[e] = total[c0 + e];
+          for (int e = 0; e < PIECE; ++e) o[e] = total[c + e];
         } else {
           tmem_load_async<PIECE>(o_at + c, o);
           tmem_load_wait();
@@ -954,7 +864,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
     const int run = CODES ? 16 : args.run;  // keys of a piece of V
     const uint32_t run_shift = run == 64 ? 2 : run == 32 ? 1 : 0, run_bytes = uint32_t(run) * D * 2;  // 2^shift steps
-    int edges = 0;
+    int edges_told = 0, edges = 0;
     // (second terms first, while the sums are small)
     auto scores = [&](int j, int i, int b) {
       const uint64_t k = operand_desc(base + T::K_AT + (j % STAGES) * T::K_BYTES, 128);
@@ -987,12 +897,20 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       return true;
     };
     auto keys_ready = [&](int j) { return wait(&k_full[j % STAGES], (j / STAGES) & 1); };
-    auto values_ready = [&](int j) {
+    // (the edge warp is told of an edge tile while the tile before is at work)
+    auto tell_edge = [&](int j) {
+      if (CODES || j >= tiles || whole(seen.key_of(tile0 + j))) return true;
       if (!wait(&v_full[j % STAGES], (j / STAGES) & 1)) return false;
-      if (CODES || whole(seen.key_of(tile0 + j))) return true;
-      // (edge tile by edge tile, in turn with the edge warps)
-      if (lane == 0) tc::mbar_arrive(edge_found);
-      return wait(edge_clean, edges++ & 1);
+      if (lane == 0) tc::mbar_arrive(&edge_found[edges_told & 1]);
+      ++edges_told;
+      return true;
+    };
+    auto values_ready = [&](int j) {
+      if (!CODES && !whole(seen.key_of(tile0 + j))) {
+        const int edge = edges++;
+        return wait(&edge_clean[edge & 1], (edge >> 1) & 1);
+      }
+      return wait(&v_full[j % STAGES], (j / STAGES) & 1);
     };
     // scores of tile j (two row tiles: when theirs of the last are read; with
     // two S, when those of the one before are)
@@ -1014,9 +932,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       for (int i = 0; i < MT && ok; ++i) ok = wait(&q_full[i], 0);
       if (ok) ok = next_scores(0);
     }
+    if (does_outputs && ok) ok = tell_edge(0);
     for (int j = 0; j < tiles && ok; ++j) {
       if (does_scores && j + 1 < tiles && !(ok = next_scores(j + 1))) break;
       if (!does_outputs) continue;
+      if (!(ok = tell_edge(j + 1))) break;
       if (!(ok = values_ready(j))) break;
       for (int i = 0; i < MT && ok; ++i) ok = outputs(j, i);
     }
@@ -1176,21 +1096,25 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     for (int j = 0; j < tiles && ok; ++j) {
       const int key0 = seen.key_of(tile0 + j);
       if (whole(key0)) continue;
-      if (!(ok = wait(edge_found, edges++ & 1))) break;
+      const int edge = edges++;
+      if (!(ok = wait(&edge_found[edge & 1], (edge >> 1) & 1))) break;
       if (!(ok = wait(&v_full[j % STAGES], (j / STAGES) & 1))) break;
       uint8_t* v = shared + T::V_AT + (j % STAGES) * T::V_STAGE;
       bool found = false;
-      for (int n = tid - 32 * T::EDGE_WARP; n < T::V_BYTES / 16; n += T::EDGE_THREADS) {
+#pragma unroll 8
+      for (int n = lane; n < T::V_BYTES / 16; n += 32) {
         uint4 x = *reinterpret_cast<uint4*>(v + 16 * n);
         uint32_t* w = reinterpret_cast<uint32_t*>(&x);
-        bool bad = false;
+        // (an exponent of all ones carries into the sign's place)
+        uint32_t bad = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= ((w[e] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+        if (!bad) continue;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool low = (w[e] & 0x7c00u) == 0x7c00u, high = (w[e] & 0x7c000000u) == 0x7c000000u;
-          bad = bad || low || high;
-          w[e] &= (low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u);
+          const uint32_t full = ((w[e] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+          w[e] &= (full & 0x8000u ? 0u : 0xffffu) | (full & 0x80000000u ? 0u : 0xffff0000u);
         }
-        if (!bad) continue;
         *reinterpret_cast<uint4*>(v + 16 * n) = x;
         // which keys: the run, and the chunk in its row before the swizzle
         // (which exchanges 16-byte chunks by the address bits 7 and up)
@@ -1202,7 +1126,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
       if (found) *taken_out = 1;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc::mbar_arrive(edge_clean);
+      tc::mbar_arrive(&edge_clean[edge & 1]);
     }
     asm volatile("bar.arrive 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");
   }
