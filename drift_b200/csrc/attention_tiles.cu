@@ -91,19 +91,19 @@ struct TileTraits {
   static constexpr bool TWO_ISSUE = !(CODES && TERMS == 2);
   static constexpr int COPY_WARP = SOFTMAX_WARPS, QK_WARP = COPY_WARP + 1, PV_WARP = QK_WARP + TWO_ISSUE;
   static constexpr int EDGE_WARP = PV_WARP + 1, EDGE_THREADS = 32;
-  // Converting codes for BF16 rows takes four warps, one to a scheduler; for
-  // F32 rows, at half the rate, two. The softmax warps take the registers that
-  // the others leave.
+  // Converting codes for BF16 rows takes eight warps, two to a scheduler (with
+  // one, latencies made a tile 6400 clocks long); for F32 rows, at half the
+  // rate, two. The softmax warps take the registers that the others leave.
   static constexpr bool WIDE = CODES && TERMS == 1;
   static constexpr int CONVERT_WARP = WIDE ? EDGE_WARP + 1 : EDGE_WARP;
-  static constexpr int CONVERT_THREADS = WIDE ? 128 : 64;
-  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4 + (WIDE ? 4 : 0));
-  static constexpr bool MOVES_REGISTERS = MT == 2;  // (128 a thread and more are there otherwise)
+  static constexpr int CONVERT_THREADS = WIDE ? 256 : 64;
+  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4 + (WIDE ? 8 : 0));
+  static constexpr bool MOVES_REGISTERS = MT == 2 || WIDE;  // (255 a thread are there otherwise)
   static constexpr int LAUNCH_REGISTERS = 65536 / THREADS / 8 * 8;
-  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : WIDE ? 64 : 88;
-  static constexpr int SOFTMAX_REGISTERS =
+  static constexpr int OTHER_REGISTERS = TERMS == 2 ? 56 : !WIDE ? 88 : MT == 2 ? 48 : 88;
+  static constexpr int SHARE =
       (THREADS * LAUNCH_REGISTERS - (THREADS - 32 * SOFTMAX_WARPS) * OTHER_REGISTERS) / (32 * SOFTMAX_WARPS) / 8 * 8;
-  static_assert(!MOVES_REGISTERS || SOFTMAX_REGISTERS <= 248, "a thread's registers");
+  static constexpr int SOFTMAX_REGISTERS = SHARE > 232 ? 232 : SHARE;
   static constexpr int ROUND_THREADS = 32 * SOFTMAX_WARPS + (CODES ? CONVERT_THREADS : EDGE_THREADS);
   static constexpr int PANELS = (D + 63) / 64;             // 64-column panels of a row
   static constexpr int Q_PANEL = ROW_TILE * 128;           // bytes
@@ -471,7 +471,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const uint32_t group_magic = a.group > 1 ? 0xffffffffu / uint32_t(a.group) + 1 : 0;  // (2^32 / group, up)
     {
       constexpr int CHUNKS = D / 8, LANES = CHUNKS <= 8 ? 8 : CHUNKS <= 16 ? 16 : 32;  // of a row
-      constexpr int AT_ONCE = 32 / LANES, PASSES = LANES, FLIGHT = 4;
+      constexpr int AT_ONCE = 32 / LANES, PASSES = LANES, FLIGHT = TERMS == 2 ? 4 : 8;
       const int c = lane % LANES, part = lane / LANES;
       const int tile_row0 = row0 + ROW_TILE * i + 32 * (warp % 4);
       const int tile_token0 = tile_row0 / a.group, tile_head0 = tile_row0 % a.group;
@@ -980,10 +980,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const uint32_t copy_phase = (j / T::COPY_STAGES) & 1;
       const uint8_t* k_codes = shared + T::CODES_AT + copy_stage * 2 * T::CODE_STAGE;
       const uint8_t* v_codes = k_codes + T::CODE_STAGE;
-      // keys: a thread takes a row (or, of 64 rows, half of one)
-      constexpr int TO_ROW = N >= 2 * KEYS ? 2 : 1;  // threads
-      const int row = TO_ROW == 2 ? t % KEYS : t;
-      const bool has_row = row < KEYS;
+      // keys: a thread takes a row, or every second or fourth chunk of one
+      constexpr int TO_ROW = CHUNKS % 4 == 0 && N >= 4 * KEYS ? 4 : CHUNKS % 2 == 0 && N >= 2 * KEYS ? 2 : 1;  // threads
+      const int row = t % KEYS, share = t / KEYS;
+      const bool has_row = share < TO_ROW;
       const float* k_from = reinterpret_cast<const float*>(shared + T::COPIED_SCALES_AT) + copy_stage * 2 * KEYS;
       const float* v_from = k_from + KEYS;
       const bool check = !whole(key0);
@@ -991,34 +991,39 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (!(ok = wait(&codes_full[2 * copy_stage], copy_phase))) break;
       float k_scale[PER];
       load_scales(key0, check, k_from, k_scale);
-      const float own_k = has_row && (!check || seen_key(key0 + row)) ? k_from[row] : 0.0f;
+      const float own_k = (!check || seen_key(key0 + row)) ? k_from[row] : 0.0f;
       // (2^-64 at least: the scores' factor stays normal with it)
       const float k_power = power_over(largest_of(k_scale), 0x1f800000u);
       if (has_row) {
         uint8_t* k = shared + T::K_AT + stage * T::K_BYTES + row * 128;
         constexpr int TAKES = CHUNKS / TO_ROW;  // chunks a thread takes
-        const int c0 = TO_ROW == 2 ? t / KEYS * TAKES : 0;
-        // the scale over the tile's power of two in two F16 terms
-        const float ratio = own_k * (1.0f / k_power);
-        const __half ratio_hi = __float2half_rn(ratio);
-        const __half2 hi = __half2half2(ratio_hi), low = __half2half2(__float2half_rn(ratio - __half2float(ratio_hi)));
+        const __half2 ratio = __float2half2_rn(own_k * (1.0f / k_power));
         auto scaled = [&](uint32_t pair) {
           if constexpr (TERMS == 2) return pair;
-          const __half2 x = *reinterpret_cast<const __half2*>(&pair);
-          const __half2 y = __hfma2(x, hi, __hmul2(x, low));
+          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), ratio);
           return *reinterpret_cast<const uint32_t*>(&y);
         };
-#pragma unroll 4
-        for (int n = 0; n < TAKES; ++n) {
-          // (each eight lanes' chunks on different banks)
-          const int c = c0 + (TAKES % 8 == 0 ? (n + t) % TAKES : TAKES == 4 ? (n + t / 2) % 4 : n);
-          const uint4 x = *reinterpret_cast<const uint4*>(k_codes + row * D + 16 * c);
-          const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
-          uint8_t* to = k + c / 4 * T::K_PANEL;
-          *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4)) ^ (row % 8))) =
-              make_uint4(scaled(y0.x), scaled(y0.y), scaled(y1.x), scaled(y1.y));
-          *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4) + 1) ^ (row % 8))) =
-              make_uint4(scaled(y2.x), scaled(y2.y), scaled(y3.x), scaled(y3.y));
+        // (each eight lanes' chunks on different banks; loads ahead of the
+        // stores, which the compiler cannot tell apart)
+        auto chunk_of = [&](int n) {
+          return CHUNKS == 4 ? (TO_ROW * n + share + row / 2) % 4 : CHUNKS % 8 == 0 ? (TO_ROW * n + share + row) % CHUNKS : n;
+        };
+        constexpr int FLIGHT = TAKES % 4 == 0 ? 4 : TAKES;
+#pragma unroll
+        for (int n0 = 0; n0 < TAKES; n0 += FLIGHT) {
+          uint4 x[FLIGHT];
+#pragma unroll
+          for (int n = 0; n < FLIGHT; ++n) x[n] = *reinterpret_cast<const uint4*>(k_codes + row * D + 16 * chunk_of(n0 + n));
+#pragma unroll
+          for (int n = 0; n < FLIGHT; ++n) {
+            const int c = chunk_of(n0 + n);
+            const uint2 y0 = code_pairs(x[n].x), y1 = code_pairs(x[n].y), y2 = code_pairs(x[n].z), y3 = code_pairs(x[n].w);
+            uint8_t* to = k + c / 4 * T::K_PANEL;
+            *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4)) ^ (row % 8))) =
+                make_uint4(scaled(y0.x), scaled(y0.y), scaled(y1.x), scaled(y1.y));
+            *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4) + 1) ^ (row % 8))) =
+                make_uint4(scaled(y2.x), scaled(y2.y), scaled(y3.x), scaled(y3.y));
+          }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1073,14 +1078,25 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), ratios[n]);
           return *reinterpret_cast<const uint32_t*>(&y);
         };
-#pragma unroll 4
-        for (int d = first_d; d < D; d += DIMS) {
-          const uint4 x = *reinterpret_cast<const uint4*>(from + d * run);
-          const uint2 y0 = code_pairs(x.x), y1 = code_pairs(x.y), y2 = code_pairs(x.z), y3 = code_pairs(x.w);
-          uint8_t* to = v + d * 32;  // (rows of 32 bytes, their halves exchanged in every other four)
-          const int c = d / 4 % 2;
-          *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(scaled(y0.x, 0), scaled(y0.y, 1), scaled(y1.x, 2), scaled(y1.y, 3));
-          *reinterpret_cast<uint4*>(to + 16 * (1 - c)) = make_uint4(scaled(y2.x, 4), scaled(y2.y, 5), scaled(y3.x, 6), scaled(y3.y, 7));
+        constexpr int TAKES = (D + DIMS - 1) / DIMS, FLIGHT = TAKES % 4 == 0 ? 4 : TAKES;
+#pragma unroll
+        for (int n0 = 0; n0 < TAKES; n0 += FLIGHT) {
+          uint4 x[FLIGHT];
+#pragma unroll
+          for (int n = 0; n < FLIGHT; ++n) {
+            const int d = first_d + DIMS * (n0 + n);
+            x[n] = d < D ? *reinterpret_cast<const uint4*>(from + d * run) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int n = 0; n < FLIGHT; ++n) {
+            const int d = first_d + DIMS * (n0 + n);
+            if (d >= D) break;
+            const uint2 y0 = code_pairs(x[n].x), y1 = code_pairs(x[n].y), y2 = code_pairs(x[n].z), y3 = code_pairs(x[n].w);
+            uint8_t* to = v + d * 32;  // (rows of 32 bytes, their halves exchanged in every other four)
+            const int c = d / 4 % 2;
+            *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(scaled(y0.x, 0), scaled(y0.y, 1), scaled(y1.x, 2), scaled(y1.y, 3));
+            *reinterpret_cast<uint4*>(to + 16 * (1 - c)) = make_uint4(scaled(y2.x, 4), scaled(y2.y, 5), scaled(y3.x, 6), scaled(y3.y, 7));
+          }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

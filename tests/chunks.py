@@ -97,10 +97,10 @@ def attention(q, cache, tables, new, counts, spec):
             rounded = coded = 0.0
             if scales is not None and q.dtype == torch.bfloat16:
                 # BF16 rows may meet keys and values rounded to F16 over a power
-                # of two under twice the largest scale: 2^-11 of each key, and
-                # 2^-25 of the power at least; a value's scale is rounded
-                # before its product, 2^-11 twice.
-                rounded = magnitude * 2.0 ** -11 + x.abs().sum(1, keepdim=True) * abs(spec.scale) * (
+                # of two under twice the largest scale: 2^-11 for the scale's
+                # rounding and 2^-11 for the product's, of each key and value,
+                # and 2^-25 of the power at least.
+                rounded = magnitude * 2 * 2.0 ** -11 + x.abs().sum(1, keepdim=True) * abs(spec.scale) * (
                     2.0 ** -25 * 2 * key_scales[seen.any(0), h // group].max())
                 coded = 2 * 2.0 ** -11
             delta = rounded + lost + magnitude * (2 * dim / 16 * 2.0 ** -22) + score.abs() * 2.0 ** -20
