@@ -13,8 +13,7 @@ namespace drift {
 namespace {
 
 struct Plan {
-  int columns;          // attention_rows' column tiles, or
-  int row_tiles;        // attention_tiles' row tiles (0: attention_rows)
+  int row_tiles;        // attention_tiles' row tiles (0: attention_rows or attention_codes)
   int rows_per_unit;    // rows of a key head that a CTA takes
   int keys_per_tile;
   int splits, tiles_per_split;
@@ -39,22 +38,33 @@ Plan plan_rows(const Call& c) {
   Plan p;
   p.row_tiles = 0;
   const long long rows = (long long)c.longest * c.group;
-  p.columns = c.head_dim > 128 || rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  p.rows_per_unit = 8 * p.columns;
-  p.keys_per_tile = attention_rows_tile(c.head_dim, c.cache_dtype == DRIFT_I8, p.columns);
+  if (c.cache_dtype == DRIFT_I8) {
+    p.rows_per_unit = rows <= 4 ? 4 : rows <= 8 || c.head_dim > 128 ? 8 : rows <= 16 ? 16 : 24;
+    p.keys_per_tile = 32;
+  } else {
+    p.rows_per_unit = rows <= 8 || c.head_dim > 128 ? 8 : 16;
+    p.keys_per_tile = 16;
+  }
   const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
   const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
-  // CTAs for every SM twice over, of a tile a warp at least
-  const long long wanted = std::max(1LL, 4LL * sm_count() / std::max(1LL, units));
-  const long long splits = std::min(wanted, (tiles + 7) / 8);
+  const int warps = c.cache_dtype == DRIFT_I8 ? attention_codes_warps(c.head_dim, p.rows_per_unit) : 8;
+  // CTAs for every SM four times over (F16 caches eight: a step of 16 x 16384
+  // keys 153 us, and 181 with four; 8-bit ones of 3 sequences 29, and 35 with
+  // eight), of a tile a warp at least
+  const long long wanted =
+      std::max(1LL, (c.cache_dtype == DRIFT_I8 ? 4LL : 8LL) * sm_count() / std::max(1LL, units));
+  const long long splits = std::min(wanted, (tiles + warps - 1) / warps);
   const long long each = (tiles + splits - 1) / splits;
-  p.tiles_per_split = int((each + 7) / 8 * 8);
+  p.tiles_per_split = int((each + warps - 1) / warps * warps);
   p.splits = int((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
   return p;
 }
 
-// Rows of a key head from which chunks go to the tensor-core tiles.
-constexpr long long TILE_ROWS = 32;
+// Whether a chunk's rows of a key head go to the tensor-core tiles.
+bool takes_tiles(const Call& c, long long rows) {
+  if (c.x_dtype == DRIFT_F32 && c.head_dim > 128) return false;
+  return rows > (c.cache_dtype == DRIFT_F16 ? 8 : c.x_dtype == DRIFT_BF16 ? 16 : 24);
+}
 
 // The split count is the one with the least time of the busiest SM, by what
 // was measured on B200 for a tile (per row tile and key: BF16 6 ns, F32 16,
@@ -63,7 +73,6 @@ constexpr long long TILE_ROWS = 32;
 Plan plan_tiles(const Call& c) {
   constexpr double CTA_NS = 5000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 4500;
   Plan p;
-  p.columns = 0;
   const long long rows = (long long)c.longest * c.group;
   p.row_tiles = c.head_dim > 128 || rows <= 128 ? 1 : 2;
   p.rows_per_unit = 128 * p.row_tiles;
@@ -92,7 +101,7 @@ Plan plan_chunks(const Call& c) {
   // (the copies' coordinates are 32-bit, the grid's unit axis 16-bit)
   const bool reachable = (long long)c.pages * c.page_size < (1ll << 31) &&
                          (long long)c.pages * c.kv_heads * c.head_dim < (1ll << 31);
-  if ((c.x_dtype == DRIFT_BF16 || c.head_dim <= 128) && reachable && rows >= TILE_ROWS) {
+  if (takes_tiles(c, rows) && reachable) {
     const Plan p = plan_tiles(c);
     if ((rows + p.rows_per_unit - 1) / p.rows_per_unit * p.splits <= 65535) return p;
   }
@@ -179,7 +188,8 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   a.softcap = softcap;
   const cudaStream_t s = cudaStream_t(stream);
   if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, x_dtype, cache_dtype, head_dim, p.row_tiles, s));
-  else DRIFT_TRY(launch_attention_rows(a, x_dtype, cache_dtype, head_dim, p.columns, s));
+  else if (cache_dtype == DRIFT_I8) DRIFT_TRY(launch_attention_codes(a, x_dtype, head_dim, p.rows_per_unit, s));
+  else DRIFT_TRY(launch_attention_rows(a, x_dtype, head_dim, p.rows_per_unit, s));
   if (!needed) return 0;
   return launch_attention_join(a, x_dtype, head_dim, p.rows_per_unit, p.keys_per_tile, s);
 }

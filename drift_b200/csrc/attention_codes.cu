@@ -1,0 +1,581 @@
+// attention_chunks over an 8-bit cache for few rows: a decoding step, drafted
+// tokens.
+//
+// A unit is a key head of one sequence with up to ROWS of the (token, query
+// head) rows that read it; a CTA takes one split of the unit's key tiles, each
+// of its warps every eighth (or twelfth) tile of 32 keys. Both products run on the int8
+// tensor cores, turned round -- scores^T = K q^T and out^T = V^T p^T by
+// mma.sync m16n8k32, keys and then dimensions as the 16 rows, the few query
+// rows as columns -- with the codes as they lie in the cache: a lane's 16
+// bytes of a key row, its 8 bytes of a dimension's positions, are A fragments
+// without a conversion (converting them to F16 was two thirds of 1470
+// instructions a tile). What is converted is the small side: a row of q and
+// a tile's weights become whole numbers, split into balanced base-256 digits
+// (bytes of (x + 0x808080) ^ 0x808080), a column for each row and digit. The
+// sums are exact; they start from the bits of 1.5 x 2^23, so that they are F32
+// numbers without a conversion (|sum| < 2^22), and their digits are joined in
+// F32. q has 30 bits (F32) or 15 (BF16) below its row's largest value, a
+// weight 2^26 steps below its row's base (BF16 rows of more than four: 2^18).
+// A key's scale multiplies its score, a value's its weight, over a power of
+// two at or above every scale so far.
+//
+// Softmax in F32, a base and a sum a row and warp; the base moves when some
+// weight passes 2^3 (and one vote a tile tells). The warps meet in shared
+// memory, the splits in a second launch (attention_chunks_join_kernel).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "chunks.cuh"
+#include "common.cuh"
+#include "registry.cuh"
+
+namespace drift {
+
+namespace {
+
+constexpr int TILE = 32;   // keys of a warp's tile
+constexpr int PITCH = 36;  // words of a row's weights in shared memory: rows on different banks
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ZERO = 0x4b400000;  // the bits of 1.5 x 2^23
+constexpr float ZERO_VALUE = 12582912.0f;
+constexpr float GROWTH = 8.0f;    // a weight that moves its base
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The digits of x, the least in the lowest byte, each -128 to 127.
+__device__ __forceinline__ uint32_t digits(int x) { return (uint32_t(x) + 0x00808080u) ^ 0x00808080u; }
+
+// Byte `digit` of each of four words.
+__device__ __forceinline__ uint32_t digit_of(const uint4& x, uint32_t digit) {
+  const uint32_t pick = digit | (digit + 4) << 4;
+  return __byte_perm(__byte_perm(x.x, x.y, pick), __byte_perm(x.z, x.w, pick), 0x5410);
+}
+
+__device__ __forceinline__ float weight_of(float score, float base) {
+  return score == -INFINITY ? 0.0f : exp2f((score - base) * LOG2E);
+}
+
+// Packed: up to four rows, column c of digit tile j being row c % 4's digit 2 j
+// + c / 4; otherwise RT tiles of eight rows, each with a tile for each digit.
+template <int D_, bool BF16_, int RT_>
+struct CodesTraits {
+  static constexpr int D = D_, RT = RT_ == 0 ? 1 : RT_;
+  static constexpr bool BF16 = BF16_, PACKED = RT_ == 0;
+  static constexpr int ROWS = PACKED ? 4 : 8 * RT;
+  // As many warps as registers leave an SM without spills: sixteen of 128, for
+  // heads of 128 twelve of 168 (a step of 16 x 16384 keys: sixteen, spilling,
+  // 191 us, twelve 113, eight 135), for more rows and wider heads eight. In
+  // CTAs of four, one's start and end run under the others.
+  static constexpr int WARPS = attention_codes_warps(D, ROWS), THREADS = 32 * WARPS;
+  static constexpr int CTAS = RT > 1 || D > 128 ? 1 : D == 128 ? 3 : 2;
+  static constexpr int Q_DIGITS = BF16 ? 2 : 4, P_DIGITS = PACKED || !BF16 ? 4 : 3;
+  static constexpr int Q_TILES = PACKED ? Q_DIGITS / 2 : RT * Q_DIGITS;
+  static constexpr int P_TILES = PACKED ? P_DIGITS / 2 : RT * P_DIGITS;
+  static constexpr int Q_BITS = BF16 ? 13 : 29;                  // of the largest value's leading bit
+  static constexpr float P_STEPS = P_DIGITS == 4 ? 67108864.0f : 262144.0f;  // of a weight of 1
+  static constexpr int CHUNKS = D / 64, TAIL = D % 64 / 16;      // 16-byte chunks a lane has of a key row; 4 bytes
+  static constexpr int STEPS = 2 * CHUNKS + TAIL, WORDS = 4 * CHUNKS + TAIL;
+  static constexpr int DM = D / 16;
+  static constexpr int Q_BYTES = STEPS * Q_TILES * 32 * 8;
+  static constexpr int P_BYTES = WARPS * ROWS * PITCH * 4;
+  static constexpr int MERGE_BYTES = WARPS * ROWS * (D + 4) * 4;
+  static constexpr int BYTES = Q_BYTES + P_BYTES > MERGE_BYTES ? Q_BYTES + P_BYTES : MERGE_BYTES;
+};
+
+template <class T>
+struct CodesWarp {
+  static constexpr int D = T::D;
+  const AttentionChunksArgs& a;
+  const Chunk& chunk;
+  const SeenTiles& seen;
+  const int head, g, t;
+  const uint32_t page_magic;              // 2^32 / page_size, up
+  int k_page[2], k_place[2], v_page, v_place;  // of the tile that is loaded next
+  uint32_t k[2][2][T::WORDS];             // [16 keys][row g, g + 8]
+  uint2 v[T::DM][2];                      // [16 dimensions][row g, g + 8], positions 8 t .. 8 t + 7
+  float k_scale[2][2], v_scale[2][2];
+
+  __device__ CodesWarp(const AttentionChunksArgs& a, const Chunk& c, const SeenTiles& s, int head, int lane)
+      : a(a), chunk(c), seen(s), head(head), g(lane / 4), t(lane % 4),
+        page_magic(0xffffffffu / uint32_t(a.at.page_size) + 1) {}
+
+  // The page that holds `position` and the place in it; -1 past the last key,
+  // or for a page that the cache does not have.
+  __device__ void find(int position, int& page, int& place) const {
+    int index = int(__umulhi(uint32_t(position), page_magic));  // (one too many at most)
+    place = position - index * a.at.page_size;
+    if (place < 0) --index, place += a.at.page_size;
+    page = -1;
+    if (position >= seen.end) return;
+    page = chunk.table[index];
+    if (page >= 0 && page < a.at.pages) return;
+    chunk_error(a.error);
+    page = -1;
+  }
+  __device__ void find_pages(int key0) {
+    find(key0, k_page[0], k_place[0]);
+    find(key0 + 16, k_page[1], k_place[1]);
+    v_page = t < 2 ? k_page[0] : k_page[1];
+    v_place = (t < 2 ? k_place[0] : k_place[1]) + 8 * (t % 2);
+  }
+
+  __device__ void load_keys() {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int place = k_place[m] + g + 8 * half;
+        const bool there = k_page[m] >= 0;
+        const uint8_t* row = static_cast<const uint8_t*>(a.keys) +
+                             (((long long)k_page[m] * a.at.page_size + place) * a.kv_heads + head) * D;
+#pragma unroll
+        for (int c = 0; c < T::CHUNKS; ++c) {
+          const uint4 x = there ? __ldg(reinterpret_cast<const uint4*>(row) + 4 * c + t) : make_uint4(0, 0, 0, 0);
+          k[m][half][4 * c] = x.x, k[m][half][4 * c + 1] = x.y, k[m][half][4 * c + 2] = x.z, k[m][half][4 * c + 3] = x.w;
+        }
+        if constexpr (T::TAIL)
+          k[m][half][4 * T::CHUNKS] = there ? __ldg(reinterpret_cast<const uint32_t*>(row + 64 * T::CHUNKS) + t) : 0;
+        const long long at = ((long long)k_page[m] * a.kv_heads + head) * a.at.page_size + place;
+        k_scale[m][half] = there ? __ldg(a.key_scales + at) : 0.0f;
+        v_scale[m][half] = there ? __ldg(a.value_scales + at) : 0.0f;
+      }
+  }
+  __device__ void load_values() {
+    const uint8_t* column = static_cast<const uint8_t*>(a.values) +
+                            ((long long)v_page * a.kv_heads + head) * D * a.at.page_size + v_place;
+#pragma unroll
+    for (int m = 0; m < T::DM; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        v[m][half] = v_page >= 0 ? __ldg(reinterpret_cast<const uint2*>(column + (16 * m + g + 8 * half) * (long long)a.at.page_size))
+                                 : make_uint2(0, 0);
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(const AttentionChunksArgs a) {
+  pdl_trigger();  // the next kernel may launch and wait for this one
+  pdl_wait();     // what the kernels before this one wrote is visible
+  constexpr int D = T::D, RT = T::RT, ROWS = T::ROWS, WARPS = T::WARPS, THREADS = T::THREADS;
+  constexpr bool PACKED = T::PACKED;
+  using X = typename std::conditional<T::BF16, __nv_bfloat16, float>::type;
+  extern __shared__ __align__(16) uint8_t shared[];
+  __shared__ float q_unit[ROWS];  // what a step of a row of q is worth
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
+  const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits, head = blockIdx.y, z = blockIdx.z;
+  const Chunk chunk(a.at, z);
+  if (!chunk.ok && blockIdx.x == 0 && head == 0 && tid == 0) chunk_error(a.error);
+  // this unit's rows [row0, row1) of the sequence's tokens x group, row r
+  // being token r / group, query head r % group of the key head
+  const int row0 = unit * ROWS, row1 = min(row0 + ROWS, chunk.tokens * a.group);
+  if (row0 >= row1) return;
+  const int token0 = row0 / a.group, token1 = (row1 - 1) / a.group + 1;
+  const SeenTiles seen(a, chunk, token0, token1, TILE);
+  const int tile0 = split * a.tiles_per_split, tile1 = min(tile0 + a.tiles_per_split, seen.count);
+  if (tile0 >= tile1) return;
+
+  CodesWarp<T> w(a, chunk, seen, head, lane);
+  int tile = tile0 + warp;
+  if (tile < tile1) {
+    w.find_pages(seen.key_of(tile));
+    w.load_keys();
+    w.load_values();
+    if (tile + WARPS < tile1) w.find_pages(seen.key_of(tile + WARPS));
+  }
+
+  // q in whole numbers of a power of two that gives its largest value
+  // Q_BITS + 1 bits, as B fragments of digits [step][digit tile][lane]: a warp
+  // takes a row, a lane four values at a time, which are a digit's word each
+  uint32_t* fragments = reinterpret_cast<uint32_t*>(shared);
+  for (int r = warp; r < ROWS; r += WARPS) {
+    constexpr int PER = (D + 127) / 128;
+    float x[PER][4] = {};
+    if (row0 + r < row1) {
+      const int row = row0 + r;
+      const X* q = static_cast<const X*>(a.q) + ((chunk.row + row / a.group) * a.q_heads + head * a.group + row % a.group) * D;
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        const int d = 4 * (lane + 32 * n);
+        if (d >= D) continue;
+        if constexpr (T::BF16) {
+          const uint2 y = *reinterpret_cast<const uint2*>(q + d);
+          x[n][0] = __uint_as_float(y.x << 16), x[n][1] = __uint_as_float(y.x & 0xffff0000u);
+          x[n][2] = __uint_as_float(y.y << 16), x[n][3] = __uint_as_float(y.y & 0xffff0000u);
+        } else {
+          const float4 y = *reinterpret_cast<const float4*>(q + d);
+          x[n][0] = y.x, x[n][1] = y.y, x[n][2] = y.z, x[n][3] = y.w;
+        }
+      }
+    }
+    float largest = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        largest = fmaxf(largest, fabsf(x[n][e]));
+        finite = finite && fabsf(x[n][e]) <= 3.402823466e38f;
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    finite = __all_sync(0xffffffffu, finite);
+    // (kept where the unit and its inverse are normal; a row that is not
+    // finite has a NaN for a unit, and so for every score)
+    constexpr uint32_t SHIFT = uint32_t(T::Q_BITS) << 23;
+    const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, SHIFT + 0x01000000u) - SHIFT;
+    if (lane == 0) q_unit[r] = finite ? __uint_as_float(exponent) : __int_as_float(0x7fc00000);
+    const float inverse = __uint_as_float(0x7f000000u - exponent);
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int d = 4 * (lane + 32 * n);
+      if (d >= D) continue;
+      const uint4 y = make_uint4(digits(__float2int_rn(x[n][0] * inverse)), digits(__float2int_rn(x[n][1] * inverse)),
+                                 digits(__float2int_rn(x[n][2] * inverse)), digits(__float2int_rn(x[n][3] * inverse)));
+      // where a lane of the product has these bytes of a key row: two steps
+      // to a chunk of 64, then the tail's first sixteen (of 32: zeros follow)
+      const bool tail = d >= 64 * T::CHUNKS;
+      const int step = tail ? 2 * T::CHUNKS : d / 64 * 2 + d / 8 % 2, lt = tail ? d / 4 % 4 : d / 16 % 4;
+      const int word = tail ? 0 : d / 4 % 2;
+#pragma unroll
+      for (int digit = 0; digit < T::Q_DIGITS; ++digit) {
+        const int tile = PACKED ? digit / 2 : r / 8 * T::Q_DIGITS + digit, column = PACKED ? digit % 2 * 4 + r : r % 8;
+        uint32_t* to = fragments + ((step * T::Q_TILES + tile) * 32 + 4 * column + lt) * 2;
+        to[word] = digit_of(y, digit);
+        if (tail) to[1] = 0;
+      }
+    }
+  }
+  __syncthreads();
+
+  // this lane's columns of row tile n: rows 8 n + 2 t and + 1 (packed: modulo 4)
+  float multiplier[RT][2];
+  int position[RT][2];
+#pragma unroll
+  for (int n = 0; n < RT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = PACKED ? (2 * t + e) % 4 : 8 * n + 2 * t + e;
+      multiplier[n][e] = a.scale * q_unit[r];
+      position[n][e] = chunk.position + min(row0 + r, row1 - 1) / a.group;
+    }
+  // what every row sees: keys below `all_end` and from `all_low` on (or below
+  // `first`)
+  const int first = a.window > 0 ? a.first : 0;
+  const int all_end = a.causal ? chunk.position + token0 + 1 : seen.end;
+  const int all_low = a.window > 0 ? chunk.position + token1 - a.window : 0;
+  const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;  // what some row sees
+  const float low_digit = PACKED && t >= 2 ? 256.0f : 1.0f;  // the worth of a packed lane's lower digit
+
+  float out[RT][T::DM][4];
+  float base[RT][2], sum[RT][2], v_unit = 0.0f;
+#pragma unroll
+  for (int n = 0; n < RT; ++n) {
+    base[n][0] = base[n][1] = -INFINITY;
+    sum[n][0] = sum[n][1] = 0.0f;
+#pragma unroll
+    for (int m = 0; m < T::DM; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
+  }
+  uint32_t* weights = reinterpret_cast<uint32_t*>(shared + T::Q_BYTES) + warp * ROWS * PITCH;
+
+  for (; tile < tile1; tile += WARPS) {
+    const int key0 = seen.key_of(tile), next = tile + WARPS;
+    const bool whole = key0 + TILE <= all_end && (key0 >= all_low || key0 + TILE <= first);
+    // scores [row tile][16 keys][(key g, columns 2 t, 2 t + 1), (key g + 8, the same)]
+    float s[RT][2][4];
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+      constexpr int TILES = T::Q_TILES / RT;
+      int acc[2][TILES][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = ZERO;
+#pragma unroll
+      for (int step = 0; step < T::STEPS; ++step) {
+        uint2 b[TILES];
+#pragma unroll
+        for (int j = 0; j < TILES; ++j)
+          b[j] = reinterpret_cast<const uint2*>(fragments)[(step * T::Q_TILES + n * TILES + j) * 32 + lane];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const bool both = step < 2 * T::CHUNKS;
+          const int word = 2 * step;
+          const uint32_t f[4] = {w.k[m][0][word], w.k[m][1][word], both ? w.k[m][0][both ? word + 1 : 0] : 0,
+                                 both ? w.k[m][1][both ? word + 1 : 0] : 0};
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) mma_s8(acc[m][j], f, b[j].x, b[j].y);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = 0.0f;
+#pragma unroll
+          for (int j = TILES - 1; j >= 0; --j) {
+            const float y = __int_as_float(acc[m][j][e]) - ZERO_VALUE;
+            x = j == TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
+          }
+          if (PACKED) {
+            x *= low_digit;
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+          }
+          s[n][m][e] = x;
+        }
+    }
+    float k_scale[2][2], v_scale[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) k_scale[m][half] = w.k_scale[m][half], v_scale[m][half] = w.v_scale[m][half];
+    if (next < tile1) w.load_keys();  // on their way under the rest of this tile
+    float top_scale = 0.0f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int key = key0 + 16 * m + g + 8 * half;
+        if (!whole && (key >= seen.end || (key < lowest && key >= first))) v_scale[m][half] = 0.0f;
+        if (v_scale[m][half] <= 3.402823466e38f) top_scale = fmaxf(top_scale, v_scale[m][half]);  // (the finite ones)
+#pragma unroll
+        for (int n = 0; n < RT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = s[n][m][2 * half + e] * multiplier[n][e] * k_scale[m][half];
+            if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
+            if (!whole) {
+              const bool sees = key < seen.end && (!a.causal || key <= position[n][e]) &&
+                                (a.window == 0 || key > position[n][e] - a.window || key < first);
+              x = sees ? x : -INFINITY;
+            }
+            s[n][m][2 * half + e] = x;
+          }
+      }
+    // weights with the bases as they are; where one passes GROWTH (or is a
+    // NaN, or a row has no base yet), or a scale the unit, they move
+    float p[RT][2][4];
+    bool move = top_scale > v_unit;
+    auto weigh = [&]() {
+#pragma unroll
+      for (int n = 0; n < RT; ++n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[n][m][e] = weight_of(s[n][m][e], base[n][e % 2]);
+            move = move || !(p[n][m][e] <= GROWTH);
+          }
+    };
+    weigh();
+    if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) top_scale = fmaxf(top_scale, __shfl_xor_sync(0xffffffffu, top_scale, o));
+      float shrink = 1.0f;
+      if (top_scale > v_unit) {
+        const uint32_t bits = __float_as_uint(top_scale);
+        const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
+        const float now = __uint_as_float(max(up, 0x01000000u));  // (its inverse is normal too)
+        shrink = v_unit / now;
+        v_unit = now;
+      }
+#pragma unroll
+      for (int n = 0; n < RT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
+#pragma unroll
+          for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float now = fmaxf(base[n][e], top), f = weight_of(base[n][e], now);
+          base[n][e] = now;
+          sum[n][e] *= f;
+#pragma unroll
+          for (int m = 0; m < T::DM; ++m) out[n][m][e] *= f * shrink, out[n][m][e + 2] *= f * shrink;
+        }
+      weigh();
+    }
+    // into digits, [row][key] in shared memory: a product's columns are rows
+    const float steps = v_unit > 0.0f ? T::P_STEPS / v_unit : 0.0f;
+    __syncwarp();  // (the tile before is read)
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float by = v_scale[m][half] * steps;
+#pragma unroll
+        for (int n = 0; n < RT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = p[n][m][2 * half + e];
+            sum[n][e] += x;
+            // (a hidden value's scale may be a NaN; a NaN that is seen stays in the sum)
+            const float y = x == 0.0f ? 0.0f : x * by;
+            if (!(y <= 2147483520.0f)) sum[n][e] = __int_as_float(0x7fc00000);
+            if (!PACKED || t < 2) weights[(8 * n + 2 * t + e) * PITCH + 16 * m + g + 8 * half] = digits(__float2int_rn(y));
+          }
+      }
+    __syncwarp();
+    uint32_t b[T::P_TILES][2];
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+      const uint4* from = reinterpret_cast<const uint4*>(weights + (PACKED ? g % 4 : 8 * n + g) * PITCH + 8 * t);
+      const uint4 x = from[0], y = from[1];
+      constexpr int TILES = T::P_TILES / RT;
+#pragma unroll
+      for (int j = 0; j < TILES; ++j) {
+        const uint32_t digit = PACKED ? 2 * j + g / 4 : j;
+        b[n * TILES + j][0] = digit_of(x, digit);
+        b[n * TILES + j][1] = digit_of(y, digit);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < T::DM; ++m) {
+      const uint32_t f[4] = {w.v[m][0].x, w.v[m][1].x, w.v[m][0].y, w.v[m][1].y};
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        constexpr int TILES = T::P_TILES / RT;
+        int acc[TILES][4];
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) {
+          acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = ZERO;
+          mma_s8(acc[j], f, b[n * TILES + j][0], b[n * TILES + j][1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = 0.0f;
+#pragma unroll
+          for (int j = TILES - 1; j >= 0; --j) {
+            const float y = __int_as_float(acc[j][e]) - ZERO_VALUE;
+            x = j == TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
+          }
+          out[n][m][e] += x;
+        }
+      }
+    }
+    if (next < tile1) {
+      w.load_values();
+      if (next + WARPS < tile1) w.find_pages(seen.key_of(next + WARPS));
+    }
+  }
+
+  // the warps' results: [warp][row][D] and [warp][row] (base, sum)
+  __syncthreads();  // (past the fragments and the weights)
+  float* merged = reinterpret_cast<float*>(shared);
+  float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
+  const float worth = v_unit / T::P_STEPS * low_digit;
+#pragma unroll
+  for (int n = 0; n < RT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float total = sum[n][e];
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const int r = 8 * n + 2 * t + e;
+      const bool writes = !PACKED || t < 2;
+      if (g == 0 && writes) stats[warp * ROWS + r] = make_float2(base[n][e], total);
+#pragma unroll
+      for (int m = 0; m < T::DM; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x = out[n][m][2 * half + e] * worth;
+          if (PACKED) x += __shfl_xor_sync(0xffffffffu, x, 2);
+          if (writes) merged[(warp * ROWS + r) * D + 16 * m + g + 8 * half] = x;
+        }
+    }
+  __syncthreads();
+  for (int i = tid; i < (row1 - row0) * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row0 + r, q_head = head * a.group + row % a.group;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) top = fmaxf(top, stats[j * ROWS + r].x);
+    float total = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) {
+      const float2 stat = stats[j * ROWS + r];
+      const float f = weight_of(stat.x, top);
+      total += stat.y * f;  // (a NaN stays one)
+      if (f == 0.0f) continue;
+      const float4 y = *reinterpret_cast<const float4*>(merged + (j * ROWS + r) * D + d);
+      x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+    }
+    const long long at = (chunk.row + row / a.group) * a.q_heads + q_head;
+    if (a.part_o) {
+      *reinterpret_cast<float4*>(a.part_o + (at * a.splits + split) * D + d) = x;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.splits + split) * 2) = make_float2(top, total);
+      continue;
+    }
+    if (a.sinks) {
+      const float sink = a.sinks[q_head], all = fmaxf(top, sink);
+      const float f = weight_of(top, all);
+      x.x *= f, x.y *= f, x.z *= f, x.w *= f;
+      total = total * f + weight_of(sink, all);
+    }
+    X* to = static_cast<X*>(a.out) + at * D + d;
+    const bool any = total != 0.0f;
+    to[0] = X(any ? x.x / total : 0.0f), to[1] = X(any ? x.y / total : 0.0f);
+    to[2] = X(any ? x.z / total : 0.0f), to[3] = X(any ? x.w / total : 0.0f);
+  }
+}
+
+template <class T>
+int launch_codes(const AttentionChunksArgs& a, cudaStream_t stream) {
+  static PerDevice configured;
+  DRIFT_TRY(ensure_shared_memory(configured, attention_codes_kernel<T>, T::BYTES));
+  const int units = (a.at.longest * a.group + T::ROWS - 1) / T::ROWS;
+  DRIFT_CUDA(launch_pdl(attention_codes_kernel<T>, dim3(unsigned(units) * a.splits, a.kv_heads, a.at.batch), T::THREADS,
+                        T::BYTES, stream, a));
+  DRIFT_LAUNCHED("attention_codes");
+  return 0;
+}
+
+template <int D, bool BF16>
+int launch_rows_of(const AttentionChunksArgs& a, int rows_per_unit, cudaStream_t stream) {
+  if (rows_per_unit == 4) return launch_codes<CodesTraits<D, BF16, 0>>(a, stream);
+  if constexpr (D <= 128) {
+    if (rows_per_unit == 24) return launch_codes<CodesTraits<D, BF16, 3>>(a, stream);
+    if (rows_per_unit == 16) return launch_codes<CodesTraits<D, BF16, 2>>(a, stream);
+  }
+  return launch_codes<CodesTraits<D, BF16, 1>>(a, stream);
+}
+
+template <int D>
+int launch_dim(const AttentionChunksArgs& a, bool bf16, int rows_per_unit, cudaStream_t stream) {
+  return bf16 ? launch_rows_of<D, true>(a, rows_per_unit, stream) : launch_rows_of<D, false>(a, rows_per_unit, stream);
+}
+
+#define DRIFT_CODES_REGISTER(D, rt, name)                                            \
+  DRIFT_REGISTER(attention_codes_f32_d##D##_##name, (attention_codes_kernel<CodesTraits<D, false, rt>>)) \
+  DRIFT_REGISTER(attention_codes_bf16_d##D##_##name, (attention_codes_kernel<CodesTraits<D, true, rt>>))
+#define DRIFT_CODES_REGISTER_NARROW(D) \
+  DRIFT_CODES_REGISTER(D, 0, r4)       \
+  DRIFT_CODES_REGISTER(D, 1, r8)       \
+  DRIFT_CODES_REGISTER(D, 2, r16)      \
+  DRIFT_CODES_REGISTER(D, 3, r24)
+DRIFT_CODES_REGISTER_NARROW(64)
+DRIFT_CODES_REGISTER_NARROW(80)
+DRIFT_CODES_REGISTER_NARROW(128)
+DRIFT_CODES_REGISTER(256, 0, r4)
+DRIFT_CODES_REGISTER(256, 1, r8)
+
+}  // namespace
+
+int launch_attention_codes(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
+                           cudaStream_t stream) {
+  const bool bf16 = x_dtype == DRIFT_BF16;
+  switch (head_dim) {
+    case 64: return launch_dim<64>(a, bf16, rows_per_unit, stream);
+    case 80: return launch_dim<80>(a, bf16, rows_per_unit, stream);
+    case 128: return launch_dim<128>(a, bf16, rows_per_unit, stream);
+    default: return launch_dim<256>(a, bf16, rows_per_unit, stream);
+  }
+}
+
+}  // namespace drift

@@ -1,19 +1,17 @@
-// attention_chunks for few rows: a decoding step, drafted tokens, and every
-// chunk in F32.
+// attention_chunks over an F16 cache for few rows: a decoding step, and every
+// chunk in F32 of heads of 256.
 //
 // A unit is a key head of one sequence with up to 8 NT of the (token, query
 // head) rows that read it; a CTA takes one split of the unit's key tiles,
-// each of its 8 warps every eighth tile. The products are turned round --
-// scores^T = K q^T and out^T = V^T p^T by mma.sync m16n8k16, keys and then
-// dimensions as the 16 rows and the query rows as the 8 columns -- because
-// there are few query rows: 8 columns leave nothing idle where 16 rows would
-// be half empty. Keys and values go from the cache straight into the
+// each of its 8 warps every eighth tile of 16 keys. The products are turned
+// round -- scores^T = K q^T and out^T = V^T p^T by mma.sync m16n8k16, keys and
+// then dimensions as the 16 rows and the query rows as the 8 columns --
+// because there are few query rows: 8 columns leave nothing idle where 16 rows
+// would be half empty. Keys and values go from the cache straight into the
 // registers that the matrix instruction reads: a lane's 16 bytes of a key row
 // (or of a dimension's consecutive positions) become its A fragments by
 // numbering the product's inner index as the bytes lie, which the query
-// fragments, laid out once in shared memory, follow. Codes become F16 by two
-// byte permutes and a subtraction, exactly; a key's scale multiplies its
-// score, and a value's its weight.
+// fragments, laid out once in shared memory, follow.
 //
 // F32 rows: q and the weights are two F16 terms each (x = hi + lo to 2^-22),
 // keys and values exact, so the products are F32-grade. BF16 rows: q is one
@@ -75,29 +73,17 @@ __device__ __forceinline__ float2 pair_value(uint32_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-// Four codes as two pairs of F16: a byte u = code + 128 under the exponent of
-// 1024 is 1024 + u, less 1152.
-__device__ __forceinline__ void code_pairs(uint32_t codes, uint32_t& first, uint32_t& second) {
-  const uint32_t u = codes ^ 0x80808080u;
-  const __half2 less = __half2half2(__ushort_as_half(0x6480));  // 1152
-  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), less);
-  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), less);
-  first = *reinterpret_cast<const uint32_t*>(&x);
-  second = *reinterpret_cast<const uint32_t*>(&y);
-}
-
 // How a lane's loads cover rows of D values, 16 of them to a k-step: chunks of
 // 16 bytes a lane while whole ones last, then (D = 80) one k-step of 4 values
 // a lane. first_of(k-step) is where lane t's four values of the step start.
-template <int D, bool CODES>
+template <int D>
 struct RowMap {
-  static constexpr int PER = CODES ? 16 : 8;            // values of a 16-byte chunk
+  static constexpr int PER = 8;                         // values of a 16-byte chunk
   static constexpr int STEPS_PER = PER / 4;             // k-steps of a chunk
   static constexpr int CHUNKS = D / (4 * PER);          // whole chunks
   static constexpr int STEPS = D / 16;
   static constexpr int TAIL = STEPS - CHUNKS * STEPS_PER;  // 0 or 1
-  static constexpr int WORDS = CODES ? STEPS : 2 * STEPS;  // 32-bit words a lane holds of a row
+  static constexpr int WORDS = 2 * STEPS;               // 32-bit words a lane holds of a row
   static_assert(TAIL <= 1, "one k-step past the chunks at most");
   __device__ static int first_of(int step, int t) {
     return step < CHUNKS * STEPS_PER ? (step / STEPS_PER) * 4 * PER + PER * t + 4 * (step % STEPS_PER)
@@ -105,16 +91,17 @@ struct RowMap {
   }
 };
 
-template <int D_, bool CODES_, bool BF16_, int NT_, int TILE_>
+constexpr int TILE = 16;  // keys of a warp's tile
+
+template <int D_, bool BF16_, int NT_>
 struct RowsTraits {
-  static constexpr int D = D_, NT = NT_, TILE = TILE_;
-  static constexpr bool CODES = CODES_, BF16 = BF16_;
+  static constexpr int D = D_, NT = NT_;
+  static constexpr bool BF16 = BF16_;
   static constexpr int TERMS = BF16 ? 1 : 2;
-  using Map = RowMap<D, CODES>;
-  static constexpr int MT = TILE / 16;   // 16-key tiles of a warp's tile
+  static constexpr int CTAS = D <= 128 && NT == 1 ? 2 : 1;  // of an SM: registers
+  using Map = RowMap<D>;
   static constexpr int ROWS = 8 * NT;
   static constexpr int DM = D / 16;      // 16-dimension tiles of the output
-  static constexpr int VWORDS = CODES ? TILE / 16 : TILE / 8;  // words a lane holds of a dimension's positions
   static constexpr int Q_BYTES = Map::STEPS * NT * TERMS * 32 * 8;
   static constexpr int MERGE_BYTES = WARPS * ROWS * (D + 4) * 4;
   static constexpr int BYTES = Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;
@@ -122,115 +109,76 @@ struct RowsTraits {
 
 template <class T>
 struct RowsWarp {
-  static constexpr int D = T::D, TILE = T::TILE, MT = T::MT, DM = T::DM;
-  static constexpr bool CODES = T::CODES;
+  static constexpr int D = T::D, DM = T::DM;
   using Map = typename T::Map;
 
   const AttentionChunksArgs& a;
   const Chunk& chunk;
   const SeenTiles& seen;
-  const int head, lane, g, t;
-  uint32_t k[MT][2][Map::WORDS];
-  uint32_t v[DM][2][T::VWORDS];
-  float k_scale[MT][2], v_scale[MT][2];
+  const int head, g, t;
+  const uint32_t page_magic;  // 2^32 / page_size, up
+  int page, place;            // of the tile that is loaded next
+  uint32_t k[2][Map::WORDS];  // [row g, g + 8]
+  uint2 v[DM][2];             // [16 dimensions][row g, g + 8], positions 4 t .. 4 t + 3
 
   __device__ RowsWarp(const AttentionChunksArgs& a, const Chunk& c, const SeenTiles& s, int head, int lane)
-      : a(a), chunk(c), seen(s), head(head), lane(lane), g(lane / 4), t(lane % 4) {}
+      : a(a), chunk(c), seen(s), head(head), g(lane / 4), t(lane % 4),
+        page_magic(0xffffffffu / uint32_t(a.at.page_size) + 1) {}
 
-  // The page that holds the sixteen positions from `position` on, or -1: past
-  // the last key, or a page that the cache does not have.
-  __device__ int page_of(int position) const {
-    if (position >= seen.end) return -1;
-    const int page = chunk.table[position / a.at.page_size];
-    if (page >= 0 && page < a.at.pages) return page;
+  // The page that holds the tile at key0 and its place in it: -1 past the last
+  // key, or for a page that the cache does not have.
+  __device__ void find_page(int key0) {
+    int index = int(__umulhi(uint32_t(key0), page_magic));  // (one too many at most)
+    place = key0 - index * a.at.page_size;
+    if (place < 0) --index, place += a.at.page_size;
+    page = -1;
+    if (key0 >= seen.end) return;
+    page = chunk.table[index];
+    if (page >= 0 && page < a.at.pages) return;
     chunk_error(a.error);
-    return -1;
+    page = -1;
   }
-  // Row r of the score tile m, r = g or g + 8, is this position of the tile:
-  // the product of weights and values then meets the positions in the order
-  // in which a lane's value words hold them.
-  __device__ int position_of(int m, int half) const {
-    return TILE / 4 * (g / 2) + 4 * m + g % 2 + 2 * half;
-  }
+  // Row r of the score tile, r = g or g + 8, is this position of the tile: the
+  // product of weights and values then meets the positions in the order in
+  // which a lane's value words hold them.
+  __device__ int position_of(int half) const { return 4 * (g / 2) + g % 2 + 2 * half; }
 
-  __device__ void load_keys(int key0) {
-    const int base = key0 + TILE / 4 * (g / 2) / 16 * 16;  // the sixteen this lane's rows are in
-    const int page = page_of(base);
-    const int in_page = base % a.at.page_size;
+  __device__ void load_keys() {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int half = 0; half < 2; ++half) {
+      const __half* row = static_cast<const __half*>(a.keys) +
+                          (((long long)page * a.at.page_size + place + position_of(half)) * a.kv_heads + head) * D;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int place = in_page + (position_of(m, half) + key0 - base);
-        const long long row = (((long long)page * a.at.page_size + place) * a.kv_heads + head) * D;
-#pragma unroll
-        for (int c = 0; c < Map::CHUNKS; ++c) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (page >= 0) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.keys) + (CODES ? row : 2 * row)) + 4 * c + t);
-          k[m][half][4 * c] = x.x, k[m][half][4 * c + 1] = x.y;
-          k[m][half][4 * c + 2] = x.z, k[m][half][4 * c + 3] = x.w;
-        }
-        if constexpr (Map::TAIL) {
-          constexpr int W = 4 * Map::CHUNKS;
-          const uint8_t* from = static_cast<const uint8_t*>(a.keys) + (CODES ? 1 : 2) * (row + Map::CHUNKS * 4 * Map::PER + 4 * t);
-          if constexpr (CODES) {
-            k[m][half][W] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0;
-          } else {
-            const uint2 x = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
-            k[m][half][W] = x.x, k[m][half][W + 1] = x.y;
-          }
-        }
-        if constexpr (CODES) {
-          const long long at = ((long long)page * a.kv_heads + head) * a.at.page_size + place;
-          k_scale[m][half] = page >= 0 ? __ldg(a.key_scales + at) : 0.0f;
-          v_scale[m][half] = page >= 0 ? __ldg(a.value_scales + at) : 0.0f;
-        }
+      for (int c = 0; c < Map::CHUNKS; ++c) {
+        const uint4 x = page >= 0 ? __ldg(reinterpret_cast<const uint4*>(row) + 4 * c + t) : make_uint4(0, 0, 0, 0);
+        k[half][4 * c] = x.x, k[half][4 * c + 1] = x.y, k[half][4 * c + 2] = x.z, k[half][4 * c + 3] = x.w;
       }
+      if constexpr (Map::TAIL) {
+        constexpr int W = 4 * Map::CHUNKS;
+        const uint2 x = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(row + Map::CHUNKS * 4 * Map::PER) + t) : make_uint2(0, 0);
+        k[half][W] = x.x, k[half][W + 1] = x.y;
+      }
+    }
   }
-
-  __device__ void load_values(int key0) {
-    const int first = key0 + TILE / 4 * t;  // this lane's TILE / 4 positions
-    const int page = page_of(first / 16 * 16);
-    const int place = first % a.at.page_size;
-    const long long column = ((long long)page * a.kv_heads + head) * D * a.at.page_size + place;
+  __device__ void load_values() {
+    const __half* column = static_cast<const __half*>(a.values) +
+                           ((long long)page * a.kv_heads + head) * D * a.at.page_size + place + 4 * t;
 #pragma unroll
     for (int m = 0; m < DM; ++m)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int d = 16 * m + g + 8 * half;
-        const uint8_t* from = static_cast<const uint8_t*>(a.values) + (CODES ? 1 : 2) * (column + (long long)d * a.at.page_size);
-        uint32_t (&to)[T::VWORDS] = v[m][half];
-        if constexpr (T::VWORDS == 1) {
-          to[0] = page >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0;
-        } else if constexpr (T::VWORDS == 2) {
-          const uint2 x = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
-          to[0] = x.x, to[1] = x.y;
-        } else {
-          const uint4 x = page >= 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
-          to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
-        }
-      }
+      for (int half = 0; half < 2; ++half)
+        v[m][half] = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(column + (16 * m + g + 8 * half) * (long long)a.at.page_size))
+                               : make_uint2(0, 0);
   }
 
-  // Score tile m's A fragment of a k-step (rows g, g + 8; the step's first and
-  // second eight).
-  __device__ void key_fragment(int m, int step, uint32_t (&f)[4]) const {
-    if constexpr (CODES) {
-      code_pairs(k[m][0][step], f[0], f[2]);
-      code_pairs(k[m][1][step], f[1], f[3]);
-    } else {
-      f[0] = k[m][0][2 * step], f[2] = k[m][0][2 * step + 1];
-      f[1] = k[m][1][2 * step], f[3] = k[m][1][2 * step + 1];
-    }
+  // The A fragments (rows g, g + 8; the step's first and second eight).
+  __device__ void key_fragment(int step, uint32_t (&f)[4]) const {
+    f[0] = k[0][2 * step], f[2] = k[0][2 * step + 1];
+    f[1] = k[1][2 * step], f[3] = k[1][2 * step + 1];
   }
-  __device__ void value_fragment(int m, int step, uint32_t (&f)[4]) const {
-    if constexpr (CODES) {
-      code_pairs(v[m][0][step], f[0], f[2]);
-      code_pairs(v[m][1][step], f[1], f[3]);
-    } else {
-      f[0] = v[m][0][2 * step], f[2] = v[m][0][2 * step + 1];
-      f[1] = v[m][1][2 * step], f[3] = v[m][1][2 * step + 1];
-    }
+  __device__ void value_fragment(int m, uint32_t (&f)[4]) const {
+    f[0] = v[m][0].x, f[2] = v[m][0].y;
+    f[1] = v[m][1].x, f[3] = v[m][1].y;
   }
 };
 
@@ -246,11 +194,10 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t word, int p, int end,
 }
 
 template <class T>
-__global__ void __launch_bounds__(THREADS) attention_rows_kernel(const AttentionChunksArgs a) {
+__global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const AttentionChunksArgs a) {
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
-  constexpr int D = T::D, NT = T::NT, TILE = T::TILE, MT = T::MT, ROWS = T::ROWS, TERMS = T::TERMS;
-  constexpr bool CODES = T::CODES;
+  constexpr int D = T::D, NT = T::NT, ROWS = T::ROWS, TERMS = T::TERMS;
   using Map = typename T::Map;
   using X = typename std::conditional<T::BF16, __nv_bfloat16, float>::type;
   extern __shared__ __align__(16) uint8_t shared[];
@@ -271,8 +218,10 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
   RowsWarp<T> w(a, chunk, seen, head, lane);
   int tile = tile0 + warp;
   if (tile < tile1) {
-    w.load_keys(seen.key_of(tile));
-    w.load_values(seen.key_of(tile));
+    w.find_page(seen.key_of(tile));
+    w.load_keys();
+    w.load_values();
+    if (tile + WARPS < tile1) w.find_page(seen.key_of(tile + WARPS));
   }
 
   // q: each row divided by a power of two near its largest value, in F16
@@ -333,7 +282,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
   const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;  // what some row sees
 
   float out[NT][T::DM][4];
-  float largest[NT][2], sum[NT][2], v_unit = 0.0f;
+  float largest[NT][2], sum[NT][2];
   bool taken_out = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -344,36 +293,24 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
   }
 
   for (; tile < tile1; tile += WARPS) {
-    const int key0 = seen.key_of(tile);
-    const int next = tile + WARPS;
-    float s[NT][MT][4];
+    const int key0 = seen.key_of(tile), next = tile + WARPS;
+    float s[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) s[n][m][0] = s[n][m][1] = s[n][m][2] = s[n][m][3] = 0.0f;
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
     for (int step = 0; step < Map::STEPS; ++step) {
-      uint32_t f[MT][4];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) w.key_fragment(m, step, f[m]);
+      uint32_t f[4];
+      w.key_fragment(step, f);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int term = TERMS - 1; term >= 0; --term) {
           const uint2 b = fragments[((step * NT + n) * TERMS + term) * 32 + lane];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) mma_f16(s[n][m], f[m], b.x, b.y);
+          mma_f16(s[n], f, b.x, b.y);
         }
     }
-    float k_scale[MT][2], v_scale[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        k_scale[m][half] = CODES ? w.k_scale[m][half] : 1.0f;
-        v_scale[m][half] = CODES ? w.v_scale[m][half] : 1.0f;
-      }
-    if (next < tile1) w.load_keys(seen.key_of(next));  // on their way under the rest of this tile
+    // (the keys' registers are the next tile's; its page was looked up a tile ago)
+    if (next < tile1) w.load_keys();
 
     // scores, and each column's largest
     const bool whole = key0 + TILE <= all_end && (key0 >= all_low || key0 + TILE <= first);
@@ -385,21 +322,18 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
       for (int e = 0; e < 2; ++e) {
         float top = -INFINITY;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float x = s[n][m][2 * half + e] * multiplier[n][e];
-            if (CODES) x *= k_scale[m][half];
-            if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-            if (!whole) {
-              const int key = key0 + w.position_of(m, half);
-              const bool sees = key < seen.end && (!a.causal || key <= position[n][e]) &&
-                                (a.window == 0 || key > position[n][e] - a.window || key < first);
-              x = sees ? x : -INFINITY;
-            }
-            s[n][m][2 * half + e] = x;
-            top = fmaxf(top, x);
+        for (int half = 0; half < 2; ++half) {
+          float x = s[n][2 * half + e] * multiplier[n][e];
+          if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
+          if (!whole) {
+            const int key = key0 + w.position_of(half);
+            const bool sees = key < seen.end && (!a.causal || key <= position[n][e]) &&
+                              (a.window == 0 || key > position[n][e] - a.window || key < first);
+            x = sees ? x : -INFINITY;
           }
+          s[n][2 * half + e] = x;
+          top = fmaxf(top, x);
+        }
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float before = largest[n][e];
@@ -408,97 +342,72 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
         grown = grown || now > before;
         largest[n][e] = now;
       }
-    // a weight is p times its value's scale over the warp's running unit, a
-    // power of two at or above every scale so far: at most 1, as F16 wants
-    float shrink = 1.0f;
-    if constexpr (CODES) {
-      float top = 0.0f;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int key = key0 + w.position_of(m, half);
-          if (key >= seen.end || (key < lowest && key >= first)) v_scale[m][half] = 0.0f;
-          if (v_scale[m][half] <= 3.402823466e38f) top = fmaxf(top, v_scale[m][half]);  // (the finite ones)
-        }
-#pragma unroll
-      for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (top > v_unit) {
-        const uint32_t bits = __float_as_uint(top);
-        const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-        const float unit = __uint_as_float(max(up, 0x01000000u));  // (its inverse is normal too)
-        shrink = v_unit / unit;
-        v_unit = unit;
-        grown = true;
-      }
-    }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         sum[n][0] *= rescale[n][0], sum[n][1] *= rescale[n][1];
-        const float f0 = rescale[n][0] * shrink, f1 = rescale[n][1] * shrink;
 #pragma unroll
         for (int m = 0; m < T::DM; ++m) {
-          out[n][m][0] *= f0, out[n][m][1] *= f1;
-          out[n][m][2] *= f0, out[n][m][3] *= f1;
+          out[n][m][0] *= rescale[n][0], out[n][m][1] *= rescale[n][1];
+          out[n][m][2] *= rescale[n][0], out[n][m][3] *= rescale[n][1];
         }
       }
     }
-    const float v_inverse = CODES && v_unit > 0.0f ? 1.0f / v_unit : 0.0f;  // exact
-    uint32_t p[NT][MT][TERMS][2];
+    uint32_t p[NT][TERMS][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int half = 0; half < 2; ++half) {
+        float y[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float y[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = s[n][m][2 * half + e];
-            const float weight = weight_of(x, largest[n][e]);
-            sum[n][e] += weight;
-            y[e] = CODES ? (x == -INFINITY ? 0.0f : weight * (v_scale[m][half] * v_inverse)) : weight;
-          }
-          const uint32_t hi = half_pair(y[0], y[1]);
-          p[n][m][0][half] = turn(hi);
-          if constexpr (TERMS == 2) {
-            const float2 u = pair_value(hi);
-            p[n][m][1][half] = turn(half_pair(y[0] - u.x, y[1] - u.y));
-          }
+        for (int e = 0; e < 2; ++e) {
+          y[e] = weight_of(s[n][2 * half + e], largest[n][e]);
+          sum[n][e] += y[e];
         }
+        const uint32_t hi = half_pair(y[0], y[1]);
+        p[n][0][half] = turn(hi);
+        if constexpr (TERMS == 2) {
+          const float2 u = pair_value(hi);
+          p[n][1][half] = turn(half_pair(y[0] - u.x, y[1] - u.y));
+        }
+      }
     // where rows differ in what they see, a value that is not finite must not
     // meet the zero weights of those that do not see it: it is taken out here
     // and added to the rows that see it at the end
-    if (!CODES && !whole) {
+    if (!whole) {
 #pragma unroll
       for (int m = 0; m < T::DM; ++m)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int j = 0; j < T::VWORDS; ++j)
-            w.v[m][half][j] = finite_halves(w.v[m][half][j], key0 + TILE / 4 * t + 2 * j, seen.end, lowest, first, taken_out);
+        for (int half = 0; half < 2; ++half) {
+          w.v[m][half].x = finite_halves(w.v[m][half].x, key0 + 4 * t, seen.end, lowest, first, taken_out);
+          w.v[m][half].y = finite_halves(w.v[m][half].y, key0 + 4 * t + 2, seen.end, lowest, first, taken_out);
+        }
     }
+    // (a tile's sums start from zero: the tensor core's drop low bits as a
+    // chain grows, F32 additions round)
 #pragma unroll
-    for (int m = 0; m < T::DM; ++m)
+    for (int m = 0; m < T::DM; ++m) {
+      uint32_t f[4];
+      w.value_fragment(m, f);
 #pragma unroll
-      for (int step = 0; step < MT; ++step) {
-        uint32_t f[4];
-        w.value_fragment(m, step, f);
+      for (int n = 0; n < NT; ++n) {
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int term = TERMS - 1; term >= 0; --term) mma_f16(o, f, p[n][term][0], p[n][term][1]);
 #pragma unroll
-          for (int term = TERMS - 1; term >= 0; --term)
-            mma_f16(out[n][m], f, p[n][step][term][0], p[n][step][term][1]);
+        for (int e = 0; e < 4; ++e) out[n][m][e] += o[e];
       }
-    if (next < tile1) w.load_values(seen.key_of(next));
+    }
+    if (next < tile1) {
+      w.load_values();
+      if (next + WARPS < tile1) w.find_page(seen.key_of(next + WARPS));
+    }
   }
 
   // the warps' results: [warp][row][D] and [warp][row] (largest, sum)
   __syncthreads();  // (past the q fragments)
   float* merged = reinterpret_cast<float*>(shared);
   float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
-  const float unit_scale = CODES ? v_unit : 1.0f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -510,8 +419,8 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
       if (g == 0) stats[warp * ROWS + r] = make_float2(largest[n][e], total);
 #pragma unroll
       for (int m = 0; m < T::DM; ++m) {
-        merged[(warp * ROWS + r) * D + 16 * m + g] = out[n][m][e] * unit_scale;
-        merged[(warp * ROWS + r) * D + 16 * m + g + 8] = out[n][m][2 + e] * unit_scale;
+        merged[(warp * ROWS + r) * D + 16 * m + g] = out[n][m][e];
+        merged[(warp * ROWS + r) * D + 16 * m + g + 8] = out[n][m][2 + e];
       }
     }
   taken_out = __syncthreads_or(taken_out);
@@ -531,7 +440,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
       const float4 y = *reinterpret_cast<const float4*>(merged + (j * ROWS + r) * D + d);
       x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
     }
-    if (!CODES && taken_out) {
+    if (taken_out) {
       const int own = chunk.position + row / a.group;
       for (int j = tile0; j < tile1; ++j) {
         const int key0 = seen.key_of(j);
@@ -594,22 +503,40 @@ __global__ void __launch_bounds__(THREADS) attention_chunks_join_kernel(const Jo
   for (int s = lane; s < splits; s += 32) top = fmaxf(top, stats[s].x);
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float total = a.sinks ? weight_of(a.sinks[head], top) : 0.0f;
-  constexpr int PER = (D + 127) / 128;
+  float total = 0.0f;
+  constexpr int PER = (D + 127) / 128, FLIGHT = 8;  // splits' rows under way
   float x[PER][4] = {};
-  for (int s = 0; s < splits; ++s) {
-    const float2 stat = stats[s];
-    const float f = weight_of(stat.x, top);
-    total += stat.y * f;  // (a NaN stays one)
-    if (f == 0.0f) continue;
+  for (int s0 = 0; s0 < splits; s0 += 32) {
+    float factor = 0.0f;
+    if (s0 + lane < splits) {
+      const float2 stat = stats[s0 + lane];
+      factor = weight_of(stat.x, top);
+      total += stat.y * factor;  // (a NaN stays one)
+    }
+    const int here = min(32, splits - s0);
+    for (int s1 = 0; s1 < here; s1 += FLIGHT) {
+      float4 y[FLIGHT][PER];
 #pragma unroll
-    for (int c = 0; c < PER; ++c) {
-      const int d = 4 * (lane + 32 * c);
-      if (d >= D) continue;
-      const float4 y = *reinterpret_cast<const float4*>(parts + (long long)s * D + d);
-      x[c][0] += y.x * f, x[c][1] += y.y * f, x[c][2] += y.z * f, x[c][3] += y.w * f;
+      for (int n = 0; n < FLIGHT; ++n)
+#pragma unroll
+        for (int c = 0; c < PER; ++c) {
+          const int d = 4 * (lane + 32 * c);
+          y[n][c] = s1 + n < here && d < D ? *reinterpret_cast<const float4*>(parts + (long long)(s0 + s1 + n) * D + d)
+                                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+      for (int n = 0; n < FLIGHT; ++n) {
+        const float f = __shfl_sync(0xffffffffu, factor, (s1 + n) % 32);
+        if (s1 + n >= here || f == 0.0f) continue;
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          x[c][0] += y[n][c].x * f, x[c][1] += y[n][c].y * f, x[c][2] += y[n][c].z * f, x[c][3] += y[n][c].w * f;
+      }
     }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (a.sinks) total += weight_of(a.sinks[head], top);
   const bool any = total != 0.0f;
 #pragma unroll
   for (int c = 0; c < PER; ++c) {
@@ -632,43 +559,27 @@ int launch_rows(const AttentionChunksArgs& a, cudaStream_t stream) {
   return 0;
 }
 
-// Keys of a warp's tile: 32 where its keys and values (16 bytes a lane and
-// key-row chunk) leave the output room in registers, else 16.
-constexpr int tile_of(int head_dim, bool codes, int columns) {
-  return codes && head_dim <= 128 && columns <= 2 ? 32 : 16;
-}
-
-template <int D, bool CODES, bool BF16>
+template <int D, bool BF16>
 int launch_columns(const AttentionChunksArgs& a, int columns, cudaStream_t stream) {
-  if constexpr (D <= 128) {
-    if (columns == 4) return launch_rows<RowsTraits<D, CODES, BF16, 4, tile_of(D, CODES, 4)>>(a, stream);
-    if (columns == 2) return launch_rows<RowsTraits<D, CODES, BF16, 2, tile_of(D, CODES, 2)>>(a, stream);
-  }
-  return launch_rows<RowsTraits<D, CODES, BF16, 1, tile_of(D, CODES, 1)>>(a, stream);
+  if constexpr (D <= 128)
+    if (columns == 2) return launch_rows<RowsTraits<D, BF16, 2>>(a, stream);
+  return launch_rows<RowsTraits<D, BF16, 1>>(a, stream);
 }
 
 template <int D>
-int launch_dim(const AttentionChunksArgs& a, bool codes, bool bf16, int columns, cudaStream_t stream) {
-  if (codes) return bf16 ? launch_columns<D, true, true>(a, columns, stream) : launch_columns<D, true, false>(a, columns, stream);
-  return bf16 ? launch_columns<D, false, true>(a, columns, stream) : launch_columns<D, false, false>(a, columns, stream);
+int launch_dim(const AttentionChunksArgs& a, bool bf16, int columns, cudaStream_t stream) {
+  return bf16 ? launch_columns<D, true>(a, columns, stream) : launch_columns<D, false>(a, columns, stream);
 }
 
-#define DRIFT_ROWS_REGISTER_AS(D, codes, bf16, nt, name) \
-  DRIFT_REGISTER(name, (attention_rows_kernel<RowsTraits<D, codes, bf16, nt, tile_of(D, codes, nt)>>))
-#define DRIFT_ROWS_REGISTER(D, nt)                                             \
-  DRIFT_ROWS_REGISTER_AS(D, true, true, nt, attention_rows_i8_bf16_d##D##_n##nt)    \
-  DRIFT_ROWS_REGISTER_AS(D, true, false, nt, attention_rows_i8_f32_d##D##_n##nt)    \
-  DRIFT_ROWS_REGISTER_AS(D, false, true, nt, attention_rows_f16_bf16_d##D##_n##nt)  \
-  DRIFT_ROWS_REGISTER_AS(D, false, false, nt, attention_rows_f16_f32_d##D##_n##nt)
+#define DRIFT_ROWS_REGISTER(D, nt)                                                                  \
+  DRIFT_REGISTER(attention_rows_bf16_d##D##_n##nt, (attention_rows_kernel<RowsTraits<D, true, nt>>))  \
+  DRIFT_REGISTER(attention_rows_f32_d##D##_n##nt, (attention_rows_kernel<RowsTraits<D, false, nt>>))
 DRIFT_ROWS_REGISTER(64, 1)
 DRIFT_ROWS_REGISTER(64, 2)
-DRIFT_ROWS_REGISTER(64, 4)
 DRIFT_ROWS_REGISTER(80, 1)
 DRIFT_ROWS_REGISTER(80, 2)
-DRIFT_ROWS_REGISTER(80, 4)
 DRIFT_ROWS_REGISTER(128, 1)
 DRIFT_ROWS_REGISTER(128, 2)
-DRIFT_ROWS_REGISTER(128, 4)
 DRIFT_ROWS_REGISTER(256, 1)
 #define DRIFT_JOIN_REGISTER(D)                                                            \
   DRIFT_REGISTER(attention_chunks_join_f32_d##D, (attention_chunks_join_kernel<D, false>)) \
@@ -680,16 +591,15 @@ DRIFT_JOIN_REGISTER(256)
 
 }  // namespace
 
-int attention_rows_tile(int head_dim, bool codes, int columns) { return tile_of(head_dim, codes, columns); }
-
-int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int columns,
+int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                           cudaStream_t stream) {
-  const bool bf16 = x_dtype == DRIFT_BF16, codes = cache_dtype == DRIFT_I8;
+  const bool bf16 = x_dtype == DRIFT_BF16;
+  const int columns = rows_per_unit / 8;
   switch (head_dim) {
-    case 64: return launch_dim<64>(a, codes, bf16, columns, stream);
-    case 80: return launch_dim<80>(a, codes, bf16, columns, stream);
-    case 128: return launch_dim<128>(a, codes, bf16, columns, stream);
-    default: return launch_dim<256>(a, codes, bf16, columns, stream);
+    case 64: return launch_dim<64>(a, bf16, columns, stream);
+    case 80: return launch_dim<80>(a, bf16, columns, stream);
+    case 128: return launch_dim<128>(a, bf16, columns, stream);
+    default: return launch_dim<256>(a, bf16, columns, stream);
   }
 }
 

@@ -11,9 +11,9 @@
 // scale is NaN and it reads back as NaNs.
 //
 // A CTA takes 16 consecutive positions (an aligned sixteenth-row of a page) of
-// one head: 16 rows in, their keys out as rows, their values out transposed,
-// through shared memory, 16 positions of a dimension in one 16-byte store (32
-// for F16). Bound by memory: (4 or 2) + 1 bytes a value.
+// one head, or of a few: their rows in, the keys out as rows, the values out
+// transposed, through shared memory, 16 positions of a dimension in one 16-byte
+// store (32 for F16). Bound by memory, (4 or 2) + 1 bytes a value.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,18 +29,33 @@ namespace drift {
 namespace {
 
 constexpr int RUN = 16;       // positions of a CTA
-constexpr int THREADS = 256;  // 8 warps, two rows of keys and two of values each
+constexpr int THREADS = 256;  // 8 warps, two rows of keys and two of values of a head each
+// Heads of a CTA that reads: enough loads under way to hide the three dependent
+// ones before them (16 x 4096 positions of 8 heads 58 us, 77 with one). One
+// that writes takes one: its rows wait in registers for their largest value,
+// and with four there were two CTAs an SM (4 x 4099 positions 110 us, 85 with one).
+constexpr int read_heads(int dim) { return dim > 128 ? 2 : 4; }
 
 // x's code for step s > 0: rint(x / s) as if in exact arithmetic. c is within
 // one of it; x - c s is exact in one fused operation (both are multiples of
 // x's or s's last place, and the difference is below s), so comparing twice
 // it with s decides.
-__device__ __forceinline__ int quantize(float x, float s) {
+__device__ __noinline__ float quantize_near_tie(float x, float s) {
   float c = rintf(x / s);
   const float r = fmaf(-c, s, x), twice = 2.0f * r;
   const bool odd = int(c) & 1;
   if (twice > s || (twice == s && odd)) c += 1.0f;
   else if (twice < -s || (twice == -s && odd)) c -= 1.0f;
+  return c;
+}
+// The same by s's reciprocal where that cannot be wrong: x times it is within
+// 127 * 2^-23 < 2^-16 of x / s, so only a product that close to a half between
+// two codes needs the above. (A step so small that its reciprocal is infinite
+// gives NaN here and goes there too.)
+__device__ __forceinline__ int quantize(float x, float s, float reciprocal) {
+  const float t = x * reciprocal;
+  float c = rintf(t);
+  if (!(fabsf(t - c) < 0.4999f)) c = quantize_near_tie(x, s);
   return int(fminf(fmaxf(c, -127.0f), 127.0f));
 }
 
@@ -135,24 +150,25 @@ __global__ void __launch_bounds__(THREADS) cache_write_chunks_kernel(const Write
   for (int i = 0; i < 4; ++i) {
     const int p = warp + 8 * (i % 2);
     const bool in = p >= run.lo && p < run.hi;
-    float scale = 0.0f;
+    float scale = 0.0f, reciprocal = 0.0f;
     if constexpr (CODES) {
       float largest = 0.0f;
-      bool finite = true;
+      float zero = 0.0f;  // NaN once a value is infinite or NaN
 #pragma unroll
       for (int j = 0; j < PER; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           largest = fmaxf(largest, fabsf(x[i][j][e]));
-          finite = finite && fabsf(x[i][j][e]) <= 3.402823466e38f;
+          zero = fmaf(x[i][j][e], 0.0f, zero);
         }
 #pragma unroll
       for (int o = 16; o > 0; o /= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-      finite = __all_sync(0xffffffffu, finite);
+      const bool finite = __all_sync(0xffffffffu, zero == 0.0f);
       scale = finite ? largest / 127.0f : __int_as_float(0x7fc00000);
       if (in && lane == 0)
         (i < 2 ? a.key_scales : a.value_scales)[(run.page * a.kv_heads + head) * a.at.page_size + run.offset + p] =
             scale;
+      reciprocal = 1.0f / scale;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -161,7 +177,7 @@ __global__ void __launch_bounds__(THREADS) cache_write_chunks_kernel(const Write
       __align__(16) Code codes[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (CODES) codes[e] = int8_t(scale > 0.0f ? quantize(x[i][j][e], scale) : 0);
+        if constexpr (CODES) codes[e] = int8_t(scale > 0.0f ? quantize(x[i][j][e], scale, reciprocal) : 0);
         else codes[e] = __float2half_rn(x[i][j][e]);
       }
       Code* to = i < 2 ? static_cast<Code*>(a.keys) +
@@ -211,62 +227,80 @@ __global__ void __launch_bounds__(THREADS) cache_read_chunks_kernel(const ReadAr
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
   constexpr bool CODES = sizeof(Code) == 1;
-  constexpr int PER = (D + 127) / 128;
-  __shared__ __align__(16) Code turned[RUN][D + 16];
-  const int block = blockIdx.x, head = blockIdx.y, z = blockIdx.z;
+  constexpr int PER = (D + 127) / 128, HEADS = read_heads(D);
+  __shared__ __align__(16) Code turned[HEADS][RUN][D + 16];
+  const int block = blockIdx.x, head0 = blockIdx.y * HEADS, z = blockIdx.z;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const Chunk chunk(a.at, z);
-  if (!chunk.ok && block == 0 && head == 0 && threadIdx.x == 0) chunk_error(a.error);
+  if (!chunk.ok && block == 0 && head0 == 0 && threadIdx.x == 0) chunk_error(a.error);
   const Run run(a.at, chunk, block, a.error);
   if (run.hi <= run.lo) return;
+  const int heads = min(HEADS, a.kv_heads - head0);
   const Code* keys = static_cast<const Code*>(a.keys) +
-                     ((run.page * a.at.page_size + run.offset) * a.kv_heads + head) * (long long)D;
+                     ((run.page * a.at.page_size + run.offset) * a.kv_heads + head0) * (long long)D;
   const Code* values = static_cast<const Code*>(a.values) +
-                       (run.page * a.kv_heads + head) * (long long)D * a.at.page_size + run.offset;
-  const long long scales = (run.page * a.kv_heads + head) * a.at.page_size + run.offset;
+                       (run.page * a.kv_heads + head0) * (long long)D * a.at.page_size + run.offset;
   // (the sixteen positions are one page's: those that are not the chunk's are
   // read with it and not written out)
   using Four = typename std::conditional<CODES, uint32_t, uint2>::type;
-  Four held[2][PER];
+  constexpr int WORDS = int(sizeof(Code)) * RUN / 16, COLUMNS = (HEADS * D + THREADS - 1) / THREADS;
+  uint4 columns[COLUMNS][WORDS];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int n = 0; n < COLUMNS; ++n) {
+    const int d = threadIdx.x + THREADS * n;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = 4 * (lane + 32 * j);
-      held[i][j] = Four{};
-      if (d < D && !run.missing) held[i][j] = *reinterpret_cast<const Four*>(keys + (long long)(warp + 8 * i) * a.kv_heads * D + d);
-    }
-  float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-  if (CODES && !run.missing) {
+    for (int j = 0; j < WORDS; ++j)
+      columns[n][j] = d < heads * D && !run.missing
+                          ? reinterpret_cast<const uint4*>(values + (long long)d * a.at.page_size)[j]
+                          : make_uint4(0, 0, 0, 0);
+  }
+  Four held[HEADS][2][PER];
+  float scale[HEADS][4];
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    const bool there = h < heads && !run.missing;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int d = 4 * (lane + 32 * j);
+        held[h][i][j] = Four{};
+        if (d < D && there)
+          held[h][i][j] = *reinterpret_cast<const Four*>(keys + ((long long)(warp + 8 * i) * a.kv_heads + h) * D + d);
+      }
+    const long long scales = (run.page * a.kv_heads + head0 + h) * a.at.page_size + run.offset;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      scale[i] = (i < 2 ? a.key_scales : a.value_scales)[scales + warp + 8 * (i % 2)];
+      scale[h][i] = CODES && there ? (i < 2 ? a.key_scales : a.value_scales)[scales + warp + 8 * (i % 2)] : 1.0f;
   }
-  for (int d = threadIdx.x; d < D; d += THREADS) {
-    __align__(16) Code column[RUN] = {};
-    if (!run.missing)
 #pragma unroll
-      for (int j = 0; j < int(sizeof(column)) / 16; ++j)
-        reinterpret_cast<uint4*>(column)[j] = reinterpret_cast<const uint4*>(values + (long long)d * a.at.page_size)[j];
+  for (int n = 0; n < COLUMNS; ++n) {
+    const int d = threadIdx.x + THREADS * n;
+    if (d >= HEADS * D) break;
+    const Code* column = reinterpret_cast<const Code*>(columns[n]);
 #pragma unroll
-    for (int p = 0; p < RUN; ++p) turned[p][d] = column[p];
+    for (int p = 0; p < RUN; ++p) turned[d / D][p][d % D] = column[p];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int p = warp + 8 * (i % 2);
-    if (p < run.lo || p >= run.hi) continue;
-    X* to = static_cast<X*>(i < 2 ? a.k : a.v) + ((run.row + p) * a.kv_heads + head) * D;
+  for (int h = 0; h < HEADS; ++h) {
+    if (h >= heads) break;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = 4 * (lane + 32 * j);
-      if (d >= D) continue;
-      const Four four = i < 2 ? held[i % 2][j] : *reinterpret_cast<const Four*>(&turned[p][d]);
-      const Code* codes = reinterpret_cast<const Code*>(&four);
-      float x[4];
+    for (int i = 0; i < 4; ++i) {
+      const int p = warp + 8 * (i % 2);
+      if (p < run.lo || p >= run.hi) continue;
+      X* to = static_cast<X*>(i < 2 ? a.k : a.v) + ((run.row + p) * a.kv_heads + head0 + h) * D;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = CODES ? float(codes[e]) * scale[i] : float(codes[e]);
-      store_four(to + d, x);
+      for (int j = 0; j < PER; ++j) {
+        const int d = 4 * (lane + 32 * j);
+        if (d >= D) continue;
+        const Four four = i < 2 ? held[h][i % 2][j] : *reinterpret_cast<const Four*>(&turned[h][p][d]);
+        const Code* codes = reinterpret_cast<const Code*>(&four);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = CODES ? float(codes[e]) * scale[h][i] : float(codes[e]);
+        store_four(to + d, x);
+      }
     }
   }
 }
@@ -303,7 +337,7 @@ int launch_read(const ReadArgs& a, int x_dtype, int cache_dtype, cudaStream_t st
   const bool bf16 = x_dtype == DRIFT_BF16, codes = cache_dtype == DRIFT_I8;
   auto kernel = codes ? (bf16 ? cache_read_chunks_kernel<D, __nv_bfloat16, int8_t> : cache_read_chunks_kernel<D, float, int8_t>)
                       : (bf16 ? cache_read_chunks_kernel<D, __nv_bfloat16, __half> : cache_read_chunks_kernel<D, float, __half>);
-  DRIFT_CUDA(launch_pdl(kernel, dim3(run_blocks(a.at.longest), a.kv_heads, a.at.batch), THREADS, 0, stream, a));
+  DRIFT_CUDA(launch_pdl(kernel, dim3(run_blocks(a.at.longest), (a.kv_heads + read_heads(D) - 1) / read_heads(D), a.at.batch), THREADS, 0, stream, a));
   DRIFT_LAUNCHED("cache_read_chunks");
   return 0;
 }

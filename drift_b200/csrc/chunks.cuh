@@ -131,11 +131,17 @@ int check_chunks(const char* call, int x_dtype, long long tokens, int kv_heads, 
                  const int32_t* positions, int batch, int longest);
 int check_rows_aligned(const char* call, const void* a, const void* b);
 
-// attention_rows.cu: `columns` tiles of 8 rows a unit (1, 2 or 4; 1 for heads
-// of 256), and the keys of one of its tiles.
-int attention_rows_tile(int head_dim, bool codes, int columns);
-int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int columns,
+// For few rows: attention_rows.cu over F16 caches (8 or 16 rows a unit, heads
+// of 256 8; 16-key tiles) and attention_codes.cu over 8-bit ones (4, 8, 16 or
+// 24, heads of 256 up to 8; 32-key tiles).
+int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                           cudaStream_t stream);
+// (the warps of a CTA of the latter)
+__host__ __device__ constexpr int attention_codes_warps(int head_dim, int rows_per_unit) {
+  return head_dim == 128 && rows_per_unit <= 8 ? 4 : 8;
+}
+int launch_attention_codes(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
+                           cudaStream_t stream);
 // attention_tiles.cu (F32 rows: heads up to 128): `row_tiles` tiles of 128 rows
 // a unit (1 or 2; 1 for heads of 256), and the keys of one of its tiles.
 int attention_tiles_keys(int head_dim, bool bf16);

@@ -91,7 +91,10 @@ def attention(q, cache, tables, new, counts, spec):
             vh = torch.where(seen.any(0)[:, None], vh, 0.0)
             score = (x @ kh.T) * spec.scale
             magnitude = (x.abs() @ kh.abs().T) * abs(spec.scale)
-            lost = (x.abs().amax(1, keepdim=True) * kh.abs().sum(1)[None]) * abs(spec.scale) * 2.0 ** -21
+            # (few BF16 rows over an 8-bit cache: q in steps of 2^-13 of its
+            # leading bit's worth, and weights in steps of 2^-18)
+            steps = 2.0 ** -14 if cache.keys.dtype == torch.int8 and q.dtype == torch.bfloat16 else 2.0 ** -21
+            lost = (x.abs().amax(1, keepdim=True) * kh.abs().sum(1)[None]) * abs(spec.scale) * steps
             if spec.softcap:
                 score = spec.softcap * torch.tanh(score / spec.softcap)
             rounded = coded = 0.0
@@ -128,7 +131,10 @@ def attention(q, cache, tables, new, counts, spec):
                 coded_floor = 2.0 ** -25 * 2 * scales[seen.any(0), h // group].max()
             else:
                 coded_floor = 0.0
-            floor = coded_floor + seen.sum(1, keepdim=True) * 2.0 ** -38 * reach / torch.where(
+            # a weight in whole steps is off by 2^-27 of one (F32, and up to four
+            # rows) or 2^-19, in F16 terms by 2^-38
+            step = (2.0 ** -27 if q.dtype == torch.float32 else 2.0 ** -19) if scales is not None else 2.0 ** -38
+            floor = coded_floor + seen.sum(1, keepdim=True) * step * reach / torch.where(
                 total > 0, torch.minimum(safe, torch.ones_like(safe)), 1.0)
             tolerance[row:row + n, h] = (mass * (2 * delta + 2.0 ** -21 + rounding + coded + chain) + floor
                                          + out[row:row + n, h].abs() * UNIT[q.dtype] + 1e-30)
