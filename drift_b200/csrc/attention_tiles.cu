@@ -538,10 +538,12 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int position = chunk.position + token;
     const int hi = a.causal ? position + 1 : seen.end;
     const int lo = a.window > 0 ? position - a.window + 1 : 0;
-    // what all of this row tile's rows see
-    const int last = min(row0 + ROW_TILE * (i + 1), row1) - 1;
-    const int tile_end = a.causal ? chunk.position + (row0 + ROW_TILE * i) / a.group + 1 : seen.end;
-    const int tile_low = a.window > 0 ? chunk.position + max(last, 0) / a.group - a.window + 1 : 0;
+    // what all of this warp's rows see (from `all_low` to `all_end`, and below
+    // `first`), and what some row sees
+    const int warp_row0 = row0 + ROW_TILE * i + 32 * (warp % 4), warp_row1 = min(warp_row0 + 32, row1);
+    const int token_first = chunk.position + warp_row0 / a.group, token_last = chunk.position + max(warp_row1 - 1, 0) / a.group;
+    const int all_end = a.causal ? token_first + 1 : seen.end, some_end = a.causal ? token_last + 1 : seen.end;
+    const int all_low = a.window > 0 ? token_last - a.window + 1 : 0, some_low = a.window > 0 ? token_first - a.window + 1 : 0;
     const uint32_t o_at = tmem + lanes + T::O_COLUMN + i * T::O_COLUMNS, p_at = tmem + lanes + T::P_COLUMN + i * T::P_COLUMNS;
 
 
@@ -567,6 +569,27 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     for (int j = 0; j < tiles; ++j) {
       const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
       if (!(ok = wait(&s_full[b], MT == 2 ? j & 1 : (j >> 1) & 1))) break;
+      // P and O are free (and O complete) when the last tile's P V is done
+      auto settled = [&]() {
+        if (j == 0) return true;
+        if (!wait(&pv_done[i], (j - 1) & 1)) return false;
+        tc::fence_after_sync();
+        return true;
+      };
+      const int key0 = seen.key_of(tile0 + j);
+      if (warp_row0 >= row1 || key0 >= some_end || (key0 + KEYS <= some_low && key0 >= first)) {
+        // no row of the warp sees the tile: weights of zero
+        tc::mbar_arrive(&s_empty[b]);
+        if (!(ok = settled())) break;
+        if (TERMS == 2 && j > 0) take_output();
+        const uint32_t zeros[8] = {};
+#pragma unroll
+        for (int c = 0; c < T::P_COLUMNS; c += 8) tmem_store_8(p_at + c, zeros);
+        tc::tmem_store_wait();
+        tc::fence_before_sync();
+        tc::mbar_arrive(&p_full[i]);
+        continue;
+      }
       if (CODES && !(ok = wait(&scales_full[stage], (j / STAGES) & 1))) break;
       tc::fence_after_sync();
       float s[KEYS];
@@ -575,7 +598,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::fence_before_sync();
       tc::mbar_arrive(&s_empty[b]);
 
-      const int key0 = seen.key_of(tile0 + j);
       const float* k_scales = scales + stage * 2 * KEYS;
       const float* v_scales = k_scales + KEYS;
       const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : 1.0f;
@@ -595,20 +617,19 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll
         for (int c = 0; c < KEYS; ++c) s[c] = capped(s[c], inverse, a.softcap);
       }
-      const bool edge = !(key0 + KEYS <= tile_end && (key0 >= tile_low || key0 + KEYS <= first));
+      const bool edge = !(key0 + KEYS <= all_end && (key0 >= all_low || key0 + KEYS <= first));
       if (edge) {
-        const int end = hi - key0, low = lo - key0, head_end = first - key0;
+        // a bit for each key that the row sees
+        auto below = [](int n) { return n <= 0 ? 0u : 0xffffffffu >> max(32 - n, 0); };
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c)
-          if (c >= end || (c < low && c >= head_end)) s[c] = -INFINITY;
+        for (int c = 0; c < KEYS; c += 32) {
+          const int at = key0 + c;
+          const uint32_t sees = below(hi - at) & (~below(lo - at) | below(first - at));
+#pragma unroll
+          for (int e = 0; e < 32 && c + e < KEYS; ++e)
+            if (!(sees >> e & 1)) s[c + e] = -INFINITY;
+        }
       }
-      // P and O are free (and O complete) when the last tile's P V is done
-      auto settled = [&]() {
-        if (j == 0) return true;
-        if (!wait(&pv_done[i], (j - 1) & 1)) return false;
-        tc::fence_after_sync();
-        return true;
-      };
       // the row's base from this tile's largest score, and what is summed in it
       bool not_a_number = false;
       auto rebase = [&](float top) {
@@ -1117,28 +1138,42 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (!(ok = wait(&v_full[j % STAGES], (j / STAGES) & 1))) break;
       uint8_t* v = shared + T::V_AT + (j % STAGES) * T::V_STAGE;
       bool found = false;
-#pragma unroll 8
-      for (int n = lane; n < T::V_BYTES / 16; n += 32) {
-        uint4 x = *reinterpret_cast<uint4*>(v + 16 * n);
-        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
-        // (an exponent of all ones carries into the sign's place)
+      // (several loads under way: the look is a chain of latencies otherwise,
+      // 2000 clocks long, and a window has an edge tile in every second)
+      constexpr int CHECKS = T::V_BYTES / 512, FLIGHT = CHECKS % 8 == 0 ? 8 : 5;
+      static_assert(T::V_BYTES % 512 == 0 && CHECKS % FLIGHT == 0, "whole rounds of a warp");
+      // (an exponent of all ones carries into the sign's place)
+      auto full = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+#pragma unroll 1
+      for (int n0 = lane; n0 < T::V_BYTES / 16; n0 += 32 * FLIGHT) {
+        uint4 held[FLIGHT];
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) held[f] = *reinterpret_cast<const uint4*>(v + 16 * (n0 + 32 * f));
         uint32_t bad = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= ((w[e] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+        for (int f = 0; f < FLIGHT; ++f) bad |= full(held[f].x) | full(held[f].y) | full(held[f].z) | full(held[f].w);
         if (!bad) continue;
+#pragma unroll 1
+        for (int n = n0; n < n0 + 32 * FLIGHT; n += 32) {
+          uint4 x = *reinterpret_cast<uint4*>(v + 16 * n);
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+          uint32_t any = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t full = ((w[e] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-          w[e] &= (full & 0x8000u ? 0u : 0xffffu) | (full & 0x80000000u ? 0u : 0xffff0000u);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t is = full(w[e]);
+            any |= is;
+            w[e] &= (is & 0x8000u ? 0u : 0xffffu) | (is & 0x80000000u ? 0u : 0xffff0000u);
+          }
+          if (!any) continue;
+          *reinterpret_cast<uint4*>(v + 16 * n) = x;
+          // which keys: the run, and the chunk in its row before the swizzle
+          // (which exchanges 16-byte chunks by the address bits 7 and up)
+          const int in_run = 16 * n % (run * D * 2), d = in_run / row_bytes;
+          const int swizzle = row_bytes == 128 ? d % 8 : row_bytes == 64 ? d / 2 % 4 : d / 4 % 2;
+          const int key = key0 + 16 * n / (run * D * 2) * run + 8 * ((n % chunks) ^ swizzle);
+          for (int e = 0; e < 8; ++e)
+            found = found || (key + e < seen.end && (key + e >= lowest || key + e < first));
         }
-        *reinterpret_cast<uint4*>(v + 16 * n) = x;
-        // which keys: the run, and the chunk in its row before the swizzle
-        // (which exchanges 16-byte chunks by the address bits 7 and up)
-        const int in_run = 16 * n % (run * D * 2), d = in_run / row_bytes;
-        const int swizzle = row_bytes == 128 ? d % 8 : row_bytes == 64 ? d / 2 % 4 : d / 4 % 2;
-        const int key = key0 + 16 * n / (run * D * 2) * run + 8 * ((n % chunks) ^ swizzle);
-        for (int e = 0; e < 8; ++e)
-          found = found || (key + e < seen.end && (key + e >= lowest || key + e < first));
       }
       if (found) *taken_out = 1;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
