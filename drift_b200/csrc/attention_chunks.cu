@@ -66,34 +66,51 @@ bool takes_tiles(const Call& c, long long rows) {
   return rows > (c.cache_dtype == DRIFT_F16 ? 8 : c.x_dtype == DRIFT_BF16 ? 16 : 24);
 }
 
-// The split count is the one with the least time of the busiest SM, by what
-// was measured on B200 for a tile (per row tile and key: BF16 6 ns, F32 16,
-// heads of 256 14, converted codes half as much again), for a CTA's start and
-// end, and for the join, whose partial rows are written and read once.
+// Two row tiles to a CTA or one, and how many splits: what ends first by a model
+// of what was measured on B200. A tile takes so many ns for each key and row
+// tile (2048 rows of 8 x 4 heads over 4096 and 8192 keys), a CTA 9 us for its
+// start and end; the join's partial rows, written and read, pass at 1.7 TB/s.
+// CTAs start with the longest (a causal chunk's last rows). Two row tiles
+// share a tile's keys: a row tile by itself takes 1.6 times as long (chunk of
+// 2048 BF16 rows, 8192 keys: 241 us, 414 with one) but keeps all SMs at work
+// where there are few (1500 F32 tokens of 4 x 4 heads: 67 us, 84 with two).
 Plan plan_tiles(const Call& c) {
-  constexpr double CTA_NS = 5000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 4500;
-  Plan p;
+  constexpr double CTA_NS = 9000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 1700;
+  const bool bf16 = c.x_dtype == DRIFT_BF16, codes = c.cache_dtype == DRIFT_I8;
+  const double key_ns = bf16 ? (c.head_dim > 128 ? 20 : c.head_dim > 64 ? 7.7 : 6.5) * (codes ? 2.2 : 1.0)
+                             : (c.head_dim > 64 ? 14.5 : 10) * (codes ? 2.5 : 1.0);
   const long long rows = (long long)c.longest * c.group;
-  p.row_tiles = c.head_dim > 128 || rows <= 128 ? 1 : 2;
-  p.rows_per_unit = 128 * p.row_tiles;
-  p.keys_per_tile = attention_tiles_keys(c.head_dim, c.x_dtype == DRIFT_BF16);
-  const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
-  const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
-  const double tile_ns = p.row_tiles * p.keys_per_tile * (c.x_dtype == DRIFT_F32 ? 16 : c.head_dim > 128 ? 14 : 6) *
-                         (c.cache_dtype == DRIFT_I8 ? 1.5 : 1.0);
-  const double parts_bytes = 8.0 * rows * c.batch * c.kv_heads * c.head_dim;  // of a split, there and back
-  double best = 0;
-  for (long long splits = 1; splits <= 64 && splits <= tiles; ++splits) {
-    const long long each = (tiles + splits - 1) / splits;
-    const double rounds = double((units * splits + sm_count() - 1) / sm_count());
-    const double cost = rounds * (each * tile_ns + CTA_NS) +
-                        (splits > 1 ? JOIN_NS + splits * parts_bytes / PARTS_BYTES_A_NS : 0);
-    if (splits > 1 && cost >= best) continue;
-    best = cost;
-    p.tiles_per_split = int(each);
-    p.splits = int((tiles + each - 1) / each);
+  Plan best;
+  double least = -1;
+  for (int row_tiles = c.head_dim > 128 || rows <= 128 ? 1 : 2; row_tiles > 0; --row_tiles) {
+    Plan p;
+    p.row_tiles = row_tiles;
+    p.rows_per_unit = 128 * row_tiles;
+    p.keys_per_tile = attention_tiles_keys(c.head_dim, bf16);
+    const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
+    const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
+    const double tile_ns = p.keys_per_tile * key_ns * (row_tiles == 2 ? 2.0 : c.head_dim > 128 ? 1.0 : 1.6);
+    const double cta_ns = row_tiles == 2 ? CTA_NS : 0.7 * CTA_NS;
+    // the fewest tiles of a unit, and the mean
+    const double fewest = c.causal && c.window == 0 ? double(tiles) * (c.max_key_count - c.longest) / c.max_key_count : double(tiles);
+    const double mean = (tiles + fewest) / 2;
+    const double parts_bytes = 8.0 * rows * c.batch * c.kv_heads * c.head_dim;  // of a split, there and back
+    for (long long splits = 1; splits <= 64 && splits <= tiles; ++splits) {
+      const long long each = (tiles + splits - 1) / splits;
+      const double ctas = units * std::max(1.0, splits * mean / tiles);
+      const double longest = each * tile_ns + cta_ns, shortest = std::min(double(each), fewest) * tile_ns + cta_ns;
+      const double shared = (units * mean * tile_ns + ctas * cta_ns) / sm_count() + shortest;
+      const double rounds = double((units * splits + sm_count() - 1) / sm_count());
+      const double cost = std::max(longest, std::min(rounds * longest, shared)) +
+                          (splits > 1 ? JOIN_NS + splits * parts_bytes / PARTS_BYTES_A_NS : 0);
+      if (least >= 0 && cost >= least) continue;
+      least = cost;
+      p.tiles_per_split = int(each);
+      p.splits = int((tiles + each - 1) / each);
+      best = p;
+    }
   }
-  return p;
+  return best;
 }
 
 Plan plan_chunks(const Call& c) {
