@@ -50,6 +50,15 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same as a new sum.
+__device__ __forceinline__ void mma_s8_new(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(ZERO));
+}
+
 // The digits of x, the least in the lowest byte, each -128 to 127.
 __device__ __forceinline__ uint32_t digits(int x) { return (uint32_t(x) + 0x00808080u) ^ 0x00808080u; }
 
@@ -295,10 +304,6 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
       constexpr int TILES = T::Q_TILES / RT;
       int acc[2][TILES][4];
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int j = 0; j < TILES; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = ZERO;
-#pragma unroll
       for (int step = 0; step < T::STEPS; ++step) {
         uint2 b[TILES];
 #pragma unroll
@@ -311,7 +316,10 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
           const uint32_t f[4] = {w.k[m][0][word], w.k[m][1][word], both ? w.k[m][0][both ? word + 1 : 0] : 0,
                                  both ? w.k[m][1][both ? word + 1 : 0] : 0};
 #pragma unroll
-          for (int j = 0; j < TILES; ++j) mma_s8(acc[m][j], f, b[j].x, b[j].y);
+          for (int j = 0; j < TILES; ++j) {
+            if (step == 0) mma_s8_new(acc[m][j], f, b[j].x, b[j].y);
+            else mma_s8(acc[m][j], f, b[j].x, b[j].y);
+          }
         }
       }
 #pragma unroll
@@ -444,8 +452,7 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
         int acc[TILES][4];
 #pragma unroll
         for (int j = 0; j < TILES; ++j) {
-          acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = ZERO;
-          mma_s8(acc[j], f, b[n * TILES + j][0], b[n * TILES + j][1]);
+          mma_s8_new(acc[j], f, b[n * TILES + j][0], b[n * TILES + j][1]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

@@ -75,7 +75,7 @@ __device__ __forceinline__ float2 pair_value(uint32_t x) {
 
 // How a lane's loads cover rows of D values, 16 of them to a k-step: chunks of
 // 16 bytes a lane while whole ones last, then (D = 80) one k-step of 4 values
-// a lane. first_of(k-step) is where lane t's four values of the step start.
+// a lane. place_of tells which step and lane t have the four values from d on.
 template <int D>
 struct RowMap {
   static constexpr int PER = 8;                         // values of a 16-byte chunk
@@ -85,9 +85,10 @@ struct RowMap {
   static constexpr int TAIL = STEPS - CHUNKS * STEPS_PER;  // 0 or 1
   static constexpr int WORDS = 2 * STEPS;               // 32-bit words a lane holds of a row
   static_assert(TAIL <= 1, "one k-step past the chunks at most");
-  __device__ static int first_of(int step, int t) {
-    return step < CHUNKS * STEPS_PER ? (step / STEPS_PER) * 4 * PER + PER * t + 4 * (step % STEPS_PER)
-                                     : CHUNKS * 4 * PER + 4 * t;
+  __device__ static void place_of(int d, int& step, int& t) {
+    const int chunk = d / (4 * PER), in = d % (4 * PER);
+    step = chunk < CHUNKS ? STEPS_PER * chunk + in % PER / 4 : STEPS_PER * CHUNKS;
+    t = chunk < CHUNKS ? in / PER : in / 4;
   }
 };
 
@@ -225,40 +226,57 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
   }
 
   // q: each row divided by a power of two near its largest value, in F16
-  // terms, as B fragments [step][column tile][term][lane]
+  // terms, as B fragments [step][column tile][term][lane]: a warp takes a row,
+  // a lane four values at a time, which are a fragment each
+  uint2* fragments = reinterpret_cast<uint2*>(shared);
   for (int r = warp; r < ROWS; r += WARPS) {
-    float largest = 0.0f;
+    constexpr int PER = (D + 127) / 128;
+    float x[PER][4] = {};
     if (row0 + r < row1) {
       const int row = row0 + r;
       const X* q = static_cast<const X*>(a.q) + ((chunk.row + row / a.group) * a.q_heads + head * a.group + row % a.group) * D;
-      for (int d = lane; d < D; d += 32) largest = fmaxf(largest, fabsf(float(q[d])));
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        const int d = 4 * (lane + 32 * n);
+        if (d >= D) continue;
+        if constexpr (T::BF16) {
+          const uint2 y = *reinterpret_cast<const uint2*>(q + d);
+          x[n][0] = __uint_as_float(y.x << 16), x[n][1] = __uint_as_float(y.x & 0xffff0000u);
+          x[n][2] = __uint_as_float(y.y << 16), x[n][3] = __uint_as_float(y.y & 0xffff0000u);
+        } else {
+          const float4 y = *reinterpret_cast<const float4*>(q + d);
+          x[n][0] = y.x, x[n][1] = y.y, x[n][2] = y.z, x[n][3] = y.w;
+        }
+      }
     }
+    float largest = 0.0f;
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(x[n][e]));
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
     // 2^(floor(log2 largest) - Q_BITS), from the exponent bits, kept where it
     // and its inverse are normal
     const uint32_t exponent = __float_as_uint(largest) & 0x7f800000u;
     const uint32_t shift = uint32_t(Q_BITS) << 23;
-    if (lane == 0) q_unit[r] = __uint_as_float(max(exponent, shift + 0x00800000u) - shift);
-  }
-  __syncthreads();
-  uint2* fragments = reinterpret_cast<uint2*>(shared);
-  for (int i = tid; i < Map::STEPS * NT * 32; i += THREADS) {
-    const int l = i % 32, n = i / 32 % NT, step = i / 32 / NT;
-    const int r = 8 * n + l / 4, row = row0 + r, d = Map::first_of(step, l % 4);
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row < row1) {
-      const X* q = static_cast<const X*>(a.q) + ((chunk.row + row / a.group) * a.q_heads + head * a.group + row % a.group) * D + d;
-      const float unit_inverse = 1.0f / q_unit[r];  // exact
+    const float unit_of_row = __uint_as_float(max(exponent, shift + 0x00800000u) - shift);
+    if (lane == 0) q_unit[r] = unit_of_row;
+    const float inverse = 1.0f / unit_of_row;  // exact
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = float(q[e]) * unit_inverse;
-    }
-    const uint2 hi = make_uint2(half_pair(x[0], x[1]), half_pair(x[2], x[3]));
-    fragments[((step * NT + n) * TERMS) * 32 + l] = hi;
-    if constexpr (TERMS == 2) {
-      const float2 u = pair_value(hi.x), y = pair_value(hi.y);
-      fragments[((step * NT + n) * TERMS + 1) * 32 + l] =
-          make_uint2(half_pair(x[0] - u.x, x[1] - u.y), half_pair(x[2] - y.x, x[3] - y.y));
+    for (int n = 0; n < PER; ++n) {
+      const int d = 4 * (lane + 32 * n);
+      if (d >= D) continue;
+      const float y[4] = {x[n][0] * inverse, x[n][1] * inverse, x[n][2] * inverse, x[n][3] * inverse};
+      const uint2 hi = make_uint2(half_pair(y[0], y[1]), half_pair(y[2], y[3]));
+      int step, lt;
+      Map::place_of(d, step, lt);
+      uint2* to = fragments + ((step * NT + r / 8) * TERMS) * 32 + 4 * (r % 8) + lt;
+      to[0] = hi;
+      if constexpr (TERMS == 2) {
+        const float2 u = pair_value(hi.x), v = pair_value(hi.y);
+        to[32] = make_uint2(half_pair(y[0] - u.x, y[1] - u.y), half_pair(y[2] - v.x, y[3] - v.y));
+      }
     }
   }
   __syncthreads();
