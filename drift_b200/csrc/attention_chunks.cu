@@ -38,32 +38,41 @@ Plan plan_rows(const Call& c) {
   Plan p;
   p.row_tiles = 0;
   const long long rows = (long long)c.longest * c.group;
-  if (c.cache_dtype == DRIFT_I8) {
-    p.rows_per_unit = rows <= 4 ? 4 : rows <= 8 || c.head_dim > 128 ? 8 : rows <= 16 ? 16 : 24;
-    p.keys_per_tile = 32;
-  } else {
-    p.rows_per_unit = rows <= 8 || c.head_dim > 128 ? 8 : 16;
-    p.keys_per_tile = 16;
-  }
+  const bool codes = c.cache_dtype == DRIFT_I8;
+  p.rows_per_unit = codes && rows <= 4 ? 4 : 8;
+  p.keys_per_tile = codes ? 32 : 16;
   const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
   const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
-  const int warps = c.cache_dtype == DRIFT_I8 ? attention_codes_warps(c.head_dim, p.rows_per_unit) : 8;
+  const int warps = codes ? attention_codes_warps(c.head_dim) : ATTENTION_ROWS_WARPS;
+  const long long slots = (long long)sm_count() * (codes ? attention_codes_ctas(c.head_dim) : attention_rows_ctas(c.head_dim));
   // CTAs for every SM four times over (F16 caches eight: a step of 16 x 16384
-  // keys 153 us, and 181 with four; 8-bit ones of 3 sequences 29, and 35 with
-  // eight), of a tile a warp at least
+  // keys 148 us, and 179 with four; 8-bit ones of 3 sequences 28, and 33 with
+  // eight), of a tile a warp at least; two splits while that leaves SMs idle
+  // (eight chunks of 40 F32 rows: 100 us, 111 with one)
   const long long wanted =
-      std::max(1LL, (c.cache_dtype == DRIFT_I8 ? 4LL : 8LL) * sm_count() / std::max(1LL, units));
+      std::max(units < slots ? 2LL : 1LL, (codes ? 4LL : 8LL) * sm_count() / std::max(1LL, units));
   const long long splits = std::min(wanted, (tiles + warps - 1) / warps);
   const long long each = (tiles + splits - 1) / splits;
-  p.tiles_per_split = int((each + warps - 1) / warps * warps);
+  long long rounds = (each + warps - 1) / warps;
+  // (a tile a warp is not worth a second round of CTAs: 12 rows of one
+  // sequence over 4096 keys 17.0 us, 18.9 with it; a windowed step of 13 x 1028
+  // keys of heads of 256 15.4, 19.2 with it)
+  if (rounds == 1 && units * ((tiles + warps - 1) / warps) > slots) rounds = 2;
+  p.tiles_per_split = int(rounds * warps);
   p.splits = int((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
   return p;
 }
 
-// Whether a chunk's rows of a key head go to the tensor-core tiles.
+// Whether a chunk's rows of a key head go to the tensor-core tiles, by what
+// both take on B200 (8 sequences x 8 key heads x 4096 keys; us, few rows' kernel
+// and tiles): F16 caches BF16 8 rows 35 and 43, 12 rows 54 and 44; F32 38 and
+// 57, 12 rows 59 and 59. 8-bit ones BF16 32 rows 61 and 75, 40 rows 80 and 77
+// (heads of 256: 24 rows 95 and 105, 32 rows 123 and 107); F32 40 rows 100 and
+// 130, and of one sequence 22 and 24, but 48 rows 31 and 24.
 bool takes_tiles(const Call& c, long long rows) {
-  if (c.x_dtype == DRIFT_F32 && c.head_dim > 128) return false;
-  return rows > (c.cache_dtype == DRIFT_F16 ? 8 : c.x_dtype == DRIFT_BF16 ? 16 : 24);
+  const bool bf16 = c.x_dtype == DRIFT_BF16;
+  if (!bf16 && c.head_dim > 128) return false;
+  return rows > (c.cache_dtype == DRIFT_F16 ? 8 : !bf16 ? 40 : c.head_dim > 128 ? 24 : 32);
 }
 
 // Two row tiles to a CTA or one, and how many splits: what ends first by a model
@@ -206,7 +215,7 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   const cudaStream_t s = cudaStream_t(stream);
   if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, x_dtype, cache_dtype, head_dim, p.row_tiles, s));
   else if (cache_dtype == DRIFT_I8) DRIFT_TRY(launch_attention_codes(a, x_dtype, head_dim, p.rows_per_unit, s));
-  else DRIFT_TRY(launch_attention_rows(a, x_dtype, head_dim, p.rows_per_unit, s));
+  else DRIFT_TRY(launch_attention_rows(a, x_dtype, head_dim, s));
   if (!needed) return 0;
   return launch_attention_join(a, x_dtype, head_dim, p.rows_per_unit, p.keys_per_tile, s);
 }

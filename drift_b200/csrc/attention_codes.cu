@@ -3,7 +3,7 @@
 //
 // A unit is a key head of one sequence with up to ROWS of the (token, query
 // head) rows that read it; a CTA takes one split of the unit's key tiles, each
-// of its warps every eighth (or twelfth) tile of 32 keys. Both products run on the int8
+// of its warps every fourth (or eighth) tile of 32 keys. Both products run on the int8
 // tensor cores, turned round -- scores^T = K q^T and out^T = V^T p^T by
 // mma.sync m16n8k32, keys and then dimensions as the 16 rows, the few query
 // rows as columns -- with the codes as they lie in the cache: a lane's 16
@@ -73,21 +73,23 @@ __device__ __forceinline__ float weight_of(float score, float base) {
 }
 
 // Packed: up to four rows, column c of digit tile j being row c % 4's digit 2 j
-// + c / 4; otherwise RT tiles of eight rows, each with a tile for each digit.
-template <int D_, bool BF16_, int RT_>
+// + c / 4; otherwise up to eight, with a tile for each digit. (Sixteen or
+// twenty-four rows to a warp shared its keys but left registers for eight warps
+// an SM: drafts of 12 rows 49 us, in units of eight 40; of 20, 70 and 51.)
+template <int D_, bool BF16_, bool PACKED_>
 struct CodesTraits {
-  static constexpr int D = D_, RT = RT_ == 0 ? 1 : RT_;
-  static constexpr bool BF16 = BF16_, PACKED = RT_ == 0;
-  static constexpr int ROWS = PACKED ? 4 : 8 * RT;
+  static constexpr int D = D_;
+  static constexpr bool BF16 = BF16_, PACKED = PACKED_;
+  static constexpr int ROWS = PACKED ? 4 : 8;
   // As many warps as registers leave an SM without spills: sixteen of 128, for
   // heads of 128 twelve of 168 (a step of 16 x 16384 keys: sixteen, spilling,
   // 191 us, twelve 113, eight 135), for more rows and wider heads eight. In
   // CTAs of four, one's start and end run under the others.
-  static constexpr int WARPS = attention_codes_warps(D, ROWS), THREADS = 32 * WARPS;
-  static constexpr int CTAS = RT > 1 || D > 128 ? 1 : D == 128 ? 3 : 2;
+  static constexpr int WARPS = attention_codes_warps(D), THREADS = 32 * WARPS;
+  static constexpr int CTAS = attention_codes_ctas(D);
   static constexpr int Q_DIGITS = BF16 ? 2 : 4, P_DIGITS = PACKED || !BF16 ? 4 : 3;
-  static constexpr int Q_TILES = PACKED ? Q_DIGITS / 2 : RT * Q_DIGITS;
-  static constexpr int P_TILES = PACKED ? P_DIGITS / 2 : RT * P_DIGITS;
+  static constexpr int Q_TILES = PACKED ? Q_DIGITS / 2 : Q_DIGITS;
+  static constexpr int P_TILES = PACKED ? P_DIGITS / 2 : P_DIGITS;
   static constexpr int Q_BITS = BF16 ? 13 : 29;                  // of the largest value's leading bit
   static constexpr float P_STEPS = P_DIGITS == 4 ? 67108864.0f : 262144.0f;  // of a weight of 1
   static constexpr int CHUNKS = D / 64, TAIL = D % 64 / 16;      // 16-byte chunks a lane has of a key row; 4 bytes
@@ -173,7 +175,7 @@ template <class T>
 __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(const AttentionChunksArgs a) {
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
-  constexpr int D = T::D, RT = T::RT, ROWS = T::ROWS, WARPS = T::WARPS, THREADS = T::THREADS;
+  constexpr int D = T::D, ROWS = T::ROWS, WARPS = T::WARPS, THREADS = T::THREADS;
   constexpr bool PACKED = T::PACKED;
   using X = typename std::conditional<T::BF16, __nv_bfloat16, float>::type;
   extern __shared__ __align__(16) uint8_t shared[];
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
       const int word = tail ? 0 : d / 4 % 2;
 #pragma unroll
       for (int digit = 0; digit < T::Q_DIGITS; ++digit) {
-        const int tile = PACKED ? digit / 2 : r / 8 * T::Q_DIGITS + digit, column = PACKED ? digit % 2 * 4 + r : r % 8;
+        const int tile = PACKED ? digit / 2 : digit, column = PACKED ? digit % 2 * 4 + r : r;
         uint32_t* to = fragments + ((step * T::Q_TILES + tile) * 32 + 4 * column + lt) * 2;
         to[word] = digit_of(y, digit);
         if (tail) to[1] = 0;
@@ -264,16 +266,14 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
   }
   __syncthreads();
 
-  // this lane's columns of row tile n: rows 8 n + 2 t and + 1 (packed: modulo 4)
-  float multiplier[RT][2];
-  int position[RT][2];
-#pragma unroll
-  for (int n = 0; n < RT; ++n)
+  // this lane's columns: rows 2 t and 2 t + 1 (packed: modulo 4)
+  float multiplier[2];
+  int position[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = PACKED ? (2 * t + e) % 4 : 8 * n + 2 * t + e;
-      multiplier[n][e] = a.scale * q_unit[r];
-      position[n][e] = chunk.position + min(row0 + r, row1 - 1) / a.group;
+      const int r = PACKED ? (2 * t + e) % 4 : 2 * t + e;
+      multiplier[e] = a.scale * q_unit[r];
+      position[e] = chunk.position + min(row0 + r, row1 - 1) / a.group;
     }
   // what every row sees: keys below `all_end` and from `all_low` on (or below
   // `first`)
@@ -283,62 +283,55 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
   const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;  // what some row sees
   const float low_digit = PACKED && t >= 2 ? 256.0f : 1.0f;  // the worth of a packed lane's lower digit
 
-  float out[RT][T::DM][4];
-  float base[RT][2], sum[RT][2], v_unit = 0.0f;
+  float out[T::DM][4];
+  float base[2], sum[2], v_unit = 0.0f;
+  base[0] = base[1] = -INFINITY;
+  sum[0] = sum[1] = 0.0f;
 #pragma unroll
-  for (int n = 0; n < RT; ++n) {
-    base[n][0] = base[n][1] = -INFINITY;
-    sum[n][0] = sum[n][1] = 0.0f;
-#pragma unroll
-    for (int m = 0; m < T::DM; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
-  }
+  for (int m = 0; m < T::DM; ++m) out[m][0] = out[m][1] = out[m][2] = out[m][3] = 0.0f;
   uint32_t* weights = reinterpret_cast<uint32_t*>(shared + T::Q_BYTES) + warp * ROWS * PITCH;
 
   for (; tile < tile1; tile += WARPS) {
     const int key0 = seen.key_of(tile), next = tile + WARPS;
     const bool whole = key0 + TILE <= all_end && (key0 >= all_low || key0 + TILE <= first);
     // scores [row tile][16 keys][(key g, columns 2 t, 2 t + 1), (key g + 8, the same)]
-    float s[RT][2][4];
+    float s[2][4];
+    int acc[2][T::Q_TILES][4];
 #pragma unroll
-    for (int n = 0; n < RT; ++n) {
-      constexpr int TILES = T::Q_TILES / RT;
-      int acc[2][TILES][4];
+    for (int step = 0; step < T::STEPS; ++step) {
+      uint2 b[T::Q_TILES];
 #pragma unroll
-      for (int step = 0; step < T::STEPS; ++step) {
-        uint2 b[TILES];
+      for (int j = 0; j < T::Q_TILES; ++j)
+        b[j] = reinterpret_cast<const uint2*>(fragments)[(step * T::Q_TILES + j) * 32 + lane];
 #pragma unroll
-        for (int j = 0; j < TILES; ++j)
-          b[j] = reinterpret_cast<const uint2*>(fragments)[(step * T::Q_TILES + n * TILES + j) * 32 + lane];
+      for (int m = 0; m < 2; ++m) {
+        const bool both = step < 2 * T::CHUNKS;
+        const int word = 2 * step;
+        const uint32_t f[4] = {w.k[m][0][word], w.k[m][1][word], both ? w.k[m][0][both ? word + 1 : 0] : 0,
+                               both ? w.k[m][1][both ? word + 1 : 0] : 0};
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const bool both = step < 2 * T::CHUNKS;
-          const int word = 2 * step;
-          const uint32_t f[4] = {w.k[m][0][word], w.k[m][1][word], both ? w.k[m][0][both ? word + 1 : 0] : 0,
-                                 both ? w.k[m][1][both ? word + 1 : 0] : 0};
-#pragma unroll
-          for (int j = 0; j < TILES; ++j) {
-            if (step == 0) mma_s8_new(acc[m][j], f, b[j].x, b[j].y);
-            else mma_s8(acc[m][j], f, b[j].x, b[j].y);
-          }
+        for (int j = 0; j < T::Q_TILES; ++j) {
+          if (step == 0) mma_s8_new(acc[m][j], f, b[j].x, b[j].y);
+          else mma_s8(acc[m][j], f, b[j].x, b[j].y);
         }
       }
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = 0.0f;
-#pragma unroll
-          for (int j = TILES - 1; j >= 0; --j) {
-            const float y = __int_as_float(acc[m][j][e]) - ZERO_VALUE;
-            x = j == TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
-          }
-          if (PACKED) {
-            x *= low_digit;
-            x += __shfl_xor_sync(0xffffffffu, x, 2);
-          }
-          s[n][m][e] = x;
-        }
     }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = 0.0f;
+#pragma unroll
+        for (int j = T::Q_TILES - 1; j >= 0; --j) {
+          const float y = __int_as_float(acc[m][j][e]) - ZERO_VALUE;
+          x = j == T::Q_TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
+        }
+        if (PACKED) {
+          x *= low_digit;
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+        }
+        s[m][e] = x;
+      }
     float k_scale[2][2], v_scale[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -354,32 +347,28 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
         if (!whole && (key >= seen.end || (key < lowest && key >= first))) v_scale[m][half] = 0.0f;
         if (v_scale[m][half] <= 3.402823466e38f) top_scale = fmaxf(top_scale, v_scale[m][half]);  // (the finite ones)
 #pragma unroll
-        for (int n = 0; n < RT; ++n)
-#pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = s[n][m][2 * half + e] * multiplier[n][e] * k_scale[m][half];
+            float x = s[m][2 * half + e] * multiplier[e] * k_scale[m][half];
             if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
             if (!whole) {
-              const bool sees = key < seen.end && (!a.causal || key <= position[n][e]) &&
-                                (a.window == 0 || key > position[n][e] - a.window || key < first);
+              const bool sees = key < seen.end && (!a.causal || key <= position[e]) &&
+                                (a.window == 0 || key > position[e] - a.window || key < first);
               x = sees ? x : -INFINITY;
             }
-            s[n][m][2 * half + e] = x;
+            s[m][2 * half + e] = x;
           }
       }
     // weights with the bases as they are; where one passes GROWTH (or is a
     // NaN, or a row has no base yet), or a scale the unit, they move
-    float p[RT][2][4];
+    float p[2][4];
     bool move = top_scale > v_unit;
     auto weigh = [&]() {
-#pragma unroll
-      for (int n = 0; n < RT; ++n)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            p[n][m][e] = weight_of(s[n][m][e], base[n][e % 2]);
-            move = move || !(p[n][m][e] <= GROWTH);
+            p[m][e] = weight_of(s[m][e], base[e % 2]);
+            move = move || !(p[m][e] <= GROWTH);
           }
     };
     weigh();
@@ -395,17 +384,15 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
         v_unit = now;
       }
 #pragma unroll
-      for (int n = 0; n < RT; ++n)
-#pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
+          float top = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float now = fmaxf(base[n][e], top), f = weight_of(base[n][e], now);
-          base[n][e] = now;
-          sum[n][e] *= f;
+          const float now = fmaxf(base[e], top), f = weight_of(base[e], now);
+          base[e] = now;
+          sum[e] *= f;
 #pragma unroll
-          for (int m = 0; m < T::DM; ++m) out[n][m][e] *= f * shrink, out[n][m][e + 2] *= f * shrink;
+          for (int m = 0; m < T::DM; ++m) out[m][e] *= f * shrink, out[m][e + 2] *= f * shrink;
         }
       weigh();
     }
@@ -418,52 +405,42 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
       for (int half = 0; half < 2; ++half) {
         const float by = v_scale[m][half] * steps;
 #pragma unroll
-        for (int n = 0; n < RT; ++n)
-#pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float x = p[n][m][2 * half + e];
-            sum[n][e] += x;
+            const float x = p[m][2 * half + e];
+            sum[e] += x;
             // (a hidden value's scale may be a NaN; a NaN that is seen stays in the sum)
             const float y = x == 0.0f ? 0.0f : x * by;
-            if (!(y <= 2147483520.0f)) sum[n][e] = __int_as_float(0x7fc00000);
-            if (!PACKED || t < 2) weights[(8 * n + 2 * t + e) * PITCH + 16 * m + g + 8 * half] = digits(__float2int_rn(y));
+            if (!(y <= 2147483520.0f)) sum[e] = __int_as_float(0x7fc00000);
+            if (!PACKED || t < 2) weights[(2 * t + e) * PITCH + 16 * m + g + 8 * half] = digits(__float2int_rn(y));
           }
       }
     __syncwarp();
     uint32_t b[T::P_TILES][2];
+    const uint4* from = reinterpret_cast<const uint4*>(weights + (PACKED ? g % 4 : g) * PITCH + 8 * t);
+    const uint4 x = from[0], y = from[1];
 #pragma unroll
-    for (int n = 0; n < RT; ++n) {
-      const uint4* from = reinterpret_cast<const uint4*>(weights + (PACKED ? g % 4 : 8 * n + g) * PITCH + 8 * t);
-      const uint4 x = from[0], y = from[1];
-      constexpr int TILES = T::P_TILES / RT;
-#pragma unroll
-      for (int j = 0; j < TILES; ++j) {
-        const uint32_t digit = PACKED ? 2 * j + g / 4 : j;
-        b[n * TILES + j][0] = digit_of(x, digit);
-        b[n * TILES + j][1] = digit_of(y, digit);
-      }
+    for (int j = 0; j < T::P_TILES; ++j) {
+      const uint32_t digit = PACKED ? 2 * j + g / 4 : j;
+      b[j][0] = digit_of(x, digit);
+      b[j][1] = digit_of(y, digit);
     }
 #pragma unroll
     for (int m = 0; m < T::DM; ++m) {
       const uint32_t f[4] = {w.v[m][0].x, w.v[m][1].x, w.v[m][0].y, w.v[m][1].y};
+      int acc[T::P_TILES][4];
 #pragma unroll
-      for (int n = 0; n < RT; ++n) {
-        constexpr int TILES = T::P_TILES / RT;
-        int acc[TILES][4];
+      for (int j = 0; j < T::P_TILES; ++j) {
+        mma_s8_new(acc[j], f, b[j][0], b[j][1]);
+      }
 #pragma unroll
-        for (int j = 0; j < TILES; ++j) {
-          mma_s8_new(acc[j], f, b[n * TILES + j][0], b[n * TILES + j][1]);
+      for (int e = 0; e < 4; ++e) {
+        float x = 0.0f;
+#pragma unroll
+        for (int j = T::P_TILES - 1; j >= 0; --j) {
+          const float y = __int_as_float(acc[j][e]) - ZERO_VALUE;
+          x = j == T::P_TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = 0.0f;
-#pragma unroll
-          for (int j = TILES - 1; j >= 0; --j) {
-            const float y = __int_as_float(acc[j][e]) - ZERO_VALUE;
-            x = j == TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
-          }
-          out[n][m][e] += x;
-        }
+        out[m][e] += x;
       }
     }
     if (next < tile1) {
@@ -478,20 +455,18 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
   float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
   const float worth = v_unit / T::P_STEPS * low_digit;
 #pragma unroll
-  for (int n = 0; n < RT; ++n)
-#pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float total = sum[n][e];
+      float total = sum[e];
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const int r = 8 * n + 2 * t + e;
+      const int r = 2 * t + e;
       const bool writes = !PACKED || t < 2;
-      if (g == 0 && writes) stats[warp * ROWS + r] = make_float2(base[n][e], total);
+      if (g == 0 && writes) stats[warp * ROWS + r] = make_float2(base[e], total);
 #pragma unroll
       for (int m = 0; m < T::DM; ++m)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float x = out[n][m][2 * half + e] * worth;
+          float x = out[m][2 * half + e] * worth;
           if (PACKED) x += __shfl_xor_sync(0xffffffffu, x, 2);
           if (writes) merged[(warp * ROWS + r) * D + 16 * m + g + 8 * half] = x;
         }
@@ -545,12 +520,8 @@ int launch_codes(const AttentionChunksArgs& a, cudaStream_t stream) {
 
 template <int D, bool BF16>
 int launch_rows_of(const AttentionChunksArgs& a, int rows_per_unit, cudaStream_t stream) {
-  if (rows_per_unit == 4) return launch_codes<CodesTraits<D, BF16, 0>>(a, stream);
-  if constexpr (D <= 128) {
-    if (rows_per_unit == 24) return launch_codes<CodesTraits<D, BF16, 3>>(a, stream);
-    if (rows_per_unit == 16) return launch_codes<CodesTraits<D, BF16, 2>>(a, stream);
-  }
-  return launch_codes<CodesTraits<D, BF16, 1>>(a, stream);
+  if (rows_per_unit == 4) return launch_codes<CodesTraits<D, BF16, true>>(a, stream);
+  return launch_codes<CodesTraits<D, BF16, false>>(a, stream);
 }
 
 template <int D>
@@ -558,19 +529,15 @@ int launch_dim(const AttentionChunksArgs& a, bool bf16, int rows_per_unit, cudaS
   return bf16 ? launch_rows_of<D, true>(a, rows_per_unit, stream) : launch_rows_of<D, false>(a, rows_per_unit, stream);
 }
 
-#define DRIFT_CODES_REGISTER(D, rt, name)                                            \
-  DRIFT_REGISTER(attention_codes_f32_d##D##_##name, (attention_codes_kernel<CodesTraits<D, false, rt>>)) \
-  DRIFT_REGISTER(attention_codes_bf16_d##D##_##name, (attention_codes_kernel<CodesTraits<D, true, rt>>))
-#define DRIFT_CODES_REGISTER_NARROW(D) \
-  DRIFT_CODES_REGISTER(D, 0, r4)       \
-  DRIFT_CODES_REGISTER(D, 1, r8)       \
-  DRIFT_CODES_REGISTER(D, 2, r16)      \
-  DRIFT_CODES_REGISTER(D, 3, r24)
-DRIFT_CODES_REGISTER_NARROW(64)
-DRIFT_CODES_REGISTER_NARROW(80)
-DRIFT_CODES_REGISTER_NARROW(128)
-DRIFT_CODES_REGISTER(256, 0, r4)
-DRIFT_CODES_REGISTER(256, 1, r8)
+#define DRIFT_CODES_REGISTER(D)                                                                          \
+  DRIFT_REGISTER(attention_codes_f32_d##D##_r4, (attention_codes_kernel<CodesTraits<D, false, true>>))  \
+  DRIFT_REGISTER(attention_codes_f32_d##D##_r8, (attention_codes_kernel<CodesTraits<D, false, false>>)) \
+  DRIFT_REGISTER(attention_codes_bf16_d##D##_r4, (attention_codes_kernel<CodesTraits<D, true, true>>))  \
+  DRIFT_REGISTER(attention_codes_bf16_d##D##_r8, (attention_codes_kernel<CodesTraits<D, true, false>>))
+DRIFT_CODES_REGISTER(64)
+DRIFT_CODES_REGISTER(80)
+DRIFT_CODES_REGISTER(128)
+DRIFT_CODES_REGISTER(256)
 
 }  // namespace
 

@@ -1,7 +1,7 @@
 // attention_chunks over an F16 cache for few rows: a decoding step, and every
 // chunk in F32 of heads of 256.
 //
-// A unit is a key head of one sequence with up to 8 NT of the (token, query
+// A unit is a key head of one sequence with up to 8 of the (token, query
 // head) rows that read it; a CTA takes one split of the unit's key tiles,
 // each of its 8 warps every eighth tile of 16 keys. The products are turned
 // round -- scores^T = K q^T and out^T = V^T p^T by mma.sync m16n8k16, keys and
@@ -19,7 +19,7 @@
 // F16 (off by 2^-11 at most, the result's own rounding is 2^-8).
 //
 // Softmax in F32, a running maximum and sum per warp; the warps meet
-// in shared memory, the splits in a second launch (attention_join_kernel).
+// in shared memory, the splits in a second launch (attention_chunks_join_kernel).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -34,7 +34,7 @@ namespace drift {
 
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = ATTENTION_ROWS_WARPS;
 constexpr int THREADS = 32 * WARPS;
 constexpr float LOG2E = 1.4426950408889634f;
 // A weight is e^WEIGHT_LOG = 2^14 at the row's largest score, and a row of q
@@ -94,16 +94,16 @@ struct RowMap {
 
 constexpr int TILE = 16;  // keys of a warp's tile
 
-template <int D_, bool BF16_, int NT_>
+template <int D_, bool BF16_>
 struct RowsTraits {
-  static constexpr int D = D_, NT = NT_;
+  static constexpr int D = D_;
   static constexpr bool BF16 = BF16_;
   static constexpr int TERMS = BF16 ? 1 : 2;
-  static constexpr int CTAS = D <= 128 && NT == 1 ? 2 : 1;  // of an SM: registers
+  static constexpr int CTAS = attention_rows_ctas(D);  // of an SM: registers
   using Map = RowMap<D>;
-  static constexpr int ROWS = 8 * NT;
+  static constexpr int ROWS = 8;
   static constexpr int DM = D / 16;      // 16-dimension tiles of the output
-  static constexpr int Q_BYTES = Map::STEPS * NT * TERMS * 32 * 8;
+  static constexpr int Q_BYTES = Map::STEPS * TERMS * 32 * 8;
   static constexpr int MERGE_BYTES = WARPS * ROWS * (D + 4) * 4;
   static constexpr int BYTES = Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;
 };
@@ -198,7 +198,7 @@ template <class T>
 __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const AttentionChunksArgs a) {
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
-  constexpr int D = T::D, NT = T::NT, ROWS = T::ROWS, TERMS = T::TERMS;
+  constexpr int D = T::D, ROWS = T::ROWS, TERMS = T::TERMS;
   using Map = typename T::Map;
   using X = typename std::conditional<T::BF16, __nv_bfloat16, float>::type;
   extern __shared__ __align__(16) uint8_t shared[];
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
       const uint2 hi = make_uint2(half_pair(y[0], y[1]), half_pair(y[2], y[3]));
       int step, lt;
       Map::place_of(d, step, lt);
-      uint2* to = fragments + ((step * NT + r / 8) * TERMS) * 32 + 4 * (r % 8) + lt;
+      uint2* to = fragments + step * TERMS * 32 + 4 * r + lt;
       to[0] = hi;
       if constexpr (TERMS == 2) {
         const float2 u = pair_value(hi.x), v = pair_value(hi.y);
@@ -282,15 +282,13 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
   __syncthreads();
 
   // this lane's columns: rows 8 n + 2 t and + 1
-  float multiplier[NT][2];
-  int position[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
+  float multiplier[2];
+  int position[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = 8 * n + 2 * t + e;
-      multiplier[n][e] = a.scale * q_unit[r];
-      position[n][e] = chunk.position + min(row0 + r, row1 - 1) / a.group;
+      const int r = 2 * t + e;
+      multiplier[e] = a.scale * q_unit[r];
+      position[e] = chunk.position + min(row0 + r, row1 - 1) / a.group;
     }
   // what every row sees: keys below `all_end` and from `all_low` on (or below
   // `first`)
@@ -299,32 +297,26 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
   const int all_low = a.window > 0 ? chunk.position + token1 - a.window : 0;
   const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;  // what some row sees
 
-  float out[NT][T::DM][4];
-  float largest[NT][2], sum[NT][2];
+  float out[T::DM][4];
+  float largest[2], sum[2];
   bool taken_out = false;
+  largest[0] = largest[1] = -INFINITY;
+  sum[0] = sum[1] = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    largest[n][0] = largest[n][1] = -INFINITY;
-    sum[n][0] = sum[n][1] = 0.0f;
-#pragma unroll
-    for (int m = 0; m < T::DM; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
-  }
+  for (int m = 0; m < T::DM; ++m) out[m][0] = out[m][1] = out[m][2] = out[m][3] = 0.0f;
 
   for (; tile < tile1; tile += WARPS) {
     const int key0 = seen.key_of(tile), next = tile + WARPS;
-    float s[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    float s[4];
+    s[0] = s[1] = s[2] = s[3] = 0.0f;
 #pragma unroll
     for (int step = 0; step < Map::STEPS; ++step) {
       uint32_t f[4];
       w.key_fragment(step, f);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
         for (int term = TERMS - 1; term >= 0; --term) {
-          const uint2 b = fragments[((step * NT + n) * TERMS + term) * 32 + lane];
-          mma_f16(s[n], f, b.x, b.y);
+          const uint2 b = fragments[(step * TERMS + term) * 32 + lane];
+          mma_f16(s, f, b.x, b.y);
         }
     }
     // (the keys' registers are the next tile's; its page was looked up a tile ago)
@@ -332,61 +324,54 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
 
     // scores, and each column's largest
     const bool whole = key0 + TILE <= all_end && (key0 >= all_low || key0 + TILE <= first);
-    float rescale[NT][2];
+    float rescale[2];
     bool grown = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float top = -INFINITY;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float x = s[n][2 * half + e] * multiplier[n][e];
+          float x = s[2 * half + e] * multiplier[e];
           if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
           if (!whole) {
             const int key = key0 + w.position_of(half);
-            const bool sees = key < seen.end && (!a.causal || key <= position[n][e]) &&
-                              (a.window == 0 || key > position[n][e] - a.window || key < first);
+            const bool sees = key < seen.end && (!a.causal || key <= position[e]) &&
+                              (a.window == 0 || key > position[e] - a.window || key < first);
             x = sees ? x : -INFINITY;
           }
-          s[n][2 * half + e] = x;
+          s[2 * half + e] = x;
           top = fmaxf(top, x);
         }
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float before = largest[n][e];
+        const float before = largest[e];
         const float now = fmaxf(before, top - WEIGHT_LOG);
-        rescale[n][e] = weight_of(before, now);
+        rescale[e] = weight_of(before, now);
         grown = grown || now > before;
-        largest[n][e] = now;
+        largest[e] = now;
       }
     if (__any_sync(0xffffffffu, grown)) {
+      sum[0] *= rescale[0], sum[1] *= rescale[1];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        sum[n][0] *= rescale[n][0], sum[n][1] *= rescale[n][1];
-#pragma unroll
-        for (int m = 0; m < T::DM; ++m) {
-          out[n][m][0] *= rescale[n][0], out[n][m][1] *= rescale[n][1];
-          out[n][m][2] *= rescale[n][0], out[n][m][3] *= rescale[n][1];
-        }
+      for (int m = 0; m < T::DM; ++m) {
+        out[m][0] *= rescale[0], out[m][1] *= rescale[1];
+        out[m][2] *= rescale[0], out[m][3] *= rescale[1];
       }
     }
-    uint32_t p[NT][TERMS][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+    uint32_t p[TERMS][2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float y[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          y[e] = weight_of(s[n][2 * half + e], largest[n][e]);
-          sum[n][e] += y[e];
+          y[e] = weight_of(s[2 * half + e], largest[e]);
+          sum[e] += y[e];
         }
         const uint32_t hi = half_pair(y[0], y[1]);
-        p[n][0][half] = turn(hi);
+        p[0][half] = turn(hi);
         if constexpr (TERMS == 2) {
           const float2 u = pair_value(hi);
-          p[n][1][half] = turn(half_pair(y[0] - u.x, y[1] - u.y));
+          p[1][half] = turn(half_pair(y[0] - u.x, y[1] - u.y));
         }
       }
     // where rows differ in what they see, a value that is not finite must not
@@ -407,14 +392,11 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
     for (int m = 0; m < T::DM; ++m) {
       uint32_t f[4];
       w.value_fragment(m, f);
+      float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int term = TERMS - 1; term >= 0; --term) mma_f16(o, f, p[term][0], p[term][1]);
 #pragma unroll
-        for (int term = TERMS - 1; term >= 0; --term) mma_f16(o, f, p[n][term][0], p[n][term][1]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[n][m][e] += o[e];
-      }
+      for (int e = 0; e < 4; ++e) out[m][e] += o[e];
     }
     if (next < tile1) {
       w.load_values();
@@ -427,18 +409,16 @@ __global__ void __launch_bounds__(THREADS, T::CTAS) attention_rows_kernel(const 
   float* merged = reinterpret_cast<float*>(shared);
   float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float total = sum[n][e];
+      float total = sum[e];
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const int r = 8 * n + 2 * t + e;
-      if (g == 0) stats[warp * ROWS + r] = make_float2(largest[n][e], total);
+      const int r = 2 * t + e;
+      if (g == 0) stats[warp * ROWS + r] = make_float2(largest[e], total);
 #pragma unroll
       for (int m = 0; m < T::DM; ++m) {
-        merged[(warp * ROWS + r) * D + 16 * m + g] = out[n][m][e];
-        merged[(warp * ROWS + r) * D + 16 * m + g + 8] = out[n][m][2 + e];
+        merged[(warp * ROWS + r) * D + 16 * m + g] = out[m][e];
+        merged[(warp * ROWS + r) * D + 16 * m + g + 8] = out[m][2 + e];
       }
     }
   taken_out = __syncthreads_or(taken_out);
@@ -577,28 +557,13 @@ int launch_rows(const AttentionChunksArgs& a, cudaStream_t stream) {
   return 0;
 }
 
-template <int D, bool BF16>
-int launch_columns(const AttentionChunksArgs& a, int columns, cudaStream_t stream) {
-  if constexpr (D <= 128)
-    if (columns == 2) return launch_rows<RowsTraits<D, BF16, 2>>(a, stream);
-  return launch_rows<RowsTraits<D, BF16, 1>>(a, stream);
-}
-
-template <int D>
-int launch_dim(const AttentionChunksArgs& a, bool bf16, int columns, cudaStream_t stream) {
-  return bf16 ? launch_columns<D, true>(a, columns, stream) : launch_columns<D, false>(a, columns, stream);
-}
-
-#define DRIFT_ROWS_REGISTER(D, nt)                                                                  \
-  DRIFT_REGISTER(attention_rows_bf16_d##D##_n##nt, (attention_rows_kernel<RowsTraits<D, true, nt>>))  \
-  DRIFT_REGISTER(attention_rows_f32_d##D##_n##nt, (attention_rows_kernel<RowsTraits<D, false, nt>>))
-DRIFT_ROWS_REGISTER(64, 1)
-DRIFT_ROWS_REGISTER(64, 2)
-DRIFT_ROWS_REGISTER(80, 1)
-DRIFT_ROWS_REGISTER(80, 2)
-DRIFT_ROWS_REGISTER(128, 1)
-DRIFT_ROWS_REGISTER(128, 2)
-DRIFT_ROWS_REGISTER(256, 1)
+#define DRIFT_ROWS_REGISTER(D)                                                            \
+  DRIFT_REGISTER(attention_rows_bf16_d##D, (attention_rows_kernel<RowsTraits<D, true>>))  \
+  DRIFT_REGISTER(attention_rows_f32_d##D, (attention_rows_kernel<RowsTraits<D, false>>))
+DRIFT_ROWS_REGISTER(64)
+DRIFT_ROWS_REGISTER(80)
+DRIFT_ROWS_REGISTER(128)
+DRIFT_ROWS_REGISTER(256)
 #define DRIFT_JOIN_REGISTER(D)                                                            \
   DRIFT_REGISTER(attention_chunks_join_f32_d##D, (attention_chunks_join_kernel<D, false>)) \
   DRIFT_REGISTER(attention_chunks_join_bf16_d##D, (attention_chunks_join_kernel<D, true>))
@@ -609,15 +574,18 @@ DRIFT_JOIN_REGISTER(256)
 
 }  // namespace
 
-int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
-                          cudaStream_t stream) {
+template <int D>
+static int launch_dim(const AttentionChunksArgs& a, bool bf16, cudaStream_t stream) {
+  return bf16 ? launch_rows<RowsTraits<D, true>>(a, stream) : launch_rows<RowsTraits<D, false>>(a, stream);
+}
+
+int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, cudaStream_t stream) {
   const bool bf16 = x_dtype == DRIFT_BF16;
-  const int columns = rows_per_unit / 8;
   switch (head_dim) {
-    case 64: return launch_dim<64>(a, bf16, columns, stream);
-    case 80: return launch_dim<80>(a, bf16, columns, stream);
-    case 128: return launch_dim<128>(a, bf16, columns, stream);
-    default: return launch_dim<256>(a, bf16, columns, stream);
+    case 64: return launch_dim<64>(a, bf16, stream);
+    case 80: return launch_dim<80>(a, bf16, stream);
+    case 128: return launch_dim<128>(a, bf16, stream);
+    default: return launch_dim<256>(a, bf16, stream);
   }
 }
 

@@ -131,15 +131,14 @@ int check_chunks(const char* call, int x_dtype, long long tokens, int kv_heads, 
                  const int32_t* positions, int batch, int longest);
 int check_rows_aligned(const char* call, const void* a, const void* b);
 
-// For few rows: attention_rows.cu over F16 caches (8 or 16 rows a unit, heads
-// of 256 8; 16-key tiles) and attention_codes.cu over 8-bit ones (4, 8, 16 or
-// 24, heads of 256 up to 8; 32-key tiles).
-int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
-                          cudaStream_t stream);
-// (the warps of a CTA of the latter)
-__host__ __device__ constexpr int attention_codes_warps(int head_dim, int rows_per_unit) {
-  return head_dim == 128 && rows_per_unit <= 8 ? 4 : 8;
-}
+// For few rows: attention_rows.cu over F16 caches (units of 8 rows, 16-key
+// tiles) and attention_codes.cu over 8-bit ones (of 4 or 8, 32-key tiles); the
+// warps of a CTA, and the CTAs that an SM holds.
+constexpr int ATTENTION_ROWS_WARPS = 8;
+constexpr int attention_rows_ctas(int head_dim) { return head_dim > 128 ? 1 : 2; }
+constexpr int attention_codes_warps(int head_dim) { return head_dim == 128 ? 4 : 8; }
+constexpr int attention_codes_ctas(int head_dim) { return head_dim > 128 ? 1 : head_dim == 128 ? 3 : 2; }
+int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, cudaStream_t stream);
 int launch_attention_codes(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                            cudaStream_t stream);
 // attention_tiles.cu (F32 rows: heads up to 128): `row_tiles` tiles of 128 rows
