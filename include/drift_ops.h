@@ -245,7 +245,7 @@ int drift_attention_decode(const float* q, int batch, int q_heads, const void* k
  * sequence stay as they are. A sequence whose starts, length or positions are
  * out of range sets the device error word (code 1) and is left out; a page id
  * outside the cache sets it too, is not written, and reads as zeros.
- * Tensors are F32 or BF16 (x_dtype), 16-byte aligned.
+ * Tensors are F32 or BF16 (x_dtype), 16-byte aligned, as are scales.
  *
  * cache_dtype DRIFT_F16 is drift_cache_write's cache. DRIFT_I8 keeps codes in
  * its place, int8 in the same two layouts, and a scale for each position and
@@ -278,8 +278,9 @@ int drift_cache_read_chunks(int x_dtype, void* k, void* v, int64_t tokens, int k
  * p - window + 1 on and, whatever the window, the sequence's first `first`
  * positions. softcap, sinks and the limits on heads are drift_attention's;
  * max_key_count bounds positions[z] plus z's tokens. F32 rows are computed to
- * F32's accuracy, BF16 rows with weights (and an 8-bit cache's keys and
- * values) rounded to F16. `workspace`
+ * F32's accuracy; BF16 rows with weights, and an 8-bit cache's keys and values,
+ * rounded to F16, or (few rows over an 8-bit cache) with q in steps of 2^-14 of
+ * its row's largest value and weights in steps of 2^-18. out may be q. `workspace`
  * (16-byte aligned, the caller's: calls that may overlap need one each) holds
  * drift_attention_chunks_workspace_bytes(...) bytes of partial results. */
 int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_heads, int kv_heads,
