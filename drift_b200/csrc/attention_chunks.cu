@@ -17,6 +17,7 @@ struct Plan {
   int rows_per_unit;    // rows of a key head that a CTA takes
   int keys_per_tile;
   int splits, tiles_per_split;
+  bool expands;         // an 8-bit cache's codes to F16 first
 };
 
 struct Call {
@@ -37,6 +38,7 @@ long long tiles_bound(const Call& c, int rows, int width) {
 Plan plan_rows(const Call& c) {
   Plan p;
   p.row_tiles = 0;
+  p.expands = false;
   const long long rows = (long long)c.longest * c.group;
   const bool codes = c.cache_dtype == DRIFT_I8;
   p.rows_per_unit = codes && rows <= 4 ? 4 : 8;
@@ -83,17 +85,18 @@ bool takes_tiles(const Call& c, long long rows) {
 // share a tile's keys: a row tile by itself takes 1.6 times as long (chunk of
 // 2048 BF16 rows, 8192 keys: 241 us, 414 with one) but keeps all SMs at work
 // where there are few (1500 F32 tokens of 4 x 4 heads: 67 us, 84 with two).
-Plan plan_tiles(const Call& c) {
+Plan plan_tiles(const Call& c, bool codes, double& least) {
   constexpr double CTA_NS = 9000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 1700;
-  const bool bf16 = c.x_dtype == DRIFT_BF16, codes = c.cache_dtype == DRIFT_I8;
+  const bool bf16 = c.x_dtype == DRIFT_BF16;
   const double key_ns = bf16 ? (c.head_dim > 128 ? 20 : c.head_dim > 64 ? 7.7 : 6.5) * (codes ? 2.2 : 1.0)
                              : (c.head_dim > 64 ? 14.5 : 10) * (codes ? 2.5 : 1.0);
   const long long rows = (long long)c.longest * c.group;
   Plan best;
-  double least = -1;
+  least = -1;
   for (int row_tiles = c.head_dim > 128 || rows <= 128 ? 1 : 2; row_tiles > 0; --row_tiles) {
     Plan p;
     p.row_tiles = row_tiles;
+    p.expands = false;
     p.rows_per_unit = 128 * row_tiles;
     p.keys_per_tile = attention_tiles_keys(c.head_dim, bf16);
     const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
@@ -104,8 +107,11 @@ Plan plan_tiles(const Call& c) {
     const double fewest = c.causal && c.window == 0 ? double(tiles) * (c.max_key_count - c.longest) / c.max_key_count : double(tiles);
     const double mean = (tiles + fewest) / 2;
     const double parts_bytes = 8.0 * rows * c.batch * c.kv_heads * c.head_dim;  // of a split, there and back
+    long long last = 0;
     for (long long splits = 1; splits <= 64 && splits <= tiles; ++splits) {
       const long long each = (tiles + splits - 1) / splits;
+      if (each == last) continue;
+      last = each;
       const double ctas = units * std::max(1.0, splits * mean / tiles);
       const double longest = each * tile_ns + cta_ns, shortest = std::min(double(each), fewest) * tile_ns + cta_ns;
       const double shared = (units * mean * tile_ns + ctas * cta_ns) / sm_count() + shortest;
@@ -122,13 +128,31 @@ Plan plan_tiles(const Call& c) {
   return best;
 }
 
+// The same with the choice of expanding an 8-bit cache's codes for BF16 rows:
+// two launches, and 3 bytes a value at about 3 TB/s (three chunks of 1001 BF16
+// tokens x 4 heads over 5003 keys: 235 us, 393 with each unit's own
+// conversion; eight of 40 tokens over 4096: 104, and 95), in at most 1 GiB.
+Plan plan_all_tiles(const Call& c) {
+  constexpr double LAUNCHES_NS = 7000, BYTES_A_NS = 3000;
+  double own;
+  const Plan p = plan_tiles(c, c.cache_dtype == DRIFT_I8, own);
+  if (c.cache_dtype != DRIFT_I8 || c.x_dtype != DRIFT_BF16) return p;
+  if (expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > (size_t(1) << 30)) return p;
+  const long long seen = c.window > 0 ? std::min((long long)c.max_key_count, (long long)c.window + c.longest + c.first) : c.max_key_count;
+  double expanded;
+  Plan q = plan_tiles(c, false, expanded);
+  q.expands = true;
+  expanded += LAUNCHES_NS + 6.0 * seen * c.batch * c.kv_heads * c.head_dim / BYTES_A_NS;
+  return expanded < own ? q : p;
+}
+
 Plan plan_chunks(const Call& c) {
   const long long rows = (long long)c.longest * c.group;
   // (the copies' coordinates are 32-bit, the grid's unit axis 16-bit)
   const bool reachable = (long long)c.pages * c.page_size < (1ll << 31) &&
                          (long long)c.pages * c.kv_heads * c.head_dim < (1ll << 31);
   if (takes_tiles(c, rows) && reachable) {
-    const Plan p = plan_tiles(c);
+    const Plan p = plan_all_tiles(c);
     if ((rows + p.rows_per_unit - 1) / p.rows_per_unit * p.splits <= 65535) return p;
   }
   return plan_rows(c);
@@ -146,8 +170,13 @@ int check_shape(int q_heads, int kv_heads, int max_key_count, int table_stride, 
   return 0;
 }
 
+// The workspace: partial results, then (from a 128-byte boundary) expanded codes.
 size_t parts_bytes(const Plan& p, long long tokens, int q_heads, int head_dim) {
-  return p.splits > 1 ? size_t(tokens) * q_heads * p.splits * (head_dim + 2) * sizeof(float) : 0;
+  return p.splits > 1 ? (size_t(tokens) * q_heads * p.splits * (head_dim + 2) * sizeof(float) + 127) / 128 * 128 : 0;
+}
+size_t workspace_bytes_of(const Plan& p, const Call& c, long long tokens, int q_heads) {
+  return parts_bytes(p, tokens, q_heads, c.head_dim) +
+         (p.expands ? expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) : 0);
 }
 
 }  // namespace
@@ -163,9 +192,9 @@ size_t drift_attention_chunks_workspace_bytes(int x_dtype, int64_t tokens, int q
   if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || pages <= 0 ||
       page_size <= 0 || batch <= 0 || longest <= 0 || max_key_count <= 0)
     return 0;
-  const Plan p = plan_chunks({x_dtype, cache_dtype, batch, longest, q_heads / kv_heads, kv_heads, head_dim, max_key_count,
-                              causal, window, first, pages, page_size});
-  return parts_bytes(p, tokens, q_heads, head_dim);
+  const Call c = {x_dtype, cache_dtype, batch, longest, q_heads / kv_heads, kv_heads, head_dim, max_key_count,
+                  causal, window, first, pages, page_size};
+  return workspace_bytes_of(plan_chunks(c), c, tokens, q_heads);
 }
 
 int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_heads, int kv_heads, int head_dim,
@@ -181,12 +210,13 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   if (tokens == 0 || batch == 0 || longest == 0) return 0;
   DRIFT_TRY(check_rows_aligned("attention", q, out));
   const int group = q_heads / kv_heads;
-  const Plan p = plan_chunks({x_dtype, cache_dtype, batch, longest, group, kv_heads, head_dim, max_key_count, causal,
-                              window, first, pages, page_size});
+  const Call c = {x_dtype, cache_dtype, batch, longest, group, kv_heads, head_dim, max_key_count, causal,
+                  window, first, pages, page_size};
+  const Plan p = plan_chunks(c);
   const long long units = ((long long)longest * group + p.rows_per_unit - 1) / p.rows_per_unit;
   if (units * p.splits > 0x7fffffffll || (long long)longest * q_heads > 0x7fffffffll)
     return invalid("attention: chunks of %d tokens of %d heads", longest, q_heads);
-  const size_t needed = parts_bytes(p, tokens, q_heads, head_dim);
+  const size_t parts = parts_bytes(p, tokens, q_heads, head_dim), needed = workspace_bytes_of(p, c, tokens, q_heads);
   if (needed > workspace_bytes || (needed && !workspace))
     return invalid("attention: a workspace of %zu bytes, %zu needed", workspace_bytes, needed);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return invalid("attention: the workspace does not start on a 16-byte boundary");
@@ -199,8 +229,9 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   a.key_scales = key_scales;
   a.value_scales = value_scales;
   a.sinks = sinks;
-  a.part_o = needed ? static_cast<float*>(workspace) : nullptr;
-  a.part_ml = needed ? a.part_o + size_t(tokens) * q_heads * p.splits * head_dim : nullptr;
+  a.units = nullptr;
+  a.part_o = parts ? static_cast<float*>(workspace) : nullptr;
+  a.part_ml = parts ? a.part_o + size_t(tokens) * q_heads * p.splits * head_dim : nullptr;
   a.error = device_error_word();
   a.q_heads = q_heads;
   a.kv_heads = kv_heads;
@@ -213,10 +244,11 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   a.scale = scale;
   a.softcap = softcap;
   const cudaStream_t s = cudaStream_t(stream);
-  if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, x_dtype, cache_dtype, head_dim, p.row_tiles, s));
+  if (p.expands) DRIFT_TRY(launch_attention_expand(a, head_dim, static_cast<uint8_t*>(workspace) + parts, s));
+  if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, x_dtype, p.expands ? DRIFT_F16 : cache_dtype, head_dim, p.row_tiles, s));
   else if (cache_dtype == DRIFT_I8) DRIFT_TRY(launch_attention_codes(a, x_dtype, head_dim, p.rows_per_unit, s));
   else DRIFT_TRY(launch_attention_rows(a, x_dtype, head_dim, s));
-  if (!needed) return 0;
+  if (!parts) return 0;
   return launch_attention_join(a, x_dtype, head_dim, p.rows_per_unit, p.keys_per_tile, s);
 }
 

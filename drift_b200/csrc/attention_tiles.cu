@@ -534,6 +534,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&q_full[i]);
     }
+    // (what expanded codes are over)
+    const float* units = !CODES && TERMS == 1 && a.units ? a.units + ((long long)z * a.kv_heads + head) * 2 : nullptr;
+    const float key_unit = units ? units[0] : 1.0f, value_unit = units ? units[1] : 1.0f;
     // (a softcap leaves natural units behind)
     // (and a factor of 2^-60 is as good as none; times a tile's power it is normal)
     const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 8.7e-19f);
@@ -602,7 +605,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 
       const float* k_scales = scales + stage * 2 * KEYS;
       const float* v_scales = k_scales + KEYS;
-      const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : 1.0f;
+      const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : key_unit;
       const float tile_m2 = a.softcap > 0.0f ? m2 : m2 * by_unit;
       const float now_unit = CODES ? float(v_unit[stage]) : 0.0f;
       if constexpr (CODES && TERMS == 2) {
@@ -741,7 +744,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     if (ok) {
       tc::fence_after_sync();
       take_output();
-      float scale = CODES ? unit : 1.0f;
+      float scale = CODES ? unit : value_unit;
       if (!a.part_o) {
         if (a.sinks) {
           // the sink's weight in the row's units, or the row's in the sink's

@@ -58,6 +58,7 @@ struct AttentionChunksArgs {
   const void* values;
   const float* key_scales;    // 8-bit caches
   const float* value_scales;
+  const float* units;         // [batch][kv_heads][2]: what keys and values are over (attention_expand), or null
   const float* sinks;
   float* part_o;   // [token row][q_heads][splits][D], or null for one split
   float* part_ml;  // [token row][q_heads][splits][2]: largest, sum
@@ -146,6 +147,11 @@ int launch_attention_codes(const AttentionChunksArgs& a, int x_dtype, int head_d
 int attention_tiles_keys(int head_dim, bool bf16);
 int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int row_tiles,
                            cudaStream_t stream);
+// attention_expand.cu: an 8-bit cache's keys and values of the chunks as F16 in
+// `memory` (16-byte aligned, expanded_bytes), which then take the cache's place
+// in `a`.
+size_t expanded_bytes(int batch, int kv_heads, int head_dim, int page_size, int max_key_count);
+int launch_attention_expand(AttentionChunksArgs& a, int head_dim, void* memory, cudaStream_t stream);
 // Joins the splits (attention_rows.cu).
 int launch_attention_join(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                           int keys_per_tile, cudaStream_t stream);
