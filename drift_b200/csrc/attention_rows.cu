@@ -20,6 +20,10 @@
 //
 // Softmax in F32, a running maximum and sum per warp; the warps meet
 // in shared memory, the splits in a second launch (attention_chunks_join_kernel).
+//
+// Bound by memory: a step of 16 sequences x 16384 keys of 8 heads of 128 148 us,
+// 1.07 GB at 7.2 TB/s; of 13 under a window of 1024 of 2 heads of 256, 15 us,
+// by the latencies of two launches.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -18,7 +18,8 @@
 // for BF16 rows times their scales over a power of two (of the tile's keys; of
 // the values so far), each rounded to F16 like the weights; for F32 rows
 // exactly, and there a key's scale multiplies its scores, and a value's its
-// weights.
+// weights. Where a chunk has several units of BF16 rows its codes come expanded
+// to an F16 cache of the call's own (attention_expand.cu).
 //
 // The order: Q K^T of the next tile is issued as soon as the softmax threads
 // have taken S into registers, P V when P is there. So the tensor core works
@@ -26,7 +27,11 @@
 // is the longer of the two: for D = 128 the tensor core's 16 + 10 products of
 // 64 and 52 clocks for 80 keys and 256 rows. (With P over S, and Q K^T behind
 // P V, a tile took both after one another: 3050 clocks for 128 keys.) TMEM's
-// 512 columns set the tile's keys: MT S, MT P, MT outputs.
+// 512 columns set the tile's keys: MT S, MT P, MT outputs. Measured: a chunk of
+// 2048 BF16 tokens of 32 heads of 128 over 8192 keys 241 us, 1000 TFLOP/s, the
+// special function unit (an exponential a score) and the tensor core each busy
+// for 59 % of a full SM's time (51 % on average: 256 CTAs on 148 SMs); 1500 F32 tokens of 16 heads 67 us; 6000 BF16 tokens of 8 heads of 64
+// under a window of 1024 51 us, the exponentials.
 //
 // BF16 rows (TERMS = 1): q is exact in F16 after a power of two per row; P's
 // rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). O stays in TMEM.
@@ -45,9 +50,9 @@
 // Warps: first the softmax, four for 128 rows; then one for the copies, two for
 // the tensor core (Q K^T, P V), and for an F16 cache one for the edges: in a
 // tile that some row sees only in part it takes values that are not finite out
-// of V, since such a value times a zero weight would reach rows that do not see
-// it
-// (they are added at the end, to the rows that do). An 8-bit cache has
+// of V, since such a value times a zero weight would reach rows that do not see it
+// (they are added at the end, to the rows that do). A softmax warp passes over
+// a tile that none of its rows sees. An 8-bit cache has
 // converting warps. Every wait is bounded; one that gives up sets device error
 // 2, and the CTA drains its copies and products, frees its TMEM and returns.
 #include <cuda.h>

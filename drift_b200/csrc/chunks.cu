@@ -13,7 +13,10 @@
 // A CTA takes 16 consecutive positions (an aligned sixteenth-row of a page) of
 // one head, or of a few: their rows in, the keys out as rows, the values out
 // transposed, through shared memory, 16 positions of a dimension in one 16-byte
-// store (32 for F16). Bound by memory, (4 or 2) + 1 bytes a value.
+// store (32 for F16). Bound by memory, (4 or 2) + 1 bytes a value: 16 x 4096
+// positions of 8 heads of 128 back to BF16 58 us, 5.4 TB/s; 4 x 4099 from BF16
+// 59 us, 2.8 TB/s (a CTA's chain of loads, largest value, codes and turned
+// stores; F32 rows, twice the bytes in, 63 us). Few rows take 3 us, a launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

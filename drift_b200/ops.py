@@ -17,6 +17,7 @@ bytes on the device), as the reference's Tensor(dtype, shape, storage) is.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -255,6 +256,9 @@ class CudaOps:
         if device is not None:
             torch.cuda.set_device(device)
         self.device = torch.cuda.current_device()
+        # (the layers of a step ask for the same sizes; the device has a say in them)
+        self._chunks_workspace = functools.lru_cache(256)(
+            lambda device, *sizes: self.lib.drift_attention_chunks_workspace_bytes(*sizes))
 
     # -- plumbing -------------------------------------------------------------------------
     @staticmethod
@@ -624,6 +628,9 @@ class CudaOps:
         (F32 or BF16), over its positions in a KvCache or a QuantizedKvCache,
         the new ones included (written before): a decoding step, drafted
         tokens, prompts or pieces of them, of different lengths in one call.
+        out may be q. Partial results (and, for BF16 rows over an 8-bit cache,
+        its keys and values as F16) are in device memory of up to a GiB that is
+        the call's own.
         With a window, the first `attention.first` positions stay visible."""
         x_dtype = self._chunk_rows("attention", q, out, cache, chunks)
         tokens, q_heads, _ = q.shape
@@ -636,8 +643,8 @@ class CudaOps:
                      f"attention: sinks {list(sinks.shape)} for {q_heads} heads")
         window, causal = attention.window or 0, int(attention.causal)
         chunk_args = self._chunk_args(chunks)
-        size = self.lib.drift_attention_chunks_workspace_bytes(
-            x_dtype, tokens, q_heads, kv_heads, dim, dtype, pages, page_size, chunk_args[4],
+        size = self._chunks_workspace(
+            q.device.index, x_dtype, tokens, q_heads, kv_heads, dim, dtype, pages, page_size, chunk_args[4],
             chunk_args[5], chunks.max_key_count, causal, window, attention.first)
         # the call's own: freed to torch's allocator behind it in the stream
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
