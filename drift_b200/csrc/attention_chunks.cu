@@ -85,11 +85,11 @@ bool takes_tiles(const Call& c, long long rows) {
 // share a tile's keys: a row tile by itself takes 1.6 times as long (chunk of
 // 2048 BF16 rows, 8192 keys: 241 us, 414 with one) but keeps all SMs at work
 // where there are few (1500 F32 tokens of 4 x 4 heads: 67 us, 84 with two).
-Plan plan_tiles(const Call& c, bool codes, double& least) {
+Plan plan_tiles(const Call& c, double slower, double& least) {
   constexpr double CTA_NS = 9000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 1700;
   const bool bf16 = c.x_dtype == DRIFT_BF16;
-  const double key_ns = bf16 ? (c.head_dim > 128 ? 20 : c.head_dim > 64 ? 7.7 : 6.5) * (codes ? 2.2 : 1.0)
-                             : (c.head_dim > 64 ? 14.5 : 10) * (codes ? 2.5 : 1.0);
+  const double key_ns = bf16 ? (c.head_dim > 128 ? 20 : c.head_dim > 64 ? 7.7 : 6.5) * slower
+                             : (c.head_dim > 64 ? 14.5 : 10) * slower;
   const long long rows = (long long)c.longest * c.group;
   Plan best;
   least = -1;
@@ -128,19 +128,22 @@ Plan plan_tiles(const Call& c, bool codes, double& least) {
   return best;
 }
 
-// The same with the choice of expanding an 8-bit cache's codes for BF16 rows:
-// two launches, and 3 bytes a value at about 3 TB/s (three chunks of 1001 BF16
-// tokens x 4 heads over 5003 keys: 235 us, 393 with each unit's own
-// conversion; eight of 40 tokens over 4096: 104, and 95), in at most 1 GiB.
+// The same with the choice of expanding an 8-bit cache's codes: two launches,
+// and 3 bytes a value at about 3 TB/s (three chunks of 1001 BF16 tokens x 4
+// heads over 5003 keys: 230 us, 395 with each unit's own conversion; eight of
+// 40 tokens over 4096: 100, and 94; 2048 F32 tokens over 8192: 592, and 984;
+// 64 over 16384: 99, and 85), in at most 1 GiB. Converting codes makes a tile
+// 2.2 (BF16) and 2.5 times as long, exact codes' scales 1.4 times.
 Plan plan_all_tiles(const Call& c) {
   constexpr double LAUNCHES_NS = 7000, BYTES_A_NS = 3000;
   double own;
-  const Plan p = plan_tiles(c, c.cache_dtype == DRIFT_I8, own);
-  if (c.cache_dtype != DRIFT_I8 || c.x_dtype != DRIFT_BF16) return p;
-  if (expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > (size_t(1) << 30)) return p;
+  const bool bf16 = c.x_dtype == DRIFT_BF16;
+  if (c.cache_dtype != DRIFT_I8) return plan_tiles(c, 1.0, own);
+  const Plan p = plan_tiles(c, bf16 ? 2.2 : 2.5, own);
+  if (expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > (size_t(1) << 30)) return p;
   const long long seen = c.window > 0 ? std::min((long long)c.max_key_count, (long long)c.window + c.longest + c.first) : c.max_key_count;
   double expanded;
-  Plan q = plan_tiles(c, false, expanded);
+  Plan q = plan_tiles(c, bf16 ? 1.0 : 1.4, expanded);
   q.expands = true;
   expanded += LAUNCHES_NS + 6.0 * seen * c.batch * c.kv_heads * c.head_dim / BYTES_A_NS;
   return expanded < own ? q : p;
@@ -176,7 +179,7 @@ size_t parts_bytes(const Plan& p, long long tokens, int q_heads, int head_dim) {
 }
 size_t workspace_bytes_of(const Plan& p, const Call& c, long long tokens, int q_heads) {
   return parts_bytes(p, tokens, q_heads, c.head_dim) +
-         (p.expands ? expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) : 0);
+         (p.expands ? expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) : 0);
 }
 
 }  // namespace
@@ -244,7 +247,7 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   a.scale = scale;
   a.softcap = softcap;
   const cudaStream_t s = cudaStream_t(stream);
-  if (p.expands) DRIFT_TRY(launch_attention_expand(a, head_dim, static_cast<uint8_t*>(workspace) + parts, s));
+  if (p.expands) DRIFT_TRY(launch_attention_expand(a, x_dtype, head_dim, static_cast<uint8_t*>(workspace) + parts, s));
   if (p.row_tiles) DRIFT_TRY(launch_attention_tiles(a, x_dtype, p.expands ? DRIFT_F16 : cache_dtype, head_dim, p.row_tiles, s));
   else if (cache_dtype == DRIFT_I8) DRIFT_TRY(launch_attention_codes(a, x_dtype, head_dim, p.rows_per_unit, s));
   else DRIFT_TRY(launch_attention_rows(a, x_dtype, head_dim, s));

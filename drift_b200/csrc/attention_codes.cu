@@ -403,13 +403,13 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
       weigh();
     }
     // into digits, [row][key] in shared memory: a product's columns are rows
-    const float steps = v_unit > 0.0f ? T::P_STEPS / v_unit : 0.0f;
+    const float v_inverse = v_unit > 0.0f ? 1.0f / v_unit : 0.0f;  // (finite; steps of it may not be)
     __syncwarp();  // (the tile before is read)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float by = v_scale[m][half] * steps;
+        const float by = v_scale[m][half] * v_inverse * T::P_STEPS;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float x = p[m][2 * half + e];
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
   __syncthreads();  // (past the fragments and the weights)
   float* merged = reinterpret_cast<float*>(shared);
   float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
-  const float worth = v_unit / T::P_STEPS * low_digit;
+  const float worth = low_digit / T::P_STEPS;  // (and v_unit, which with it may be below F32's range)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float total = sum[e];
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
       for (int m = 0; m < T::DM; ++m)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float x = out[m][2 * half + e] * worth;
+          float x = out[m][2 * half + e] * worth * v_unit;
           if (PACKED) x += __shfl_xor_sync(0xffffffffu, x, 2);
           if (writes) merged[(warp * ROWS + r) * D + 16 * m + g + 8 * half] = x;
         }

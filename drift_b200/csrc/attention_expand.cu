@@ -1,9 +1,11 @@
-// For attention_chunks of BF16 rows over an 8-bit cache where a chunk has
-// several units of rows: the sequences' keys and values as F16, once, for
-// attention_tiles' F16 kernel. Its own converting warps make each tile anew
-// for every unit, and bound it (a tile 5900 clocks, 2700 from an F16 cache).
+// For attention_chunks over an 8-bit cache where a chunk has several units of
+// rows: the sequences' keys and values as F16, once, for attention_tiles' F16
+// kernel. Its own converting warps make each tile anew for every unit, and
+// bound it (a tile of BF16 rows 5900 clocks, 2700 from an F16 cache).
 //
-//   keys16, values16 = code scale / unit, rounded to F16
+//   BF16 rows: keys16, values16 = code scale / unit, rounded to F16
+//   F32 rows:  keys16, values16 = code, exactly; and a row of scales for each
+//              sequence and head, the values' over their unit
 //
 // with a power of two for each sequence, key head and side: at or above the
 // largest finite scale that a row sees, so that a quotient is at most 127 (508
@@ -25,7 +27,8 @@ namespace drift {
 
 namespace {
 
-constexpr int UNIT_THREADS = 512;
+constexpr int UNIT_THREADS = 1024;
+constexpr int FLIGHT = 4;
 constexpr int THREADS = 256;
 constexpr int RUN = 16;    // positions of a code chunk, in one page
 constexpr int runs_of(int dim) { return dim % 64 ? 8 : 4; }  // of a CTA: as many chunks to every thread
@@ -39,6 +42,8 @@ struct ExpandArgs {
   __half* keys16;
   __half* values16;
   float* units;    // [batch][kv_heads][2]
+  float* key_scales32;    // [batch][kv_heads][page_row page_size], F32 rows
+  float* value_scales32;
   int* table;      // [batch][page_row]
   int* error;
   int kv_heads, page_row, window, first;
@@ -55,12 +60,12 @@ struct SeenPositions {
   __device__ bool sees(int position) const { return position < end && (position >= low || position < first); }
 };
 
-// A power of two at or above x whose inverse is normal, 2^-64 at least (the
-// scores' factor stays normal with it).
-__device__ __forceinline__ float power_over(float x) {
+// A power of two at or above x, `least` (in exponent bits) at least, whose
+// inverse is normal.
+__device__ __forceinline__ float power_over(float x, uint32_t least) {
   const uint32_t bits = __float_as_uint(x);
   const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-  return __uint_as_float(max(up, 0x1f800000u));
+  return __uint_as_float(max(up, least));
 }
 
 __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const ExpandArgs a) {
@@ -74,14 +79,37 @@ __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const Exp
   const SeenPositions seen(a, chunk);
   float top[2] = {0.0f, 0.0f};
   auto look = [&](int from, int to) {
-#pragma unroll 4
-    for (int p = from + int(threadIdx.x); p < to; p += UNIT_THREADS) {
-      const int page = chunk.table[p / a.at.page_size];
-      if (page < 0 || page >= a.at.pages) continue;
-      const long long at = ((long long)page * a.kv_heads + head) * a.at.page_size + p % a.at.page_size;
-      const float k = a.key_scales[at], v = a.value_scales[at];
-      if (k <= 3.402823466e38f) top[0] = fmaxf(top[0], k);  // (the finite ones)
-      if (v <= 3.402823466e38f) top[1] = fmaxf(top[1], v);
+    // four positions of a page to a thread, four times over: two latencies
+    // for 16384 positions
+#pragma unroll 1
+    for (int p0 = from / 4 * 4 + 4 * int(threadIdx.x); p0 < to; p0 += 4 * FLIGHT * UNIT_THREADS) {
+      int page[FLIGHT];
+#pragma unroll
+      for (int n = 0; n < FLIGHT; ++n) {
+        const long long p = p0 + 4ll * n * UNIT_THREADS;
+        page[n] = p < to ? chunk.table[p / a.at.page_size] : -1;
+      }
+      float4 x[FLIGHT][2];
+#pragma unroll
+      for (int n = 0; n < FLIGHT; ++n) {
+        const long long p = p0 + 4ll * n * UNIT_THREADS;
+        const bool there = page[n] >= 0 && page[n] < a.at.pages;
+        const long long at = ((long long)page[n] * a.kv_heads + head) * a.at.page_size + p % a.at.page_size;
+        x[n][0] = there ? *reinterpret_cast<const float4*>(a.key_scales + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        x[n][1] = there ? *reinterpret_cast<const float4*>(a.value_scales + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int n = 0; n < FLIGHT; ++n)
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          const float y[4] = {x[n][side].x, x[n][side].y, x[n][side].z, x[n][side].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const long long p = p0 + 4ll * n * UNIT_THREADS + e;
+            // (the finite ones)
+            if (p >= from && p < to && y[e] <= 3.402823466e38f) top[side] = fmaxf(top[side], y[e]);
+          }
+        }
     }
   };
   if (chunk.tokens > 0) {
@@ -98,13 +126,16 @@ __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const Exp
   if (threadIdx.x < 2) {
     float most = 0.0f;
     for (int w = 0; w < UNIT_THREADS / 32; ++w) most = fmaxf(most, tops[threadIdx.x][w]);
-    a.units[((long long)z * a.kv_heads + head) * 2 + threadIdx.x] = power_over(most);
+    // (F32 rows' keys are over nothing: their scales meet the scores; 2^-64 at
+    // least for the others', so that the scores' factor stays normal with it)
+    a.units[((long long)z * a.kv_heads + head) * 2 + threadIdx.x] =
+        a.key_scales32 && threadIdx.x == 0 ? 1.0f : power_over(most, threadIdx.x == 0 ? 0x1f800000u : 0x01000000u);
   }
 }
 
 // 64 positions of a head (128 where D = 80): a thread takes 16 codes at a time, of a position's
 // key or of a dimension's values.
-template <int D>
+template <int D, bool EXACT>
 __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -156,9 +187,20 @@ __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandA
     const bool key = in < D;
     float by[RUN];
     if (key) {
-      const float scale = there[n] ? a.key_scales[from_scales[n] + in / (D / 16)] * key_inverse : 0.0f;
+      float scale = there[n] ? a.key_scales[from_scales[n] + in / (D / 16)] * key_inverse : 0.0f;
+      if constexpr (EXACT) {
+        if (in % (D / 16) == 0) {
+          const long long to = ((long long)z * a.kv_heads + head) * a.page_row * a.at.page_size + first + in / (D / 16);
+          a.key_scales32[to] = scale;
+          a.value_scales32[to] = there[n] ? a.value_scales[from_scales[n] + in / (D / 16)] * value_inverse : 0.0f;
+        }
+        scale = 1.0f;
+      }
 #pragma unroll
       for (int e = 0; e < RUN; ++e) by[e] = scale;
+    } else if constexpr (EXACT) {
+#pragma unroll
+      for (int e = 0; e < RUN; ++e) by[e] = 1.0f;
     } else {
 #pragma unroll
       for (int e = 0; e < RUN; e += 4) {
@@ -180,18 +222,28 @@ __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandA
   }
 }
 
-#define DRIFT_EXPAND_REGISTER(D) DRIFT_REGISTER(attention_expand_d##D, attention_expand_kernel<D>)
+#define DRIFT_EXPAND_REGISTER(D)                                               \
+  DRIFT_REGISTER(attention_expand_bf16_d##D, (attention_expand_kernel<D, false>)) \
+  DRIFT_REGISTER(attention_expand_f32_d##D, (attention_expand_kernel<D, true>))
 DRIFT_EXPAND_REGISTER(64)
 DRIFT_EXPAND_REGISTER(80)
 DRIFT_EXPAND_REGISTER(128)
-DRIFT_EXPAND_REGISTER(256)
+DRIFT_REGISTER(attention_expand_bf16_d256, (attention_expand_kernel<256, false>))
 DRIFT_REGISTER(attention_units, attention_units_kernel)
 
 template <int D>
 int launch_dim(const ExpandArgs& a, cudaStream_t stream) {
   constexpr int POSITIONS = RUN * runs_of(D);
   const unsigned runs = unsigned(((long long)a.at.max_keys + POSITIONS - 1) / POSITIONS);
-  DRIFT_CUDA(launch_pdl(attention_expand_kernel<D>, dim3(runs, a.kv_heads, a.at.batch), THREADS, 0, stream, a));
+  const dim3 grid(runs, a.kv_heads, a.at.batch);
+  if constexpr (D <= 128) {
+    if (a.key_scales32) {
+      DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, true>, grid, THREADS, 0, stream, a));
+      DRIFT_LAUNCHED("attention_expand");
+      return 0;
+    }
+  }
+  DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, false>, grid, THREADS, 0, stream, a));
   DRIFT_LAUNCHED("attention_expand");
   return 0;
 }
@@ -202,13 +254,17 @@ constexpr size_t round_up(size_t bytes) { return (bytes + 127) / 128 * 128; }
 
 int expanded_page_row(int max_key_count, int page_size) { return int(((long long)max_key_count + page_size - 1) / page_size); }
 
-size_t expanded_bytes(int batch, int kv_heads, int head_dim, int page_size, int max_key_count) {
+// (a tile's scales are read whole past the last page)
+static size_t scales_bytes(size_t positions, int kv_heads) { return round_up((positions * kv_heads + 128) * sizeof(float)); }
+
+size_t expanded_bytes(int x_dtype, int batch, int kv_heads, int head_dim, int page_size, int max_key_count) {
   const size_t pages = size_t(batch) * expanded_page_row(max_key_count, page_size);
   return round_up(size_t(batch) * kv_heads * 2 * sizeof(float)) + round_up(pages * sizeof(int)) +
-         2 * round_up(pages * page_size * kv_heads * head_dim * sizeof(__half));
+         2 * round_up(pages * page_size * kv_heads * head_dim * sizeof(__half)) +
+         (x_dtype == DRIFT_F32 ? 2 * scales_bytes(pages * page_size, kv_heads) : 0);
 }
 
-int launch_attention_expand(AttentionChunksArgs& a, int head_dim, void* memory, cudaStream_t stream) {
+int launch_attention_expand(AttentionChunksArgs& a, int x_dtype, int head_dim, void* memory, cudaStream_t stream) {
   ExpandArgs e;
   e.at = a.at;
   e.keys = static_cast<const uint8_t*>(a.keys);
@@ -229,6 +285,10 @@ int launch_attention_expand(AttentionChunksArgs& a, int head_dim, void* memory, 
   const size_t side = round_up(pages * a.at.page_size * a.kv_heads * head_dim * sizeof(__half));
   e.keys16 = reinterpret_cast<__half*>(at);
   e.values16 = reinterpret_cast<__half*>(at + side);
+  at += 2 * side;
+  const size_t scales = scales_bytes(pages * a.at.page_size, a.kv_heads);
+  e.key_scales32 = x_dtype == DRIFT_F32 ? reinterpret_cast<float*>(at) : nullptr;
+  e.value_scales32 = x_dtype == DRIFT_F32 ? reinterpret_cast<float*>(at + scales) : nullptr;
   DRIFT_CUDA(launch_pdl(attention_units_kernel, dim3(a.kv_heads, a.at.batch), UNIT_THREADS, 0, stream, e));
   DRIFT_LAUNCHED("attention_units");
   switch (head_dim) {
@@ -240,7 +300,8 @@ int launch_attention_expand(AttentionChunksArgs& a, int head_dim, void* memory, 
   // the copies in the cache's place
   a.keys = e.keys16;
   a.values = e.values16;
-  a.key_scales = a.value_scales = nullptr;
+  a.key_scales = e.key_scales32;
+  a.value_scales = e.value_scales32;
   a.units = e.units;
   a.at.tables = e.table;
   a.at.table_stride = e.page_row;

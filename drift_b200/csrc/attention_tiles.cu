@@ -18,8 +18,9 @@
 // for BF16 rows times their scales over a power of two (of the tile's keys; of
 // the values so far), each rounded to F16 like the weights; for F32 rows
 // exactly, and there a key's scale multiplies its scores, and a value's its
-// weights. Where a chunk has several units of BF16 rows its codes come expanded
-// to an F16 cache of the call's own (attention_expand.cu).
+// weights. Where a chunk has several units of rows its codes come expanded to an
+// F16 cache of the call's own (attention_expand.cu): scaled for BF16 rows, and
+// exactly, with their scales by position, for F32 ones (SCALED).
 //
 // The order: Q K^T of the next tile is issued as soon as the softmax threads
 // have taken S into registers, P V when P is there. So the tensor core works
@@ -84,10 +85,10 @@ constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f, MOST_WEIGHT = 32768.0f;
 // terms end far below F16's last bit, 2^-24.
 constexpr int Q_BITS = 8;
 
-template <int D_, int KEYS_, int MT_, bool CODES_, int TERMS_>
+template <int D_, int KEYS_, int MT_, bool CODES_, int TERMS_, bool SCALED_>
 struct TileTraits {
   static constexpr int D = D_, KEYS = KEYS_, MT = MT_, TERMS = TERMS_;
-  static constexpr bool CODES = CODES_;
+  static constexpr bool CODES = CODES_, SCALED = SCALED_;  // SCALED: expanded codes of F32 rows
   static constexpr int UNIT = ROW_TILE * MT;
   static constexpr int SOFTMAX_WARPS = 4 * MT;
   // Q K^T and P V have a warp each: a wait costs one about 100 clocks even when
@@ -125,7 +126,8 @@ struct TileTraits {
   // its stage is free are a tile's time)
   static constexpr int bytes_of(int stages, int code_stages) {
     return K_AT + stages * (K_BYTES + V_STAGE) + (CODES ? code_stages * 2 * CODE_STAGE : 0) +
-           (CODES && TERMS == 2 ? stages * 2 * KEYS * 4 : 0) + (CODES ? code_stages * 2 * KEYS * 4 : 0) + 384;
+           (CODES && TERMS == 2 ? stages * 2 * KEYS * 4 : 0) + (CODES ? code_stages * 2 * KEYS * 4 : 0) +
+           (SCALED ? SOFTMAX_WARPS * KEYS * 4 : 0) + 384;
   }
   static constexpr int LIMIT = 232448;
   static constexpr int CODE_STAGES = bytes_of(2, 2) <= LIMIT ? 2 : 1;
@@ -135,7 +137,8 @@ struct TileTraits {
   static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;  // [COPY_STAGES][2]
   static constexpr int SCALES_AT = CODES_AT + (CODES ? COPY_STAGES * 2 * CODE_STAGE : 0);  // [STAGES][2][KEYS]
   static constexpr int COPIED_SCALES_AT = SCALES_AT + (CODES && TERMS == 2 ? STAGES * 2 * KEYS * 4 : 0);  // [COPY_STAGES][2][KEYS]
-  static constexpr int BARRIERS_AT = COPIED_SCALES_AT + (CODES ? COPY_STAGES * 2 * KEYS * 4 : 0);
+  static constexpr int WARP_SCALES_AT = COPIED_SCALES_AT + (CODES ? COPY_STAGES * 2 * KEYS * 4 : 0);  // [SOFTMAX_WARPS][KEYS]
+  static constexpr int BARRIERS_AT = WARP_SCALES_AT + (SCALED ? SOFTMAX_WARPS * KEYS * 4 : 0);
   static constexpr int BYTES = BARRIERS_AT + 384;  // 38 barriers and a few words
   // TMEM: S of row tile i, or (MT = 1) of every other tile; P and O of row tile i
   static constexpr int S_COLUMNS = (KEYS + 31) / 32 * 32;
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(T::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                        const TileArgs args) {
   constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
-  constexpr bool CODES = T::CODES;
+  constexpr bool CODES = T::CODES, SCALED = T::SCALED;
   using X = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
@@ -540,7 +543,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_arrive(&q_full[i]);
     }
     // (what expanded codes are over)
-    const float* units = !CODES && TERMS == 1 && a.units ? a.units + ((long long)z * a.kv_heads + head) * 2 : nullptr;
+    const float* units = !CODES && a.units ? a.units + ((long long)z * a.kv_heads + head) * 2 : nullptr;
     const float key_unit = units ? units[0] : 1.0f, value_unit = units ? units[1] : 1.0f;
     // (a softcap leaves natural units behind)
     // (and a factor of 2^-60 is as good as none; times a tile's power it is normal)
@@ -578,6 +581,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
+      float held_k[2], held_v[2];
+      if constexpr (SCALED) {
+        static_assert(!SCALED || KEYS == 64, "two scales a lane");
+        const long long at = ((long long)z * a.kv_heads + head) * a.at.table_stride * a.at.page_size + seen.key_of(tile0 + j) + lane;
+        held_k[0] = a.key_scales[at], held_k[1] = a.key_scales[at + 32];
+        held_v[0] = a.value_scales[at], held_v[1] = a.value_scales[at + 32];
+      }
       if (!(ok = wait(&s_full[b], MT == 2 ? j & 1 : (j >> 1) & 1))) break;
       // P and O are free (and O complete) when the last tile's P V is done
       auto settled = [&]() {
@@ -608,12 +618,19 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::fence_before_sync();
       tc::mbar_arrive(&s_empty[b]);
 
-      const float* k_scales = scales + stage * 2 * KEYS;
-      const float* v_scales = k_scales + KEYS;
+      // (expanded codes' scales: the keys', then the values', in a row of the warp's own)
+      float* warp_scales = reinterpret_cast<float*>(shared + T::WARP_SCALES_AT) + warp * KEYS;
+      const float* k_scales = SCALED ? warp_scales : scales + stage * 2 * KEYS;
+      const float* v_scales = SCALED ? warp_scales : k_scales + KEYS;
+      if constexpr (SCALED) {
+        __syncwarp();
+        warp_scales[lane] = held_k[0], warp_scales[lane + 32] = held_k[1];
+        __syncwarp();
+      }
       const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : key_unit;
       const float tile_m2 = a.softcap > 0.0f ? m2 : m2 * by_unit;
       const float now_unit = CODES ? float(v_unit[stage]) : 0.0f;
-      if constexpr (CODES && TERMS == 2) {
+      if constexpr (SCALED || (CODES && TERMS == 2)) {
 #pragma unroll
         for (int c = 0; c < KEYS; c += 4) {
           const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
@@ -640,6 +657,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll
           for (int c = 0; c < KEYS; ++c) s[c] = a.softcap * capped_near(s[c] * inverse);
         }
+      }
+      if constexpr (SCALED) {
+        __syncwarp();
+        warp_scales[lane] = held_v[0], warp_scales[lane + 32] = held_v[1];
+        __syncwarp();
       }
       const bool edge = !(key0 + KEYS <= all_end && (key0 >= all_low || key0 + KEYS <= first));
       if (edge) {
@@ -700,7 +722,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           float2 w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
           w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
           part = add2(part, w);
-          if constexpr (CODES && TERMS == 2) {
+          if constexpr (SCALED || (CODES && TERMS == 2)) {
             w = mul2(w, *reinterpret_cast<const float2*>(v_scales + 2 * e));
             if (edge) {  // (a hidden value's scale may be a NaN)
               w.x = s[2 * e] == -INFINITY ? 0.0f : w.x;
@@ -1232,9 +1254,9 @@ constexpr int tile_of(int head_dim, int terms) {
   return terms == 2 || head_dim > 128 ? 64 : head_dim > 80 ? 80 : head_dim > 64 ? 96 : 128;
 }
 
-template <int D, int MT, bool CODES, int TERMS>
+template <int D, int MT, bool CODES, int TERMS, bool SCALED>
 int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
-  using T = TileTraits<D, tile_of(D, TERMS), MT, CODES, TERMS>;
+  using T = TileTraits<D, tile_of(D, TERMS), MT, CODES, TERMS, SCALED>;
   TileArgs args;
   args.a = a;
   const int ps = a.at.page_size;
@@ -1274,20 +1296,24 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
 
 template <int D, int MT>
 int launch_types(const AttentionChunksArgs& a, bool codes, bool bf16, cudaStream_t stream) {
-  if (bf16) return codes ? launch_tiles<D, MT, true, 1>(a, stream) : launch_tiles<D, MT, false, 1>(a, stream);
-  if constexpr (D <= 128) return codes ? launch_tiles<D, MT, true, 2>(a, stream) : launch_tiles<D, MT, false, 2>(a, stream);
+  if (bf16) return codes ? launch_tiles<D, MT, true, 1, false>(a, stream) : launch_tiles<D, MT, false, 1, false>(a, stream);
+  if constexpr (D <= 128) {
+    if (codes) return launch_tiles<D, MT, true, 2, false>(a, stream);
+    return a.units ? launch_tiles<D, MT, false, 2, true>(a, stream) : launch_tiles<D, MT, false, 2, false>(a, stream);
+  }
   else return invalid("attention: no F32 tiles for heads of %d", D);
 }
 
-#define DRIFT_TILES_REGISTER_AS(D, MT, codes, terms, name) \
-  DRIFT_REGISTER(name, (attention_tiles_kernel<TileTraits<D, tile_of(D, terms), MT, codes, terms>>))
+#define DRIFT_TILES_REGISTER_AS(D, MT, codes, terms, scaled, name) \
+  DRIFT_REGISTER(name, (attention_tiles_kernel<TileTraits<D, tile_of(D, terms), MT, codes, terms, scaled>>))
 #define DRIFT_TILES_REGISTER_BF16(D, MT)                                            \
-  DRIFT_TILES_REGISTER_AS(D, MT, false, 1, attention_tiles_f16_bf16_d##D##_m##MT)    \
-  DRIFT_TILES_REGISTER_AS(D, MT, true, 1, attention_tiles_i8_bf16_d##D##_m##MT)
+  DRIFT_TILES_REGISTER_AS(D, MT, false, 1, false, attention_tiles_f16_bf16_d##D##_m##MT)    \
+  DRIFT_TILES_REGISTER_AS(D, MT, true, 1, false, attention_tiles_i8_bf16_d##D##_m##MT)
 #define DRIFT_TILES_REGISTER(D, MT)                                                 \
   DRIFT_TILES_REGISTER_BF16(D, MT)                                                  \
-  DRIFT_TILES_REGISTER_AS(D, MT, false, 2, attention_tiles_f16_f32_d##D##_m##MT)     \
-  DRIFT_TILES_REGISTER_AS(D, MT, true, 2, attention_tiles_i8_f32_d##D##_m##MT)
+  DRIFT_TILES_REGISTER_AS(D, MT, false, 2, false, attention_tiles_f16_f32_d##D##_m##MT)     \
+  DRIFT_TILES_REGISTER_AS(D, MT, true, 2, false, attention_tiles_i8_f32_d##D##_m##MT)  \
+  DRIFT_TILES_REGISTER_AS(D, MT, false, 2, true, attention_tiles_expanded_f32_d##D##_m##MT)
 DRIFT_TILES_REGISTER(64, 1)
 DRIFT_TILES_REGISTER(64, 2)
 DRIFT_TILES_REGISTER(80, 1)

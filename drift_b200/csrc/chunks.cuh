@@ -56,7 +56,7 @@ struct AttentionChunksArgs {
   void* out;
   const void* keys;
   const void* values;
-  const float* key_scales;    // 8-bit caches
+  const float* key_scales;    // 8-bit caches (expanded: [batch][kv_heads][positions], F32 rows)
   const float* value_scales;
   const float* units;         // [batch][kv_heads][2]: what keys and values are over (attention_expand), or null
   const float* sinks;
@@ -150,8 +150,8 @@ int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_
 // attention_expand.cu: an 8-bit cache's keys and values of the chunks as F16 in
 // `memory` (16-byte aligned, expanded_bytes), which then take the cache's place
 // in `a`.
-size_t expanded_bytes(int batch, int kv_heads, int head_dim, int page_size, int max_key_count);
-int launch_attention_expand(AttentionChunksArgs& a, int head_dim, void* memory, cudaStream_t stream);
+size_t expanded_bytes(int x_dtype, int batch, int kv_heads, int head_dim, int page_size, int max_key_count);
+int launch_attention_expand(AttentionChunksArgs& a, int x_dtype, int head_dim, void* memory, cudaStream_t stream);
 // Joins the splits (attention_rows.cu).
 int launch_attention_join(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                           int keys_per_tile, cudaStream_t stream);

@@ -628,8 +628,8 @@ class CudaOps:
         (F32 or BF16), over its positions in a KvCache or a QuantizedKvCache,
         the new ones included (written before): a decoding step, drafted
         tokens, prompts or pieces of them, of different lengths in one call.
-        out may be q. Partial results (and, for BF16 rows over an 8-bit cache,
-        its keys and values as F16) are in device memory of up to a GiB that is
+        out may be q. Partial results (and, for many rows over an 8-bit cache,
+        its keys and values as F16, up to a GiB) are in device memory that is
         the call's own.
         With a window, the first `attention.first` positions stay visible."""
         x_dtype = self._chunk_rows("attention", q, out, cache, chunks)

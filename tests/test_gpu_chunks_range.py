@@ -144,6 +144,52 @@ def test_hidden_positions_in_wide_chunks(ops, tokens, kind, quantized):
     assert torch.equal(out, clean)
 
 
+@KINDS
+@pytest.mark.parametrize("size", [-110, -40, 90])
+def test_small_and_large_scales(ops, size, kind):
+    """All of a cache's scales around 2^size (the keys' smaller by as much as
+    keeps scores ordinary), for few rows, tiles, and codes expanded first."""
+    for tokens in (1, 6, 60, 500):
+        new, counts, tables, page_size, cache, q, spec = attention_case(
+            ([tokens], [tokens + 150], 8, 2, 64, 16, 100, 3, None, False, True), kind, True)
+        cache.value_scales.mul_(2.0 ** size)
+        if size < 0:
+            cache.key_scales.mul_(2.0 ** size)
+        out = torch.empty_like(q)
+        ops.attention_chunks(q, cache, plain.chunks_of(new, counts, tables, page_size), spec, out)
+        held(out, *plain.attention(q, cache, tables, new, counts, spec))
+
+
+@KINDS
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+def test_expanded_codes(ops, dim, kind):
+    """Many units of rows over an 8-bit cache: a window, tokens that are not
+    finite for those that see them, bad pages, other bounds."""
+    for new, counts, window, first, softcap in (([700, 5, 0, 333], [1100, 500, 40, 333], 0, 0, 20.0),
+                                                ([700, 5, 0, 333], [1100, 500, 40, 333], 120, 6, None)):
+        case = (new, counts, 8, 2, dim, 48, window, first, softcap, True, True)
+        checked(ops, case, kind, True)
+        checked(ops, case, kind, True, longest=1000, max_keys=1104)
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        ([900], [1400], 8, 2, dim, 16, 0, 0, None, False, True), kind, True)
+    chunks = plain.chunks_of(new, counts, tables, page_size)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    ops.attention_chunks(q, cache, chunks, spec, clean)
+    cache.value_scales[int(tables[0][1000 // 16]), 1, 1000 % 16] = math.nan  # rows 500 and later see it
+    ops.attention_chunks(q, cache, chunks, spec, out)
+    assert torch.equal(out[:, :4], clean[:, :4]) and out[500:, 4:].isnan().all()
+    expected, tolerance = plain.attention(q[:500], cache, tables, [500], [1000], spec)
+    held(out[:500], expected, tolerance)
+    broken = tables.copy()
+    broken[0, 3] = cache.pages
+    ops.attention_chunks(q, cache, plain.chunks_of(new, counts, broken, page_size), spec, out)
+    assert ops.take_device_error() == 1
+    zeroed = type(cache)(*[torch.cat((t, torch.zeros_like(t[:1]))) for t in
+                           (cache.keys, cache.values, cache.key_scales, cache.value_scales)], page_size)
+    expected, tolerance = plain.attention(q[:500], zeroed, broken, [500], [1000], spec)
+    held(out[:500], expected, tolerance)
+
+
 @CACHES
 @pytest.mark.parametrize("tokens", [1, 5, 40])
 def test_shared_pages(ops, tokens, quantized):
