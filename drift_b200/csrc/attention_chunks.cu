@@ -12,6 +12,8 @@ namespace drift {
 
 namespace {
 
+constexpr size_t EXPANDED_MOST = size_t(1) << 30;  // bytes
+
 struct Plan {
   int row_tiles;        // attention_tiles' row tiles (0: attention_rows or attention_codes)
   int rows_per_unit;    // rows of a key head that a CTA takes
@@ -70,11 +72,14 @@ Plan plan_rows(const Call& c) {
 // and tiles): F16 caches BF16 8 rows 35 and 43, 12 rows 54 and 44; F32 38 and
 // 57, 12 rows 59 and 59. 8-bit ones BF16 32 rows 61 and 75, 40 rows 80 and 77
 // (heads of 256: 24 rows 95 and 105, 32 rows 123 and 107); F32 40 rows 100 and
-// 130, and of one sequence 22 and 24, but 48 rows 31 and 24.
+// 130, and of one sequence 22 and 24, but 48 rows 31 and 24. F32 heads of 256
+// (8 x 2 key heads): F16 16 rows 35 and 43, 24 rows 46 and 45; 8-bit 64 rows 78
+// and 83, 128 rows 133 and 82.
 bool takes_tiles(const Call& c, long long rows) {
   const bool bf16 = c.x_dtype == DRIFT_BF16;
-  if (!bf16 && c.head_dim > 128) return false;
-  return rows > (c.cache_dtype == DRIFT_F16 ? 8 : !bf16 ? 40 : c.head_dim > 128 ? 24 : 32);
+  const bool wide = c.head_dim > 128;
+  if (c.cache_dtype == DRIFT_F16) return rows > (wide && !bf16 ? 16 : 8);
+  return rows > (bf16 ? (wide ? 24 : 32) : wide ? 64 : 40);
 }
 
 // Two row tiles to a CTA or one, and how many splits: what ends first by a model
@@ -89,7 +94,7 @@ Plan plan_tiles(const Call& c, double slower, double& least) {
   constexpr double CTA_NS = 9000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 1700;
   const bool bf16 = c.x_dtype == DRIFT_BF16;
   const double key_ns = bf16 ? (c.head_dim > 128 ? 20 : c.head_dim > 64 ? 7.7 : 6.5) * slower
-                             : (c.head_dim > 64 ? 14.5 : 10) * slower;
+                             : (c.head_dim > 128 ? 35 : c.head_dim > 64 ? 14.5 : 10) * slower;
   const long long rows = (long long)c.longest * c.group;
   Plan best;
   least = -1;
@@ -99,7 +104,8 @@ Plan plan_tiles(const Call& c, double slower, double& least) {
     p.expands = false;
     p.rows_per_unit = 128 * row_tiles;
     p.keys_per_tile = attention_tiles_keys(c.head_dim, bf16);
-    const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads;
+    // (F32 rows of heads of 256 have two CTAs)
+    const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads * (!bf16 && c.head_dim > 128 ? 2 : 1);
     const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
     const double tile_ns = p.keys_per_tile * key_ns * (row_tiles == 2 ? 2.0 : c.head_dim > 128 ? 1.0 : 1.6);
     const double cta_ns = row_tiles == 2 ? CTA_NS : 0.7 * CTA_NS;
@@ -140,13 +146,14 @@ Plan plan_all_tiles(const Call& c) {
   const bool bf16 = c.x_dtype == DRIFT_BF16;
   if (c.cache_dtype != DRIFT_I8) return plan_tiles(c, 1.0, own);
   const Plan p = plan_tiles(c, bf16 ? 2.2 : 2.5, own);
-  if (expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > (size_t(1) << 30)) return p;
+  if (expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > EXPANDED_MOST) return p;
   const long long seen = c.window > 0 ? std::min((long long)c.max_key_count, (long long)c.window + c.longest + c.first) : c.max_key_count;
   double expanded;
   Plan q = plan_tiles(c, bf16 ? 1.0 : 1.4, expanded);
   q.expands = true;
   expanded += LAUNCHES_NS + 6.0 * seen * c.batch * c.kv_heads * c.head_dim / BYTES_A_NS;
-  return expanded < own ? q : p;
+  // (no tiles convert codes for F32 heads of 256)
+  return expanded < own || (!bf16 && c.head_dim > 128) ? q : p;
 }
 
 Plan plan_chunks(const Call& c) {
@@ -154,7 +161,9 @@ Plan plan_chunks(const Call& c) {
   // (the copies' coordinates are 32-bit, the grid's unit axis 16-bit)
   const bool reachable = (long long)c.pages * c.page_size < (1ll << 31) &&
                          (long long)c.pages * c.kv_heads * c.head_dim < (1ll << 31);
-  if (takes_tiles(c, rows) && reachable) {
+  const bool expandable = expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) <= EXPANDED_MOST;
+  const bool has_tiles = c.cache_dtype == DRIFT_F16 || c.x_dtype == DRIFT_BF16 || c.head_dim <= 128 || expandable;
+  if (takes_tiles(c, rows) && reachable && has_tiles) {
     const Plan p = plan_all_tiles(c);
     if ((rows + p.rows_per_unit - 1) / p.rows_per_unit * p.splits <= 65535) return p;
   }
@@ -223,6 +232,10 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
   if (needed > workspace_bytes || (needed && !workspace))
     return invalid("attention: a workspace of %zu bytes, %zu needed", workspace_bytes, needed);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return invalid("attention: the workspace does not start on a 16-byte boundary");
+  // (two CTAs of F32 heads of 256 read the same rows of q)
+  const uintptr_t row_bytes = uintptr_t(tokens) * q_heads * head_dim * (x_dtype == DRIFT_F32 ? 4 : 2);
+  const uintptr_t q_at = reinterpret_cast<uintptr_t>(q), out_at = reinterpret_cast<uintptr_t>(out);
+  if (q_at < out_at + row_bytes && out_at < q_at + row_bytes) return invalid("attention: q and out overlap");
   AttentionChunksArgs a;
   a.at = {starts, positions, page_tables, tokens, table_stride, pages, page_size, batch, longest, max_key_count};
   a.q = q;

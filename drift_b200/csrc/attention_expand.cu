@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandA
 DRIFT_EXPAND_REGISTER(64)
 DRIFT_EXPAND_REGISTER(80)
 DRIFT_EXPAND_REGISTER(128)
-DRIFT_REGISTER(attention_expand_bf16_d256, (attention_expand_kernel<256, false>))
+DRIFT_EXPAND_REGISTER(256)
 DRIFT_REGISTER(attention_units, attention_units_kernel)
 
 template <int D>
@@ -236,14 +236,8 @@ int launch_dim(const ExpandArgs& a, cudaStream_t stream) {
   constexpr int POSITIONS = RUN * runs_of(D);
   const unsigned runs = unsigned(((long long)a.at.max_keys + POSITIONS - 1) / POSITIONS);
   const dim3 grid(runs, a.kv_heads, a.at.batch);
-  if constexpr (D <= 128) {
-    if (a.key_scales32) {
-      DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, true>, grid, THREADS, 0, stream, a));
-      DRIFT_LAUNCHED("attention_expand");
-      return 0;
-    }
-  }
-  DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, false>, grid, THREADS, 0, stream, a));
+  if (a.key_scales32) DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, true>, grid, THREADS, 0, stream, a));
+  else DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, false>, grid, THREADS, 0, stream, a));
   DRIFT_LAUNCHED("attention_expand");
   return 0;
 }

@@ -1,5 +1,4 @@
-// attention_chunks over an F16 cache for few rows: a decoding step, and every
-// chunk in F32 of heads of 256.
+// attention_chunks over an F16 cache for few rows: a decoding step.
 //
 // A unit is a key head of one sequence with up to 8 of the (token, query
 // head) rows that read it; a CTA takes one split of the unit's key tiles,

@@ -45,6 +45,8 @@
 // grows, so a tile's P V starts a new O, and the softmax threads add it to
 // their row's running output in registers.
 //
+// F32 rows of heads of 256 have a CTA for each half of the values' dimensions.
+//
 // MT = 2 (D <= 128) shares a tile's keys and values between two row tiles. MT =
 // 1 (heads of 256, whose outputs fill TMEM, and units of 128 rows) has two S.
 //
@@ -88,6 +90,9 @@ constexpr int Q_BITS = 8;
 template <int D_, int KEYS_, int MT_, bool CODES_, int TERMS_, bool SCALED_>
 struct TileTraits {
   static constexpr int D = D_, KEYS = KEYS_, MT = MT_, TERMS = TERMS_;
+  // F32 rows of heads of 256: a CTA takes 128 of the values' dimensions (a row's
+  // running output is in registers), and both make the weights
+  static constexpr int DV = TERMS == 2 && D > 128 ? 128 : D, PARTS = D / DV;
   static constexpr bool CODES = CODES_, SCALED = SCALED_;  // SCALED: expanded codes of F32 rows
   static constexpr int UNIT = ROW_TILE * MT;
   static constexpr int SOFTMAX_WARPS = 4 * MT;
@@ -116,7 +121,7 @@ struct TileTraits {
   static constexpr int Q_BYTES = PANELS * Q_PANEL;         // one term of one row tile
   static constexpr int K_PANEL = KEYS * 128;
   static constexpr int K_BYTES = PANELS * K_PANEL;
-  static constexpr int V_BYTES = KEYS * D * 2;
+  static constexpr int V_BYTES = KEYS * DV * 2;
   static constexpr int V_STAGE = (V_BYTES + 1023) / 1024 * 1024;
   static constexpr int CODE_BYTES = KEYS * D;              // of one side of a tile
   static constexpr int CODE_STAGE = (CODE_BYTES + 127) / 128 * 128;
@@ -143,10 +148,10 @@ struct TileTraits {
   // TMEM: S of row tile i, or (MT = 1) of every other tile; P and O of row tile i
   static constexpr int S_COLUMNS = (KEYS + 31) / 32 * 32;
   static constexpr int P_COLUMN = S_COLUMNS + KEYS, P_COLUMNS = TERMS * KEYS / 2;
-  static constexpr int O_COLUMN = int(TMEM_COLUMNS) - MT * ((D + 31) / 32 * 32), O_COLUMNS = (D + 31) / 32 * 32;
+  static constexpr int O_COLUMN = int(TMEM_COLUMNS) - MT * ((DV + 31) / 32 * 32), O_COLUMNS = (DV + 31) / 32 * 32;
   static_assert(P_COLUMN + MT * P_COLUMNS <= O_COLUMN, "TMEM");
   static_assert(KEYS % 16 == 0 && KEYS <= 128 && P_COLUMN % 8 == 0, "whole steps");
-  static_assert(TERMS == 1 || (D <= 128 && KEYS == 64), "the running output of a row in registers");
+  static_assert(TERMS == 1 || (DV <= 128 && KEYS == 64), "the running output of a row in registers");
   static_assert(BYTES <= LIMIT, "shared memory");
 };
 
@@ -368,18 +373,18 @@ template <class T>
 __global__ void __launch_bounds__(T::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                        const TileArgs args) {
-  constexpr int D = T::D, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
+  constexpr int D = T::D, DV = T::DV, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
   constexpr bool CODES = T::CODES, SCALED = T::SCALED;
   using X = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
   const AttentionChunksArgs& a = args.a;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int head = blockIdx.x, z = blockIdx.y;
+  const int head = blockIdx.x / T::PARTS, part = blockIdx.x % T::PARTS, z = blockIdx.y;
   // the last rows first: under a causal mask they see the most keys
   const int at = gridDim.z - 1 - blockIdx.z, split = at % a.splits, unit = at / a.splits;
   const Chunk chunk(a.at, z);
-  if (!chunk.ok && head == 0 && blockIdx.z == 0 && tid == 0) chunk_error(a.error);
+  if (!chunk.ok && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) chunk_error(a.error);
   const int row0 = unit * T::UNIT, row1 = min(row0 + T::UNIT, chunk.tokens * a.group);
   if (row0 >= row1) return;
   const int token0 = row0 / a.group, token1 = (row1 - 1) / a.group + 1;
@@ -562,12 +567,12 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 
     float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
     float unit = 0.0f;                    // and, for codes, values are over this
-    float total[TERMS == 2 ? D : 1] = {};  // the running output (F32 rows)
+    float total[TERMS == 2 ? DV : 1] = {};  // the running output (F32 rows)
     // the last tile's output, which the tensor core has left in O
     auto take_output = [&]() {
       if constexpr (TERMS == 2) {
 #pragma unroll
-        for (int c = 0; c < D; c += 16) {
+        for (int c = 0; c < DV; c += 16) {
           float o[16];
           tmem_load_16(o_at + c, o);
 #pragma unroll
@@ -689,10 +694,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         sum *= f;
         if constexpr (TERMS == 2) {
 #pragma unroll
-          for (int c = 0; c < D; ++c) total[c] *= g;
+          for (int c = 0; c < DV; ++c) total[c] *= g;
         } else if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = 0; c < DV; c += 16) {
             float o[16];
             tmem_load_16(o_at + c, o);
 #pragma unroll
@@ -781,24 +786,25 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           scale *= f;
         }
         scale = all_sum != 0.0f ? scale / all_sum : 0.0f;
-      } else if (real) {
+      } else if (real && part == 0) {
         *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, all_sum);
       }
       // PIECE dimensions of every row at a time, through this warp's part of the
       // row tile's q (which no product reads any more): a row to a thread goes
       // in, a row to neighbouring threads comes out
-      constexpr int PIECE = D % 32 == 0 && ROW_TILE * 144 <= TERMS * T::Q_BYTES ? 32 : 16;
+      constexpr int PIECE = DV % 32 == 0 && ROW_TILE * 144 <= TERMS * T::Q_BYTES ? 32 : 16;
       const bool wide = TERMS == 2 || a.part_o;
       const int size = wide ? 4 : 2, pitch = PIECE * size + 16;
       const long long row_bytes = (a.part_o ? (long long)a.splits : 1ll) * D * size;
       uint8_t* out = a.part_o ? reinterpret_cast<uint8_t*>(a.part_o + (long long)split * D) : static_cast<uint8_t*>(a.out);
+      out += part * DV * size;
       uint8_t* stage = shared + i * TERMS * T::Q_BYTES + 32 * (warp % 4) * pitch;
       static_assert(ROW_TILE * (PIECE * 4 + 16) <= TERMS * T::Q_BYTES, "a piece of every row");
       const int lanes_to_row = PIECE * size / 16, at_once = 32 / lanes_to_row;  // 2 to 8, 16 to 4
       const int tile_row0 = row0 + ROW_TILE * i + 32 * (warp % 4);
       const int tile_token0 = tile_row0 / a.group, tile_head0 = tile_row0 % a.group;
 #pragma unroll
-      for (int c = 0; c < D; c += PIECE) {
+      for (int c = 0; c < DV; c += PIECE) {
         float o[PIECE];
         if constexpr (TERMS == 2) {
 #pragma unroll
@@ -823,7 +829,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             } else {
 #pragma unroll
               for (int e = 0; e < PIECE; e += 4) {
-                const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + c + e) * a.at.page_size,
+                const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + part * DV + c + e) * a.at.page_size,
                                             (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
                                             a.at.page_size, key0, end, lo, first);
                 o[e] += y.x, o[e + 1] += y.y, o[e + 2] += y.z, o[e + 3] += y.w;
@@ -877,7 +883,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
       const int place = key % a.at.page_size;
       const int k_row = page * a.at.page_size + (page < a.at.pages ? place : 0);
-      const int v_row = (page * a.kv_heads + (page < a.at.pages ? head : 0)) * D;
+      const int v_row = (page * a.kv_heads + (page < a.at.pages ? head : 0)) * D + part * DV;
       const uint32_t codes = base + T::CODES_AT + stage * 2 * T::CODE_STAGE + lane * run * D;
       // codes come with the scales of their pages' runs (zeros for the others')
       const long long scales_row = ((long long)page * a.kv_heads + head) * a.at.page_size + place;
@@ -921,16 +927,16 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       }
       __syncwarp();
       if (lane < runs)
-        tma_load_2d(CODES ? codes + T::CODE_STAGE : base + T::V_AT + stage * T::V_STAGE + lane * run * D * 2, &value_map,
+        tma_load_2d(CODES ? codes + T::CODE_STAGE : base + T::V_AT + stage * T::V_STAGE + lane * run * DV * 2, &value_map,
                     full, place, v_row);
       if (CODES && lane < runs) copy_scales(a.value_scales, copied_scales + KEYS, full);
       __syncwarp();
     }
   } else if (warp == T::QK_WARP || warp == T::PV_WARP) {
     // ---- tensor core --------------------------------------------------------------------
-    constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, D);
+    constexpr uint32_t qk = tc::instr_desc_f16(ROW_TILE, KEYS), pv = tc::instr_desc_f16(ROW_TILE, DV);
     const int run = CODES ? 16 : args.run;  // keys of a piece of V
-    const uint32_t run_shift = run == 64 ? 2 : run == 32 ? 1 : 0, run_bytes = uint32_t(run) * D * 2;  // 2^shift steps
+    const uint32_t run_shift = run == 64 ? 2 : run == 32 ? 1 : 0, run_bytes = uint32_t(run) * DV * 2;  // 2^shift steps
     int edges_told = 0, edges = 0;
     // (second terms first, while the sums are small)
     auto scores = [&](int j, int i, int b) {
@@ -1214,9 +1220,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           *reinterpret_cast<uint4*>(v + 16 * n) = x;
           // which keys: the run, and the chunk in its row before the swizzle
           // (which exchanges 16-byte chunks by the address bits 7 and up)
-          const int in_run = 16 * n % (run * D * 2), d = in_run / row_bytes;
+          const int in_run = 16 * n % (run * DV * 2), d = in_run / row_bytes;
           const int swizzle = row_bytes == 128 ? d % 8 : row_bytes == 64 ? d / 2 % 4 : d / 4 % 2;
-          const int key = key0 + 16 * n / (run * D * 2) * run + 8 * ((n % chunks) ^ swizzle);
+          const int key = key0 + 16 * n / (run * DV * 2) * run + 8 * ((n % chunks) ^ swizzle);
           for (int e = 0; e < 8; ++e)
             found = found || (key + e < seen.end && (key + e >= lowest || key + e < first));
         }
@@ -1274,7 +1280,7 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
   {
     const uint64_t dims[2] = {uint64_t(ps), uint64_t(a.at.pages) * a.kv_heads * D};
     const uint64_t strides[1] = {uint64_t(ps) * SIZE};
-    const uint32_t box[2] = {uint32_t(args.run), uint32_t(D)};
+    const uint32_t box[2] = {uint32_t(args.run), uint32_t(T::DV)};
     DRIFT_TRY(encode_cache_tiles(&value_map, a.values, CODES, 2, dims, strides, box, CODES ? 0 : 2 * args.run));
   }
   static PerDevice configured;
@@ -1288,7 +1294,7 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
   }
   DRIFT_TRY(ensure_shared_memory(configured, attention_tiles_kernel<T>, T::BYTES));
   const unsigned units = unsigned((a.at.longest * a.group + T::UNIT - 1) / T::UNIT);
-  DRIFT_CUDA(launch_pdl(attention_tiles_kernel<T>, dim3(a.kv_heads, a.at.batch, units * a.splits), T::THREADS, T::BYTES,
+  DRIFT_CUDA(launch_pdl(attention_tiles_kernel<T>, dim3(a.kv_heads * T::PARTS, a.at.batch, units * a.splits), T::THREADS, T::BYTES,
                         stream, key_map, value_map, args));
   DRIFT_LAUNCHED("attention_tiles");
   return 0;
@@ -1297,11 +1303,9 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
 template <int D, int MT>
 int launch_types(const AttentionChunksArgs& a, bool codes, bool bf16, cudaStream_t stream) {
   if (bf16) return codes ? launch_tiles<D, MT, true, 1, false>(a, stream) : launch_tiles<D, MT, false, 1, false>(a, stream);
-  if constexpr (D <= 128) {
-    if (codes) return launch_tiles<D, MT, true, 2, false>(a, stream);
-    return a.units ? launch_tiles<D, MT, false, 2, true>(a, stream) : launch_tiles<D, MT, false, 2, false>(a, stream);
-  }
-  else return invalid("attention: no F32 tiles for heads of %d", D);
+  if (!codes) return a.units ? launch_tiles<D, MT, false, 2, true>(a, stream) : launch_tiles<D, MT, false, 2, false>(a, stream);
+  if constexpr (D <= 128) return launch_tiles<D, MT, true, 2, false>(a, stream);
+  else return invalid("attention: no tiles that convert codes for F32 heads of %d", D);
 }
 
 #define DRIFT_TILES_REGISTER_AS(D, MT, codes, terms, scaled, name) \
@@ -1321,6 +1325,8 @@ DRIFT_TILES_REGISTER(80, 2)
 DRIFT_TILES_REGISTER(128, 1)
 DRIFT_TILES_REGISTER(128, 2)
 DRIFT_TILES_REGISTER_BF16(256, 1)
+DRIFT_TILES_REGISTER_AS(256, 1, false, 2, false, attention_tiles_f16_f32_d256_m1)
+DRIFT_TILES_REGISTER_AS(256, 1, false, 2, true, attention_tiles_expanded_f32_d256_m1)
 
 }  // namespace
 

@@ -142,7 +142,7 @@ constexpr int attention_codes_ctas(int head_dim) { return head_dim > 128 ? 1 : h
 int launch_attention_rows(const AttentionChunksArgs& a, int x_dtype, int head_dim, cudaStream_t stream);
 int launch_attention_codes(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,
                            cudaStream_t stream);
-// attention_tiles.cu (F32 rows: heads up to 128): `row_tiles` tiles of 128 rows
+// attention_tiles.cu: `row_tiles` tiles of 128 rows
 // a unit (1 or 2; 1 for heads of 256), and the keys of one of its tiles.
 int attention_tiles_keys(int head_dim, bool bf16);
 int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int row_tiles,

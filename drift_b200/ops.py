@@ -628,7 +628,7 @@ class CudaOps:
         (F32 or BF16), over its positions in a KvCache or a QuantizedKvCache,
         the new ones included (written before): a decoding step, drafted
         tokens, prompts or pieces of them, of different lengths in one call.
-        out may be q. Partial results (and, for many rows over an 8-bit cache,
+        q and out do not overlap. Partial results (and, for many rows over an 8-bit cache,
         its keys and values as F16, up to a GiB) are in device memory that is
         the call's own.
         With a window, the first `attention.first` positions stay visible."""

@@ -205,16 +205,17 @@ def test_shared_pages(ops, tokens, quantized):
 @CACHES
 @KINDS
 @pytest.mark.parametrize("tokens", [1, 5, 40, 300])
-def test_in_place_and_again(ops, tokens, kind, quantized):
-    """out may be q, and a call repeats bit for bit."""
+def test_again(ops, tokens, kind, quantized):
+    """A call repeats bit for bit, and is refused in place."""
     new, counts, tables, page_size, cache, q, spec = attention_case(
         ([tokens, 1], [tokens + 700, 900], 8, 2, 128, 16, 0, 0, None, False, True), kind, quantized)
     chunks = plain.chunks_of(new, counts, tables, page_size)
     out, again = torch.empty_like(q), torch.empty_like(q)
     ops.attention_chunks(q, cache, chunks, spec, out)
     ops.attention_chunks(q, cache, chunks, spec, again)
-    ops.attention_chunks(q, cache, chunks, spec, q)
-    assert torch.equal(out, again) and torch.equal(out, q)
+    assert torch.equal(out, again)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attention_chunks(q, cache, chunks, spec, q)
 
 
 @CACHES
@@ -305,3 +306,30 @@ def test_writes_of_one_position_at_every_place(ops):
         ops.cache_write_chunks(x, -x, once, plain.chunks_of([64], [64], tables, 32))
         for name in ("keys", "values") + (("key_scales", "value_scales") if quantized else ()):
             assert torch.equal(getattr(cache, name), getattr(once, name))
+
+
+@CACHES
+@pytest.mark.parametrize("tokens", [2, 3, 9, 100, 515])
+def test_f32_heads_of_256(ops, tokens, quantized):
+    """A CTA for each half of a value, with and without splits, windows and
+    values that are not finite."""
+    checked(ops, ([tokens, 1], [tokens + 277, 300], 16, 2, 256, 16, 0, 0, 10.0, True, True), "f32", quantized)
+    checked(ops, ([tokens] * 9, [tokens + 40] * 9, 16, 2, 256, 32, 90, 5, None, False, True), "f32", quantized)
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        ([tokens], [tokens + 99], 16, 2, 256, 16, 0, 0, None, False, True), "f32", quantized)
+    chunks = plain.chunks_of(new, counts, tables, page_size)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    ops.attention_chunks(q, cache, chunks, spec, clean)
+    position = tokens + 97  # the last two tokens' and the last's
+    page, place = int(tables[0][position // page_size]), position % page_size
+    if quantized:
+        cache.value_scales[page, 1, place] = math.nan
+    else:
+        cache.values[page, 1, 200, place] = math.inf
+    ops.attention_chunks(q, cache, chunks, spec, out)
+    assert torch.equal(out[:-2], clean[:-2]) and torch.equal(out[:, :8], clean[:, :8])
+    if quantized:
+        assert out[-2:, 8:].isnan().all()
+    else:
+        assert not out[-2:, 8:, 200].isfinite().any()
+        assert torch.equal(out[-2:, 8:, :200], clean[-2:, 8:, :200])
