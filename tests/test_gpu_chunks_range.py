@@ -333,3 +333,37 @@ def test_f32_heads_of_256(ops, tokens, quantized):
     else:
         assert not out[-2:, 8:, 200].isfinite().any()
         assert torch.equal(out[-2:, 8:, :200], clean[-2:, 8:, :200])
+
+
+@CACHES
+@KINDS
+def test_wide_chunks_captured_and_replayed(ops, kind, quantized):
+    """Chunks of several units (an 8-bit cache's codes expanded in the launch)
+    captured once and replayed at other lengths, positions and pages."""
+    rng = np.random.default_rng(31)
+    q_heads, kv_heads, dim, page_size = 8, 2, 128, 16
+    tables, pages = plain.tables_of(rng, 2, 80)
+    cache = plain.random_cache(rng, quantized, pages, page_size, kv_heads, dim)
+    chunks = plain.chunks_of([500, 500], [500, 1200], tables, page_size, max_keys=1280)
+    q = torch.from_numpy(rng.standard_normal((1000, q_heads, dim)).astype(np.float32)).to(TYPES[kind]).cuda()
+    out = torch.empty_like(q)
+    spec = Attention(1 / math.sqrt(dim), window=300, first=5)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ops.attention_chunks(q, cache, chunks, spec, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ops.attention_chunks(q, cache, chunks, spec, out)
+    for new, counts in (([500, 130], [1280, 131]), ([0, 400], [3, 900]), ([1, 500], [700, 500])):
+        tables = tables[::-1].copy()
+        fresh = plain.chunks_of(new, counts, tables, page_size)
+        for name in ("starts", "positions", "page_tables"):
+            getattr(chunks, name).copy_(getattr(fresh, name))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        n = sum(new)
+        held(out[:n], *plain.attention(q[:n], cache, tables, new, counts, spec))
+        assert (out[n:] == 7.0).all()
+    assert ops.take_device_error() == 0
