@@ -564,7 +564,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int all_low = a.window > 0 ? token_last - a.window + 1 : 0, some_low = a.window > 0 ? token_first - a.window + 1 : 0;
     const uint32_t o_at = tmem + lanes + T::O_COLUMN + i * T::O_COLUMNS, p_at = tmem + lanes + T::P_COLUMN + i * T::P_COLUMNS;
 
-
     float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
     float unit = 0.0f;                    // and, for codes, values are over this
     float total[TERMS == 2 ? DV : 1] = {};  // the running output (F32 rows)

@@ -16,7 +16,7 @@
 // store (32 for F16). Bound by memory, (4 or 2) + 1 bytes a value: 16 x 4096
 // positions of 8 heads of 128 back to BF16 58 us, 5.4 TB/s; 4 x 4099 from BF16
 // 59 us, 2.8 TB/s (a CTA's chain of loads, largest value, codes and turned
-// stores; F32 rows, twice the bytes in, 63 us). Few rows take 3 us, a launch.
+// stores; F32 rows, twice the bytes in, 61 us). Few rows take 3 us, a launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -43,23 +43,37 @@ constexpr int read_heads(int dim) { return dim > 128 ? 2 : 4; }
 // one of it; x - c s is exact in one fused operation (both are multiples of
 // x's or s's last place, and the difference is below s), so comparing twice
 // it with s decides.
-__device__ __noinline__ float quantize_near_tie(float x, float s) {
+__device__ __forceinline__ int quantize(float x, float s) {
   float c = rintf(x / s);
   const float r = fmaf(-c, s, x), twice = 2.0f * r;
   const bool odd = int(c) & 1;
   if (twice > s || (twice == s && odd)) c += 1.0f;
   else if (twice < -s || (twice == -s && odd)) c -= 1.0f;
-  return c;
-}
-// The same by s's reciprocal where that cannot be wrong: x times it is within
-// 127 * 2^-23 < 2^-16 of x / s, so only a product that close to a half between
-// two codes needs the above. (A step so small that its reciprocal is infinite
-// gives NaN here and goes there too.)
-__device__ __forceinline__ int quantize(float x, float s, float reciprocal) {
-  const float t = x * reciprocal;
-  float c = rintf(t);
-  if (!(fabsf(t - c) < 0.4999f)) c = quantize_near_tie(x, s);
   return int(fminf(fmaxf(c, -127.0f), 127.0f));
+}
+__device__ __noinline__ uint32_t quantize_exactly(float x0, float x1, float x2, float x3, float s) {
+  return (uint32_t(quantize(x0, s)) & 255) | (uint32_t(quantize(x1, s)) & 255) << 8 |
+         (uint32_t(quantize(x2, s)) & 255) << 16 | uint32_t(quantize(x3, s)) << 24;
+}
+// Four codes by s's reciprocal where that cannot be wrong: x times it is within
+// 127 * 2^-23 < 2^-16 of x / s, so only a product that close to a half between
+// two codes needs the above, as do steps so small that they lost bits. Added to
+// 1.5 x 2^23 a product rounds to a whole number in the sum's low bits. (With
+// a conversion and a branch a value 4 x 4099 positions of 8 heads of 64 took 62
+// us, 56 so, of 2 heads of 256 30 and 27.)
+__device__ __forceinline__ uint32_t quantize_four(const float (&x)[4], float s, float reciprocal) {
+  constexpr float ZERO = 12582912.0f;
+  uint32_t codes[4];
+  float off = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float sum = fmaf(x[e], reciprocal, ZERO);
+    codes[e] = __float_as_uint(sum);
+    off = fmaxf(off, fabsf(fmaf(x[e], reciprocal, ZERO - sum)));
+  }
+  if (!(s > 0.0f)) return 0;  // a row of zeros, or one without a step
+  if (off >= 0.4999f || s < 7.9e-31f) return quantize_exactly(x[0], x[1], x[2], x[3], s);
+  return __byte_perm(__byte_perm(codes[0], codes[1], 0x0040), __byte_perm(codes[2], codes[3], 0x0040), 0x5410);
 }
 
 template <typename X>
@@ -123,7 +137,7 @@ struct WriteArgs {
 
 // Codes are int8_t or __half (no scale).
 template <int D, typename X, typename Code>
-__global__ void __launch_bounds__(THREADS) cache_write_chunks_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(THREADS, D <= 128 ? 6 : 4) cache_write_chunks_kernel(const WriteArgs a) {
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
   constexpr bool CODES = sizeof(Code) == 1;
@@ -178,11 +192,10 @@ __global__ void __launch_bounds__(THREADS) cache_write_chunks_kernel(const Write
       const int d = 4 * (lane + 32 * j);
       if (d >= D) continue;
       __align__(16) Code codes[4];
+      if constexpr (CODES) *reinterpret_cast<uint32_t*>(codes) = quantize_four(x[i][j], scale, reciprocal);
+      else
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (CODES) codes[e] = int8_t(scale > 0.0f ? quantize(x[i][j][e], scale, reciprocal) : 0);
-        else codes[e] = __float2half_rn(x[i][j][e]);
-      }
+        for (int e = 0; e < 4; ++e) codes[e] = __float2half_rn(x[i][j][e]);
       Code* to = i < 2 ? static_cast<Code*>(a.keys) +
                              ((run.page * a.at.page_size + run.offset + p) * a.kv_heads + head) * D + d
                        : &turned[p][d];
