@@ -215,7 +215,8 @@ def _require(condition: bool, message: str) -> None:
 
 
 def _check_cache(name: str, keys, values, page_size: int, dtype) -> None:
-    """A paged cache's two sides."""
+    """A paged cache's two sides (kernels get their addresses alone: codes of
+    a QuantizedKvCache read as F16 would be half of what is read)."""
     shape = keys.shape
     if len(shape) != 4 or shape[1] != page_size or \
             values.shape != (shape[0], shape[2], shape[3], page_size):
@@ -446,6 +447,7 @@ class CudaOps:
         """k, v [tokens, kv_heads, D] into the cache at positions start..
         (AttentionOps.scala:58-64; checks L225-257)."""
         _f32("cacheWrite", k, v)
+        _check_cache("cacheWrite", cache.keys, cache.values, cache.page_size, torch.float16)
         _require(k.shape == v.shape and k.dim() == 3 and
                  tuple(k.shape[1:]) == (cache.kv_heads, cache.head_dim),
                  f"cacheWrite: {list(k.shape)} into a cache of {cache.kv_heads} heads of "
@@ -464,6 +466,7 @@ class CudaOps:
         positions (AttentionOps.scala:113-121; checks L259-294)."""
         _f32("attention", q, out)
         _same_shape("attention", q, out)
+        _check_cache("attention", cache.keys, cache.values, cache.page_size, torch.float16)
         _require(q.dim() == 3 and q.shape[2] == cache.head_dim,
                  f"attention: queries {list(q.shape)} against heads of {cache.head_dim}")
         _require(page_table.dtype == torch.int32 and page_table.dim() == 1,
@@ -493,6 +496,7 @@ class CudaOps:
         [b]; page_tables I32 [b, pages per sequence]."""
         _f32("attentionInputs", q, k, v, q_out)
         _same_shape("attentionInputs", k, v)
+        _check_cache("attentionInputs", cache.keys, cache.values, cache.page_size, torch.float16)
         split = q.shape[-1] == 2 * q_out.shape[-1]
         _require(split or tuple(q.shape) == tuple(q_out.shape),
                  f"attentionInputs: q {list(q.shape)} for out {list(q_out.shape)}")
@@ -524,6 +528,7 @@ class CudaOps:
         with `prepared`, the records of out as [b, q_heads D] too."""
         _f32("attention", q, out)
         _same_shape("attention", q, out)
+        _check_cache("attention", cache.keys, cache.values, cache.page_size, torch.float16)
         b, q_heads, dim = q.shape
         _require(dim == cache.head_dim,
                  f"attention: queries {list(q.shape)} against heads of {cache.head_dim}")

@@ -1,0 +1,45 @@
+"""What the chunk operators' 8-bit cache and its neighbours refuse, and the
+accuracy that they keep where weights, scales and bounds are far apart."""
+
+import pytest
+import torch
+
+from drift_b200.ops import Attention, CudaOps, KvCache, QuantizedKvCache, Rope
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return CudaOps()
+
+
+# ---- caches ---------------------------------------------------------------------
+
+def test_the_f16_calls_refuse_an_8_bit_cache(ops):
+    """cache_write, attention and the decode step's two calls read and write
+    F16 values: an 8-bit cache's buffers are half as long."""
+    zeros = lambda *s, **k: torch.zeros(*s, device="cuda", **k)  # noqa: E731
+    codes = QuantizedKvCache.allocate(4, 16, 2, 64)
+    halves = KvCache.allocate(4, 16, 2, 64)
+    floats = KvCache(halves.keys.float(), halves.values.float(), 16)
+    turned = KvCache(halves.keys, halves.keys, 16)
+    k, q, norm = zeros(1, 2, 64), zeros(1, 4, 64), zeros(64)
+    table, positions = zeros(4, dtype=torch.int32), zeros(1, dtype=torch.int32)
+    spec, rope = Attention(0.125), Rope(10000.0, 64, 0)
+    calls = [
+        ("cacheWrite", lambda cache: ops.cache_write(k, k, cache, table, 0)),
+        ("attention", lambda cache: ops.attention(q, cache, table, 0, 1, spec, q.clone())),
+        ("attentionInputs", lambda cache: ops.attention_inputs_decode(
+            q, k, k, norm, norm, 1e-6, positions, rope, q.clone(), cache, table[None])),
+        ("attention", lambda cache: ops.attention_decode(q, cache, table[None], positions, 64, spec, q.clone())),
+    ]
+    for name, call in calls:
+        for cache in (codes, floats):
+            with pytest.raises(ValueError, match=f"{name}: the cache is contiguous device memory, torch.float16"):
+                call(cache)
+        with pytest.raises(ValueError, match=f"{name}: a cache of keys"):
+            call(turned)
+        call(halves)
+    assert ops.take_device_error() == 0
+    assert not codes.keys.any() and not codes.values.any()
