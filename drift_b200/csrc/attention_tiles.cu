@@ -555,7 +555,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 8.7e-19f);
     const int position = chunk.position + token;
     const int hi = a.causal ? position + 1 : seen.end;
-    const int lo = a.window > 0 ? position - a.window + 1 : 0;
+    // (not below 0: a window of no limit less a key's position is past 32 bits)
+    const int lo = a.window > 0 ? max(position - a.window + 1, 0) : 0;
     // what all of this warp's rows see (from `all_low` to `all_end`, and below
     // `first`), and what some row sees
     const int warp_row0 = row0 + ROW_TILE * i + 32 * (warp % 4), warp_row1 = min(warp_row0 + 32, row1);

@@ -1,12 +1,19 @@
 """What the chunk operators' 8-bit cache and its neighbours refuse, and the
 accuracy that they keep where weights, scales and bounds are far apart."""
 
+import math
+
 import pytest
 import torch
 
 from drift_b200.ops import Attention, CudaOps, KvCache, QuantizedKvCache, Rope
+from tests import chunks as plain
+from tests.test_gpu_chunks import attention_case, held
 
 pytestmark = pytest.mark.gpu
+
+CACHES = pytest.mark.parametrize("quantized", [True, False], ids=["i8", "f16"])
+KINDS = pytest.mark.parametrize("kind", ["f32", "bf16"])
 
 
 @pytest.fixture(scope="module")
@@ -43,3 +50,23 @@ def test_the_f16_calls_refuse_an_8_bit_cache(ops):
         call(halves)
     assert ops.take_device_error() == 0
     assert not codes.keys.any() and not codes.values.any()
+
+
+# ---- bounds ---------------------------------------------------------------------
+
+@CACHES
+@KINDS
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("tokens", [1, 5, 60, 300])
+def test_a_window_of_no_limit(ops, tokens, causal, kind, quantized):
+    """The largest window that an int holds is no window, for few rows and
+    many, and so is one of the positions that there are."""
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        ([tokens, 1], [tokens + 211, 130], 8, 2, 64, 16, 0, 0, None, False, causal), kind, quantized)
+    chunks = plain.chunks_of(new, counts, tables, page_size)
+    for window in (2 ** 31 - 1, 2 ** 31 - 2 - tokens, tokens + 211):
+        for first in (0, 7):
+            out = torch.full_like(q, 7.0)
+            wide = Attention(1 / math.sqrt(64), causal, window, first=first)
+            ops.attention_chunks(q, cache, chunks, wide, out)
+            held(out, *plain.attention(q, cache, tables, new, counts, spec))
