@@ -226,7 +226,8 @@ int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_hea
                   window, first, pages, page_size};
   const Plan p = plan_chunks(c);
   const long long units = ((long long)longest * group + p.rows_per_unit - 1) / p.rows_per_unit;
-  if (units * p.splits > 0x7fffffffll || (long long)longest * q_heads > 0x7fffffffll)
+  // (the kernels count rows of whole units in 32 bits)
+  if (units * p.splits > 0x7fffffffll || (long long)longest * q_heads > 0x7fffffffll - 1024)
     return invalid("attention: chunks of %d tokens of %d heads", longest, q_heads);
   const size_t parts = parts_bytes(p, tokens, q_heads, head_dim), needed = workspace_bytes_of(p, c, tokens, q_heads);
   if (needed > workspace_bytes || (needed && !workspace))

@@ -113,3 +113,12 @@ def test_workspace_bytes(lib):
     assert size(window=16) < size()         # a window bounds the splits
     # a split's partial row: the output, the largest score and the sum
     assert size() % (8 * 32 * (128 + 2) * 4) == 0
+
+
+def test_rows_past_32_bits_are_refused(lib):
+    """`longest` bounds a launch's rows: sixteen heads of 2^27 - 1 tokens fit in
+    31 bits, but not with the rest of their last unit."""
+    for longest in (2 ** 27 - 1, 2 ** 27):
+        for cache_dtype in (I8, F16):
+            refused(attention_call(lib, longest=longest, max_keys=2 ** 27, stride=2 ** 23, q_heads=16, kv_heads=1, batch=1,
+                                   cache_dtype=cache_dtype, out=AT + (1 << 20)), f"chunks of {longest} tokens of 16 heads")
