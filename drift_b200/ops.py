@@ -165,6 +165,9 @@ class Chunks:
                  and self.page_tables.dim() == 2 and self.page_tables.shape[0] == batch,
                  f"chunks: starts {list(self.starts.shape)}, page tables "
                  f"{list(self.page_tables.shape)} for {batch} sequences")
+        # (as 32-bit arguments they would wrap)
+        _require(0 <= self.longest < 2 ** 31 and 0 <= self.max_key_count < 2 ** 31,
+                 f"chunks: {self.longest} tokens of one sequence, {self.max_key_count} positions at most")
 
 
 @dataclass
@@ -647,6 +650,8 @@ class CudaOps:
             _require(tuple(sinks.shape) == (q_heads,) and sinks.device == q.device,
                      f"attention: sinks {list(sinks.shape)} for {q_heads} heads")
         window, causal = attention.window or 0, int(attention.causal)
+        if not (0 <= window < 2 ** 31 and 0 <= attention.first < 2 ** 31):
+            raise ValueError(f"attention: a window of {window} with {attention.first} first keys")
         chunk_args = self._chunk_args(chunks)
         size = self._chunks_workspace(
             q.device.index, x_dtype, tokens, q_heads, kv_heads, dim, dtype, pages, page_size, chunk_args[4],

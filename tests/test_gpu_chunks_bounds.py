@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from drift_b200.ops import Attention, CudaOps, KvCache, QuantizedKvCache, Rope
+from drift_b200.ops import Attention, Chunks, CudaOps, KvCache, QuantizedKvCache, Rope
 from tests import chunks as plain
 from tests.test_gpu_chunks import attention_case, held
 
@@ -70,3 +70,19 @@ def test_a_window_of_no_limit(ops, tokens, causal, kind, quantized):
             wide = Attention(1 / math.sqrt(64), causal, window, first=first)
             ops.attention_chunks(q, cache, chunks, wide, out)
             held(out, *plain.attention(q, cache, tables, new, counts, spec))
+
+
+def test_bounds_past_32_bits_are_refused(ops):
+    """2^32 + 5 is not a window of 5."""
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        ([3], [30], 8, 2, 64, 16, 0, 0, None, False, True), "f32", True)
+    chunks = plain.chunks_of(new, counts, tables, page_size)
+    out = torch.full_like(q, 7.0)
+    for changes in (dict(window=2 ** 32 + 5), dict(window=2 ** 31), dict(window=-1), dict(window=5, first=2 ** 32),
+                    dict(window=5, first=-2 ** 32)):
+        with pytest.raises(ValueError, match="a window of"):
+            ops.attention_chunks(q, cache, chunks, Attention(0.125, **changes), out)
+    for longest, max_keys in ((2 ** 32 + 3, 30), (3, 2 ** 32 + 30), (-1, 30), (3, -1)):
+        with pytest.raises(ValueError, match="of one sequence"):
+            Chunks(chunks.starts, chunks.positions, chunks.page_tables, longest, max_keys)
+    assert (out == 7.0).all()
