@@ -14,10 +14,17 @@
 // (bytes of (x + 0x808080) ^ 0x808080), a column for each row and digit. The
 // sums are exact; they start from the bits of 1.5 x 2^23, so that they are F32
 // numbers without a conversion (|sum| < 2^22), and their digits are joined in
-// F32. q has 30 bits (F32) or 15 (BF16) below its row's largest value, a
-// weight 2^26 steps below its row's base (BF16 rows of more than four: 2^18).
-// A key's scale multiplies its score, a value's its weight, over a power of
-// two at or above every scale so far.
+// F32. A key's scale multiplies its score, a value's its weight.
+//
+// What the conversion rounds: q to 2^-30 (F32) or 2^-14 (BF16) of its row's
+// largest value; a row's 32 products of weight and value scale in a tile to
+// 2^-30 of the largest of them (BF16 rows of more than four: 2^-22), each row
+// and tile over a power of two of its own. So a row does not depend on what it
+// does not see, a key of much weight costs no other tile's keys bits, and in
+// its own none if its value is small (a row's largest code is 127, so its scale
+// is its size). Steps of the warp's largest weight instead lost a tenth of the
+// result where one of 16384 keys has ten times the weight of the others and a
+// value of zero.
 //
 // Softmax in F32, a base and a sum a row and warp; the base moves when some
 // weight passes 2^3 (and one vote a tile tells). The warps meet in shared
@@ -47,6 +54,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ZERO = 0x4b400000;  // the bits of 1.5 x 2^23
 constexpr float ZERO_VALUE = 12582912.0f;
 constexpr float GROWTH = 8.0f;    // a weight that moves its base
+constexpr int UNIT_GROWTH = 40 << 23;  // a tile's unit over the output's, in exponent bits, that moves the latter
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -74,6 +82,13 @@ __device__ __forceinline__ uint32_t digit_of(const uint4& x, uint32_t digit) {
   return __byte_perm(__byte_perm(x.x, x.y, pick), __byte_perm(x.z, x.w, pick), 0x5410);
 }
 
+// The larger, a NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+
 __device__ __forceinline__ float weight_of(float score, float base) {
   return score == -INFINITY ? 0.0f : exp2f((score - base) * LOG2E);
 }
@@ -97,7 +112,7 @@ struct CodesTraits {
   static constexpr int Q_TILES = PACKED ? Q_DIGITS / 2 : Q_DIGITS;
   static constexpr int P_TILES = PACKED ? P_DIGITS / 2 : P_DIGITS;
   static constexpr int Q_BITS = BF16 ? 13 : 29;                  // of the largest value's leading bit
-  static constexpr float P_STEPS = P_DIGITS == 4 ? 67108864.0f : 262144.0f;  // of a weight of 1
+  static constexpr int P_BITS = P_DIGITS == 4 ? 29 : 21;         // the same for a tile's products
   static constexpr int CHUNKS = D / 64, TAIL = D % 64 / 16;      // 16-byte chunks a lane has of a key row; 4 bytes
   static constexpr int STEPS = 2 * CHUNKS + TAIL, WORDS = 4 * CHUNKS + TAIL;
   static constexpr int DM = D / 16;
@@ -286,16 +301,17 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
   const int first = a.window > 0 ? a.first : 0;
   const int all_end = a.causal ? chunk.position + token0 + 1 : seen.end;
   const int all_low = a.window > 0 ? chunk.position + token1 - a.window : 0;
-  const int lowest = a.window > 0 ? chunk.position + token0 - a.window + 1 : 0;  // what some row sees
   const float low_digit = PACKED && t >= 2 ? 256.0f : 1.0f;  // the worth of a packed lane's lower digit
 
   float out[T::DM][4];
-  float base[2], sum[2], v_unit = 0.0f;
+  float base[2], sum[2];
+  int o_unit[2];  // what a row's output is over, a power of two as exponent bits
+  o_unit[0] = o_unit[1] = 1 << 23;
   base[0] = base[1] = -INFINITY;
   sum[0] = sum[1] = 0.0f;
 #pragma unroll
   for (int m = 0; m < T::DM; ++m) out[m][0] = out[m][1] = out[m][2] = out[m][3] = 0.0f;
-  uint32_t* weights = reinterpret_cast<uint32_t*>(shared + T::Q_BYTES) + warp * ROWS * PITCH;
+  float* weights = reinterpret_cast<float*>(shared + T::Q_BYTES) + warp * ROWS * PITCH;
 
   for (; tile < tile1; tile += WARPS) {
     const int key0 = seen.key_of(tile), next = tile + WARPS;
@@ -344,14 +360,11 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
 #pragma unroll
       for (int half = 0; half < 2; ++half) k_scale[m][half] = w.k_scale[m][half], v_scale[m][half] = w.v_scale[m][half];
     if (next < tile1) w.load_keys();  // on their way under the rest of this tile
-    float top_scale = 0.0f;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int key = key0 + 16 * m + g + 8 * half;
-        if (!whole && (key >= seen.end || (key < lowest && key >= first))) v_scale[m][half] = 0.0f;
-        if (v_scale[m][half] <= 3.402823466e38f) top_scale = fmaxf(top_scale, v_scale[m][half]);  // (the finite ones)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float x = s[m][2 * half + e] * multiplier[e] * k_scale[m][half];
@@ -365,9 +378,9 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
           }
       }
     // weights with the bases as they are; where one passes GROWTH (or is a
-    // NaN, or a row has no base yet), or a scale the unit, they move
+    // NaN, or a row has no base yet) they move
     float p[2][4];
-    bool move = top_scale > v_unit;
+    bool move = false;
     auto weigh = [&]() {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -380,16 +393,6 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
     weigh();
     if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-      for (int o = 4; o < 32; o *= 2) top_scale = fmaxf(top_scale, __shfl_xor_sync(0xffffffffu, top_scale, o));
-      float shrink = 1.0f;
-      if (top_scale > v_unit) {
-        const uint32_t bits = __float_as_uint(top_scale);
-        const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-        const float now = __uint_as_float(max(up, 0x01000000u));  // (its inverse is normal too)
-        shrink = v_unit / now;
-        v_unit = now;
-      }
-#pragma unroll
         for (int e = 0; e < 2; ++e) {
           float top = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
 #pragma unroll
@@ -398,37 +401,79 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
           base[e] = now;
           sum[e] *= f;
 #pragma unroll
-          for (int m = 0; m < T::DM; ++m) out[m][e] *= f * shrink, out[m][e + 2] *= f * shrink;
+          for (int m = 0; m < T::DM; ++m) out[m][e] *= f, out[m][e + 2] *= f;
         }
       weigh();
     }
-    // into digits, [row][key] in shared memory: a product's columns are rows
-    const float v_inverse = v_unit > 0.0f ? 1.0f / v_unit : 0.0f;  // (finite; steps of it may not be)
+    // products of weights and values' scales, [row][key] in shared memory: a
+    // product's columns are rows
     __syncwarp();  // (the tile before is read)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float by = v_scale[m][half] * v_inverse * T::P_STEPS;
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = p[m][2 * half + e];
-            sum[e] += x;
-            // (a hidden value's scale may be a NaN; a NaN that is seen stays in the sum)
-            const float y = x == 0.0f ? 0.0f : x * by;
-            if (!(y <= 2147483520.0f)) sum[e] = __int_as_float(0x7fc00000);
-            if (!PACKED || t < 2) weights[(2 * t + e) * PITCH + 16 * m + g + 8 * half] = digits(__float2int_rn(y));
-          }
-      }
+        for (int e = 0; e < 2; ++e) {
+          const float x = p[m][2 * half + e];
+          sum[e] += x;
+          float y = x * v_scale[m][half];
+          if (!whole && x == 0.0f) y = 0.0f;  // (a hidden value's scale may be a NaN)
+          if (!PACKED || t < 2) weights[(2 * t + e) * PITCH + 16 * m + g + 8 * half] = y;
+        }
     __syncwarp();
+    // a row's largest, the power of two at or below it, and the products as
+    // whole numbers of steps: this lane has eight keys' of row g (packed: g % 4)
+    const float4* from = reinterpret_cast<const float4*>(weights + (PACKED ? g % 4 : g) * PITCH + 8 * t);
+    const float4 y0 = from[0], y1 = from[1];
+    float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+    float top = max_nan(max_nan(max_nan(y[0], y[1]), max_nan(y[2], y[3])), max_nan(max_nan(y[4], y[5]), max_nan(y[6], y[7])));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    int tile_unit = max(__float_as_int(top) & 0x7f800000, 1 << 23);
+    if (tile_unit < 64 << 23) {  // (its inverse times the steps would be past F32's range)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= 18446744073709551616.0f;
+    }
+    const float steps = __uint_as_float((uint32_t(254 + T::P_BITS) << 23) - uint32_t(tile_unit + (tile_unit < 64 << 23 ? 64 << 23 : 0)));
+    uint4 x0, x1;
+    x0.x = digits(__float2int_rn(y[0] * steps)), x0.y = digits(__float2int_rn(y[1] * steps));
+    x0.z = digits(__float2int_rn(y[2] * steps)), x0.w = digits(__float2int_rn(y[3] * steps));
+    x1.x = digits(__float2int_rn(y[4] * steps)), x1.y = digits(__float2int_rn(y[5] * steps));
+    x1.z = digits(__float2int_rn(y[6] * steps)), x1.w = digits(__float2int_rn(y[7] * steps));
     uint32_t b[T::P_TILES][2];
-    const uint4* from = reinterpret_cast<const uint4*>(weights + (PACKED ? g % 4 : g) * PITCH + 8 * t);
-    const uint4 x = from[0], y = from[1];
 #pragma unroll
     for (int j = 0; j < T::P_TILES; ++j) {
       const uint32_t digit = PACKED ? 2 * j + g / 4 : j;
-      b[j][0] = digit_of(x, digit);
-      b[j][1] = digit_of(y, digit);
+      b[j][0] = digit_of(x0, digit);
+      b[j][1] = digit_of(x1, digit);
+    }
+    // what a step is worth to this lane's columns, over their outputs' units;
+    // a product that is not finite makes its row NaNs
+    float worth[2];
+    {
+      int over[2];
+      bool grown = false;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = PACKED ? (2 * t + e) % 4 : 2 * t + e;
+        over[e] = __shfl_sync(0xffffffffu, tile_unit, 4 * r);
+        if (over[e] == 0x7f800000) sum[e] = __int_as_float(0x7fc00000);
+        over[e] -= o_unit[e];
+        grown = grown || over[e] > UNIT_GROWTH;
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (over[e] <= UNIT_GROWTH) continue;
+          const float f = __int_as_float(max((127 << 23) - over[e], 0));
+          o_unit[e] += over[e];
+          over[e] = 0;
+#pragma unroll
+          for (int m = 0; m < T::DM; ++m) out[m][e] *= f, out[m][e + 2] *= f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) worth[e] = __int_as_float(max(over[e] + ((127 - T::P_BITS) << 23), 0));
     }
 #pragma unroll
     for (int m = 0; m < T::DM; ++m) {
@@ -446,7 +491,7 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
           const float y = __int_as_float(acc[j][e]) - ZERO_VALUE;
           x = j == T::P_TILES - 1 ? y : fmaf(x, PACKED ? 65536.0f : 256.0f, y);
         }
-        out[m][e] += x;
+        out[m][e] = fmaf(x, worth[e % 2], out[m][e]);
       }
     }
     if (next < tile1) {
@@ -459,7 +504,6 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
   __syncthreads();  // (past the fragments and the weights)
   float* merged = reinterpret_cast<float*>(shared);
   float2* stats = reinterpret_cast<float2*>(merged + WARPS * ROWS * D);
-  const float worth = low_digit / T::P_STEPS;  // (and v_unit, which with it may be below F32's range)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float total = sum[e];
@@ -472,7 +516,7 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) attention_codes_kernel(co
       for (int m = 0; m < T::DM; ++m)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float x = out[m][2 * half + e] * worth * v_unit;
+          float x = out[m][2 * half + e] * low_digit * __int_as_float(o_unit[e]);
           if (PACKED) x += __shfl_xor_sync(0xffffffffu, x, 2);
           if (writes) merged[(warp * ROWS + r) * D + 16 * m + g + 8 * half] = x;
         }

@@ -1,0 +1,131 @@
+"""attention_chunks held to what its kernels' roundings allow
+(tests/chunk_accuracy.py): ordinary scores, a key that takes most of the weight
+and has no value, scales far apart, scales that a row's mask hides."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from drift_b200.ops import Attention, CudaOps, KvCache, QuantizedKvCache
+from tests import chunk_accuracy
+from tests import chunks as plain
+from tests.test_gpu_chunks import TYPES, attention_case
+
+pytestmark = pytest.mark.gpu
+
+KINDS = pytest.mark.parametrize("kind", ["f32", "bf16"])
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return CudaOps()
+
+
+def floats(rng, *shape):
+    return torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).cuda()
+
+
+def holds(ops, q, cache, tables, new, counts, spec, **bounds):
+    """Runs the call and holds it to the bound; the result."""
+    out = torch.full_like(q, 7.0)
+    ops.attention_chunks(q, cache, plain.chunks_of(new, counts, tables, cache.page_size, **bounds), spec, out)
+    expected, off = chunk_accuracy.attention(q, cache, tables, new, counts, spec, bounds.get("longest"))
+    error = (out.double() - expected).abs()
+    worst = (error / off).max().item()
+    assert (error <= off).all(), f"{worst:.3g} of the bound, largest error {error.max().item():.3g}"
+    assert ops.take_device_error() == 0
+    return out
+
+
+def written(ops, rng, quantized, k, v, page_size=16):
+    """A cache with k, v [count, kv_heads, D] as one sequence, and its table."""
+    count, kv_heads, dim = k.shape
+    tables, pages = plain.tables_of(rng, 1, -(-count // page_size))
+    cache = (QuantizedKvCache if quantized else KvCache).allocate(pages, page_size, kv_heads, dim)
+    ops.cache_write_chunks(k, v, cache, plain.chunks_of([count], [count], tables, page_size))
+    return cache, tables
+
+
+# (new tokens, positions with them, q heads, kv heads, dim): four rows at most,
+# eight, several units of eight
+FEW = [
+    ([1, 1], [4097, 700], 4, 1, 128),
+    ([1, 1, 1], [2000, 16, 33], 16, 2, 256),
+    ([2, 1], [3001, 5], 16, 4, 64),
+    ([1, 1], [1500, 6000], 16, 1, 128),
+    ([3, 1], [5000, 900], 10, 2, 80),
+    ([5, 4], [2500, 2500], 8, 2, 128),
+]
+
+
+@pytest.mark.parametrize("window,softcap,sinks", [(0, None, False), (300, 20.0, True)], ids=["plain", "window-cap-sinks"])
+@KINDS
+@pytest.mark.parametrize("case", FEW, ids=lambda c: f"{c[0]}of{c[1]}h{c[2]}/{c[3]}d{c[4]}".replace(" ", ""))
+def test_few_rows_over_8_bits(ops, case, kind, window, softcap, sinks):
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        (*case, 16, window, 4 if window else 0, softcap, sinks, True), kind, True)
+    holds(ops, q, cache, tables, new, counts, spec)
+    holds(ops, q * 4, cache, tables, new, counts, spec)  # scores of up to sixteen and more
+
+
+def dominated(ops, rng, kind, quantized, tokens, count, q_heads, kv_heads, dim, rest, spread, value):
+    """One early key that has 1 / `rest` times the weight of all others
+    together, `value` times their values; theirs are of both signs."""
+    group = q_heads // kv_heads
+    along = floats(rng, kv_heads, 1, dim)
+    along = along / along.norm(dim=2, keepdim=True)
+    k, v = floats(rng, count, kv_heads, dim), floats(rng, count, kv_heads, dim)
+    u = along[None, :, 0]
+    k = k - (k * u).sum(2, keepdim=True) * u
+    q = floats(rng, tokens, kv_heads, group, dim) * spread + math.sqrt(dim) * along
+    k[3] = math.log(count * math.exp(spread ** 2 / 2) / rest) * u[0]
+    v[3] *= value
+    cache, tables = written(ops, rng, quantized, k, v)
+    return q.reshape(tokens, q_heads, dim).to(TYPES[kind]), cache, tables
+
+
+@pytest.mark.parametrize("rest,spread", [(0.1, 0.5), (0.5, 1.5)])
+@pytest.mark.parametrize("value", [0.0, 1e-3])
+@pytest.mark.parametrize("count", [500, 16384, 65536])
+@KINDS
+@pytest.mark.parametrize("tokens,heads", [(1, (4, 1)), (1, (16, 2)), (3, (16, 2))], ids=str)
+def test_a_key_of_most_weight_and_no_value_over_8_bits(ops, tokens, heads, kind, count, value, rest, spread):
+    """As an attention sink: what is left of the result is the other keys'
+    small weights, which keep their own bits."""
+    rng = np.random.default_rng(count + tokens)
+    q, cache, tables = dominated(ops, rng, kind, True, tokens, count, *heads, 64, rest, spread, value)
+    holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(64)))
+
+
+@pytest.mark.parametrize("power", [8, 20, 60, 100])
+@KINDS
+@pytest.mark.parametrize("heads", [(4, 2), (8, 2)], ids=str)
+def test_hidden_scales_do_not_reach_earlier_rows_of_few(ops, heads, kind, power):
+    """The last token's value scale is 2^power times the others': the rows
+    before it are what they are without it, bit for bit."""
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        ([2], [258], *heads, 128, 16, 0, 0, None, False, True), kind, True)
+    clean = holds(ops, q, cache, tables, new, counts, spec)
+    page, place = int(tables[0][257 // 16]), 257 % 16
+    cache.value_scales[page, :, place] *= 2.0 ** power
+    out = holds(ops, q, cache, tables, new, counts, spec)
+    assert torch.equal(out[:1], clean[:1])
+
+
+@KINDS
+def test_values_of_far_scales_in_one_tile_of_few_rows(ops, kind):
+    """Scales from 2^-126 to 2^100, among them zeros: a tile's products are in
+    steps of its own largest, whatever other tiles hold."""
+    rng = np.random.default_rng(12)
+    tables, pages = plain.tables_of(rng, 1, 40)
+    cache = plain.random_cache(rng, True, pages, 16, 2, 128)
+    for size in ([-126, -20], [-30, 100], [-110, -100], [95, 100]):
+        spread = rng.uniform(*size, (pages, 2, 16)) if size[1] - size[0] < 50 else np.repeat(
+            rng.uniform(*size, (pages, 2, 1)), 16, 2)
+        cache.value_scales.copy_(torch.from_numpy(np.exp2(spread).astype(np.float32)).cuda())
+        cache.value_scales[int(tables[0][0])] = 0.0
+        q = floats(rng, 2, 8, 128).to(TYPES[kind])
+        for count in (20, 600):
+            holds(ops, q, cache, tables, [2], [count], Attention(1 / math.sqrt(128)))
