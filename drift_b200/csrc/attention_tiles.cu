@@ -80,9 +80,13 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROW_TILE = 128;
 constexpr uint32_t TMEM_COLUMNS = 512;
 // A weight is 2^WEIGHT_BITS at the row's largest score when its base is set,
-// and the base moves when a tile's weights sum to more than MOST_WEIGHT (F32
-// rows: when one would pass 2^(WEIGHT_BITS + GROWTH_BITS)).
-constexpr float WEIGHT_BITS = 8.0f, GROWTH_BITS = 6.0f, MOST_WEIGHT = 32768.0f;
+// and the base moves when a tile's weights sum to more than MOST_WEIGHT. F32
+// rows: 2^WEIGHT_BITS_2, and it moves when one would pass 8 times that; a
+// second term stops at F16's 2^-24, so a weight is off by 2^-37 of the largest
+// (with 2^8 and a growth of 2^6 by 2^-33: 4e-5 of the result where an early
+// key has ten times the weight of 65536 others, and no value).
+constexpr float WEIGHT_BITS = 8.0f, MOST_WEIGHT = 32768.0f;
+constexpr float WEIGHT_BITS_2 = 12.0f, GROWTH_BITS_2 = 3.0f;
 // A row of q is 2^Q_BITS and more at its largest value, so that its second
 // terms end far below F16's last bit, 2^-24.
 constexpr int Q_BITS = 8;
@@ -686,7 +690,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       auto rebase = [&](float top) {
         not_a_number = top != top;
         // (a row without a base takes one; a base that is too high stays)
-        const float now = fmaxf(base2, top - WEIGHT_BITS);
+        const float now = fmaxf(base2, top - (TERMS == 2 ? WEIGHT_BITS_2 : WEIGHT_BITS));
         const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
         const float g = CODES && now_unit > unit ? f * (unit / now_unit) : f;
         if (CODES) unit = fmaxf(unit, now_unit);
@@ -743,7 +747,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         if (!(ok = settled())) break;
         if (j > 0) take_output();
         const float top = largest();
-        const bool grown = !(top <= base2 + (WEIGHT_BITS + GROWTH_BITS)) || (CODES && now_unit > unit);
+        const bool grown = !(top <= base2 + (WEIGHT_BITS_2 + GROWTH_BITS_2)) || (CODES && now_unit > unit);
         if (__any_sync(0xffffffffu, grown)) rebase(top);
         sum += weigh();
       } else {

@@ -43,15 +43,15 @@ def roundings(dtype, quantized, rows, dim):
     `rows` rows of a key head goes to."""
     f32 = dtype == torch.float32
     if not quantized:
-        # two F16 terms, or one; the largest weight is 2^13 or more (tiles: 2^8 for BF16)
+        # two F16 terms, or one; the largest weight is 2^12 or more (BF16: 2^8)
         if f32:
-            return 2.0 ** -21, 2.0 ** -22, 2.0 ** -38, 0.0
+            return 2.0 ** -21, 2.0 ** -22, 2.0 ** -37, 0.0
         return 0.0, 2.0 ** -11, 2.0 ** -33, 0.0
     if rows <= FEW_ROWS[dtype][dim]:
         # whole numbers, of 30 or 14 bits for q, 29 or (BF16, more than four rows) 21 for a product
         return 2.0 ** -29 if f32 else 2.0 ** -13, 0.0, 0.0, 2.0 ** -29 if f32 or rows <= 4 else 2.0 ** -21
     if f32:
-        return 2.0 ** -21, 2.0 ** -22, 2.0 ** -38, 0.0
+        return 2.0 ** -21, 2.0 ** -22, 2.0 ** -37, 0.0
     return 0.0, 2.0 ** -11, 2.0 ** -33, 0.0
 
 

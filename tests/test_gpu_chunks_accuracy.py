@@ -129,3 +129,17 @@ def test_values_of_far_scales_in_one_tile_of_few_rows(ops, kind):
         q = floats(rng, 2, 8, 128).to(TYPES[kind])
         for count in (20, 600):
             holds(ops, q, cache, tables, [2], [count], Attention(1 / math.sqrt(128)))
+
+
+# ---- many rows --------------------------------------------------------------------
+
+@pytest.mark.parametrize("rest,spread", [(0.1, 0.5), (0.5, 1.5)])
+@pytest.mark.parametrize("count", [500, 16384, 65536])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind,quantized", [("f32", True), ("f32", False), ("bf16", False)], ids=["f32-i8", "f32-f16", "bf16-f16"])
+def test_a_key_of_most_weight_and_no_value(ops, dim, count, kind, quantized, rest, spread):
+    """The same for a chunk of 40 tokens and for a step over an F16 cache."""
+    rng = np.random.default_rng(count + dim)
+    for tokens in (40, 1):
+        q, cache, tables = dominated(ops, rng, kind, quantized, tokens, count, 4, 2, dim, rest, spread, 0.0)
+        holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim)))
