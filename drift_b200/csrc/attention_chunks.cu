@@ -90,7 +90,7 @@ bool takes_tiles(const Call& c, long long rows) {
 // share a tile's keys: a row tile by itself takes 1.6 times as long (chunk of
 // 2048 BF16 rows, 8192 keys: 241 us, 414 with one) but keeps all SMs at work
 // where there are few (1500 F32 tokens of 4 x 4 heads: 67 us, 84 with two).
-Plan plan_tiles(const Call& c, double slower, double& least) {
+Plan plan_tiles(const Call& c, bool converts, double slower, double& least) {
   constexpr double CTA_NS = 9000, JOIN_NS = 3000, PARTS_BYTES_A_NS = 1700;
   const bool bf16 = c.x_dtype == DRIFT_BF16;
   const double key_ns = bf16 ? (c.head_dim > 128 ? 20 : c.head_dim > 64 ? 7.7 : 6.5) * slower
@@ -103,7 +103,7 @@ Plan plan_tiles(const Call& c, double slower, double& least) {
     p.row_tiles = row_tiles;
     p.expands = false;
     p.rows_per_unit = 128 * row_tiles;
-    p.keys_per_tile = attention_tiles_keys(c.head_dim, bf16);
+    p.keys_per_tile = attention_tiles_keys(c.head_dim, bf16, converts);
     // (F32 rows of heads of 256 have two CTAs)
     const long long units = (rows + p.rows_per_unit - 1) / p.rows_per_unit * c.batch * c.kv_heads * (!bf16 && c.head_dim > 128 ? 2 : 1);
     const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
@@ -134,24 +134,25 @@ Plan plan_tiles(const Call& c, double slower, double& least) {
   return best;
 }
 
-// The same with the choice of expanding an 8-bit cache's codes: two launches,
-// and 3 bytes a value at about 3 TB/s (three chunks of 1001 BF16 tokens x 4
-// heads over 5003 keys: 230 us, 395 with each unit's own conversion; eight of
-// 40 tokens over 4096: 100, and 94; 2048 F32 tokens over 8192: 592, and 984;
-// 64 over 16384: 99, and 85), in at most 1 GiB. Converting codes makes a tile
+// The same with the choice of expanding an 8-bit cache's codes: two launches
+// more (BF16 rows: three), and 3 bytes a value at about 3 TB/s (three chunks of 1001 BF16 tokens x 4
+// heads over 5003 keys: 290 us, 395 with each unit's own conversion; three of
+// 100 over 2000: 55, and 49; 2048 F32 tokens over 8192: 660, and 1000; 64 over
+// 16384: 109, and 88), in at most 1 GiB. Converting codes makes a tile
 // 2.2 (BF16) and 2.5 times as long, exact codes' scales 1.4 times.
 Plan plan_all_tiles(const Call& c) {
-  constexpr double LAUNCHES_NS = 7000, BYTES_A_NS = 3000;
+  constexpr double BYTES_A_NS = 3000;
   double own;
   const bool bf16 = c.x_dtype == DRIFT_BF16;
-  if (c.cache_dtype != DRIFT_I8) return plan_tiles(c, 1.0, own);
-  const Plan p = plan_tiles(c, bf16 ? 2.2 : 2.5, own);
-  if (expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > EXPANDED_MOST) return p;
+  const double launches_ns = bf16 ? 16000 : 14000;
+  if (c.cache_dtype != DRIFT_I8) return plan_tiles(c, false, 1.0, own);
+  const Plan p = plan_tiles(c, true, bf16 ? 2.2 : 2.5, own);
+  if (expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) > EXPANDED_MOST) return p;
   const long long seen = c.window > 0 ? std::min((long long)c.max_key_count, (long long)c.window + c.longest + c.first) : c.max_key_count;
   double expanded;
-  Plan q = plan_tiles(c, bf16 ? 1.0 : 1.4, expanded);
+  Plan q = plan_tiles(c, false, bf16 ? 1.0 : 1.4, expanded);
   q.expands = true;
-  expanded += LAUNCHES_NS + 6.0 * seen * c.batch * c.kv_heads * c.head_dim / BYTES_A_NS;
+  expanded += launches_ns + 6.0 * seen * c.batch * c.kv_heads * c.head_dim / BYTES_A_NS;
   // (no tiles convert codes for F32 heads of 256)
   return expanded < own || (!bf16 && c.head_dim > 128) ? q : p;
 }
@@ -161,7 +162,7 @@ Plan plan_chunks(const Call& c) {
   // (the copies' coordinates are 32-bit, the grid's unit axis 16-bit)
   const bool reachable = (long long)c.pages * c.page_size < (1ll << 31) &&
                          (long long)c.pages * c.kv_heads * c.head_dim < (1ll << 31);
-  const bool expandable = expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) <= EXPANDED_MOST;
+  const bool expandable = expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) <= EXPANDED_MOST;
   const bool has_tiles = c.cache_dtype == DRIFT_F16 || c.x_dtype == DRIFT_BF16 || c.head_dim <= 128 || expandable;
   if (takes_tiles(c, rows) && reachable && has_tiles) {
     const Plan p = plan_all_tiles(c);
@@ -188,7 +189,7 @@ size_t parts_bytes(const Plan& p, long long tokens, int q_heads, int head_dim) {
 }
 size_t workspace_bytes_of(const Plan& p, const Call& c, long long tokens, int q_heads) {
   return parts_bytes(p, tokens, q_heads, c.head_dim) +
-         (p.expands ? expanded_bytes(c.x_dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) : 0);
+         (p.expands ? expanded_bytes(c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_key_count) : 0);
 }
 
 }  // namespace

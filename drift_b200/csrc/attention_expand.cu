@@ -3,14 +3,17 @@
 // kernel. Its own converting warps make each tile anew for every unit, and
 // bound it (a tile of BF16 rows 5900 clocks, 2700 from an F16 cache).
 //
-//   BF16 rows: keys16, values16 = code scale / unit, rounded to F16
-//   F32 rows:  keys16, values16 = code, exactly; and a row of scales for each
-//              sequence and head, the values' over their unit
+//   BF16 rows: keys16, values16 = code scale / unit, rounded to F16 once
+//   F32 rows:  keys16, values16 = code, exactly; and rows of scales for each
+//              sequence and head, the values' over their unit (by key)
 //
-// with a power of two for each sequence, key head and side: at or above the
-// largest finite scale that a row sees, so that a quotient is at most 127 (508
-// at the ends of F32's range) and is off by 2^-11 of itself, or 2^-25, at most.
-// The tiles multiply scores by the keys' unit and results by the values'.
+// with powers of two for each sequence, key head and side. BF16 rows' are
+// 2^-8 of what the largest scale that a row sees rounds up to, so that a
+// quotient is at most 2^15, and 2^-14 and more for scales down to 2^-22 of that,
+// where F16 has its 11 bits: what a row has of its keys does not depend on the
+// scales beside them. Scales that are farther apart (than 2^20), not finite or at
+// the ends of F32's range go by key as F32 rows' do, at a third more time in the
+// tiles. The tiles multiply scores by the keys' unit and results by the values'.
 //
 // The copies are a paged cache of their own, in the F16 cache's layouts, with
 // sequence z's pages from z * page_row on and the table that says so. Only what
@@ -41,12 +44,13 @@ struct ExpandArgs {
   const float* value_scales;
   __half* keys16;
   __half* values16;
-  float* units;    // [batch][kv_heads][2]
-  float* key_scales32;    // [batch][kv_heads][page_row page_size], F32 rows
+  float4* units;   // [batch][kv_heads]
+  float* key_scales32;    // [batch][kv_heads][page_row page_size]
   float* value_scales32;
   int* table;      // [batch][page_row]
   int* error;
   int kv_heads, page_row, window, first;
+  bool always_by_key;
 };
 
 // What the rows of a chunk see between them: [low, end) and [0, first).
@@ -60,24 +64,27 @@ struct SeenPositions {
   __device__ bool sees(int position) const { return position < end && (position >= low || position < first); }
 };
 
-// A power of two at or above x, `least` (in exponent bits) at least, whose
-// inverse is normal.
-__device__ __forceinline__ float power_over(float x, uint32_t least) {
+// A power of two at or above x whose inverse is normal.
+__device__ __forceinline__ float power_over(float x) {
   const uint32_t bits = __float_as_uint(x);
   const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-  return __uint_as_float(max(up, least));
+  return __uint_as_float(max(up, 0x01000000u));
 }
 
 __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const ExpandArgs a) {
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
-  __shared__ float tops[2][UNIT_THREADS / 32];
+  __shared__ uint32_t ends[4][UNIT_THREADS / 32];
   const int head = blockIdx.x, z = blockIdx.y;
   if (head == 0)
     for (int i = threadIdx.x; i < a.page_row; i += UNIT_THREADS) a.table[(long long)z * a.page_row + i] = z * a.page_row + i;
   const Chunk chunk(a.at, z);
   const SeenPositions seen(a, chunk);
-  float top[2] = {0.0f, 0.0f};
+  // the largest and (upside down) the smallest of either side's, as bits, which
+  // order as numbers do; zeros need none, and of what is no finite positive
+  // number it is enough that there is some
+  uint32_t most[4] = {0, 0, 0, 0};
+  bool odd = false;
   auto look = [&](int from, int to) {
     // four positions of a page to a thread, four times over: two latencies
     // for 16384 positions
@@ -106,8 +113,12 @@ __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const Exp
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const long long p = p0 + 4ll * n * UNIT_THREADS + e;
-            // (the finite ones)
-            if (p >= from && p < to && y[e] <= 3.402823466e38f) top[side] = fmaxf(top[side], y[e]);
+            const uint32_t bits = __float_as_uint(y[e]);
+            if (p < from || p >= to || bits == 0) continue;
+            odd = odd || bits >= 0x7f800000u;
+            if (bits >= 0x7f800000u) continue;
+            most[2 * side] = max(most[2 * side], bits);
+            most[2 * side + 1] = max(most[2 * side + 1], ~bits);
           }
         }
     }
@@ -117,25 +128,31 @@ __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const Exp
     look(seen.low, seen.end);
   }
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
+  for (int i = 0; i < 4; ++i) {
+    most[i] = __reduce_max_sync(0xffffffffu, most[i]);
+    if (threadIdx.x % 32 == 0) ends[i][threadIdx.x / 32] = most[i];
+  }
+  odd = __syncthreads_or(odd);
+  if (threadIdx.x >= 32) return;
+  float top[2];
+  bool by_key = a.always_by_key || odd;
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2) top[side] = fmaxf(top[side], __shfl_xor_sync(0xffffffffu, top[side], o));
-    if (threadIdx.x % 32 == 0) tops[side][threadIdx.x / 32] = top[side];
+  for (int side = 0; side < 2; ++side) {
+    const uint32_t high = __reduce_max_sync(0xffffffffu, ends[2 * side][threadIdx.x]);
+    const uint32_t low = ~__reduce_max_sync(0xffffffffu, ends[2 * side + 1][threadIdx.x]);
+    top[side] = __uint_as_float(high);
+    // (a side without scales is 0 and 2^32 - 1)
+    if (high != 0) by_key = by_key || high - low > 20 << 23 || high > 247 << 23 || high < (side == 0 ? 77 : 27) << 23;
   }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    float most = 0.0f;
-    for (int w = 0; w < UNIT_THREADS / 32; ++w) most = fmaxf(most, tops[threadIdx.x][w]);
-    // (F32 rows' keys are over nothing: their scales meet the scores; 2^-64 at
-    // least for the others', so that the scores' factor stays normal with it)
-    a.units[((long long)z * a.kv_heads + head) * 2 + threadIdx.x] =
-        a.key_scales32 && threadIdx.x == 0 ? 1.0f : power_over(most, threadIdx.x == 0 ? 0x1f800000u : 0x01000000u);
-  }
+  if (threadIdx.x > 0) return;
+  constexpr float LESS = 1.0f / 256.0f;
+  a.units[(long long)z * a.kv_heads + head] = by_key ? make_float4(power_over(top[1]), 1.0f, 1.0f, 0.0f)
+                                                     : make_float4(power_over(top[1]) * LESS, power_over(top[0]) * LESS, 0.0f, 0.0f);
 }
 
 // 64 positions of a head (128 where D = 80): a thread takes 16 codes at a time, of a position's
 // key or of a dimension's values.
-template <int D, bool EXACT>
+template <int D>
 __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -147,8 +164,9 @@ __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandA
   const SeenPositions seen(a, chunk);
   const int start = blockIdx.x * RUN * RUNS;
   if (start >= seen.end || (start + RUN * RUNS <= seen.low && start >= seen.first)) return;
-  const float* units = a.units + ((long long)z * a.kv_heads + head) * 2;
-  const float key_inverse = 1.0f / units[0], value_inverse = 1.0f / units[1];  // exact
+  const float4 units = a.units[(long long)z * a.kv_heads + head];
+  const bool by_key = units.z != 0.0f;
+  const float value_inverse = 1.0f / units.x, key_inverse = 1.0f / units.y;  // exact
   uint4 codes[PER];
   long long from_scales[PER];
   bool there[PER];
@@ -186,21 +204,18 @@ __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandA
     const long long page = (long long)z * a.page_row + index;
     const bool key = in < D;
     float by[RUN];
-    if (key) {
-      float scale = there[n] ? a.key_scales[from_scales[n] + in / (D / 16)] * key_inverse : 0.0f;
-      if constexpr (EXACT) {
-        if (in % (D / 16) == 0) {
-          const long long to = ((long long)z * a.kv_heads + head) * a.page_row * a.at.page_size + first + in / (D / 16);
-          a.key_scales32[to] = scale;
-          a.value_scales32[to] = there[n] ? a.value_scales[from_scales[n] + in / (D / 16)] * value_inverse : 0.0f;
-        }
-        scale = 1.0f;
+    if (by_key) {
+      if (key && in % (D / 16) == 0) {
+        const long long to = ((long long)z * a.kv_heads + head) * a.page_row * a.at.page_size + first + in / (D / 16);
+        a.key_scales32[to] = there[n] ? a.key_scales[from_scales[n] + in / (D / 16)] : 0.0f;
+        a.value_scales32[to] = there[n] ? a.value_scales[from_scales[n] + in / (D / 16)] * value_inverse : 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < RUN; ++e) by[e] = scale;
-    } else if constexpr (EXACT) {
-#pragma unroll
       for (int e = 0; e < RUN; ++e) by[e] = 1.0f;
+    } else if (key) {
+      const float scale = there[n] ? a.key_scales[from_scales[n] + in / (D / 16)] * key_inverse : 0.0f;
+#pragma unroll
+      for (int e = 0; e < RUN; ++e) by[e] = scale;
     } else {
 #pragma unroll
       for (int e = 0; e < RUN; e += 4) {
@@ -222,9 +237,7 @@ __global__ void __launch_bounds__(THREADS) attention_expand_kernel(const ExpandA
   }
 }
 
-#define DRIFT_EXPAND_REGISTER(D)                                               \
-  DRIFT_REGISTER(attention_expand_bf16_d##D, (attention_expand_kernel<D, false>)) \
-  DRIFT_REGISTER(attention_expand_f32_d##D, (attention_expand_kernel<D, true>))
+#define DRIFT_EXPAND_REGISTER(D) DRIFT_REGISTER(attention_expand_d##D, (attention_expand_kernel<D>))
 DRIFT_EXPAND_REGISTER(64)
 DRIFT_EXPAND_REGISTER(80)
 DRIFT_EXPAND_REGISTER(128)
@@ -236,8 +249,7 @@ int launch_dim(const ExpandArgs& a, cudaStream_t stream) {
   constexpr int POSITIONS = RUN * runs_of(D);
   const unsigned runs = unsigned(((long long)a.at.max_keys + POSITIONS - 1) / POSITIONS);
   const dim3 grid(runs, a.kv_heads, a.at.batch);
-  if (a.key_scales32) DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, true>, grid, THREADS, 0, stream, a));
-  else DRIFT_CUDA(launch_pdl(attention_expand_kernel<D, false>, grid, THREADS, 0, stream, a));
+  DRIFT_CUDA(launch_pdl(attention_expand_kernel<D>, grid, THREADS, 0, stream, a));
   DRIFT_LAUNCHED("attention_expand");
   return 0;
 }
@@ -251,11 +263,11 @@ int expanded_page_row(int max_key_count, int page_size) { return int(((long long
 // (a tile's scales are read whole past the last page)
 static size_t scales_bytes(size_t positions, int kv_heads) { return round_up((positions * kv_heads + 128) * sizeof(float)); }
 
-size_t expanded_bytes(int x_dtype, int batch, int kv_heads, int head_dim, int page_size, int max_key_count) {
+size_t expanded_bytes(int batch, int kv_heads, int head_dim, int page_size, int max_key_count) {
   const size_t pages = size_t(batch) * expanded_page_row(max_key_count, page_size);
-  return round_up(size_t(batch) * kv_heads * 2 * sizeof(float)) + round_up(pages * sizeof(int)) +
+  return round_up(size_t(batch) * kv_heads * sizeof(float4)) + round_up(pages * sizeof(int)) +
          2 * round_up(pages * page_size * kv_heads * head_dim * sizeof(__half)) +
-         (x_dtype == DRIFT_F32 ? 2 * scales_bytes(pages * page_size, kv_heads) : 0);
+         2 * scales_bytes(pages * page_size, kv_heads);
 }
 
 int launch_attention_expand(AttentionChunksArgs& a, int x_dtype, int head_dim, void* memory, cudaStream_t stream) {
@@ -270,10 +282,11 @@ int launch_attention_expand(AttentionChunksArgs& a, int x_dtype, int head_dim, v
   e.page_row = expanded_page_row(a.at.max_keys, a.at.page_size);
   e.window = a.window;
   e.first = a.first;
+  e.always_by_key = x_dtype == DRIFT_F32;
   const size_t pages = size_t(a.at.batch) * e.page_row;
   uint8_t* at = static_cast<uint8_t*>(memory);
-  e.units = reinterpret_cast<float*>(at);
-  at += round_up(size_t(a.at.batch) * a.kv_heads * 2 * sizeof(float));
+  e.units = reinterpret_cast<float4*>(at);
+  at += round_up(size_t(a.at.batch) * a.kv_heads * sizeof(float4));
   e.table = reinterpret_cast<int*>(at);
   at += round_up(pages * sizeof(int));
   const size_t side = round_up(pages * a.at.page_size * a.kv_heads * head_dim * sizeof(__half));
@@ -281,8 +294,8 @@ int launch_attention_expand(AttentionChunksArgs& a, int x_dtype, int head_dim, v
   e.values16 = reinterpret_cast<__half*>(at + side);
   at += 2 * side;
   const size_t scales = scales_bytes(pages * a.at.page_size, a.kv_heads);
-  e.key_scales32 = x_dtype == DRIFT_F32 ? reinterpret_cast<float*>(at) : nullptr;
-  e.value_scales32 = x_dtype == DRIFT_F32 ? reinterpret_cast<float*>(at + scales) : nullptr;
+  e.key_scales32 = reinterpret_cast<float*>(at);
+  e.value_scales32 = reinterpret_cast<float*>(at + scales);
   DRIFT_CUDA(launch_pdl(attention_units_kernel, dim3(a.kv_heads, a.at.batch), UNIT_THREADS, 0, stream, e));
   DRIFT_LAUNCHED("attention_units");
   switch (head_dim) {

@@ -14,13 +14,19 @@
 // largest that divides the page): runs of keys are rows of the 128-byte
 // swizzled tile, and a run of values is a tile of its own, in the swizzle as
 // wide as the run. An 8-bit cache's codes come the same way into a buffer of
-// their own, from which converting warps write them as F16 into the operands:
-// for BF16 rows times their scales over a power of two (of the tile's keys; of
-// the values so far), each rounded to F16 like the weights; for F32 rows
-// exactly, and there a key's scale multiplies its scores, and a value's its
-// weights. Where a chunk has several units of rows its codes come expanded to an
-// F16 cache of the call's own (attention_expand.cu): scaled for BF16 rows, and
-// exactly, with their scales by position, for F32 ones (SCALED).
+// their own, from which converting warps write them as F16 into the operands,
+// exactly; a key's scale multiplies its scores, and a value's its weights, in
+// F32 (BY_KEY). Where a chunk has several units of rows its codes come expanded to
+// an F16 cache of the call's own (attention_expand.cu), with their scales by
+// position (SCALED), or for BF16 rows with them
+// in the values where they are of like size. Values' scales are over a power of two, of all that some
+// row sees (SCALED) or of those so far.
+//
+// Where scales are by key, a row's base is set by its largest product of weight
+// and value scale, since that is what is rounded to F16: so its bits are its own,
+// whatever scales the rows beside it see. (With codes converted over the largest
+// scale, as was, a key's scale and its product were rounded one after the other,
+// twice the error, and a hidden scale of 2^25 times the rest left a row no bits.)
 //
 // The order: Q K^T of the next tile is issued as soon as the softmax threads
 // have taken S into registers, P V when P is there. So the tensor core works
@@ -86,7 +92,11 @@ constexpr uint32_t TMEM_COLUMNS = 512;
 // (with 2^8 and a growth of 2^6 by 2^-33: 4e-5 of the result where an early
 // key has ten times the weight of 65536 others, and no value).
 constexpr float WEIGHT_BITS = 8.0f, MOST_WEIGHT = 32768.0f;
-constexpr float WEIGHT_BITS_2 = 12.0f, GROWTH_BITS_2 = 3.0f;
+constexpr float WEIGHT_BITS_2 = 12.0f, MOST_BITS_2 = 15.0f;
+// By key it is products that this holds for, and a bound of them (the largest
+// score and the tile's largest scale) that moves a base: a little lower, so that
+// the two's difference seldom does.
+constexpr float WEIGHT_BITS_BY_KEY = 6.0f, WEIGHT_BITS_2_BY_KEY = 11.0f;
 // A row of q is 2^Q_BITS and more at its largest value, so that its second
 // terms end far below F16's last bit, 2^-24.
 constexpr int Q_BITS = 8;
@@ -97,7 +107,8 @@ struct TileTraits {
   // F32 rows of heads of 256: a CTA takes 128 of the values' dimensions (a row's
   // running output is in registers), and both make the weights
   static constexpr int DV = TERMS == 2 && D > 128 ? 128 : D, PARTS = D / DV;
-  static constexpr bool CODES = CODES_, SCALED = SCALED_;  // SCALED: expanded codes of F32 rows
+  static constexpr bool CODES = CODES_, SCALED = SCALED_;  // SCALED: expanded codes
+  static constexpr bool BY_KEY = CODES || SCALED;
   static constexpr int UNIT = ROW_TILE * MT;
   static constexpr int SOFTMAX_WARPS = 4 * MT;
   // Q K^T and P V have a warp each: a wait costs one about 100 clocks even when
@@ -119,7 +130,7 @@ struct TileTraits {
   static constexpr int SHARE =
       (THREADS * LAUNCH_REGISTERS - (THREADS - 32 * SOFTMAX_WARPS) * OTHER_REGISTERS) / (32 * SOFTMAX_WARPS) / 8 * 8;
   static constexpr int SOFTMAX_REGISTERS = SHARE > 232 ? 232 : SHARE;
-  static constexpr int ROUND_THREADS = 32 * SOFTMAX_WARPS + (CODES ? CONVERT_THREADS : EDGE_THREADS);
+  static constexpr int ROUND_THREADS = 32 * SOFTMAX_WARPS + EDGE_THREADS;
   static constexpr int PANELS = (D + 63) / 64;             // 64-column panels of a row
   static constexpr int Q_PANEL = ROW_TILE * 128;           // bytes
   static constexpr int Q_BYTES = PANELS * Q_PANEL;         // one term of one row tile
@@ -133,9 +144,10 @@ struct TileTraits {
   // what the copies fill: the operands, or codes, twice where that fits; and
   // the operands three times where that does (a copy's 1400 clocks from when
   // its stage is free are a tile's time)
+  static constexpr int SCALE_ROWS = TERMS == 1 ? 2 : 3;    // the keys', the values' and (there is room) their logarithms
   static constexpr int bytes_of(int stages, int code_stages) {
     return K_AT + stages * (K_BYTES + V_STAGE) + (CODES ? code_stages * 2 * CODE_STAGE : 0) +
-           (CODES && TERMS == 2 ? stages * 2 * KEYS * 4 : 0) + (CODES ? code_stages * 2 * KEYS * 4 : 0) +
+           (CODES ? stages * SCALE_ROWS * KEYS * 4 + code_stages * 2 * KEYS * 4 : 0) +
            (SCALED ? SOFTMAX_WARPS * KEYS * 4 : 0) + 384;
   }
   static constexpr int LIMIT = 232448;
@@ -144,8 +156,8 @@ struct TileTraits {
   static constexpr int COPY_STAGES = CODES ? CODE_STAGES : STAGES;
   static constexpr int V_AT = K_AT + STAGES * K_BYTES;
   static constexpr int CODES_AT = V_AT + STAGES * V_STAGE;  // [COPY_STAGES][2]
-  static constexpr int SCALES_AT = CODES_AT + (CODES ? COPY_STAGES * 2 * CODE_STAGE : 0);  // [STAGES][2][KEYS]
-  static constexpr int COPIED_SCALES_AT = SCALES_AT + (CODES && TERMS == 2 ? STAGES * 2 * KEYS * 4 : 0);  // [COPY_STAGES][2][KEYS]
+  static constexpr int SCALES_AT = CODES_AT + (CODES ? COPY_STAGES * 2 * CODE_STAGE : 0);  // [STAGES][SCALE_ROWS][KEYS]
+  static constexpr int COPIED_SCALES_AT = SCALES_AT + (CODES ? STAGES * SCALE_ROWS * KEYS * 4 : 0);  // [COPY_STAGES][2][KEYS]
   static constexpr int WARP_SCALES_AT = COPIED_SCALES_AT + (CODES ? COPY_STAGES * 2 * KEYS * 4 : 0);  // [SOFTMAX_WARPS][KEYS]
   static constexpr int BARRIERS_AT = WARP_SCALES_AT + (SCALED ? SOFTMAX_WARPS * KEYS * 4 : 0);
   static constexpr int BYTES = BARRIERS_AT + 384;  // 38 barriers and a few words
@@ -378,7 +390,7 @@ __global__ void __launch_bounds__(T::THREADS, 1)
 attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                        const TileArgs args) {
   constexpr int D = T::D, DV = T::DV, KEYS = T::KEYS, MT = T::MT, TERMS = T::TERMS, STAGES = T::STAGES;
-  constexpr bool CODES = T::CODES, SCALED = T::SCALED;
+  constexpr bool CODES = T::CODES, SCALED = T::SCALED, BY_KEY = T::BY_KEY;
   using X = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   pdl_trigger();  // the next kernel may launch and wait for this one
   pdl_wait();     // what the kernels before this one wrote is visible
@@ -396,6 +408,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   const int tile0 = split * a.tiles_per_split, tile1 = min(tile0 + a.tiles_per_split, seen.count);
   if (tile0 >= tile1) return;
   const int tiles = tile1 - tile0;
+  // (BF16 rows' expanded codes: those of a head whose scales are by key are the
+  // SCALED launch's, the others' the F16 cache's)
+  float4 units = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
+  if (!CODES && a.units) {
+    units = a.units[(long long)z * a.kv_heads + head];
+    if (SCALED != (units.z != 0.0f)) return;
+  }
   // what some row sees: keys below seen.end that are `lowest` or later or
   // below `first`; what every row sees: below all_end, from all_low on (or
   // below `first`)
@@ -431,8 +450,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* taken_out = abort + 1;
   volatile int* copied = abort + 2;         // [2]: tiles whose keys, values were asked for
-  volatile float* k_unit = reinterpret_cast<volatile float*>(abort + 4);  // [STAGES]: the scales' powers of two
-  volatile float* v_unit = k_unit + STAGES;
+  volatile float* v_unit = reinterpret_cast<volatile float*>(abort + 4);  // [STAGES]: what values' scales are over,
+  volatile float* v_most = v_unit + STAGES;                               // and the largest of a tile's
   float* scales = reinterpret_cast<float*>(shared + T::SCALES_AT);
 
   if (tid == 0) {
@@ -551,11 +570,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(&q_full[i]);
     }
-    // (what expanded codes are over)
-    const float* units = !CODES && a.units ? a.units + ((long long)z * a.kv_heads + head) * 2 : nullptr;
-    const float key_unit = units ? units[0] : 1.0f, value_unit = units ? units[1] : 1.0f;
-    // (a softcap leaves natural units behind)
-    // (and a factor of 2^-60 is as good as none; times a tile's power it is normal)
+    const float value_unit = units.x;
+    multiplier *= units.y;
+    // (a softcap leaves natural units behind; a factor of 2^-60 is as good as none)
     const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 8.7e-19f);
     const int position = chunk.position + token;
     const int hi = a.causal ? position + 1 : seen.end;
@@ -570,7 +587,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const uint32_t o_at = tmem + lanes + T::O_COLUMN + i * T::O_COLUMNS, p_at = tmem + lanes + T::P_COLUMN + i * T::P_COLUMNS;
 
     float base2 = -INFINITY, sum = 0.0f;  // weights are 2^(score in base 2 - base2)
-    float unit = 0.0f;                    // and, for codes, values are over this
+    float unit = 0.0f;                    // and, for codes, values' scales are over this
     float total[TERMS == 2 ? DV : 1] = {};  // the running output (F32 rows)
     // the last tile's output, which the tensor core has left in O
     auto take_output = [&]() {
@@ -590,12 +607,18 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       const int b = MT == 2 ? i : j & 1, stage = j % STAGES;
-      float held_k[2], held_v[2];
+      // (expanded codes' scales, and the largest of the values', off the way)
+      constexpr int HELD = (KEYS + 31) / 32;  // a lane has of a tile (reads up to 31 past it)
+      float held_k[HELD], held_v[HELD], most_scale = 1.0f;
       if constexpr (SCALED) {
-        static_assert(!SCALED || KEYS == 64, "two scales a lane");
         const long long at = ((long long)z * a.kv_heads + head) * a.at.table_stride * a.at.page_size + seen.key_of(tile0 + j) + lane;
-        held_k[0] = a.key_scales[at], held_k[1] = a.key_scales[at + 32];
-        held_v[0] = a.value_scales[at], held_v[1] = a.value_scales[at + 32];
+#pragma unroll
+        for (int n = 0; n < HELD; ++n) held_k[n] = a.key_scales[at + 32 * n], held_v[n] = a.value_scales[at + 32 * n];
+        uint32_t most = 0;  // (what is past the last key may be anything)
+#pragma unroll
+        for (int n = 0; n < HELD; ++n)
+          if (__float_as_uint(held_v[n]) <= 0x3f800000u) most = max(most, __float_as_uint(held_v[n]));
+        most_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
       }
       if (!(ok = wait(&s_full[b], MT == 2 ? j & 1 : (j >> 1) & 1))) break;
       // P and O are free (and O complete) when the last tile's P V is done
@@ -627,19 +650,21 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::fence_before_sync();
       tc::mbar_arrive(&s_empty[b]);
 
-      // (expanded codes' scales: the keys', then the values', in a row of the warp's own)
+      // (expanded codes' scales: one kind after the other in a row of the warp's own)
       float* warp_scales = reinterpret_cast<float*>(shared + T::WARP_SCALES_AT) + warp * KEYS;
-      const float* k_scales = SCALED ? warp_scales : scales + stage * 2 * KEYS;
+      const float* k_scales = SCALED ? warp_scales : scales + stage * T::SCALE_ROWS * KEYS;
       const float* v_scales = SCALED ? warp_scales : k_scales + KEYS;
-      if constexpr (SCALED) {
+      const float* logarithms = SCALED ? warp_scales : v_scales + KEYS;
+      auto share = [&](const float (&x)[HELD]) {
+        __syncwarp();  // (what it held before is read)
+#pragma unroll
+        for (int n = 0; n < HELD; ++n)
+          if (KEYS % 32 == 0 || lane + 32 * n < KEYS) warp_scales[lane + 32 * n] = x[n];
         __syncwarp();
-        warp_scales[lane] = held_k[0], warp_scales[lane + 32] = held_k[1];
-        __syncwarp();
-      }
-      const float by_unit = CODES && TERMS == 1 ? float(k_unit[stage]) : key_unit;
-      const float tile_m2 = a.softcap > 0.0f ? m2 : m2 * by_unit;
+      };
+      if constexpr (SCALED) share(held_k);
       const float now_unit = CODES ? float(v_unit[stage]) : 0.0f;
-      if constexpr (SCALED || (CODES && TERMS == 2)) {
+      if constexpr (BY_KEY) {
 #pragma unroll
         for (int c = 0; c < KEYS; c += 4) {
           const float4 x = *reinterpret_cast<const float4*>(k_scales + c);
@@ -652,7 +677,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         // (where no score of the warp's rows is far from zero, the usual case,
         // the far form's two special functions a score are left out: of 1500 F32
         // rows of 16 heads, 98 us with them)
-        const float inverse = multiplier * by_unit / a.softcap;
+        const float inverse = multiplier / a.softcap;
         float far = 0.0f;
 #pragma unroll
         for (int c = 0; c < KEYS; c += 2) far = max3(far, fabsf(s[c]), fabsf(s[c + 1]));
@@ -667,11 +692,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           for (int c = 0; c < KEYS; ++c) s[c] = a.softcap * capped_near(s[c] * inverse);
         }
       }
-      if constexpr (SCALED) {
-        __syncwarp();
-        warp_scales[lane] = held_v[0], warp_scales[lane + 32] = held_v[1];
-        __syncwarp();
-      }
       const bool edge = !(key0 + KEYS <= all_end && (key0 >= all_low || key0 + KEYS <= first));
       if (edge) {
         // a bit for each key that the row sees
@@ -685,15 +705,32 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             if (!(sees >> e & 1)) s[c + e] = -INFINITY;
         }
       }
-      // the row's base from this tile's largest score, and what is summed in it
+      // the row's base from this tile's largest score (BY_KEY: its largest
+      // product's logarithm), and what is summed in it
       bool not_a_number = false;
       auto rebase = [&](float top) {
         not_a_number = top != top;
+        float g = 1.0f;
+        if constexpr (CODES) {
+          if (now_unit > unit) {
+            // values' scales are over 2^over times as much: as products stay
+            // what they are, the base falls and the weights' sum grows, as far
+            // as it has room (the outputs take the rest)
+            if (unit > 0.0f) {
+              const int over = (__float_as_int(now_unit) - __float_as_int(unit)) >> 23;
+              const int falls = min(over, max(227 - (__float_as_int(sum) >> 23), 0));
+              base2 -= float(falls);
+              sum = ldexpf(sum, falls);
+              g = exp2f(float(falls - over));
+            }
+            unit = now_unit;
+          }
+        }
         // (a row without a base takes one; a base that is too high stays)
-        const float now = fmaxf(base2, top - (TERMS == 2 ? WEIGHT_BITS_2 : WEIGHT_BITS));
+        constexpr float BITS = TERMS == 2 ? (BY_KEY ? WEIGHT_BITS_2_BY_KEY : WEIGHT_BITS_2) : BY_KEY ? WEIGHT_BITS_BY_KEY : WEIGHT_BITS;
+        const float now = fmaxf(base2, top - BITS);
         const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - now);
-        const float g = CODES && now_unit > unit ? f * (unit / now_unit) : f;
-        if (CODES) unit = fmaxf(unit, now_unit);
+        g *= f;
         base2 = now;
         sum *= f;
         if constexpr (TERMS == 2) {
@@ -710,7 +747,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           }
         }
       };
-      auto largest = [&]() {
+      auto largest_score = [&]() {
         float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
         for (int c = 4; c < KEYS - 4; c += 8)
@@ -718,8 +755,30 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], s[c + 2 * n], s[c + 2 * n + 1]);
 #pragma unroll
         for (int n = 0; n < 4; ++n) tops[n] = max3(tops[n], tops[n], s[KEYS - 4 + n]);
-        return max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * tile_m2;
+        return max3(tops[0], tops[1], max3(tops[2], tops[2], tops[3])) * m2;
       };
+      // by key: of a product. (NaNs do not count: a hidden key's scale may be one,
+      // and a score that is makes its row NaNs by its weight.)
+      auto largest_product = [&]() {
+        if constexpr (SCALED) {
+          float x[HELD];
+#pragma unroll
+          for (int n = 0; n < HELD; ++n) x[n] = logarithm(held_v[n]);
+          share(x);
+        }
+        float tops[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 4) {
+          float4 l;
+          if constexpr (SCALED || T::SCALE_ROWS == 3) l = *reinterpret_cast<const float4*>(logarithms + c);
+          else l = make_float4(logarithm(v_scales[c]), logarithm(v_scales[c + 1]), logarithm(v_scales[c + 2]), logarithm(v_scales[c + 3]));
+          const float2 x = fma2(make_float2(s[c], s[c + 1]), make_float2(m2, m2), make_float2(l.x, l.y));
+          const float2 y = fma2(make_float2(s[c + 2], s[c + 3]), make_float2(m2, m2), make_float2(l.z, l.w));
+          tops[0] = fmaxf(tops[0], fmaxf(x.x, x.y)), tops[1] = fmaxf(tops[1], fmaxf(y.x, y.y));
+        }
+        return fmaxf(tops[0], tops[1]);
+      };
+      if constexpr (CODES) most_scale = v_most[stage];
       uint32_t p[KEYS / 2], p_low[TERMS == 2 ? KEYS / 2 : 1];
       // the weights and their sum (a tile's own: short chains)
       auto weigh = [&]() {
@@ -727,43 +786,58 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         const float less = not_a_number ? __int_as_float(0x7fc00000) : base2 == -INFINITY ? 0.0f : -base2;
         float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int e = 0; e < KEYS / 2; ++e) {
-          float2 w = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(tile_m2, tile_m2), make_float2(less, less));
-          w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
-          part = add2(part, w);
-          if constexpr (SCALED || (CODES && TERMS == 2)) {
-            w = mul2(w, *reinterpret_cast<const float2*>(v_scales + 2 * e));
-            if (edge) {  // (a hidden value's scale may be a NaN)
-              w.x = s[2 * e] == -INFINITY ? 0.0f : w.x;
-              w.y = s[2 * e + 1] == -INFINITY ? 0.0f : w.y;
+        for (int e = 0; e < KEYS / 2; e += 2) {
+          float4 by;
+          if constexpr (BY_KEY) by = *reinterpret_cast<const float4*>(v_scales + 2 * e);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float s0 = s[2 * (e + n)], s1 = s[2 * (e + n) + 1];
+            float2 w = fma2(make_float2(s0, s1), make_float2(m2, m2), make_float2(less, less));
+            w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
+            part = add2(part, w);
+            if constexpr (BY_KEY) {
+              w = mul2(w, n == 0 ? make_float2(by.x, by.y) : make_float2(by.z, by.w));
+              if (edge) {  // (a hidden value's scale may be a NaN)
+                w.x = s0 == -INFINITY ? 0.0f : w.x;
+                w.y = s1 == -INFINITY ? 0.0f : w.y;
+              }
             }
+            p[e + n] = half_pair(w.x, w.y);
+            if constexpr (TERMS == 2) p_low[e + n] = left_pair(w.x, w.y, p[e + n]);
           }
-          p[e] = half_pair(w.x, w.y);
-          if constexpr (TERMS == 2) p_low[e] = left_pair(w.x, w.y, p[e]);
         }
         return part.x + part.y;
       };
       if constexpr (TERMS == 2) {
         if (!(ok = settled())) break;
         if (j > 0) take_output();
-        const float top = largest();
-        const bool grown = !(top <= base2 + (WEIGHT_BITS_2 + GROWTH_BITS_2)) || (CODES && now_unit > unit);
-        if (__any_sync(0xffffffffu, grown)) rebase(top);
+        // (no product is past its weight times the tile's largest scale)
+        float top = largest_score();
+        if constexpr (BY_KEY) top += logarithm(most_scale);
+        const bool grown = !(top <= base2 + MOST_BITS_2) || (CODES && now_unit > unit);
+        if (__any_sync(0xffffffffu, grown)) {
+          if constexpr (BY_KEY) top = largest_product();
+          rebase(top);
+        }
+        if constexpr (SCALED) share(held_v);
         sum += weigh();
       } else {
         // the bases stay unless a weight might not fit; in the first tile, and
         // where a row without one sees keys, they are set
         bool slow = j == 0;
+        if constexpr (SCALED) share(held_v);
         float part = 0.0f;
         if (!slow) {
           part = weigh();
           const bool sees = key0 < hi && (key0 + KEYS > lo || key0 < first);
-          const bool over = !(part <= MOST_WEIGHT) || (base2 == -INFINITY && sees) || (CODES && now_unit > unit);
+          const bool over = !(part * most_scale <= MOST_WEIGHT) || (base2 == -INFINITY && sees) ||
+                            (CODES && now_unit > unit);
           slow = __any_sync(0xffffffffu, over);
         }
         if (!(ok = settled())) break;
         if (slow) {
-          rebase(largest());
+          rebase(BY_KEY ? largest_product() : largest_score());
+          if constexpr (SCALED) share(held_v);
           part = weigh();
         }
         sum += part;
@@ -776,22 +850,29 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
     if (ok) ok = wait(&pv_done[i], (tiles - 1) & 1);
     float all_sum = sum;
-    if constexpr (!(CODES && TERMS == 2)) asm volatile("bar.sync 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");  // (taken_out is final)
+    if constexpr (!CODES) asm volatile("bar.sync 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");  // (taken_out is final)
     if (ok) {
       tc::fence_after_sync();
       take_output();
-      float scale = CODES ? unit : value_unit;
+      // (two factors: what values are over may be at either end of F32's range)
+      const float over = CODES ? unit : value_unit;  // (an F16 cache's is 1)
+      float scale = 1.0f;
       if (!a.part_o) {
         if (a.sinks) {
           // the sink's weight in the row's units, or the row's in the sink's
           const float sink = a.sinks[q_head] * LOG2E, all = fmaxf(base2, sink);
           const float f = base2 == -INFINITY ? 0.0f : exp2f(base2 - all);
           all_sum = all_sum * f + exp2f(sink - all);
-          scale *= f;
+          scale = f;
         }
         scale = all_sum != 0.0f ? scale / all_sum : 0.0f;
-      } else if (real && part == 0) {
-        *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) = make_float2(base2 * LN2, all_sum);
+      } else {
+        // (BY_KEY over 2^15: products up to that, times what values are over, may pass F32's range)
+        constexpr float PART_BITS = BY_KEY ? 15.0f : 0.0f;
+        scale = BY_KEY ? 1.0f / 32768.0f : 1.0f;
+        if (real && part == 0)
+          *reinterpret_cast<float2*>(a.part_ml + (row_at * a.splits + split) * 2) =
+              make_float2((base2 + PART_BITS) * LN2, all_sum * scale);
       }
       // PIECE dimensions of every row at a time, through this warp's part of the
       // row tile's q (which no product reads any more): a row to a thread goes
@@ -818,26 +899,19 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           tmem_load_wait();
         }
 #pragma unroll
-        for (int e = 0; e < PIECE; ++e) o[e] *= scale;
-        if (!(CODES && TERMS == 2) && *taken_out && real) {
+        for (int e = 0; e < PIECE; ++e) o[e] = o[e] * scale * over;
+        if (!BY_KEY && *taken_out && real) {
 #pragma unroll 1
           for (int j = 0; j < tiles; ++j) {
             const int key0 = seen.key_of(tile0 + j);
             if (whole(key0)) continue;
             const int end = min(key0 + KEYS, hi);
-            if constexpr (CODES) {
-              const float y = not_finite_scale(a.value_scales + (long long)head * a.at.page_size, (long long)a.kv_heads * a.at.page_size,
-                                               chunk.table, a.at.pages, a.at.page_size, key0, end, lo, first);
 #pragma unroll
-              for (int e = 0; e < PIECE; ++e) o[e] += y;
-            } else {
-#pragma unroll
-              for (int e = 0; e < PIECE; e += 4) {
-                const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + part * DV + c + e) * a.at.page_size,
-                                            (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
-                                            a.at.page_size, key0, end, lo, first);
-                o[e] += y.x, o[e + 1] += y.y, o[e + 2] += y.z, o[e + 3] += y.w;
-              }
+            for (int e = 0; e < PIECE; e += 4) {
+              const float4 y = not_finite(static_cast<const __half*>(a.values) + ((long long)head * D + part * DV + c + e) * a.at.page_size,
+                                          (long long)a.kv_heads * D * a.at.page_size, chunk.table, a.at.pages,
+                                          a.at.page_size, key0, end, lo, first);
+              o[e] += y.x, o[e + 1] += y.y, o[e + 2] += y.z, o[e + 3] += y.w;
             }
           }
         }
@@ -1033,7 +1107,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         x[n] = k < KEYS && (!check || seen_key(key0 + k)) ? from[k] : 0.0f;
       }
     };
-    auto largest_of = [](const float (&x)[PER]) {  // of those that are finite
+    auto largest_scale = [](const float (&x)[PER]) {  // of those that are finite
       float most = 0.0f;
 #pragma unroll
       for (int n = 0; n < PER; ++n) most = x[n] <= 3.402823466e38f ? fmaxf(most, x[n]) : most;
@@ -1041,12 +1115,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       return most;
     };
-    // a power of two at or above x, `least` (in exponent bits) at least, whose
-    // inverse is normal
-    auto power_over = [](float x, uint32_t least) {
+    // a power of two at or above x whose inverse is normal
+    auto power_over = [](float x) {
       const uint32_t bits = __float_as_uint(x);
       const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-      return __uint_as_float(max(up, least));
+      return __uint_as_float(max(up, 0x01000000u));
     };
     float v_power = 0.0f;
     bool ok = true;
@@ -1066,20 +1139,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       const bool check = !whole(key0);
       if (j >= STAGES && !(ok = wait(&k_empty[stage], used))) break;
       if (!(ok = wait(&codes_full[2 * copy_stage], copy_phase))) break;
-      float k_scale[PER];
-      load_scales(key0, check, k_from, k_scale);
       const float own_k = (!check || seen_key(key0 + row)) ? k_from[row] : 0.0f;
-      // (2^-64 at least: the scores' factor stays normal with it)
-      const float k_power = power_over(largest_of(k_scale), 0x1f800000u);
       if (has_row) {
         uint8_t* k = shared + T::K_AT + stage * T::K_BYTES + row * 128;
         constexpr int TAKES = CHUNKS / TO_ROW;  // chunks a thread takes
-        const __half2 ratio = __float2half2_rn(own_k * (1.0f / k_power));
-        auto scaled = [&](uint32_t pair) {
-          if constexpr (TERMS == 2) return pair;
-          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), ratio);
-          return *reinterpret_cast<const uint32_t*>(&y);
-        };
         // (each eight lanes' chunks on different banks; loads ahead of the
         // stores, which the compiler cannot tell apart)
         auto chunk_of = [&](int n) {
@@ -1097,9 +1160,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             const uint2 y0 = code_pairs(x[n].x), y1 = code_pairs(x[n].y), y2 = code_pairs(x[n].z), y3 = code_pairs(x[n].w);
             uint8_t* to = k + c / 4 * T::K_PANEL;
             *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4)) ^ (row % 8))) =
-                make_uint4(scaled(y0.x), scaled(y0.y), scaled(y1.x), scaled(y1.y));
+                make_uint4(y0.x, y0.y, y1.x, y1.y);
             *reinterpret_cast<uint4*>(to + 16 * ((2 * (c % 4) + 1) ^ (row % 8))) =
-                make_uint4(scaled(y2.x), scaled(y2.y), scaled(y3.x), scaled(y3.y));
+                make_uint4(y2.x, y2.y, y3.x, y3.y);
           }
         }
       }
@@ -1112,49 +1175,24 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       if (!(ok = wait(&codes_full[2 * copy_stage + 1], copy_phase))) break;
       float v_scale[PER];
       load_scales(key0, check, v_from, v_scale);
-      const float most = largest_of(v_scale);
-      if (most > v_power) v_power = power_over(most, 0x01000000u);
+      const float most = largest_scale(v_scale);
+      if (most > v_power) v_power = power_over(most);
       const float v_inverse = 1.0f / (v_power > 0.0f ? v_power : 1.0f);
-      if (TERMS == 2) {
-        scales[stage * 2 * KEYS + row] = own_k;
-        scales[stage * 2 * KEYS + KEYS + row] = !check || seen_key(key0 + row) ? v_from[row] * v_inverse : 0.0f;
-      }
-      if (t == 0) k_unit[stage] = k_power, v_unit[stage] = v_power;
+      float* to_scales = scales + stage * T::SCALE_ROWS * KEYS + row;
+      const float own_v = !check || seen_key(key0 + row) ? v_from[row] * v_inverse : 0.0f;
+      to_scales[0] = own_k;
+      to_scales[KEYS] = own_v;
+      if constexpr (T::SCALE_ROWS == 3) to_scales[2 * KEYS] = logarithm(own_v);
+      if (t == 0) v_unit[stage] = v_power, v_most[stage] = most * v_inverse;
       tc::mbar_arrive(&scales_full[stage]);
       // values: a thread takes sixteen positions of every (DIMS)th dimension
       constexpr int GROUPS = KEYS / 16, DIMS = N / GROUPS;
       const int per = run / 16;
       const int group = t % per + per * (t / (DIMS * per)), first_d = t / per % DIMS;
       const bool has_group = group < GROUPS;
-      __half2 ratios[8];
-      if constexpr (TERMS == 1) {
-        const int key = key0 + 16 * group;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (has_group) x = *reinterpret_cast<const float4*>(v_from + 16 * group + 4 * n);
-          float y[4] = {x.x, x.y, x.z, x.w};
-          if (check) {
-            // (at an edge, what is not finite is taken out for the rows that
-            // do not see it)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (!has_group || !seen_key(key + 4 * n + e)) y[e] = 0.0f;
-              else if (!isfinite(y[e])) y[e] = 0.0f, *taken_out = 1;
-            }
-          }
-          ratios[2 * n] = __floats2half2_rn(y[0] * v_inverse, y[1] * v_inverse);
-          ratios[2 * n + 1] = __floats2half2_rn(y[2] * v_inverse, y[3] * v_inverse);
-        }
-      }
       if (has_group) {
         uint8_t* v = shared + T::V_AT + stage * T::V_STAGE + group * (D * 32);
         const uint8_t* from = v_codes + group / per * (run * D) + group % per * 16;
-        auto scaled = [&](uint32_t pair, int n) {
-          if constexpr (TERMS == 2) return pair;
-          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), ratios[n]);
-          return *reinterpret_cast<const uint32_t*>(&y);
-        };
         constexpr int TAKES = (D + DIMS - 1) / DIMS, FLIGHT = TAKES % 4 == 0 ? 4 : TAKES;
 #pragma unroll
         for (int n0 = 0; n0 < TAKES; n0 += FLIGHT) {
@@ -1171,8 +1209,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             const uint2 y0 = code_pairs(x[n].x), y1 = code_pairs(x[n].y), y2 = code_pairs(x[n].z), y3 = code_pairs(x[n].w);
             uint8_t* to = v + d * 32;  // (rows of 32 bytes, their halves exchanged in every other four)
             const int c = d / 4 % 2;
-            *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(scaled(y0.x, 0), scaled(y0.y, 1), scaled(y1.x, 2), scaled(y1.y, 3));
-            *reinterpret_cast<uint4*>(to + 16 * (1 - c)) = make_uint4(scaled(y2.x, 4), scaled(y2.y, 5), scaled(y3.x, 6), scaled(y3.y, 7));
+            *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+            *reinterpret_cast<uint4*>(to + 16 * (1 - c)) = make_uint4(y2.x, y2.y, y3.x, y3.y);
           }
         }
       }
@@ -1180,7 +1218,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
       tc::mbar_arrive(&v_full[stage]);
       tc::mbar_arrive(&codes_empty[2 * copy_stage + 1]);
     }
-    if constexpr (TERMS == 1) asm volatile("bar.arrive 1, %0;" ::"n"(T::ROUND_THREADS) : "memory");
   } else if (!CODES && warp == T::EDGE_WARP) {
     // ---- edges: values that are not finite, out of the tiles seen in part -----------------
     bool ok = true;
@@ -1260,13 +1297,15 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 
 // Keys of a tile: what TMEM holds beside the outputs (P_COLUMN's assertion);
 // F32 rows and heads of 256 have no room in registers or shared memory for more.
-constexpr int tile_of(int head_dim, int terms) {
-  return terms == 2 || head_dim > 128 ? 64 : head_dim > 80 ? 80 : head_dim > 64 ? 96 : 128;
+// Codes of heads of 64 go by 64 for BF16 rows, whose softmax takes scales as well
+// (a chunk of 2 x 100 tokens x 4 heads over 2048 keys 18 us, 22 by 128, spilling).
+constexpr int tile_of(int head_dim, int terms, bool codes) {
+  return terms == 2 || head_dim > 128 ? 64 : head_dim > 80 ? 80 : head_dim > 64 ? 96 : codes ? 64 : 128;
 }
 
 template <int D, int MT, bool CODES, int TERMS, bool SCALED>
 int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
-  using T = TileTraits<D, tile_of(D, TERMS), MT, CODES, TERMS, SCALED>;
+  using T = TileTraits<D, tile_of(D, TERMS, CODES), MT, CODES, TERMS, SCALED>;
   TileArgs args;
   args.a = a;
   const int ps = a.at.page_size;
@@ -1306,17 +1345,24 @@ int launch_tiles(const AttentionChunksArgs& a, cudaStream_t stream) {
 
 template <int D, int MT>
 int launch_types(const AttentionChunksArgs& a, bool codes, bool bf16, cudaStream_t stream) {
-  if (bf16) return codes ? launch_tiles<D, MT, true, 1, false>(a, stream) : launch_tiles<D, MT, false, 1, false>(a, stream);
+  if (bf16 && codes) return launch_tiles<D, MT, true, 1, false>(a, stream);
+  if (bf16) {
+    // (expanded codes with their scales in them, and by key: what is the other's
+    // returns at once)
+    DRIFT_TRY((launch_tiles<D, MT, false, 1, false>(a, stream)));
+    return a.units ? launch_tiles<D, MT, false, 1, true>(a, stream) : 0;
+  }
   if (!codes) return a.units ? launch_tiles<D, MT, false, 2, true>(a, stream) : launch_tiles<D, MT, false, 2, false>(a, stream);
   if constexpr (D <= 128) return launch_tiles<D, MT, true, 2, false>(a, stream);
   else return invalid("attention: no tiles that convert codes for F32 heads of %d", D);
 }
 
 #define DRIFT_TILES_REGISTER_AS(D, MT, codes, terms, scaled, name) \
-  DRIFT_REGISTER(name, (attention_tiles_kernel<TileTraits<D, tile_of(D, terms), MT, codes, terms, scaled>>))
+  DRIFT_REGISTER(name, (attention_tiles_kernel<TileTraits<D, tile_of(D, terms, codes), MT, codes, terms, scaled>>))
 #define DRIFT_TILES_REGISTER_BF16(D, MT)                                            \
   DRIFT_TILES_REGISTER_AS(D, MT, false, 1, false, attention_tiles_f16_bf16_d##D##_m##MT)    \
-  DRIFT_TILES_REGISTER_AS(D, MT, true, 1, false, attention_tiles_i8_bf16_d##D##_m##MT)
+  DRIFT_TILES_REGISTER_AS(D, MT, true, 1, false, attention_tiles_i8_bf16_d##D##_m##MT)      \
+  DRIFT_TILES_REGISTER_AS(D, MT, false, 1, true, attention_tiles_expanded_bf16_d##D##_m##MT)
 #define DRIFT_TILES_REGISTER(D, MT)                                                 \
   DRIFT_TILES_REGISTER_BF16(D, MT)                                                  \
   DRIFT_TILES_REGISTER_AS(D, MT, false, 2, false, attention_tiles_f16_f32_d##D##_m##MT)     \
@@ -1334,7 +1380,7 @@ DRIFT_TILES_REGISTER_AS(256, 1, false, 2, true, attention_tiles_expanded_f32_d25
 
 }  // namespace
 
-int attention_tiles_keys(int head_dim, bool bf16) { return tile_of(head_dim, bf16 ? 1 : 2); }
+int attention_tiles_keys(int head_dim, bool bf16, bool codes) { return tile_of(head_dim, bf16 ? 1 : 2, codes); }
 
 int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int row_tiles,
                            cudaStream_t stream) {

@@ -56,9 +56,10 @@ struct AttentionChunksArgs {
   void* out;
   const void* keys;
   const void* values;
-  const float* key_scales;    // 8-bit caches (expanded: [batch][kv_heads][positions], F32 rows)
+  const float* key_scales;    // 8-bit caches (expanded: [batch][kv_heads][positions])
   const float* value_scales;
-  const float* units;         // [batch][kv_heads][2]: what keys and values are over (attention_expand), or null
+  const float4* units;        // [batch][kv_heads], of expanded codes (attention_expand): what values are over, what
+                              // keys are over, whether scales are by key; or null
   const float* sinks;
   float* part_o;   // [token row][q_heads][splits][D], or null for one split
   float* part_ml;  // [token row][q_heads][splits][2]: largest, sum
@@ -68,6 +69,15 @@ struct AttentionChunksArgs {
   int splits, tiles_per_split;  // key tiles a split takes, of the tiles its rows see
   float scale, softcap;
 };
+
+// A value's scale (over a power of two, 1 at most) to base 2, as it moves a
+// row's base: 2^-80 at least, so that no weight is past F32's range because its
+// value has none.
+__device__ __forceinline__ float logarithm(float scale) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(scale));
+  return scale > 0.0f ? fminf(fmaxf(y, -80.0f), 0.0f) : -80.0f;
+}
 
 // The keys some row among the chunk's tokens [token0, token1) sees, as key
 // tiles of `keys_per_tile`: the first `head` tiles hold the first positions
@@ -110,21 +120,6 @@ static __device__ __noinline__ float4 not_finite(const __half* values, long long
   return x;
 }
 
-// The same for codes: a scale that is not finite makes NaNs of the key's
-// values in every dimension. `scales`: the key head's in page 0.
-static __device__ __noinline__ float not_finite_scale(const float* scales, long long page_stride, const int* table,
-                                                      int pages, int page_size, int key0, int end, int lowest, int first) {
-  float x = 0.0f;
-  for (int key = key0; key < end; ++key) {
-    if (key < lowest && key >= first) continue;
-    const int page = table[key / page_size];
-    if (page < 0 || page >= pages) continue;
-    const float s = scales[page * page_stride + key % page_size];
-    if (!isfinite(s)) x += s - s;
-  }
-  return x;
-}
-
 // The checks that the calls share (chunks.cu).
 int check_chunks(const char* call, int x_dtype, long long tokens, int kv_heads, int head_dim, int cache_dtype,
                  const void* keys, const void* values, const float* key_scales, const float* value_scales,
@@ -144,13 +139,13 @@ int launch_attention_codes(const AttentionChunksArgs& a, int x_dtype, int head_d
                            cudaStream_t stream);
 // attention_tiles.cu: `row_tiles` tiles of 128 rows
 // a unit (1 or 2; 1 for heads of 256), and the keys of one of its tiles.
-int attention_tiles_keys(int head_dim, bool bf16);
+int attention_tiles_keys(int head_dim, bool bf16, bool codes);
 int launch_attention_tiles(const AttentionChunksArgs& a, int x_dtype, int cache_dtype, int head_dim, int row_tiles,
                            cudaStream_t stream);
 // attention_expand.cu: an 8-bit cache's keys and values of the chunks as F16 in
 // `memory` (16-byte aligned, expanded_bytes), which then take the cache's place
 // in `a`.
-size_t expanded_bytes(int x_dtype, int batch, int kv_heads, int head_dim, int page_size, int max_key_count);
+size_t expanded_bytes(int batch, int kv_heads, int head_dim, int page_size, int max_key_count);
 int launch_attention_expand(AttentionChunksArgs& a, int x_dtype, int head_dim, void* memory, cudaStream_t stream);
 // Joins the splits (attention_rows.cu).
 int launch_attention_join(const AttentionChunksArgs& a, int x_dtype, int head_dim, int rows_per_unit,

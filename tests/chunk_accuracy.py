@@ -39,20 +39,21 @@ def sequence(cache, table, count):
 def roundings(dtype, quantized, rows, dim):
     """(q's step over its largest value, a weight's relative half step, its
     absolute half step over the row's largest, the step of a tile's products of
-    weight and scale over the largest of 32 keys) of the kernel that a chunk of
-    `rows` rows of a key head goes to."""
+    weight and scale over the largest of 32 keys, a key's and value's relative
+    half step) of the kernel that a chunk of `rows` rows of a key head goes to."""
     f32 = dtype == torch.float32
     if not quantized:
         # two F16 terms, or one; the largest weight is 2^12 or more (BF16: 2^8)
         if f32:
-            return 2.0 ** -21, 2.0 ** -22, 2.0 ** -37, 0.0
-        return 0.0, 2.0 ** -11, 2.0 ** -33, 0.0
+            return 2.0 ** -21, 2.0 ** -22, 2.0 ** -37, 0.0, 0.0
+        return 0.0, 2.0 ** -11, 2.0 ** -33, 0.0, 0.0
     if rows <= FEW_ROWS[dtype][dim]:
         # whole numbers, of 30 or 14 bits for q, 29 or (BF16, more than four rows) 21 for a product
-        return 2.0 ** -29 if f32 else 2.0 ** -13, 0.0, 0.0, 2.0 ** -29 if f32 or rows <= 4 else 2.0 ** -21
+        return 2.0 ** -29 if f32 else 2.0 ** -13, 0.0, 0.0, 2.0 ** -29 if f32 or rows <= 4 else 2.0 ** -21, 0.0
     if f32:
-        return 2.0 ** -21, 2.0 ** -22, 2.0 ** -37, 0.0
-    return 0.0, 2.0 ** -11, 2.0 ** -33, 0.0
+        return 2.0 ** -21, 2.0 ** -22, 2.0 ** -36, 0.0, 0.0
+    # (codes expanded first: with their scales, in F16)
+    return 0.0, 2.0 ** -11, 2.0 ** -31, 0.0, 2.0 ** -11
 
 
 def attention(q, cache, tables, new, counts, spec, longest=None):
@@ -61,7 +62,7 @@ def attention(q, cache, tables, new, counts, spec, longest=None):
     group = q_heads // cache.keys.shape[2]
     quantized = isinstance(cache, QuantizedKvCache) or hasattr(cache, "key_scales")
     rows = (longest or max(new)) * group
-    q_step, relative, absolute, product = roundings(q.dtype, quantized, rows, dim)
+    q_step, relative, absolute, product, coded = roundings(q.dtype, quantized, rows, dim)
     # (many BF16 rows: all keys of a split are one chain; else a tile's are)
     in_place = q.dtype == torch.bfloat16 and rows > (FEW_ROWS[q.dtype][dim] if quantized else 8)
     out = torch.zeros(tokens, q_heads, dim, dtype=torch.float64, device=q.device)
@@ -98,9 +99,14 @@ def attention(q, cache, tables, new, counts, spec, longest=None):
             # one key's own: q's steps in its score, its weight's rounding
             step = q_step * x.abs().amax(1, keepdim=True) / 2 * UNIFORM * abs(spec.scale)
             own = (step * kh.norm(dim=1)[None]) ** 2 + (relative * UNIFORM) ** 2
+            if coded:
+                own = own + (coded * UNIFORM * spec.scale) ** 2 * ((x * x) @ (kh * kh).T)
             mass = p * p * own
             square = mass @ (vh * vh) - 2 * o * (mass @ vh) + o * o * mass.sum(1, keepdim=True)
-            # rounded with its value's scale in it, of which the largest counts
+            if coded:
+                square = square + (coded * UNIFORM) ** 2 * ((p * p) @ (vh * vh))
+            # rounded with its value's scale in it, of which the largest counts (or
+            # without, where scales are in the values)
             if absolute:
                 reach = p if scales is None else p * scales[None, :, h // group].nan_to_num(0.0)
                 reach = torch.where(seen, reach, 0.0).amax(1, keepdim=True)

@@ -15,6 +15,7 @@ from tests.test_gpu_chunks import TYPES, attention_case
 
 pytestmark = pytest.mark.gpu
 
+CACHES = pytest.mark.parametrize("quantized", [True, False], ids=["i8", "f16"])
 KINDS = pytest.mark.parametrize("kind", ["f32", "bf16"])
 
 
@@ -136,10 +137,74 @@ def test_values_of_far_scales_in_one_tile_of_few_rows(ops, kind):
 @pytest.mark.parametrize("rest,spread", [(0.1, 0.5), (0.5, 1.5)])
 @pytest.mark.parametrize("count", [500, 16384, 65536])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("kind,quantized", [("f32", True), ("f32", False), ("bf16", False)], ids=["f32-i8", "f32-f16", "bf16-f16"])
+@pytest.mark.parametrize("kind,quantized", [("f32", True), ("f32", False), ("bf16", True), ("bf16", False)],
+                         ids=["f32-i8", "f32-f16", "bf16-i8", "bf16-f16"])
 def test_a_key_of_most_weight_and_no_value(ops, dim, count, kind, quantized, rest, spread):
     """The same for a chunk of 40 tokens and for a step over an F16 cache."""
     rng = np.random.default_rng(count + dim)
     for tokens in (40, 1):
         q, cache, tables = dominated(ops, rng, kind, quantized, tokens, count, 4, 2, dim, rest, spread, 0.0)
         holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim)))
+
+
+# (as FEW: units of 128 rows and of 256; codes converted tile by tile, or
+# expanded first, which is where there are several units)
+MANY = [
+    ([12, 40], [3000, 700], 8, 2, 128),
+    ([40, 1], [2000, 16], 16, 2, 256),
+    ([70, 30], [1300, 30], 16, 4, 64),
+    ([33], [1500], 10, 2, 80),
+    ([150, 20], [4000, 2000], 8, 2, 128),
+    ([700, 5], [1100, 500], 8, 2, 64),
+    ([400], [400], 16, 2, 256),
+    ([900], [1400], 8, 2, 128),
+]
+
+
+@pytest.mark.parametrize("window,softcap,sinks", [(0, None, False), (300, 20.0, True)], ids=["plain", "window-cap-sinks"])
+@KINDS
+@CACHES
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{c[0]}of{c[1]}h{c[2]}/{c[3]}d{c[4]}".replace(" ", ""))
+def test_many_rows(ops, case, quantized, kind, window, softcap, sinks):
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        (*case, 16, window, 4 if window else 0, softcap, sinks, True), kind, quantized)
+    holds(ops, q, cache, tables, new, counts, spec)
+
+
+@pytest.mark.parametrize("power", [8, 20, 40, 70])
+@KINDS
+@pytest.mark.parametrize("tokens", [48, 600])
+def test_hidden_scales_do_not_reach_earlier_rows_of_many(ops, tokens, kind, power):
+    """The last token's value scale, and its key's, is 2^power times the
+    others', for converted codes and expanded ones: the rows before it keep
+    their own bits."""
+    for dim in (64, 128):
+        new, counts, tables, page_size, cache, q, spec = attention_case(
+            ([tokens], [tokens + 200], 8, 2, dim, 16, 0, 0, None, False, True), kind, True)
+        page, place = int(tables[0][(tokens + 199) // 16]), (tokens + 199) % 16
+        cache.value_scales[page, :, place] *= 2.0 ** power
+        holds(ops, q, cache, tables, new, counts, spec)
+        cache.key_scales[page, :, place] *= 2.0 ** power
+        out = torch.empty_like(q)
+        ops.attention_chunks(q, cache, plain.chunks_of(new, counts, tables, 16), spec, out)
+        expected, off = chunk_accuracy.attention(q[:-1], cache, tables, [tokens - 1], [tokens + 199], spec, tokens)
+        assert ((out[:-1].double() - expected).abs() <= off).all()
+
+
+@KINDS
+@pytest.mark.parametrize("tokens", [48, 600])
+def test_values_of_far_scales_for_many_rows(ops, tokens, kind):
+    """As for few rows; and scales that grow, or fall, from tile to tile."""
+    rng = np.random.default_rng(13)
+    count = tokens + 500
+    tables, pages = plain.tables_of(rng, 1, -(-count // 16))
+    cache = plain.random_cache(rng, True, pages, 16, 2, 128)
+    position = np.zeros((pages, 1, 16))
+    position[tables[0]] = np.arange(tables.size * 16).reshape(-1, 1, 16)
+    grows = position / count * np.ones((1, 2, 1))
+    q = floats(rng, tokens, 8, 128).to(TYPES[kind])
+    for size in (rng.uniform(-40, 0, (pages, 2, 16)), rng.uniform(-110, -100, (pages, 2, 1)) * np.ones((1, 1, 16)),
+                 rng.uniform(95, 100, (pages, 2, 1)) * np.ones((1, 1, 16)), 60 * grows, -60 * grows, 120 * grows - 100):
+        cache.value_scales.copy_(torch.from_numpy(np.exp2(size).astype(np.float32)).cuda())
+        cache.value_scales[int(tables[0][0])] = 0.0
+        holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(128)))
