@@ -549,7 +549,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
           constexpr uint32_t SHIFT = uint32_t(Q_BITS) << 23;
           const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, SHIFT + 0x01000000u) - SHIFT;
           const float unit_inverse = __uint_as_float(0x7f000000u - exponent);
-          const float by = a.scale < 0.0f ? -unit_inverse : unit_inverse;
+          const float by = a.scale < 0.0f ? -unit_inverse : a.scale > 0.0f ? unit_inverse : 0.0f;
           const int pass = pass0 + n;
           const uint32_t own = __shfl_sync(0xffffffffu, exponent, lane % AT_ONCE * LANES);
           if (lane / AT_ONCE == pass) multiplier = fabsf(a.scale) * __uint_as_float(own);
@@ -572,8 +572,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
     const float value_unit = units.x;
     multiplier *= units.y;
-    // (a softcap leaves natural units behind; a factor of 2^-60 is as good as none)
-    const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 8.7e-19f);
+    // (a softcap leaves natural units behind; and never zero, which a hidden
+    // score of -infinity may not meet: with a scale of zero it is q that is)
+    const float m2 = a.softcap > 0.0f ? LOG2E : fmaxf(multiplier * LOG2E, 1.17549435e-38f);
     const int position = chunk.position + token;
     const int hi = a.causal ? position + 1 : seen.end;
     // (not below 0: a window of no limit less a key's position is past 32 bits)

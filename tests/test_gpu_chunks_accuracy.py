@@ -208,3 +208,16 @@ def test_values_of_far_scales_for_many_rows(ops, tokens, kind):
         cache.value_scales.copy_(torch.from_numpy(np.exp2(size).astype(np.float32)).cuda())
         cache.value_scales[int(tables[0][0])] = 0.0
         holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(128)))
+
+
+@pytest.mark.parametrize("power", [-70, -40, 40, 70])
+@KINDS
+@pytest.mark.parametrize("tokens", [1, 5, 48, 600])
+def test_small_queries_of_large_keys(ops, tokens, kind, power):
+    """q times 2^-power and keys' scales times 2^power: the same scores."""
+    new, counts, tables, page_size, cache, q, spec = attention_case(
+        ([tokens], [tokens + 200], 8, 2, 64, 16, 0, 0, None, False, True), kind, True)
+    cache.key_scales.mul_(2.0 ** power)
+    holds(ops, q * 2.0 ** -power, cache, tables, new, counts, spec)
+    none = Attention(0.0)
+    holds(ops, q * 2.0 ** -power, cache, tables, new, counts, none)
