@@ -62,3 +62,26 @@ def test_mistakes_are_outside_the_bound(count, tokens, kind, quantized):
     assert outside(other)[-1].any()
     # and its results rounded once to their type are inside
     assert not outside(expected.to(q.dtype).double()).any()
+
+
+@pytest.mark.parametrize("quantized", [True, False], ids=["i8", "f16"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_a_missing_rescale_is_outside_the_bound(tokens, kind, quantized):
+    """Scores that rise: a row's base moves, and the results so far with it. The
+    last move left out of them is far outside, if keys before it count."""
+    rng = np.random.default_rng(tokens)
+    count, dim = 1500, 64
+    cache = random_cache(rng, quantized, 94, 16, 1, dim)
+    tables = np.arange(94, dtype=np.int32)[None]
+    q = torch.from_numpy(rng.standard_normal((tokens, 1, dim)).astype(np.float32)).to(TYPES[kind])
+    spec = Attention(1 / math.sqrt(dim))
+    expected, off = chunk_accuracy.attention(q, cache, tables, [tokens], [count], spec)
+    _, v, _ = chunk_accuracy.sequence(cache, tables[0], count)
+    k = chunk_accuracy.sequence(cache, tables[0], count)[0]
+    for i in range(tokens):
+        score = k[:count - tokens + i + 1, 0] @ q[i, 0].double() * spec.scale
+        p = torch.softmax(score, 0)
+        for moved in (64, 640, 1216):  # keys before the move; it was by 2^3
+            other = expected[i, 0] + 7 * (p[:moved] @ v[:moved, 0])
+            assert ((other - expected[i, 0]).abs() > off[i, 0]).any()

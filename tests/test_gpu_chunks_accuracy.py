@@ -1,6 +1,7 @@
 """attention_chunks held to what its kernels' roundings allow
 (tests/chunk_accuracy.py): ordinary scores, a key that takes most of the weight
-and has no value, scales far apart, scales that a row's mask hides."""
+and has no value, scales far apart, scales that a row's mask hides, scores that
+grow along the keys."""
 
 import math
 
@@ -221,3 +222,51 @@ def test_small_queries_of_large_keys(ops, tokens, kind, power):
     holds(ops, q * 2.0 ** -power, cache, tables, new, counts, spec)
     none = Attention(0.0)
     holds(ops, q * 2.0 ** -power, cache, tables, new, counts, none)
+
+
+# ---- scores and scales that change along the keys --------------------------------------
+
+def ramped(ops, rng, kind, quantized, tokens, count, q_heads, kv_heads, dim, height, shape):
+    """Scores that rise by `height` (in powers of e) along the keys, fall, or
+    stand in steps of 200 keys, under noise of about one."""
+    along = floats(rng, kv_heads, 1, dim)
+    along = along / along.norm(dim=2, keepdim=True)
+    at = torch.arange(count, device="cuda", dtype=torch.float32)[:, None, None] / count
+    ramp = {"rises": at, "falls": 1 - at, "steps": torch.floor(at * count / 200) * 200 / count,
+            "peaks": torch.exp(-((at - 0.5) * 8) ** 2)}[shape] * height
+    q = floats(rng, tokens, kv_heads, q_heads // kv_heads, dim) + math.sqrt(dim) * along
+    k = floats(rng, count, kv_heads, dim) + ramp * along[None, :, 0]
+    cache, tables = written(ops, rng, quantized, k, floats(rng, count, kv_heads, dim))
+    return q.reshape(tokens, q_heads, dim).to(TYPES[kind]), cache, tables
+
+
+@pytest.mark.parametrize("shape", ["rises", "falls", "steps", "peaks"])
+@pytest.mark.parametrize("height", [4.0, 15.0, 60.0])
+@CACHES
+@KINDS
+def test_scores_that_grow_along_the_keys(ops, kind, quantized, height, shape):
+    """Bases move in the middle of a chain of tiles, outputs with them: for few
+    rows and many, whole and in splits, with a sink between the first score
+    and the last."""
+    rng = np.random.default_rng(int(height))
+    for tokens, count, dim in ((1, 3000, 128), (5, 1500, 64), (40, 2500, 128), (300, 1700, 64), (130, 900, 256), (48, 20000, 80)):
+        q, cache, tables = ramped(ops, rng, kind, quantized, tokens, count, 4, 2, dim, height, shape)
+        for sinks in (None, torch.full((4,), height / 2, device="cuda")):
+            holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim), sinks=sinks))
+
+
+@pytest.mark.parametrize("grows", [1.0, 3.0, -3.0])
+@KINDS
+def test_scales_that_grow_from_tile_to_tile(ops, kind, grows):
+    """Key and value scales that double (or halve) every 64 positions once and
+    thrice, under scores that rise."""
+    rng = np.random.default_rng(17)
+    for tokens, count, dim in ((1, 2000, 128), (5, 1500, 64), (40, 1500, 128), (300, 1400, 64), (130, 900, 256)):
+        q, cache, tables = ramped(ops, rng, kind, True, tokens, count, 4, 2, dim, 10.0, "rises")
+        position = np.zeros((cache.pages, 1, 16))
+        position[tables[0]] = np.arange(tables.size * 16).reshape(-1, 1, 16)
+        by = torch.from_numpy(np.exp2(position // 64 * grows).astype(np.float32)).cuda()
+        cache.value_scales.mul_(by)
+        holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim)))
+        cache.key_scales.mul_(by ** 0.1)
+        holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim)))
