@@ -49,8 +49,8 @@ Plan plan_rows(const Call& c) {
   const long long tiles = std::max(1LL, tiles_bound(c, p.rows_per_unit, p.keys_per_tile));
   const int warps = codes ? attention_codes_warps(c.head_dim) : ATTENTION_ROWS_WARPS;
   const long long slots = (long long)sm_count() * (codes ? attention_codes_ctas(c.head_dim) : attention_rows_ctas(c.head_dim));
-  // CTAs for every SM four times over (F16 caches eight: a step of 16 x 16384
-  // keys 148 us, and 179 with four; 8-bit ones of 3 sequences 28, and 33 with
+  // CTAs for every SM four times over (F16 caches eight: a step of 16 x 8700 to
+  // 16384 keys 148 us, and 179 with four; 8-bit ones of 3 sequences 28, and 33 with
   // eight), of a tile a warp at least; two splits while that leaves SMs idle
   // (eight chunks of 40 F32 rows: 100 us, 111 with one)
   const long long wanted =
@@ -68,13 +68,14 @@ Plan plan_rows(const Call& c) {
 }
 
 // Whether a chunk's rows of a key head go to the tensor-core tiles, by what
-// both take on B200 (8 sequences x 8 key heads x 4096 keys; us, few rows' kernel
-// and tiles): F16 caches BF16 8 rows 35 and 43, 12 rows 54 and 44; F32 38 and
-// 57, 12 rows 59 and 59. 8-bit ones BF16 32 rows 61 and 75, 40 rows 80 and 77
-// (heads of 256: 24 rows 95 and 105, 32 rows 123 and 107); F32 40 rows 100 and
-// 130, and of one sequence 22 and 24, but 48 rows 31 and 24. F32 heads of 256
-// (8 x 2 key heads): F16 16 rows 35 and 43, 24 rows 46 and 45; 8-bit 64 rows 78
-// and 83, 128 rows 133 and 82.
+// both take on B200 (8 sequences x 8 key heads of 128, the longest of so many
+// rows over 4096 keys, the others down to half; us, few rows' kernel and tiles):
+// F16 caches BF16 8 rows 35 and 43, 12 rows 40 and 44 (all of them as long: 56 and
+// 45); F32 8 rows 37 and 57, 12 rows 43 and 58 (60 and 59). 8-bit ones BF16 32
+// rows 63 and 77, 40 rows 90 and 76 (heads of 256: 24 rows 92 and 91, 32 rows 113
+// and 93); F32 40 rows 104 and 129, and of one sequence 22 and 25, but 48 rows
+// 33 and 25. F32 heads of 256 (8 x 2 key heads): F16 16 rows 35 and 42, 24 rows
+// 46 and 43; 8-bit 64 rows 79 and 86, 128 rows 136 and 88.
 bool takes_tiles(const Call& c, long long rows) {
   const bool bf16 = c.x_dtype == DRIFT_BF16;
   const bool wide = c.head_dim > 128;
@@ -135,11 +136,12 @@ Plan plan_tiles(const Call& c, bool converts, double slower, double& least) {
 }
 
 // The same with the choice of expanding an 8-bit cache's codes: two launches
-// more (BF16 rows: three), and 3 bytes a value at about 3 TB/s (three chunks of 1001 BF16 tokens x 4
-// heads over 5003 keys: 290 us, 395 with each unit's own conversion; three of
-// 100 over 2000: 55, and 49; 2048 F32 tokens over 8192: 660, and 1000; 64 over
-// 16384: 109, and 88), in at most 1 GiB. Converting codes makes a tile
-// 2.2 (BF16) and 2.5 times as long, exact codes' scales 1.4 times.
+// more (BF16 rows: three), and 3 bytes a value at about 3 TB/s, in at most 1 GiB
+// (us, with each unit's own conversion and expanded: three chunks of 1001 BF16
+// tokens x 4 heads over 5003 keys 527 and 293, three of 100 over 2000 49 and 55,
+// eight of 40 over 4096 104 and 120; 2048 F32 tokens over 8192 1031 and 640, 64
+// over 16384 89 and 109). Converting codes makes a tile 2.2 (BF16) and 2.5 times
+// as long, scales by key 1.4 times.
 Plan plan_all_tiles(const Call& c) {
   constexpr double BYTES_A_NS = 3000;
   double own;

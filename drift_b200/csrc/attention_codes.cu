@@ -30,11 +30,13 @@
 // weight passes 2^3 (and one vote a tile tells). The warps meet in shared
 // memory, the splits in a second launch (attention_chunks_join_kernel).
 //
-// Bound by the issue of about 930 instructions a tile of 32 keys (57 % of the
-// slots; the rest waits on loads and on the products' chains), above memory: a
-// step of 16 sequences x 16384 keys of 8 heads of 128, F32, 110 us, 4 TB/s of
-// codes and scales; one of 4096 keys 11 us, by two launches' latencies; 8 x 5
-// drafts over 4096 keys 51 us, three units of eight rows a sequence and head.
+// Bound by latency at 12 warps an SM (168 registers: a tile of codes on its way
+// in each): about 1200 instructions a tile of 32 keys take 51 % of the issue
+// slots and 37 % of DRAM's rate; a warp waits on fixed latencies and on global
+// loads, about an issue's time each. A step of 16 sequences of 8700 to 16384
+// keys of 8 heads of 128, F32, 115 us, 3.7 TB/s of codes and scales; one of 4096
+// keys 11 us, two launches' latencies; 8 sequences' up to 5 drafts over up to
+// 4096 keys 53 us, three units of eight rows a sequence and head.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -50,7 +52,6 @@ namespace {
 
 constexpr int TILE = 32;   // keys of a warp's tile
 constexpr int PITCH = 36;  // words of a row's weights in shared memory: rows on different banks
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ZERO = 0x4b400000;  // the bits of 1.5 x 2^23
 constexpr float ZERO_VALUE = 12582912.0f;
 constexpr float GROWTH = 8.0f;    // a weight that moves its base
@@ -89,10 +90,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return c;
 }
 
-__device__ __forceinline__ float weight_of(float score, float base) {
-  return score == -INFINITY ? 0.0f : exp2f((score - base) * LOG2E);
-}
-
 // Packed: up to four rows, column c of digit tile j being row c % 4's digit 2 j
 // + c / 4; otherwise up to eight, with a tile for each digit. (Sixteen or
 // twenty-four rows to a warp shared its keys but left registers for eight warps
@@ -103,7 +100,7 @@ struct CodesTraits {
   static constexpr bool BF16 = BF16_, PACKED = PACKED_;
   static constexpr int ROWS = PACKED ? 4 : 8;
   // As many warps as registers leave an SM without spills: sixteen of 128, for
-  // heads of 128 twelve of 168 (a step of 16 x 16384 keys: sixteen, spilling,
+  // heads of 128 twelve of 168 (a step of 16 x 8700 to 16384 keys: sixteen, spilling,
   // 191 us, twelve 113, eight 135), for more rows and wider heads eight. In
   // CTAs of four, one's start and end run under the others.
   static constexpr int WARPS = attention_codes_warps(D), THREADS = 32 * WARPS;

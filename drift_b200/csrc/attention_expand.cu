@@ -1,7 +1,7 @@
 // For attention_chunks over an 8-bit cache where a chunk has several units of
 // rows: the sequences' keys and values as F16, once, for attention_tiles' F16
-// kernel. Its own converting warps make each tile anew for every unit, and
-// bound it (a tile of BF16 rows 5900 clocks, 2700 from an F16 cache).
+// kernel. The tiles' own converting warps make each tile anew for every unit (one
+// takes 2.2 times as long as from an F16 cache).
 //
 //   BF16 rows: keys16, values16 = code scale / unit, rounded to F16 once
 //   F32 rows:  keys16, values16 = code, exactly; and rows of scales for each
@@ -11,9 +11,10 @@
 // 2^-8 of what the largest scale that a row sees rounds up to, so that a
 // quotient is at most 2^15, and 2^-14 and more for scales down to 2^-22 of that,
 // where F16 has its 11 bits: what a row has of its keys does not depend on the
-// scales beside them. Scales that are farther apart (than 2^20), not finite or at
-// the ends of F32's range go by key as F32 rows' do, at a third more time in the
-// tiles. The tiles multiply scores by the keys' unit and results by the values'.
+// scales beside them. Heads whose scales are farther apart (than 2^20), not
+// finite or at the ends of F32's range go by key as F32 rows' do, in a launch of
+// the tiles of their own, by a third slower. The tiles multiply scores by the
+// keys' unit and results by the values'.
 //
 // The copies are a paged cache of their own, in the F16 cache's layouts, with
 // sequence z's pages from z * page_row on and the table that says so. Only what
@@ -63,13 +64,6 @@ struct SeenPositions {
   }
   __device__ bool sees(int position) const { return position < end && (position >= low || position < first); }
 };
-
-// A power of two at or above x whose inverse is normal.
-__device__ __forceinline__ float power_over(float x) {
-  const uint32_t bits = __float_as_uint(x);
-  const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-  return __uint_as_float(max(up, 0x01000000u));
-}
 
 __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const ExpandArgs a) {
   pdl_trigger();  // the next kernel may launch and wait for this one

@@ -18,9 +18,9 @@
 // exactly; a key's scale multiplies its scores, and a value's its weights, in
 // F32 (BY_KEY). Where a chunk has several units of rows its codes come expanded to
 // an F16 cache of the call's own (attention_expand.cu), with their scales by
-// position (SCALED), or for BF16 rows with them
-// in the values where they are of like size. Values' scales are over a power of two, of all that some
-// row sees (SCALED) or of those so far.
+// position (SCALED), or for BF16 rows with their scales in them where those are of
+// like size. Values' scales are over a power of two, of all that some row sees
+// (SCALED) or of those so far.
 //
 // Where scales are by key, a row's base is set by its largest product of weight
 // and value scale, since that is what is rounded to F16: so its bits are its own,
@@ -32,13 +32,13 @@
 // have taken S into registers, P V when P is there. So the tensor core works
 // under the softmax and the softmax under the products, and what bounds a tile
 // is the longer of the two: for D = 128 the tensor core's 16 + 10 products of
-// 64 and 52 clocks for 80 keys and 256 rows. (With P over S, and Q K^T behind
-// P V, a tile took both after one another: 3050 clocks for 128 keys.) TMEM's
-// 512 columns set the tile's keys: MT S, MT P, MT outputs. Measured: a chunk of
-// 2048 BF16 tokens of 32 heads of 128 over 8192 keys 241 us, 1000 TFLOP/s, the
-// special function unit (an exponential a score) and the tensor core each busy
-// for 59 % of a full SM's time (51 % on average: 256 CTAs on 148 SMs); 1500 F32 tokens of 16 heads 67 us; 6000 BF16 tokens of 8 heads of 64
-// under a window of 1024 51 us, the exponentials.
+// 64 and 52 clocks for 80 keys and 256 rows. TMEM's 512 columns set the tile's
+// keys: MT S, MT P, MT outputs. Measured: a chunk of 2048 BF16 tokens of 32 heads
+// of 128 over 8192 keys 241 us, 1000 TFLOP/s, the special function unit (an
+// exponential a score) and the tensor core each busy for 59 % of a full SM's time
+// (51 % on average: 256 CTAs on 148 SMs); 1500 F32 tokens of 16 heads 71 us; 6000
+// BF16 tokens of 8 heads of 64 under a window of 1024 52 us: 192 CTAs on 148 SMs, each 11 tiles, 4 of them at an edge, and its
+// start and end (the exponentials are under half of it on an SM with two CTAs).
 //
 // BF16 rows (TERMS = 1): q is exact in F16 after a power of two per row; P's
 // rounding to F16 (2^-11) is 1/8 of the result's own (2^-8). O stays in TMEM.
@@ -81,7 +81,6 @@ namespace drift {
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int ROW_TILE = 128;
 constexpr uint32_t TMEM_COLUMNS = 512;
@@ -342,10 +341,6 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-__device__ __forceinline__ uint32_t half_pair(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // What F16 leaves of a pair.
 __device__ __forceinline__ uint32_t left_pair(float a, float b, uint32_t pair) {
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pair));
@@ -365,8 +360,9 @@ __device__ __forceinline__ uint2 code_pairs(uint32_t codes) {
 
 // softcap tanh(y): near zero y times a polynomial in its square (least squares
 // on Chebyshev points of |y| <= NEAR, reweighted towards the least largest
-// relative error, 1e-9), farther off 1 - 2 / (1 + e^(2 y)), which loses bits
-// only near zero.
+// relative error, 1e-9), farther off 1 - 2 / (1 + e^(2 y)). The cut is where
+// tanh is 1/2: from there on the difference is no smaller than what is taken from
+// 1, and loses one bit at most.
 constexpr float NEAR = 0.55f;
 __device__ __forceinline__ float capped_near(float y) {
   const float u = y * y;
@@ -1115,12 +1111,6 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
 #pragma unroll
       for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       return most;
-    };
-    // a power of two at or above x whose inverse is normal
-    auto power_over = [](float x) {
-      const uint32_t bits = __float_as_uint(x);
-      const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
-      return __uint_as_float(max(up, 0x01000000u));
     };
     float v_power = 0.0f;
     bool ok = true;

@@ -70,6 +70,25 @@ struct AttentionChunksArgs {
   float scale, softcap;
 };
 
+constexpr float LOG2E = 1.4426950408889634f;
+
+// e^(score - base), 0 for a score that is not seen.
+__device__ __forceinline__ float weight_of(float score, float base) {
+  return score == -INFINITY ? 0.0f : exp2f((score - base) * LOG2E);
+}
+
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A power of two at or above x whose inverse is normal.
+__device__ __forceinline__ float power_over(float x) {
+  const uint32_t bits = __float_as_uint(x);
+  const uint32_t up = min((bits & 0x7f800000u) + ((bits & 0x7fffffu) ? 0x800000u : 0u), 0x7e800000u);
+  return __uint_as_float(max(up, 0x01000000u));
+}
+
 // A value's scale (over a power of two, 1 at most) to base 2, as it moves a
 // row's base: 2^-80 at least, so that no weight is past F32's range because its
 // value has none.
