@@ -16,10 +16,10 @@
 // numbers without a conversion (|sum| < 2^22), and their digits are joined in
 // F32. A key's scale multiplies its score, a value's its weight.
 //
-// What the conversion rounds: q to 2^-30 (F32) or 2^-14 (BF16) of its row's
-// largest value; a row's 32 products of weight and value scale in a tile to
-// 2^-30 of the largest of them (BF16 rows of more than four: 2^-22), each row
-// and tile over a power of two of its own. So a row does not depend on what it
+// What the conversion rounds: q to 2^-30 of its row's largest value and a row's
+// 32 products of weight and value scale in a tile to 2^-30 of the largest of them
+// (BF16 rows of more than four, in three digits: 2^-22), each row and tile over a
+// power of two of its own. So a row does not depend on what it
 // does not see, a key of much weight costs no other tile's keys bits, and in
 // its own none if its value is small (a row's largest code is 127, so its scale
 // is its size). Steps of the warp's largest weight instead lost a tenth of the
@@ -105,10 +105,10 @@ struct CodesTraits {
   // CTAs of four, one's start and end run under the others.
   static constexpr int WARPS = attention_codes_warps(D), THREADS = 32 * WARPS;
   static constexpr int CTAS = attention_codes_ctas(D);
-  static constexpr int Q_DIGITS = BF16 ? 2 : 4, P_DIGITS = PACKED || !BF16 ? 4 : 3;
+  static constexpr int DIGITS = PACKED || !BF16 ? 4 : 3, Q_DIGITS = DIGITS, P_DIGITS = DIGITS;
   static constexpr int Q_TILES = PACKED ? Q_DIGITS / 2 : Q_DIGITS;
   static constexpr int P_TILES = PACKED ? P_DIGITS / 2 : P_DIGITS;
-  static constexpr int Q_BITS = BF16 ? 13 : 29;                  // of the largest value's leading bit
+  static constexpr int Q_BITS = DIGITS == 4 ? 29 : 21;           // of the largest value's leading bit
   static constexpr int P_BITS = P_DIGITS == 4 ? 29 : 21;         // the same for a tile's products
   static constexpr int CHUNKS = D / 64, TAIL = D % 64 / 16;      // 16-byte chunks a lane has of a key row; 4 bytes
   static constexpr int STEPS = 2 * CHUNKS + TAIL, WORDS = 4 * CHUNKS + TAIL;

@@ -279,7 +279,7 @@ int drift_cache_read_chunks(int x_dtype, void* k, void* v, int64_t tokens, int k
  * positions. softcap, sinks and the limits on heads are drift_attention's;
  * max_key_count bounds positions[z] plus z's tokens. F32 rows are computed to
  * F32's accuracy; BF16 rows with weights, and an 8-bit cache's keys and values,
- * rounded to F16, or (few rows over an 8-bit cache) with q in steps of 2^-13 of
+ * rounded to F16, or (few rows over an 8-bit cache) with q in steps of 2^-21 of
  * its row's largest value and the products of 32 keys' weights and value scales
  * in steps of 2^-21 of the largest of them. q and out do not overlap. `workspace`
  * (16-byte aligned, the caller's: calls that may overlap need one each) holds

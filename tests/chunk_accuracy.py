@@ -48,8 +48,9 @@ def roundings(dtype, quantized, rows, dim):
             return 2.0 ** -21, 2.0 ** -22, 2.0 ** -37, 0.0, 0.0
         return 0.0, 2.0 ** -11, 2.0 ** -33, 0.0, 0.0
     if rows <= FEW_ROWS[dtype][dim]:
-        # whole numbers, of 30 or 14 bits for q, 29 or (BF16, more than four rows) 21 for a product
-        return 2.0 ** -29 if f32 else 2.0 ** -13, 0.0, 0.0, 2.0 ** -29 if f32 or rows <= 4 else 2.0 ** -21, 0.0
+        # whole numbers, of 29 bits or (BF16, more than four rows) 21
+        step = 2.0 ** -29 if f32 or rows <= 4 else 2.0 ** -21
+        return step, 0.0, 0.0, step, 0.0
     if f32:
         return 2.0 ** -21, 2.0 ** -22, 2.0 ** -36, 0.0, 0.0
     # (codes expanded first: with their scales, in F16)

@@ -270,3 +270,34 @@ def test_scales_that_grow_from_tile_to_tile(ops, kind, grows):
         holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim)))
         cache.key_scales.mul_(by ** 0.1)
         holds(ops, q, cache, tables, [tokens], [count], Attention(1 / math.sqrt(dim)))
+
+
+@CACHES
+@KINDS
+@pytest.mark.parametrize("tokens", [1, 2, 6, 48, 300])
+def test_a_query_of_one_large_value(ops, tokens, kind, quantized):
+    """A dimension in which q is 4000 times as large as elsewhere and the keys
+    are nothing: the others' scores keep their bits."""
+    rng = np.random.default_rng(tokens)
+    for dim, heads in ((64, (4, 2)), (128, (4, 1)), (256, (16, 2))):
+        k, v = floats(rng, 900, heads[1], dim), floats(rng, 900, heads[1], dim)
+        k[..., 7] = 0.0
+        cache, tables = written(ops, rng, quantized, k, v)
+        q = floats(rng, tokens, heads[0], dim)
+        q[..., 7] *= 4000.0
+        holds(ops, q.to(TYPES[kind]), cache, tables, [tokens], [900], Attention(2 / math.sqrt(dim)))
+
+
+@KINDS
+def test_heads_and_sequences_of_far_scales_beside_others(ops, kind):
+    """One head of one sequence has scales far apart and the others do not:
+    each goes its own way (BF16 rows' expanded codes in two launches), with
+    splits and without."""
+    for new, counts in (([300, 250], [4000, 700]), ([1200, 700], [1300, 2400]), ([40, 48], [2000, 900])):
+        new, counts, tables, page_size, cache, q, spec = attention_case(
+            (new, counts, 8, 2, 128, 16, 0, 0, None, True, True), kind, True)
+        cache.value_scales[int(tables[0][3]), 1, 5] *= 2.0 ** 30
+        cache.key_scales[int(tables[1][20]), 0, 9] *= 2.0 ** -30
+        holds(ops, q, cache, tables, new, counts, spec)
+        windowed = Attention(spec.scale, window=200, first=3, sinks=spec.sinks)
+        holds(ops, q, cache, tables, new, counts, windowed)
