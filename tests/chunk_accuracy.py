@@ -1,10 +1,12 @@
 """attention_chunks in 64 bits with the error to expect of each kernel, tight
 enough to tell a key left out or taken from another page.
 
-A result is o = sum_k p_k v_k over the keys that a row sees. If key k's weight
-is off by a factor 1 + e_k, o is off by sum_k p_k e_k (v_k - o): the sum of the
-weights is off with them. Roundings of different keys are independent, so
-their squares add, and a result may be off by SIGMAS times the root; a uniform
+A result is o = sum_k p_k v_k over the keys that a row sees. If key k's score
+is off by e_k, o is off by sum_k p_k e_k (v_k - o): the sum of the weights is off
+with them. A weight's rounding for the product with its value is not in that
+sum: there o is off by sum_k p_k e_k v_k (a row of one key, whose weight over
+the sum is one: by all of a half step). Roundings of different keys are
+independent, so their squares add, and a result may be off by SIGMAS times the root; a uniform
 error of a half step h has a deviation of h / sqrt(3). What repeats from key to
 key (F32 and tensor-core sums of a score, the functions of one score) is added
 in the open. The result's own rounding is half a step of its type."""
@@ -97,15 +99,15 @@ def attention(q, cache, tables, new, counts, spec, longest=None):
                 total = total + torch.exp(spec.sinks[h].double() - largest)
             p = weight / total
             o = p @ vh
-            # one key's own: q's steps in its score, its weight's rounding
+            # one key's own: q's steps in its score
             step = q_step * x.abs().amax(1, keepdim=True) / 2 * UNIFORM * abs(spec.scale)
-            own = (step * kh.norm(dim=1)[None]) ** 2 + (relative * UNIFORM) ** 2
+            own = (step * kh.norm(dim=1)[None]) ** 2
             if coded:
                 own = own + (coded * UNIFORM * spec.scale) ** 2 * ((x * x) @ (kh * kh).T)
             mass = p * p * own
             square = mass @ (vh * vh) - 2 * o * (mass @ vh) + o * o * mass.sum(1, keepdim=True)
-            if coded:
-                square = square + (coded * UNIFORM) ** 2 * ((p * p) @ (vh * vh))
+            # its weight's rounding, and its value's
+            square = square + (relative ** 2 + coded ** 2) * UNIFORM ** 2 * ((p * p) @ (vh * vh))
             # rounded with its value's scale in it, of which the largest counts (or
             # without, where scales are in the values)
             if absolute:
