@@ -139,9 +139,10 @@ __global__ void __launch_bounds__(UNIT_THREADS) attention_units_kernel(const Exp
     if (high != 0) by_key = by_key || high - low > 20 << 23 || high > 247 << 23 || high < (side == 0 ? 77 : 27) << 23;
   }
   if (threadIdx.x > 0) return;
-  constexpr float LESS = 1.0f / 256.0f;
-  a.units[(long long)z * a.kv_heads + head] = by_key ? make_float4(power_over(top[1]), 1.0f, 1.0f, 0.0f)
-                                                     : make_float4(power_over(top[1]) * LESS, power_over(top[0]) * LESS, 0.0f, 0.0f);
+  // (all zeros are over one: what they would be over has no inverse)
+  auto over = [](float x) { return x > 0.0f ? power_over(x) * (1.0f / 256.0f) : 1.0f; };
+  a.units[(long long)z * a.kv_heads + head] =
+      by_key ? make_float4(power_over(top[1]), 1.0f, 1.0f, 0.0f) : make_float4(over(top[1]), over(top[0]), 0.0f, 0.0f);
 }
 
 // 64 positions of a head (128 where D = 80): a thread takes 16 codes at a time, of a position's

@@ -278,10 +278,11 @@ int drift_cache_read_chunks(int x_dtype, void* k, void* v, int64_t tokens, int k
  * p - window + 1 on and, whatever the window, the sequence's first `first`
  * positions. softcap, sinks and the limits on heads are drift_attention's;
  * max_key_count bounds positions[z] plus z's tokens. F32 rows are computed to
- * F32's accuracy; BF16 rows with weights, and an 8-bit cache's keys and values,
- * rounded to F16, or (few rows over an 8-bit cache) with q in steps of 2^-21 of
- * its row's largest value and the products of 32 keys' weights and value scales
- * in steps of 2^-21 of the largest of them. q and out do not overlap. `workspace`
+ * F32's accuracy; BF16 rows with weights (by 2^-33 of a row's largest at least),
+ * and an 8-bit cache's keys and values, rounded to F16, or (few rows over an 8-bit
+ * cache) with q in steps of 2^-21 of its row's largest value and the products of
+ * 32 keys' weights and value scales in steps of 2^-21 of the largest of them. q
+ * and out do not overlap. `workspace`
  * (16-byte aligned, the caller's: calls that may overlap need one each) holds
  * drift_attention_chunks_workspace_bytes(...) bytes of partial results and copies. */
 int drift_attention_chunks(int x_dtype, const void* q, int64_t tokens, int q_heads, int kv_heads,

@@ -108,14 +108,16 @@ def attention(q, cache, tables, new, counts, spec, longest=None):
             square = mass @ (vh * vh) - 2 * o * (mass @ vh) + o * o * mass.sum(1, keepdim=True)
             # its weight's rounding, and its value's
             square = square + (relative ** 2 + coded ** 2) * UNIFORM ** 2 * ((p * p) @ (vh * vh))
-            # rounded with its value's scale in it, of which the largest counts (or
-            # without, where scales are in the values)
+            # rounded with its value's scale in it, of which the largest counts; where
+            # scales are in the values (BF16 rows' expanded codes) of the largest weight
             if absolute:
                 reach = p if scales is None else p * scales[None, :, h // group].nan_to_num(0.0)
                 reach = torch.where(seen, reach, 0.0).amax(1, keepdim=True)
                 size = vh if scales is None else torch.where(scales[:, h // group, None] > 0,
                                                              vh / scales[:, h // group, None], 0.0)
                 square = square + (absolute * UNIFORM * reach) ** 2 * (seen.double() @ (size * size))
+                if coded:
+                    square = square + (absolute * UNIFORM * p.amax(1, keepdim=True)) ** 2 * (seen.double() @ (vh * vh))
             if product:
                 s = torch.where(any_row, scales[:, h // group], 0.0)
                 tiles = torch.nn.functional.pad(torch.where(seen, p * s, 0.0), (0, -count % 32)).view(n, -1, 32)

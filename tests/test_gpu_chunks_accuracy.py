@@ -301,3 +301,21 @@ def test_heads_and_sequences_of_far_scales_beside_others(ops, kind):
         holds(ops, q, cache, tables, new, counts, spec)
         windowed = Attention(spec.scale, window=200, first=3, sinks=spec.sinks)
         holds(ops, q, cache, tables, new, counts, windowed)
+
+
+@KINDS
+@pytest.mark.parametrize("tokens", [1, 5, 48, 600])
+def test_keys_or_values_of_zeros(ops, tokens, kind):
+    """Scales of zero in all that a head sees, or in all of its keys."""
+    for dim in (64, 128, 256):
+        new, counts, tables, page_size, cache, q, spec = attention_case(
+            ([tokens, 1], [tokens + 90, 1], 8, 2, dim, 16, 0, 0, None, dim == 128, True), kind, True)
+        cache.value_scales[:, 0] = 0.0
+        cache.key_scales[:, 1] = 0.0
+        bounds = dict(longest=tokens + 100, max_keys=tokens + 105)
+        for b in ({}, bounds):
+            out = holds(ops, q, cache, tables, new, counts, spec, **b)
+            assert (out[:, :4] == 0.0).all()
+        cache.value_scales.zero_()
+        cache.key_scales.zero_()
+        assert (holds(ops, q, cache, tables, new, counts, spec) == 0.0).all()
