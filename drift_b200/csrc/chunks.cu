@@ -5,7 +5,8 @@
 // either side, [pages][kv_heads][page offset].
 //
 // A row x of D values is kept as scale s = fl(max |x| / 127) and codes
-// c = rint(x / s), halves to the even code: a value is off by at most s / 2.
+// c = rint(x / s), halves to the even code: a value is off by at most s / 2 (codes
+// end at 127, which only subnormal scales, rounded by more than 2^-8, can pass).
 // The quotient is decided exactly (quantize()), so a code never depends on how
 // a division rounds. A row that holds a NaN or an infinity has no step: its
 // scale is NaN and it reads back as NaNs.

@@ -253,8 +253,9 @@ int drift_attention_decode(const float* q, int batch, int q_heads, const void* k
  * values is scale = max |x| / 127 (rounded to F32) and codes x / scale
  * rounded to the nearest whole number, halves to the even one, as in exact
  * arithmetic -- (head_dim + 4) bytes for 2 head_dim, each value within half a
- * scale of x. A row with a NaN or an infinity reads back as NaNs. Scales are
- * NULL for DRIFT_F16. */
+ * scale of x (in rows of less than 2^-135, whose scales have few bits, codes end
+ * at 127; those of less than 2^-143 are zeros). A row with a NaN or an infinity
+ * reads back as NaNs. Scales are NULL for DRIFT_F16. */
 /* drift_cache_write for all sequences. Two sequences may share pages if they
  * write none of them. */
 int drift_cache_write_chunks(int x_dtype, const void* k, const void* v, int64_t tokens, int kv_heads,
